@@ -1,0 +1,560 @@
+"""Performance cases of the attention operators between the FP8 projections
+and the expert layer: what a serving program calls, at the sizes it calls it
+with.
+
+Four kinds of call (colormlm_amd.attention):
+
+  norm_rope  per-head RMS norms of the query and key projections with the
+             position rotation in the same pass
+  append     keys and values of new tokens into the paged 8-bit cache (E4M3
+             codes, one E8M0 scale a page, head and side), the keys' norm and
+             rotation on the way
+  paged      attention of the new tokens over that cache: decode, speculative
+             verify, a prompt's later chunks
+  prompt     causal attention over whole packed prompts in bf16
+
+Head layouts: 32 query heads over 8 key heads of 128 and 64 over 8 of 64, the
+generic ones at hidden size 4,096, and 64 query heads over one key head of
+512, the layout of the package's own projections (wq_b [32768, 1024], wkv
+[512, 4096]).  Projections are N(0, 1) rows, pages lie in the cache in random
+order, sequence lengths are log-uniform.  Every input is drawn from the seed.
+"""
+
+from __future__ import annotations
+
+import functools
+import math
+import random
+
+import torch
+
+own = False
+
+EPS = 1e-6
+THETA = 10000.0
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def listed():
+    return [
+        # decode of one token: the rows of one projection call, where the launch is what counts
+        {"name": "norm_rope_1", "op": "norm_rope", "tokens": 1, "heads": 32, "kv": 8, "dim": 128, "rot": 128,
+         "layout": "half", "norm": True, "dtype": "f32", "table": 32768},
+        # a long prompt's projections as fp8_linear leaves them
+        {"name": "norm_rope_16384", "op": "norm_rope", "tokens": 16384, "heads": 32, "kv": 8, "dim": 128, "rot": 128,
+         "layout": "half", "norm": True, "dtype": "f32", "table": 32768},
+        # the package's own projections: 512 wide heads, the last 64 dimensions rotated in pairs
+        {"name": "norm_rope_333_wide", "op": "norm_rope", "tokens": 333, "heads": 64, "kv": 1, "dim": 512, "rot": 64,
+         "layout": "interleaved", "norm": True, "dtype": "bf16", "table": 131072},
+        # one speculative-verify block of one sequence, one wide key head
+        {"name": "append_verify_8", "op": "append", "seqs": 1, "new": 8, "ragged": False, "past": 299, "kv": 1,
+         "dim": 512, "page": 64, "rot": 64, "layout": "interleaved", "norm": True, "dtype": "f32", "spread": 1},
+        # one decode step of a batch
+        {"name": "append_decode_96", "op": "append", "seqs": 96, "new": 1, "ragged": False, "past": 700, "kv": 8,
+         "dim": 128, "page": 64, "rot": 128, "layout": "half", "norm": True, "dtype": "f32", "spread": 2},
+        # packed prompts whose keys are rotated already
+        {"name": "append_prompts", "op": "append", "seqs": 21, "new": 4000, "ragged": True, "past": 100, "kv": 8,
+         "dim": 128, "page": 64, "rot": 0, "layout": "half", "norm": False, "dtype": "bf16", "spread": 3},
+        # decode of one sequence of an odd length: few rows, a long axis
+        {"name": "paged_1_4097", "op": "paged", "seqs": 1, "new": 1, "ragged": False, "len": 4097, "same": True,
+         "heads": 32, "kv": 8, "dim": 128, "page": 64, "window": 0, "lse": False, "spread": 4},
+        # a speculative-verify block at a long context
+        {"name": "paged_verify8_40000", "op": "paged", "seqs": 1, "new": 8, "ragged": False, "len": 40000, "same": True,
+         "heads": 32, "kv": 8, "dim": 128, "page": 64, "window": 0, "lse": True, "spread": 5},
+        # one decode step of a batch of ragged lengths
+        {"name": "paged_decode_128", "op": "paged", "seqs": 128, "new": 1, "ragged": False, "len": 8192, "same": False,
+         "heads": 32, "kv": 8, "dim": 128, "page": 64, "window": 0, "lse": False, "spread": 6},
+        # 64 query heads over one wide key head: matrix work, not bytes
+        {"name": "paged_wide_4x9000", "op": "paged", "seqs": 4, "new": 4, "ragged": False, "len": 9000, "same": False,
+         "heads": 64, "kv": 1, "dim": 512, "page": 64, "window": 0, "lse": False, "spread": 7},
+        # one long prompt
+        {"name": "prompt_8192", "op": "prompt", "seqs": 1, "len": 8192, "same": True, "heads": 32, "kv": 8, "dim": 128,
+         "window": 0, "lse": True, "spread": 8},
+        # packed prompts of different lengths
+        {"name": "prompt_packed", "op": "prompt", "seqs": 17, "len": 2500, "same": False, "heads": 32, "kv": 8,
+         "dim": 128, "window": 0, "lse": False, "spread": 9},
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+LAYOUTS = [(32, 8, 128), (32, 8, 128), (64, 8, 64), (32, 4, 128), (16, 16, 64), (64, 1, 512), (12, 2, 256)]
+
+
+def draw(rng):
+    op = rng.choice(["norm_rope", "append", "paged", "paged", "prompt"])
+    heads, kv, dim = rng.choice(LAYOUTS)
+    spread = rng.randint(10, 1 << 20)
+    rot, layout = rng.choice([(dim, "half"), (dim, "half"), (dim // 2, "half"), (32, "interleaved"),
+                              (64, "interleaved")])
+    norm, dtype = rng.random() < 0.7, rng.choice(["f32", "bf16"])
+    if op == "norm_rope":
+        tokens = min(_log_int(rng, 1, 16384), 80_000_000 // ((heads + kv) * dim))
+        return {"op": op, "tokens": tokens, "heads": heads, "kv": kv, "dim": dim, "rot": rot, "layout": layout,
+                "norm": norm, "dtype": dtype, "table": 65536}
+    page = rng.choice([16, 32, 64, 64, 128])
+    if op == "append":
+        seqs = _log_int(rng, 1, 128)
+        new = _log_int(rng, 1, max(8, min(4000, 24000000 // (seqs * kv * dim))))
+        return {"op": op, "seqs": seqs, "new": new, "ragged": rng.random() < 0.6, "past": _log_int(rng, 1, 700),
+                "kv": kv, "dim": dim, "page": page, "rot": rng.choice([0, rot]), "layout": layout, "norm": norm,
+                "dtype": dtype, "spread": spread}
+    window = rng.choice([0, 0, 0, _log_int(rng, 16, 2048)])
+    lse = rng.random() < 0.5
+    if op == "paged":
+        seqs = _log_int(rng, 1, 100)
+        most = 300_000_000 // (seqs * kv * dim * 2)
+        length = _log_int(rng, 20, max(40, min(60000, most)))
+        new = rng.choice([1, 1, 2, 4, 8, 8, _log_int(rng, 9, 64)]) if heads // kv <= 8 else rng.choice([1, 2, 4])
+        return {"op": op, "seqs": seqs, "new": min(new, length), "ragged": rng.random() < 0.3, "len": length,
+                "same": rng.random() < 0.3, "heads": heads, "kv": kv, "dim": dim, "page": page, "window": window,
+                "lse": lse, "spread": spread}
+    if dim > 256:
+        heads, kv, dim = 32, 8, 128
+    same = rng.random() < 0.3
+    length = _log_int(rng, 1, 4000)
+    seqs = min(_log_int(rng, 1, 32), max(1, 25_000_000 // (length * length) if same else 120_000_000 // (length * length)))
+    return {"op": op, "seqs": seqs, "len": length, "same": same, "heads": heads, "kv": kv, "dim": dim,
+            "window": window, "lse": lse, "spread": spread}
+
+
+# ---------------------------------------------------------------------------
+# the sizes of a case
+# ---------------------------------------------------------------------------
+
+
+def _ragged(case, n, top, salt, low=1):
+    """n lengths, log-uniform in [low, top], the first one top itself."""
+    rng = random.Random(case["spread"] * 31 + salt)
+    return [top] + [_log_int(rng, low, top) for _ in range(n - 1)]
+
+
+def _lengths(case):
+    """new, past (append) or len (paged, prompt) of each sequence."""
+    n = case["seqs"]
+    if case["op"] == "append":
+        new = _ragged(case, n, case["new"], 1) if case["ragged"] else [case["new"]] * n
+        past = _ragged(case, n, case["past"], 2)
+        return new, past
+    low = 1 + case["len"] // 16 if case["op"] == "paged" else 1
+    length = [case["len"]] * n if case["same"] else _ragged(case, n, case["len"], 3, low)
+    if case["op"] == "prompt":
+        return length, length
+    new = _ragged(case, n, case["new"], 4) if case["ragged"] else [case["new"]] * n
+    return [min(a, b) for a, b in zip(new, length)], length
+
+
+def _visible(new, length, window):
+    """Pairs (query, key) that a sequence's new tokens at the end of `length` see."""
+    first, last = length - new + 1, length
+    if not window:
+        return (first + last) * new // 2
+    return sum(min(window, p) for p in range(first, last + 1))
+
+
+def work(case):
+    op, dim, kv = case["op"], case["dim"], case["kv"]
+    if op == "norm_rope":
+        values = case["tokens"] * (case["heads"] + kv) * dim
+        size = 4 if case["dtype"] == "f32" else 2
+        return {"bytes": values * (size + 2) + 4 * case["tokens"] * (1 + case["rot"]), "flops": 8 * values}
+    if op == "append":
+        values = 2 * sum(_lengths(case)[0]) * kv * dim
+        size = 4 if case["dtype"] == "f32" else 2
+        return {"bytes": values * (size + 1) + 4 * sum(_lengths(case)[0]) * case["rot"], "flops": 8 * values}
+    new, length = _lengths(case)
+    rows = sum(new) * case["heads"] * dim * 2 * 2
+    pairs = sum(_visible(a, b, case["window"]) for a, b in zip(new, length))
+    if op == "paged":
+        read = [min(b, case["window"] + a - 1) if case["window"] else b for a, b in zip(new, length)]
+        cache = sum(read) * kv * dim * 2 + sum(-(-b // case["page"]) for b in read) * (2 * kv + 4)
+    else:
+        cache = sum(length) * kv * dim * 2 * 2
+    return {"bytes": rows + cache + (4 * sum(new) * case["heads"] if case["lse"] else 0),
+            "flops": 4 * pairs * case["heads"] * dim}
+
+
+# ---------------------------------------------------------------------------
+# inputs
+# ---------------------------------------------------------------------------
+
+
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(int(seed) * 1000003 + 17)
+    return g
+
+
+def _randn(g, *shape, dtype="f32"):
+    return torch.randn(*shape, generator=g, device="cuda", dtype=torch.float32).to(DTYPES[dtype])
+
+
+def _ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _cumulative(lengths):
+    total = [0]
+    for n in lengths:
+        total.append(total[-1] + n)
+    return _ints(total)
+
+
+@functools.lru_cache(maxsize=4)
+def _table(positions, rot):
+    """cos | sin of each position, f32 from angles in 64 bits."""
+    inv = THETA ** (-torch.arange(0, rot, 2, dtype=torch.float64, device="cuda") / rot)
+    angle = torch.arange(positions, dtype=torch.float64, device="cuda")[:, None] * inv
+    return torch.cat([angle.cos(), angle.sin()], 1).float()
+
+
+def _codes(g, *shape):
+    """E4M3 codes of normal values, some of them past the largest."""
+    out = torch.empty(shape, dtype=torch.uint8, device="cuda")
+    for part in out.view(shape[0], -1).split(max(1, (1 << 28) // max(1, out[0].numel()))):
+        x = torch.randn(part.shape, generator=g, device="cuda") * 100.0
+        part.copy_(x.clamp_(-448.0, 448.0).to(torch.float8_e4m3fn).view(torch.uint8))
+    return out
+
+
+def _cache(g, pages, case):
+    kv, page, dim = case["kv"], case["page"], case["dim"]
+    scale = lambda: torch.randint(118, 121, (pages, kv), generator=g, device="cuda", dtype=torch.uint8)  # noqa: E731
+    return {"k_pages": _codes(g, pages, kv, page, dim), "k_scales": scale(),
+            "v_pages": _codes(g, pages, kv, dim, page), "v_scales": scale()}
+
+
+def _page_table(g, lengths, page):
+    """Each sequence's pages, in random places of the cache; entries past its
+    last page are 0 and not read.  Also the pages in all."""
+    need = [-(-n // page) for n in lengths]
+    order = torch.randperm(sum(need), generator=g, device="cuda").to(torch.int32)
+    table = torch.zeros((len(need), max(need)), dtype=torch.int32, device="cuda")
+    at = 0
+    for i, n in enumerate(need):
+        table[i, :n] = order[at:at + n]
+        at += n
+    return table, at
+
+
+def prepare(case, seed):
+    g = _gen(seed)
+    op, kv, dim = case["op"], case["kv"], case["dim"]
+    s = {"case": case}
+    if op == "norm_rope":
+        t = case["tokens"]
+        s["q"] = _randn(g, t, case["heads"], dim, dtype=case["dtype"])
+        s["k"] = _randn(g, t, kv, dim, dtype=case["dtype"])
+        for name in ("q_weight", "k_weight"):
+            s[name] = 1.0 + 0.1 * _randn(g, dim) if case["norm"] else None
+        s["table"] = _table(case["table"], case["rot"])
+        first = int(torch.randint(0, case["table"] - t + 1, (1,), generator=g, device="cuda"))
+        s["positions"] = torch.arange(first, first + t, dtype=torch.int32, device="cuda")
+        return s
+    new, length = _lengths(case)
+    s["cu"], s["total"], s["most"] = _cumulative(new), sum(new), max(new)
+    if op == "append":
+        past, length = length, [a + b for a, b in zip(new, length)]
+        s["past"] = _ints(past)
+        s["k"] = _randn(g, s["total"], kv, dim, dtype=case["dtype"])
+        s["v"] = _randn(g, s["total"], kv, dim, dtype=case["dtype"])
+        s["k_weight"] = 1.0 + 0.1 * _randn(g, dim) if case["norm"] else None
+        s["table"] = _table(8192, case["rot"]) if case["rot"] else None
+        s["pages"], n = _page_table(g, length, case["page"])
+        s.update(_cache(g, n, case))
+        return s
+    s["q"] = _randn(g, s["total"], case["heads"], dim, dtype="bf16")
+    s["longest"] = max(length)
+    if op == "paged":
+        s["lengths"] = _ints(length)
+        s["pages"], n = _page_table(g, length, case["page"])
+        s.update(_cache(g, n, case))
+        return s
+    s["k"] = _randn(g, s["total"], kv, dim, dtype="bf16")
+    s["v"] = _randn(g, s["total"], kv, dim, dtype="bf16")
+    return s
+
+
+# ---------------------------------------------------------------------------
+# plain forms
+# ---------------------------------------------------------------------------
+
+
+def _rotate(x, c, s, layout, start):
+    """x [..., dim] with dimensions start .. start + rot rotated, c and s [tokens, 1, rot / 2]."""
+    half = c.shape[-1]
+    part = x[..., start:start + 2 * half]
+    if layout == "half":
+        a, b = part[..., :half], part[..., half:]
+        part = torch.cat([a * c - b * s, b * c + a * s], -1)
+    else:
+        a, b = part[..., 0::2], part[..., 1::2]
+        part = torch.stack([a * c - b * s, b * c + a * s], -1).flatten(-2)
+    return torch.cat([x[..., :start], part, x[..., start + 2 * half:]], -1)
+
+
+def _norm_rope(x, weight, table, positions, case):
+    x = x.float()
+    if weight is not None:
+        x = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + EPS) * weight
+    if table is not None:
+        c, s = table[positions.long()][:, None].chunk(2, -1)
+        x = _rotate(x, c, s, case["layout"], case["dim"] - case["rot"])
+    return x
+
+
+def _power(code):
+    """2^(code - 127) in f32, code 1 to 254."""
+    return (code.int() << 23).view(torch.float32)
+
+
+def _e4m3(x):
+    return x.clamp(-448.0, 448.0).to(torch.float8_e4m3fn).view(torch.uint8)
+
+
+def _place(s):
+    """Sequence, position, page and slot of each new token, and each sequence's first page."""
+    case, cu, past = s["case"], s["cu"].long(), s["past"].long()
+    row = torch.arange(s["total"], device="cuda")
+    seq = torch.searchsorted(cu, row, right=True) - 1
+    pos = past[seq] + row - cu[seq]
+    page = s["pages"].long()[seq, pos // case["page"]]
+    kept = past % case["page"]  # earlier tokens in the first page
+    first = s["pages"].long().gather(1, (past // case["page"])[:, None])[:, 0]
+    return pos, page, pos % case["page"], first[kept > 0], kept[kept > 0]
+
+
+def _side(x, codes, scales, page, slot, first, kept, slot_dim):
+    """One side (K or V) of the cache with the new rows x [tokens, kv, dim] in it."""
+    amax = torch.zeros(scales.shape, device="cuda").index_reduce_(0, page, x.abs().amax(-1), "amax")
+    bits = (amax.clamp(min=1e-4) / 448.0).view(torch.int32)
+    need = (bits >> 23) + ((bits & 0x7FFFFF) != 0).int()
+    need[first] = torch.maximum(need[first], scales[first].int())
+    touched = torch.zeros(scales.shape[0], dtype=torch.bool, device="cuda")
+    touched[page] = True
+    code = torch.where(touched[:, None], need, scales.int())
+    ratio = (scales[first].int() - code[first]).clamp(min=-126) + 127
+    old = codes[first]
+    moved = _e4m3(old.view(torch.float8_e4m3fn).float() * _power(ratio)[..., None, None])
+    at = torch.arange(codes.shape[slot_dim], device="cuda").view([-1 if d == slot_dim else 1 for d in range(4)])
+    codes[first] = torch.where(at < kept[:, None, None, None], moved, old)
+    fresh = _e4m3(x / _power(code[page])[..., None])
+    if slot_dim == 2:
+        codes[page, :, slot] = fresh
+    else:
+        codes[page, :, :, slot] = fresh
+    scales.copy_(code)
+
+
+def _attend(q, k, v, visible, scale):
+    """q [n, h, g * t, d], k and v [n, h, l, d] f32, visible [n, 1, g * t, l]: the outputs and each row's log sum."""
+    score = q @ k.transpose(-1, -2).contiguous()
+    score.mul_(scale).masked_fill_(~visible, -math.inf)
+    top = score.amax(-1, keepdim=True)
+    top = torch.where(top == -math.inf, 0.0, top)
+    p = score.sub_(top).exp_()
+    total = p.sum(-1, keepdim=True)
+    out = (p @ v) / torch.where(total == 0, 1.0, total)
+    return out, (top + total.log())[..., 0]
+
+
+def _padded(s, kv_len):
+    """Row of q for each (sequence, new token), whether there is one, and its position."""
+    cu = s["cu"].long()
+    step = torch.arange(s["most"], device="cuda")
+    count = cu[1:] - cu[:-1]
+    real = step < count[:, None]
+    row = (cu[:-1, None] + step).clamp(max=s["total"] - 1)
+    return row, real, kv_len[:, None] - count[:, None] + step
+
+
+def _plain_attention(s, k, v, kv_len):
+    """k, v [n, kv, length, dim] f32 padded; the packed rows' outputs."""
+    case = s["case"]
+    kv, dim, group = case["kv"], case["dim"], case["heads"] // case["kv"]
+    row, real, pos = _padded(s, kv_len)
+    n, most = row.shape
+    q = s["q"].float()[row].view(n, most, kv, group, dim).permute(0, 2, 3, 1, 4).reshape(n, kv, group * most, dim)
+    j = torch.arange(k.shape[2], device="cuda")
+    seen = (j <= pos[..., None]) & (j < kv_len[:, None, None]) & real[..., None]
+    if case["window"]:
+        seen &= j > pos[..., None] - case["window"]
+    seen = seen[:, None, None].expand(n, 1, group, most, k.shape[2]).reshape(n, 1, group * most, k.shape[2])
+    out, lse = _attend(q, k, v, seen, 1.0 / math.sqrt(dim))
+    out = out.view(n, kv, group, most, dim).permute(0, 3, 1, 2, 4).reshape(n, most, case["heads"], dim)
+    lse = lse.view(n, kv, group, most).permute(0, 3, 1, 2).reshape(n, most, case["heads"])
+    return (out[real].to(torch.bfloat16), lse[real]) if case["lse"] else out[real].to(torch.bfloat16)
+
+
+def _pages_f32(codes, scales, table):
+    return codes[table].view(torch.float8_e4m3fn).float() * _power(scales[table])[..., None, None]
+
+
+def _codes_out(s):
+    """The cache as the values that its codes and scales stand for."""
+    return [s["k_pages"].view(torch.float8_e4m3fn), s["k_scales"].view(torch.float8_e8m0fnu),
+            s["v_pages"].view(torch.float8_e4m3fn), s["v_scales"].view(torch.float8_e8m0fnu)]
+
+
+def _run_plain(s):
+    case = s["case"]
+    op = case["op"]
+    if op == "norm_rope":
+        return [_norm_rope(s[x], s[x + "_weight"], s["table"], s["positions"], case).to(torch.bfloat16)
+                for x in ("q", "k")]
+    if op == "append":
+        pos, page, slot, first, kept = _place(s)
+        k = _norm_rope(s["k"], s["k_weight"], s["table"], pos, case)
+        _side(k, s["k_pages"], s["k_scales"], page, slot, first, kept, 2)
+        _side(s["v"].float(), s["v_pages"], s["v_scales"], page, slot, first, kept, 3)
+        return _codes_out(s)
+    kv, dim = case["kv"], case["dim"]
+    if op == "paged":
+        table = s["pages"].long()
+        n, length = table.shape[0], table.shape[1] * case["page"]
+        k = _pages_f32(s["k_pages"], s["k_scales"], table).permute(0, 2, 1, 3, 4).reshape(n, kv, length, dim)
+        v = _pages_f32(s["v_pages"], s["v_scales"], table).permute(0, 2, 1, 4, 3).reshape(n, kv, length, dim)
+        return _plain_attention(s, k, v, s["lengths"].long())
+    row, _, _ = _padded(s, s["cu"].long()[1:] - s["cu"].long()[:-1])
+    k, v = (s[x].float()[row].permute(0, 2, 1, 3).contiguous() for x in ("k", "v"))
+    return _plain_attention(s, k, v, s["cu"].long()[1:] - s["cu"].long()[:-1])
+
+
+# ---------------------------------------------------------------------------
+# the framework's calls
+# ---------------------------------------------------------------------------
+
+
+@functools.lru_cache(maxsize=1)
+def _context():
+    from colormlm_amd import s14
+
+    return s14.Context(0)  # a program keeps one
+
+
+def _kept(s):
+    """What a program makes once: its rotation and its cache."""
+    if "rope" not in s:
+        from colormlm_amd import attention as A
+
+        case = s["case"]
+        table = s.get("table")
+        s["rope"] = None if table is None else A.Rope(table, case["layout"], start=case["dim"] - case["rot"])
+        s["cache"] = A.KvCache(s["k_pages"], s["k_scales"], s["v_pages"], s["v_scales"]) if "k_pages" in s else None
+    return s["rope"], s["cache"]
+
+
+def _run_own(s):
+    from colormlm_amd import attention as A
+
+    case, ctx = s["case"], _context()
+    op = case["op"]
+    rope, cache = _kept(s)
+    if op == "norm_rope":
+        out = [torch.empty(s[x].shape, dtype=torch.bfloat16, device="cuda") for x in ("q", "k")]
+        A.qk_norm_rope(ctx, s["q"], s["k"], out[0], out[1], q_weight=s["q_weight"], k_weight=s["k_weight"], eps=EPS,
+                       rope=rope, positions=s["positions"])
+        return out
+    if op == "append":
+        A.kv_append(ctx, cache, s["k"], s["v"], s["pages"], s["cu"], s["past"], k_weight=s["k_weight"], eps=EPS,
+                    rope=rope, max_new=s["most"])
+        return _codes_out(s)
+    out = torch.empty_like(s["q"])
+    lse = torch.empty(s["q"].shape[:2], dtype=torch.float32, device="cuda") if case["lse"] else None
+    if op == "paged":
+        A.paged_attention(ctx, s["q"], cache, s["pages"], s["cu"], s["lengths"], out, lse=lse, window=case["window"],
+                          max_new=s["most"], max_len=s["longest"])
+    else:
+        A.prompt_attention(ctx, s["q"], s["k"], s["v"], s["cu"], out, lse=lse, window=case["window"],
+                           max_len=s["longest"])
+    return out if lse is None else (out, lse)
+
+
+def run(state):
+    return _run_own(state) if own else _run_plain(state)
+
+
+# ---------------------------------------------------------------------------
+# the definition in 64 bits
+# ---------------------------------------------------------------------------
+
+
+def _exact_rows(x, weight, positions, case):
+    y = x.double()
+    if weight is not None:
+        y = y / (y.pow(2).sum(-1, keepdim=True) / case["dim"] + EPS).sqrt() * weight.double()
+    if case["rot"]:
+        rot, start = case["rot"], case["dim"] - case["rot"]
+        i = torch.arange(rot // 2, device="cuda")
+        angle = positions.double()[:, None] / THETA ** (2.0 * i.double() / rot)
+        turn = torch.polar(torch.ones_like(angle), angle)[:, None]
+        at = (start + i, start + i + rot // 2) if case["layout"] == "half" else (start + 2 * i, start + 2 * i + 1)
+        z = torch.complex(y[..., at[0]], y[..., at[1]]) * turn
+        y[..., at[0]], y[..., at[1]] = z.real, z.imag
+    return y
+
+
+def _exact_append(s):
+    case = s["case"]
+    page, cu, past = case["page"], s["cu"].tolist(), s["past"].tolist()
+    position = torch.cat([torch.arange(p, p + b - a) for p, a, b in zip(past, cu, cu[1:])]).cuda()
+    rows = [_exact_rows(s["k"], s["k_weight"], position, case), s["v"].double()]
+    sides = []
+    for y, name in zip(rows, ("k", "v")):
+        codes = s[name + "_pages"].view(torch.float8_e4m3fn).double()
+        codes = codes if name == "k" else codes.transpose(2, 3)
+        scale = s[name + "_scales"].double() - 127.0
+        for i, table in enumerate(s["pages"].tolist()):
+            for p in range(past[i] // page, -(-(past[i] + cu[i + 1] - cu[i]) // page)):
+                lo, hi = max(past[i], p * page), min(past[i] + cu[i + 1] - cu[i], p * page + page)
+                new = y[cu[i] + lo - past[i]:cu[i] + hi - past[i]].transpose(0, 1)
+                # the nearest f32 of the quotient: a maximum at a border goes the operator's way
+                most = (new.abs().amax((1, 2)).clamp(min=1e-4) / 448.0).float().double()
+                need = most.log2().ceil()
+                if lo > p * page:
+                    need = torch.maximum(need, scale[table[p]])
+                    codes[table[p], :, :lo - p * page] *= (scale[table[p]] - need).exp2()[:, None, None]
+                scale[table[p]] = need
+                codes[table[p], :, lo - p * page:hi - p * page] = new / need.exp2()[:, None, None]
+        sides += [codes if name == "k" else codes.transpose(2, 3).contiguous(), scale.exp2()]
+    return sides
+
+
+def _exact_sequence(q, k, v, case):
+    """q [t, heads, dim] at the end of k, v [l, kv, dim], all in 64 bits."""
+    t, length, group = q.shape[0], k.shape[0], case["heads"] // case["kv"]
+    at = torch.arange(length - t, length, device="cuda")[:, None]
+    j = torch.arange(length, device="cuda")
+    hidden = (j > at) | (j <= at - case["window"]) if case["window"] else j > at
+    out, lse = torch.empty_like(q), torch.empty(q.shape[:2], dtype=torch.float64, device="cuda")
+    for h in range(case["heads"]):
+        score = (q[:, h] @ k[:, h // group].T) / math.sqrt(case["dim"])
+        score.masked_fill_(hidden, -math.inf)
+        lse[:, h] = score.logsumexp(-1)
+        out[:, h] = (score - lse[:, h, None]).exp() @ v[:, h // group]
+    return out, lse
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    op = case["op"]
+    if op == "norm_rope":
+        return [_exact_rows(s[x], s[x + "_weight"], s["positions"], case) for x in ("q", "k")]
+    if op == "append":
+        return _exact_append(s)
+    outs, cu = [], s["cu"].tolist()
+    for i, (a, b) in enumerate(zip(cu, cu[1:])):
+        if op == "paged":
+            length = int(s["lengths"][i])
+            ids = s["pages"][i, :-(-length // case["page"])].long()
+            power = [(s[x][ids].double() - 127.0).exp2()[..., None, None] for x in ("k_scales", "v_scales")]
+            k = (s["k_pages"][ids].view(torch.float8_e4m3fn).double() * power[0]).permute(0, 2, 1, 3).flatten(0, 1)
+            v = (s["v_pages"][ids].view(torch.float8_e4m3fn).double() * power[1]).permute(0, 3, 1, 2).flatten(0, 1)
+            k, v = k[:length], v[:length]
+        else:
+            k, v = s["k"][a:b].double(), s["v"][a:b].double()
+        outs.append(_exact_sequence(s["q"][a:b].double(), k, v, case))
+    out, lse = (torch.cat(x) for x in zip(*outs))
+    return (out, lse) if case["lse"] else out
