@@ -467,8 +467,7 @@ def _run_own(s):
         A.paged_attention(ctx, s["q"], cache, s["pages"], s["cu"], s["lengths"], out, lse=lse, window=case["window"],
                           max_new=s["most"], max_len=s["longest"])
     else:
-        A.prompt_attention(ctx, s["q"], s["k"], s["v"], s["cu"], out, lse=lse, window=case["window"],
-                           max_len=s["longest"])
+        A.prompt_attention(ctx, s["q"], s["k"], s["v"], s["cu"], out, lse=lse, window=case["window"])
     return out if lse is None else (out, lse)
 
 
