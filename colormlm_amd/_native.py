@@ -44,6 +44,8 @@ S14_MODE_OFFICIAL = 2
 S14_LINEAR_ROUND_BF16 = 1
 S14_X_F32 = 0
 S14_X_BF16 = 1
+S14_ROPE_HALF = 0
+S14_ROPE_INTERLEAVED = 1
 S14_SCALE_UE8M0 = 0
 S14_SCALE_F32 = 1
 S14_PAGE_MXFP4 = 0
@@ -184,6 +186,49 @@ class LoadingReservationC(C.Structure):
     ]
 
 
+class Rows(C.Structure):
+    _fields_ = [
+        ("buf", Buffer),
+        ("dtype", C.c_int),
+        ("heads", C.c_uint32),
+        ("token_stride", C.c_uint64),
+        ("head_stride", C.c_uint32),
+    ]
+
+
+class Rope(C.Structure):
+    _fields_ = [
+        ("table", Buffer),
+        ("positions", C.c_uint32),
+        ("rot", C.c_uint32),
+        ("start", C.c_uint32),
+        ("layout", C.c_int),
+    ]
+
+
+class RopeScaling(C.Structure):
+    _fields_ = [
+        ("factor", C.c_double),
+        ("original", C.c_double),
+        ("beta_fast", C.c_double),
+        ("beta_slow", C.c_double),
+        ("amplitude", C.c_double),
+    ]
+
+
+class KvCache(C.Structure):
+    _fields_ = [
+        ("k", Buffer),
+        ("v", Buffer),
+        ("k_scale", Buffer),
+        ("v_scale", Buffer),
+        ("pages", C.c_uint32),
+        ("heads", C.c_uint32),
+        ("page_tokens", C.c_uint32),
+        ("dim", C.c_uint32),
+    ]
+
+
 class RouteDecisionC(C.Structure):
     _fields_ = [
         ("layer", C.c_uint8),
@@ -242,6 +287,27 @@ SIGNATURES = {
     "s14_requant_e4m3": (I, [P, P, U32, U32, P, P, P]),
     "s14_act_quant_e4m3": (I, [P, P, U32, U32, U32, P, P, P]),
     "s14_fp8_linear": (I, [P, P, U32, U32, U32, Buffer, Buffer, I, Buffer, Buffer, I, Buffer, Buffer, I, I]),
+    "s14_rope_table": (I, [P, P, U32, U32, C.c_double, C.POINTER(RopeScaling), Buffer]),
+    "s14_qk_norm_rope": (
+        I,
+        [P, P, U32, U32, C.POINTER(Rows), C.POINTER(Rows), C.POINTER(Rows), C.POINTER(Rows), Buffer, Buffer, F,
+         C.POINTER(Rope), Buffer],
+    ),
+    "s14_kv_append": (
+        I,
+        [P, P, C.POINTER(KvCache), U32, U32, U32, C.POINTER(Rows), C.POINTER(Rows), Buffer, U32, Buffer, Buffer, Buffer,
+         F, C.POINTER(Rope)],
+    ),
+    "s14_paged_attention": (
+        I,
+        [P, P, C.POINTER(Rows), C.POINTER(KvCache), U32, U32, U32, U32, Buffer, U32, Buffer, Buffer, C.POINTER(Rows),
+         Buffer, F, U32],
+    ),
+    "s14_prompt_attention": (
+        I,
+        [P, P, U32, C.POINTER(Rows), C.POINTER(Rows), C.POINTER(Rows), U32, U32, Buffer, C.POINTER(Rows), Buffer, F,
+         U32],
+    ),
     "s14_last_prefill_view": (I, [P, C.POINTER(PrefillView)]),
     "s14_fill_mxfp4_page": (I, [P, P, P, U64, U32, U32, U32, U32, I, I]),
     "s14_pool_create": (I, [P, U32, U64, C.POINTER(P)]),

@@ -34,6 +34,7 @@ struct s14_ctx {
   void *prefill_base = nullptr;  // prefill workspace, made on the first prefill call
   void *lin_base = nullptr;      // fp8_linear FAST split-K workspace, made on the first FAST call
   s14::LinearWorkspace lws{};
+  void *attn_base = nullptr;     // partial results of a split paged attention, made on the first split call
   uint32_t prefill_tokens = 0;   // token count of the last prefill
   s14::PrefillWorkspace pws{};
   s14::Workspace ws{};
@@ -159,6 +160,7 @@ extern "C" void s14_ctx_destroy(s14_ctx *ctx) {
   if (ctx->ws_base) (void)hipFree(ctx->ws_base);
   if (ctx->prefill_base) (void)hipFree(ctx->prefill_base);
   if (ctx->lin_base) (void)hipFree(ctx->lin_base);
+  if (ctx->attn_base) (void)hipFree(ctx->attn_base);
   if (ctx->compute) (void)hipStreamDestroy(ctx->compute);
   if (ctx->copy) (void)hipStreamDestroy(ctx->copy);
   if (ctx->fork.side) (void)hipStreamDestroy(ctx->fork.side);
@@ -171,6 +173,23 @@ extern "C" void s14_ctx_destroy(s14_ctx *ctx) {
 
 extern "C" void *s14_ctx_compute_stream(s14_ctx *ctx) { return ctx ? ctx->compute : nullptr; }
 int s14::ctx_device(const s14_ctx *ctx) { return ctx->device; }
+uint32_t *s14::ctx_status(const s14_ctx *ctx) { return status_word(ctx->ws); }
+int s14::ctx_attn_workspace(s14_ctx *ctx, uint64_t bytes, float **out) {
+  if (!ctx->attn_base) {
+    // the call may be under capture, where this thread's mode forbids hipMalloc
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    S14_HIP(hipThreadExchangeStreamCaptureMode(&mode), "hipThreadExchangeStreamCaptureMode");
+    const hipError_t e = hipMalloc(&ctx->attn_base, bytes);
+    const hipError_t r = hipThreadExchangeStreamCaptureMode(&mode);  // the caller's mode again
+    if (e != hipSuccess) {
+      ctx->attn_base = nullptr;
+      return hip_fail(e, "hipMalloc(attention workspace)");
+    }
+    if (r != hipSuccess) return hip_fail(r, "hipThreadExchangeStreamCaptureMode");
+  }
+  *out = static_cast<float *>(ctx->attn_base);
+  return S14_OK;
+}
 extern "C" void *s14_ctx_copy_stream(s14_ctx *ctx) { return ctx ? ctx->copy : nullptr; }
 
 extern "C" int s14_ctx_synchronize(s14_ctx *ctx) {
@@ -630,6 +649,12 @@ int read_launch_status(const Workspace &ws, int device) {
   S14_HIP(hipMemcpy(word, &zero, sizeof(zero), hipMemcpyHostToDevice), "hipMemcpy(status clear)");
   if (bits & kStatusNullPage)
     return fail(S14_ERR_INVALID, "a routed expert's page address was 0 (page not resident); outputs are NaN");
+  if (bits & kStatusBadCachePage)
+    return fail(S14_ERR_INVALID,
+                "a sequence's cache page lies outside the cache or past its page table; its new rows are not stored "
+                "and its outputs are NaN");
+  if (bits & kStatusBadPosition)
+    return fail(S14_ERR_INVALID, "a position lies outside the rotation table; its rows are NaN");
   return fail(S14_ERR_ROUTE,
               "a token's route failed RouteDecision::validate_for (expert id out of range or repeated, weight "
               "not finite or negative, or weight sum off route_scale by more than 1e-4); its outputs are NaN");

@@ -1,0 +1,74 @@
+// Device helpers of the attention kernels (s14_attn_*.hip).  Unnamed
+// namespace: each kernel file gets its own inline copy.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "s14_attn.hpp"
+
+namespace s14 {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// A row bound from device memory, held inside the packed rows.
+__device__ __forceinline__ int64_t clamp_row(int32_t r, uint32_t rows) {
+  return r < 0 ? 0 : int64_t(r) > int64_t(rows) ? int64_t(rows) : int64_t(r);
+}
+
+__device__ __forceinline__ float power_of_two(int e) { return __builtin_ldexpf(1.0f, e); }
+
+// a and b rounded to bf16 (ties to even, NaN stays NaN), a in the low half.
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+  const bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+// The positions a row sees, base .. base + count - 1: those up to its own, of
+// a window the last ones.  One unsigned comparison answers for a position.
+// (Masks are selects of plain floats everywhere: writing an element of a
+// matrix result in a divergent branch has been compiled into a copy of that
+// element over its neighbours, clang 20 of ROCm 7.2, when registers spill.)
+struct Visible {
+  int32_t base;
+  uint32_t count;
+  __device__ __forceinline__ Visible(int32_t pos, uint32_t window) {
+    base = window && pos >= 0 && window <= uint32_t(pos) ? pos - int32_t(window) + 1 : 0;
+    count = pos < 0 ? 0u : uint32_t(pos - base) + 1u;
+  }
+  Visible() = default;
+  __device__ __forceinline__ bool operator()(int32_t j) const { return uint32_t(j - base) < count; }
+};
+
+// The result of a max or sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float max_lane16(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_lane16(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Eight E4M3 codes as bf16, exactly (a NaN code gives NaN).
+__device__ __forceinline__ bf16x8 e4m3_bf16(uint32_t lo, uint32_t hi) {
+  const u32x4 v = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true))};
+  return __builtin_bit_cast(bf16x8, v);
+}
+
+}  // namespace
+}  // namespace s14

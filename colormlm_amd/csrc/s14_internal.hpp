@@ -35,6 +35,11 @@ int read_launch_status(const Workspace &ws, int device);
 
 // The device a context was created on.
 int ctx_device(const s14_ctx *ctx);
+// Its device status word (kStatus* bits).
+uint32_t *ctx_status(const s14_ctx *ctx);
+// Its workspace for a split paged attention's partial results, allocated on
+// the first call (always the same `bytes`), on the current device.
+int ctx_attn_workspace(s14_ctx *ctx, uint64_t bytes, float **out);
 
 // Records `msg` as this thread's last error and returns `code`.
 int fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));

@@ -431,6 +431,116 @@ int s14_fp8_linear(s14_ctx *ctx, void *stream, uint32_t m, uint32_t n, uint32_t 
                    int weight_scale_dtype, s14_buffer bias, s14_buffer y, int flags, int mode);
 
 /* ======================================================================
+ * Attention between the FP8 projections and the expert layer: per-head norms
+ * with the position rotation, a paged key/value cache in 8 bits, attention
+ * over it, and causal attention over packed prompts.  No counterpart in the
+ * reference, whose GPU code has no S14 attention; the projections (s14_fp8_linear)
+ * give these calls their rows and take their outputs.
+ *
+ * Token t, head h of a packed [tokens][heads][dim] operand starts at element
+ * t * token_stride + h * head_stride; a row's dim values are contiguous.  dim
+ * is 64, 128, 256 or 512 (prompt: to 256).  Operands start on 16 bytes and
+ * have strides that are multiples of 8 elements.  Device index arrays (cu, past, lens, page tables, positions) are
+ * checked on the device: no value makes a launch read or write outside its
+ * operands, and one that is wrong is reported by s14_launch_status.
+ * Launches of one context share its workspace and must not overlap.
+ * ====================================================================== */
+typedef struct {
+  s14_buffer buf;
+  int dtype;             /* S14_X_F32 or S14_X_BF16 */
+  uint32_t heads;
+  uint64_t token_stride; /* in elements */
+  uint32_t head_stride;
+} s14_rows;
+
+/* Rotation of dimensions start .. start + rot - 1 of each head: the pair
+ * (a, b) becomes (a cos - b sin, b cos + a sin).  rot and start are multiples
+ * of 8.  HALF: pairs are (i, i + rot / 2); INTERLEAVED: (2 i, 2 i + 1).
+ * table: f32 [positions][rot], cos of the rot / 2 angles and then their
+ * sines (s14_rope_table). */
+enum { S14_ROPE_HALF = 0, S14_ROPE_INTERLEAVED = 1 };
+typedef struct {
+  s14_buffer table; /* ptr NULL: no rotation */
+  uint32_t positions;
+  uint32_t rot;
+  uint32_t start;
+  int layout;
+} s14_rope;
+
+/* Stretching of the rotation for contexts longer than the trained one:
+ * frequencies divided by `factor`; with original > 0 (the trained length)
+ * only those that turn less than beta_slow times in it, not those that turn
+ * more than beta_fast times, and those between in proportion.  cos and sin
+ * are multiplied by `amplitude`. */
+typedef struct {
+  double factor, original, beta_fast, beta_slow, amplitude;
+} s14_rope_scaling;
+/* table[p] = cos | sin of p * theta^(-2 i / rot), from angles in 64 bits.
+ * scaling may be NULL. */
+int s14_rope_table(s14_ctx *ctx, void *stream, uint32_t positions, uint32_t rot, double theta,
+                   const s14_rope_scaling *scaling, s14_buffer table);
+
+/* Per-head RMS norm x * rsqrt(mean(x^2) + eps) * weight of queries and keys,
+ * then the rotation at positions[t] (device int32 [tokens]), f32 throughout,
+ * each output rounded once to its dtype.  A weight (f32 [dim]) of NULL leaves that side's norm out; rope
+ * NULL leaves the rotation out; k.heads 0 leaves the keys out.  Outputs may be
+ * their inputs.  A position outside the table gives NaN rows. */
+int s14_qk_norm_rope(s14_ctx *ctx, void *stream, uint32_t tokens, uint32_t dim, const s14_rows *q,
+                     const s14_rows *k, const s14_rows *q_out, const s14_rows *k_out,
+                     s14_buffer q_weight, s14_buffer k_weight, float eps, const s14_rope *rope,
+                     s14_buffer positions);
+
+/* The paged cache: E4M3 codes with one E8M0 scale for each page, key head and
+ * side (value = code * 2^(scale - 127), as everywhere in this library).
+ *   k codes [page][head][slot][dim], v codes [page][head][dim][slot],
+ *   k and v scales [page][head]
+ * page_tokens is 16, 32, 64 or 128.  Position p of a sequence is slot p %
+ * page_tokens of the page its page-table row (int32) names at p / page_tokens. */
+typedef struct {
+  s14_buffer k, v, k_scale, v_scale;
+  uint32_t pages, heads, page_tokens, dim;
+} s14_kv_cache;
+
+/* Rows cu[i] .. cu[i + 1] - 1 of k and v become positions past[i] .. of
+ * sequence i (cu, past: device int32 [seqs + 1], [seqs]; page_table device
+ * int32 [seqs][table_width]; max_new >= the largest count).  K takes the norm
+ * and rotation of s14_qk_norm_rope on the way, at those positions.
+ * A page's scale is 2^ceil(log2(max(amax, 1e-4) / 448)) of the values put in,
+ * never less than the one that its earlier tokens have (slots below past[i]):
+ * where it grows their codes are divided by the power of two, rounded to
+ * nearest even.  Slots past the last new token stay as they were.  A NaN is
+ * stored as NaN (it sets no scale), an infinity as the largest value of the
+ * largest scale.  A page outside the cache or past the table takes nothing.
+ * Pages written by one call belong to one sequence each. */
+int s14_kv_append(s14_ctx *ctx, void *stream, const s14_kv_cache *cache, uint32_t tokens,
+                  uint32_t seqs, uint32_t max_new, const s14_rows *k, const s14_rows *v,
+                  s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer past,
+                  s14_buffer k_weight, float eps, const s14_rope *rope);
+
+/* Attention of the rows cu[i] .. cu[i + 1] - 1 of q (bf16), the last tokens of
+ * sequence i, over its lens[i] cached tokens (these rows' own among them:
+ * append first).  Row j of n sees positions <= lens[i] - n + j, with window >
+ * 0 only the last `window` of them; heads of q share a key head in groups of
+ * heads / cache heads.  out (bf16 or f32) = softmax(scale q.k) v (scale > 0), the
+ * softmax in f32, its weights rounded to bf16 for the second product; lse (f32
+ * [tokens][heads], or ptr NULL) the natural log of the weights' sum.  A row
+ * that sees nothing is 0 with lse -inf.  max_new and max_len: at least the
+ * largest count of rows, and about the longest sequence (it only sets how the
+ * work is split). */
+int s14_paged_attention(s14_ctx *ctx, void *stream, const s14_rows *q, const s14_kv_cache *cache,
+                        uint32_t tokens, uint32_t seqs, uint32_t max_new, uint32_t max_len,
+                        s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer lens,
+                        const s14_rows *out, s14_buffer lse, float scale, uint32_t window);
+
+/* Causal attention over packed prompts: sequence i is the rows cu[i] .. cu[i
+ * + 1] - 1 of q, k and v (bf16), and row j of it sees its rows <= j (with
+ * window > 0 the last `window` of them).  out and lse as above. */
+int s14_prompt_attention(s14_ctx *ctx, void *stream, uint32_t dim, const s14_rows *q,
+                         const s14_rows *k, const s14_rows *v, uint32_t tokens, uint32_t seqs,
+                         s14_buffer cu, const s14_rows *out, s14_buffer lse, float scale,
+                         uint32_t window);
+
+/* ======================================================================
  * Synthetic page fill (bench / tests): integer hash, same spec as the
  * oracle's generator, computed on the device.
  * ====================================================================== */
