@@ -70,6 +70,13 @@ __device__ __forceinline__ int32_t page_of(const PagedArgs &a, const int32_t *ta
   return id;
 }
 
+// A row of a chunk's partial result: D sums, the maximum and the weights' sum.
+template <int D>
+constexpr uint32_t kRecord = D + 4;
+
+// The top bit of each byte that is a NaN code (0x7f, 0xff).
+__device__ __forceinline__ uint32_t nan_codes(uint32_t c) { return ((c & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
 template <int D, int NT, int T>
 __global__ __launch_bounds__(256) void k_paged_attention(PagedArgs a, PagedPlan p, float *part) {
   constexpr int C = D / 64;   // 16-byte pieces of a K row a lane holds
@@ -111,22 +118,34 @@ __global__ __launch_bounds__(256) void k_paged_attention(PagedArgs a, PagedPlan 
   float m[NT], sum[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) m[nt] = -INFINITY, sum[nt] = 0.0f;
-  bool bad = false;
+  bool bad = false, odd = false;
   const float scale = a.scale * kLog2e;
   const uint64_t page_bytes = uint64_t(P) * D;
 
-  for (int32_t b = begin + 16 * T * int32_t(wave); b < end; b += 4 * 16 * T) {
-    const int32_t tk = b + 4 * T * int32_t(n / 4), tv = b + 4 * T * int32_t(g);
-    const int32_t idk = page_of(a, table, tk, sp.len, bad), idv = page_of(a, table, tv, sp.len, bad);
-    const uint8_t *kp = a.cache.k + (uint64_t(idk) * kvh + head) * page_bytes +
-                        (uint32_t(tk) % P + (n & 3u)) * uint32_t(D) + 16 * g;
-    const uint8_t *vp = a.cache.v + (uint64_t(idv) * kvh + head) * page_bytes + n * P + uint32_t(tv) % P;
-    uint4 kk[T][C];
+  // A step's operands: codes in registers, loaded one step ahead (K as soon as
+  // the first product has read the step before, V after the second), their
+  // pages' ids another step ahead.
+  uint4 kk[T][C];
+  uint32_t vv[DT][W];
+  uint32_t ksc = 0, vsc = 0;
+  int32_t idk = 0, idv = 0;
+  auto load_ids = [&](int32_t b) {
+    idk = page_of(a, table, b + 4 * T * int32_t(n / 4), sp.len, bad);
+    idv = page_of(a, table, b + 4 * T * int32_t(g), sp.len, bad);
+  };
+  auto load_k = [&](int32_t b) {
+    const uint32_t at = uint32_t(b + 4 * T * int32_t(n / 4)) % P + (n & 3u);
+    const uint8_t *kp = a.cache.k + (uint64_t(idk) * kvh + head) * page_bytes + at * uint32_t(D) + 16 * g;
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int c = 0; c < C; ++c) kk[t][c] = *reinterpret_cast<const uint4 *>(kp + 4 * t * D + 64 * c);
-    uint32_t vv[DT][W];
+    const uint64_t sat = uint64_t(idv) * kvh + head;
+    ksc = a.cache.ks[sat], vsc = a.cache.vs[sat];
+  };
+  auto load_v = [&](int32_t b) {
+    const uint8_t *vp = a.cache.v + (uint64_t(idv) * kvh + head) * page_bytes + n * P +
+                        uint32_t(b + 4 * T * int32_t(g)) % P;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       if constexpr (T == 4) {
@@ -137,10 +156,21 @@ __global__ __launch_bounds__(256) void k_paged_attention(PagedArgs a, PagedPlan 
         vv[dt][0] = x.x, vv[dt][1] = x.y;
       }
     }
-    const uint64_t sat = uint64_t(idv) * kvh + head;
-    const float ks = scale * power_of_two(int(a.cache.ks[sat]) - 127);
-    const float vs = power_of_two(int(a.cache.vs[sat]) - 127);
+  };
+  constexpr int32_t kStride = 4 * 16 * T;  // the wavefronts' steps interleave
+  int32_t b = begin + 16 * T * int32_t(wave);
+  if (b < end) {
+    load_ids(b);
+    load_k(b);
+    load_v(b);
+    if (b + kStride < end) load_ids(b + kStride);
+  }
 
+  for (; b < end; b += kStride) {
+    const int32_t tv = b + 4 * T * int32_t(g);
+    const bool more = b + kStride < end;
+    const float ks = scale * power_of_two(int(ksc) - 127);
+    const float vs = power_of_two(int(vsc) - 127);
     f32x4 s[NT][T];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -157,6 +187,7 @@ __global__ __launch_bounds__(256) void k_paged_attention(PagedArgs a, PagedPlan 
           s[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q[nt][2 * c + 1], s[nt][t], 0, 0, 0);
         }
       }
+    if (more) load_k(b + kStride);
     const bool partial = b + 16 * T - 1 > pos_lo || (a.window && int64_t(b) <= int64_t(pos_hi) - a.window);
     bf16x8 pb[NT][T / 2];
 #pragma unroll
@@ -196,43 +227,22 @@ __global__ __launch_bounds__(256) void k_paged_attention(PagedArgs a, PagedPlan 
     }
     if (partial) {
       // what lies behind the sequence is not read; a NaN code that some row
-      // must not see leaves the product (0 * NaN is NaN) and reaches the rows
-      // that see it afterwards, as the count of such codes they see
-      bool nan = false;
-      uint32_t hit[DT][W];
+      // must not see leaves the product (0 * NaN is NaN), and the rows that see
+      // it get it back below
+      uint32_t nan = 0;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+      for (int k = 0; k < W; ++k) {
+        const int32_t left = sp.len - (tv + 4 * k);
+        const uint32_t keep = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
 #pragma unroll
-        for (int k = 0; k < W; ++k) {
-          const int32_t left = sp.len - (tv + 4 * k);
-          const uint32_t keep = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
-          uint32_t c = vv[dt][k] & keep;
-          const uint32_t is = ((c & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // byte's top bit: a NaN code
-          hit[dt][k] = is;
-          nan |= is != 0;
-          vv[dt][k] = c & ~((is >> 7) * 0xffu);
-        }
-      if (__any(nan)) {
+        for (int dt = 0; dt < DT; ++dt) vv[dt][k] &= keep, nan |= nan_codes(vv[dt][k]);
+      }
+      if (__any(nan != 0)) {
+        odd = true;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int k = 0; k < W; ++k)
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            f32x4 count = {};
-#pragma unroll
-            for (int u = 0; u < T / 2; ++u) {
-              u32x4 seen;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int32_t j = tv + 8 * u + 2 * k;
-                seen[k] = (see[nt](j) ? 0x3f80u : 0u) | (see[nt](j + 1) ? 0x3f800000u : 0u);
-              }
-              const uint32_t h0 = (hit[dt][2 * u] >> 7) * 0x38u, h1 = (hit[dt][2 * u + 1] >> 7) * 0x38u;  // 1 in E4M3
-              count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3_bf16(h0, h1), __builtin_bit_cast(bf16x8, seen),
-                                                              count, 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[nt][dt][i] += count[i] > 0.0f ? __uint_as_float(0x7fc00000u) : 0.0f;
-          }
+          for (int dt = 0; dt < DT; ++dt) vv[dt][k] &= ~((nan_codes(vv[dt][k]) >> 7) * 0xffu);
       }
     }
 #pragma unroll
@@ -244,6 +254,33 @@ __global__ __launch_bounds__(256) void k_paged_attention(PagedArgs a, PagedPlan 
         for (int nt = 0; nt < NT; ++nt)
           o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pb[nt][u], o[nt][dt], 0, 0, 0);
       }
+    if (more) load_v(b + kStride);
+    if (b + 2 * kStride < end) load_ids(b + 2 * kStride);
+  }
+
+  if (odd) {  // uniform, and rare: one token after the other
+    for (int32_t b0 = begin + 16 * T * int32_t(wave); b0 < end; b0 += kStride) {
+      if (b0 + 16 * T - 1 <= pos_lo && !(a.window && int64_t(b0) <= int64_t(pos_hi) - a.window)) continue;
+      for (int32_t j = b0; j < min(b0 + 16 * T, sp.len); ++j) {
+        const int32_t id = page_of(a, table, j, sp.len, bad);
+        const uint8_t *vp = a.cache.v + (uint64_t(id) * kvh + head) * page_bytes + uint32_t(j) % P;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          f32x4 nan;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            nan[i] = (vp[(16 * dt + 4 * g + i) * P] & 0x7fu) == 0x7fu ? __uint_as_float(0x7fc00000u) : 0.0f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const bool in = see[nt](j);
+            f32x4 back;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) back[i] = in ? nan[i] : 0.0f;
+            o[nt][dt] += back;
+          }
+        }
+      }
+    }
   }
 
   // join the four wavefronts: 2 and 3 into 0 and 1, then 1 into 0
@@ -309,57 +346,73 @@ __global__ __launch_bounds__(256) void k_paged_attention(PagedArgs a, PagedPlan 
     }
     return;
   }
-  float *rec = part + uint64_t(blockIdx.x) * (16 * NT * (D + 2));
+  float *rec = part + uint64_t(blockIdx.x) * (p.rec_rows * kRecord<D>);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    float *row = rec + (16 * nt + n) * (D + 2);
+    if (16 * nt + n >= p.rec_rows) continue;
+    float *row = rec + (16 * nt + n) * kRecord<D>;
     if (g == 0) row[D] = m[nt], row[D + 1] = sum[nt];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      float2 *to = reinterpret_cast<float2 *>(row + 16 * dt + 4 * g);  // rows of D + 2 floats: 8-byte aligned
-      to[0] = make_float2(o[nt][dt][0], o[nt][dt][1]);
-      to[1] = make_float2(o[nt][dt][2], o[nt][dt][3]);
+      *reinterpret_cast<f32x4 *>(row + 16 * dt + 4 * g) = o[nt][dt];
     }
   }
 }
 
-// Joins the chunks of one row a wavefront, in their order.
+// Joins the chunks of one row a workgroup, in an order that its size alone
+// sets: the chunks' maxima in the lanes, then their rows in groups of
+// threads at once.
 template <int D>
 __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, PagedPlan p, const float *part) {
-  constexpr int V = D / 64;
-  const uint32_t kvh = a.cache.heads, group = a.heads / kvh, l = threadIdx.x & 63u;
-  const uint32_t seq = blockIdx.y, head = blockIdx.z;
-  const int64_t r = int64_t(blockIdx.x) * 4 + threadIdx.x / 64;
-  const uint32_t per = 16 * p.row_tiles, tile = uint32_t(r / per);
+  constexpr uint32_t kLanes = D / 4 < 64 ? D / 4 : 64, kSpan = D / (4 * kLanes);  // float4s of a row a thread
+  constexpr uint32_t kGroups = 256 / kLanes;
+  const uint32_t kvh = a.cache.heads, group = a.heads / kvh, tid = threadIdx.x;
+  const uint32_t seq = blockIdx.y, head = blockIdx.z, r = blockIdx.x;
+  const uint32_t per = 16 * p.row_tiles, tile = r / per;
   const Span sp = paged_span(a, p, seq, tile * per);
-  if (r >= sp.rows || sp.chunks <= 1) return;
-  const uint64_t rec = uint64_t(per) * (D + 2);
+  if (int64_t(r) >= sp.rows || sp.chunks <= 1) return;
+  const uint64_t rec = uint64_t(p.rec_rows) * kRecord<D>;
   const float *row = part + (uint64_t(tile) * kvh * p.chunks * a.seqs + uint64_t(seq) * p.chunks * kvh + head) * rec +
-                     uint32_t(r % per) * (D + 2);
+                     uint32_t(r % per) * kRecord<D>;
   const uint64_t next = kvh * rec;  // the next chunk's record
   float top = -INFINITY;
-  for (uint32_t c = 0; c < sp.chunks; ++c) top = fmaxf(top, row[c * next + D]);
+  for (uint32_t c = tid & 63u; c < sp.chunks; c += 64) top = fmaxf(top, row[c * next + D]);
+#pragma unroll
+  for (int m = 32; m; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
   const float at = top == -INFINITY ? 0.0f : top;
-  float total = 0.0f, o[V] = {};
-  for (uint32_t c = 0; c < sp.chunks; ++c) {
+  const uint32_t lane = tid % kLanes, first = tid / kLanes;
+  float total = 0.0f;
+  f32x4 o[kSpan] = {};
+#pragma unroll 4
+  for (uint32_t c = first; c < sp.chunks; c += kGroups) {
     const float *x = row + c * next;
     const float fade = __builtin_amdgcn_exp2f(x[D] - at);
     total += x[D + 1] * fade;
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] += x[V * l + i] * fade;
+    for (uint32_t i = 0; i < kSpan; ++i) o[i] += *reinterpret_cast<const f32x4 *>(x + 4 * (lane + kLanes * i)) * fade;
+  }
+  __shared__ f32x4 s_o[kGroups][kSpan][kLanes];
+  __shared__ float s_l[kGroups];
+#pragma unroll
+  for (uint32_t i = 0; i < kSpan; ++i) s_o[first][i][lane] = o[i];
+  if (lane == 0) s_l[first] = total;
+  __syncthreads();
+  if (first) return;
+#pragma unroll
+  for (uint32_t w = 1; w < kGroups; ++w) {
+    total += s_l[w];
+#pragma unroll
+    for (uint32_t i = 0; i < kSpan; ++i) o[i] += s_o[w][i][lane];
   }
   const uint64_t t = uint64_t(sp.first + r / group);
-  const uint32_t h = head * group + uint32_t(r % group);
+  const uint32_t h = head * group + r % group;
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  const uint64_t to = t * a.out.token + uint64_t(h) * a.out.head + V * l;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if (a.out.bf16)
-      static_cast<uint16_t *>(a.out.p)[to + i] = uint16_t(bf16_pair(o[i] * inv, 0.0f));
-    else
-      static_cast<float *>(a.out.p)[to + i] = o[i] * inv;
+  for (uint32_t i = 0; i < kSpan; ++i) {
+    const f32x4 y = o[i] * inv;
+    store_out(a.out, t * a.out.token + uint64_t(h) * a.out.head + 4 * (lane + kLanes * i), y[0], y[1], y[2], y[3]);
   }
-  if (a.lse && l == 0) a.lse[t * a.heads + h] = total == 0.0f ? -INFINITY : top * kLn2 + __logf(total);
+  if (a.lse && lane == 0) a.lse[t * a.heads + h] = total == 0.0f ? -INFINITY : top * kLn2 + __logf(total);
 }
 
 template <int D, int NT, int T>
@@ -367,7 +420,7 @@ hipError_t launch(hipStream_t s, const PagedArgs &a, const PagedPlan &p, float *
   k_paged_attention<D, NT, T><<<uint32_t(p.blocks), 256, 0, s>>>(a, p, part);
   if (p.chunks > 1) {
     const uint32_t rows = uint32_t(a.max_new) * (a.heads / a.cache.heads);
-    k_paged_join<D><<<dim3((rows + 3) / 4, a.seqs, a.cache.heads), 256, 0, s>>>(a, p, part);
+    k_paged_join<D><<<dim3(rows, a.seqs, a.cache.heads), 256, 0, s>>>(a, p, part);
   }
   return hipGetLastError();
 }
@@ -397,9 +450,17 @@ PagedPlan paged_plan(const PagedArgs &a) {
   const uint64_t base = tiles * a.cache.heads * a.seqs;  // workgroups of an uncut launch
   uint64_t span = a.max_len;
   if (a.window && uint64_t(a.window) + a.max_new + 63 < span) span = uint64_t(a.window) + a.max_new + 63;
-  constexpr uint64_t kWant = 2048, kLeast = 256;
-  const uint64_t rec = 16ull * p.row_tiles * (dim + 2);
+  #ifndef KWANT
+#define KWANT 512
+#endif
+#ifndef KMOST
+#define KMOST 2048
+#endif
+  constexpr uint64_t kWant = KWANT, kLeast = 256, kMost = KMOST;
+  p.rec_rows = uint32_t(rows < 16 * p.row_tiles ? rows : 16 * p.row_tiles);
+  const uint64_t rec = uint64_t(p.rec_rows) * (dim + 4);
   uint64_t chunks = (kWant + base - 1) / base;
+  if (chunks < (span + kMost - 1) / kMost) chunks = (span + kMost - 1) / kMost;
   const uint64_t fit = kPagedPartFloats / (rec * base);
   if (chunks > fit) chunks = fit;
   if (chunks > (span + kLeast - 1) / kLeast) chunks = (span + kLeast - 1) / kLeast;

@@ -23,6 +23,7 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr uint32_t kPromptRows = 128;
+constexpr float kRise = 8.0f;
 
 // Row block `index` of the packed sequences: its sequence's first token and
 // length, and the block within it.  Every sequence has its rows in whole
@@ -53,9 +54,10 @@ __device__ __forceinline__ bool find_block(const PromptArgs &a, uint32_t index, 
     if (here) {
       const int lane = __builtin_ctzll(here);
       const uint32_t end = __shfl(sum, lane);
-      out.first = __shfl(first, lane);
-      out.len = int32_t(__shfl(len, lane));
-      out.row0 = (end - 1 - (index - before)) * kPromptRows;
+      // packed rows fit 31 bits; a uniform block lets its descriptors and bounds stay scalar
+      out.first = __builtin_amdgcn_readfirstlane(int32_t(__shfl(int32_t(first), lane)));
+      out.len = __builtin_amdgcn_readfirstlane(int32_t(__shfl(int32_t(len), lane)));
+      out.row0 = __builtin_amdgcn_readfirstlane((end - 1 - (index - before)) * kPromptRows);
       return true;
     }
     before += __shfl(sum, 63);
@@ -74,12 +76,19 @@ template <int D, int KT>
 __device__ __forceinline__ void stage(const uint16_t *base, uint32_t stride, int32_t valid, uint16_t *lds) {
   constexpr uint32_t kPieces = D / 8, kPasses = KT * kPieces / 256;
   const uint32_t rows = valid < KT ? uint32_t(valid) : uint32_t(KT);
-  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(base), 0, int((rows - 1) * stride + 2 * D), 0x00020000);
+  const uint64_t at0 = reinterpret_cast<uint64_t>(base);
+  const u32x4 r = {uint32_t(at0), uint32_t(at0 >> 32), (rows - 1) * stride + 2 * D, 0x00020000u};
+  const uint32_t to = uint32_t(reinterpret_cast<uintptr_t>((lds_void *)lds));
+  // In asm: the compiler would let every LDS read wait for these loads, whose
+  // halves of the double buffer it cannot tell apart.  No register waits for
+  // them; the wait at the head of the next tile does.
 #pragma unroll
   for (uint32_t i = 0; i < kPasses; ++i) {
     const uint32_t at = i * 256 + threadIdx.x, row = at / kPieces, piece = (at % kPieces) ^ swizzle<D>(row);
-    const uint32_t wave_at = i * 256 + (threadIdx.x & ~63u);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(lds + wave_at * 8), 16, row * stride + piece * 16, 0, 0, 0);
+    const uint32_t wave_at = __builtin_amdgcn_readfirstlane(to + (i * 256 + (threadIdx.x & ~63u)) * 16);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(wave_at),
+                 "v"(row * stride + piece * 16), "s"(r)
+                 : "memory");
   }
 }
 
@@ -89,7 +98,7 @@ __device__ __forceinline__ uint32_t odd_halves(uint32_t w) {  // 0x8000 in each 
 }
 
 template <int D, int KT>
-__global__ __launch_bounds__(256) void k_prompt_attention(PromptArgs a) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(PromptArgs a) {
   constexpr int KS = D / 16, DT = D / 32, ST = KT / 32, U = KT / 16;
   __shared__ __align__(16) uint16_t lds_k[2][KT * D], lds_v[2][KT * D];
   const uint32_t group = a.heads / a.kv_heads, head = blockIdx.x % a.kv_heads;
@@ -108,6 +117,10 @@ __global__ __launch_bounds__(256) void k_prompt_attention(PromptArgs a) {
                           uint64_t(head * group + uint32_t(r % group)) * a.q_head;
 #pragma unroll
     for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const bf16x8 *>(row + 16 * k + 8 * h);
+    // Q is here before any tile is asked for: its first use, in the loop,
+    // would otherwise wait for every load in flight, each time round
+#pragma unroll
+    for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(q[k]));
   }
   // tokens that the workgroup, and this wavefront, walk
   const uint64_t blk_last = (blk.row0 + kPromptRows < rows ? blk.row0 + kPromptRows : rows) - 1;
@@ -120,14 +133,23 @@ __global__ __launch_bounds__(256) void k_prompt_attention(PromptArgs a) {
 
   f32x16 o[DT] = {};
   float m = -INFINITY, sum = 0.0f;
+  bool odd = false;
   const float scale = a.scale * kLog2e;
   const uint16_t *kb = a.k + uint64_t(blk.first) * a.k_token + uint64_t(head) * a.k_head;
   const uint16_t *vb = a.v + uint64_t(blk.first) * a.v_token + uint64_t(head) * a.v_head;
   const uint32_t ks = uint32_t(a.k_token * 2), vs = uint32_t(a.v_token * 2);
 
-  // this lane's places in LDS: its K row (per 32-token tile), and its piece of
-  // a V row for the transposing read
-  const uint32_t v_row = 4 * h + (l & 15u) / 4, v_piece = ((l >> 4) & 1u) * 2 + ((l & 3u) >> 1), v_byte = (l & 1u) * 8;
+  // This lane's places in an LDS tile, the rest of a read's address being a
+  // constant: the pieces of its K row (rows 32 apart have the same swizzle),
+  // and its part of a V row for the transposing read (rows 8 apart).
+  constexpr int KA = KS < 8 ? KS : 8, VA = DT < 4 ? DT : 4;
+  uint32_t k_at[KA], v_at[VA];
+#pragma unroll
+  for (int k = 0; k < KA; ++k) k_at[k] = n * (2 * D) + ((2 * k + h) ^ swizzle<D>(n)) * 16;
+  const uint32_t v_row = 4 * h + (l & 15u) / 4;
+#pragma unroll
+  for (int dt = 0; dt < VA; ++dt)
+    v_at[dt] = v_row * (2 * D) + ((4 * dt + ((l >> 4) & 1u) * 2 + ((l & 3u) >> 1)) ^ swizzle<D>(v_row)) * 16 + (l & 1u) * 8;
 
   stage<D, KT>(kb + uint64_t(lo) * a.k_token, ks, blk.len - lo, lds_k[0]);
   stage<D, KT>(vb + uint64_t(lo) * a.v_token, vs, blk.len - lo, lds_v[0]);
@@ -140,17 +162,16 @@ __global__ __launch_bounds__(256) void k_prompt_attention(PromptArgs a) {
       stage<D, KT>(vb + uint64_t(b + KT) * a.v_token, vs, blk.len - b - KT, lds_v[buf ^ 1]);
     }
     if (b > wpos_hi || (a.window && int64_t(b) + KT - 1 <= int64_t(wpos_lo) - a.window)) continue;
-    const uint8_t *lk = reinterpret_cast<const uint8_t *>(lds_k[buf]);
-    const uint16_t *lv = lds_v[buf];
+    const auto *lk = (const __attribute__((address_space(3))) uint8_t *)lds_k[buf];
+    const auto *lv = (const __attribute__((address_space(3))) uint8_t *)lds_v[buf];
 
     f32x16 s[ST];
 #pragma unroll
     for (int t = 0; t < ST; ++t) {
       s[t] = f32x16{};
-      const uint32_t row = 32 * t + n;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        const bf16x8 kf = *reinterpret_cast<const bf16x8 *>(lk + row * (2 * D) + ((2 * k + h) ^ swizzle<D>(row)) * 16);
+        const bf16x8 kf = *(const __attribute__((address_space(3))) bf16x8 *)(lk + k_at[k % KA] + 64 * D * t + 32 * (k - k % KA));
         s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[k], s[t], 0, 0, 0);
       }
     }
@@ -167,15 +188,17 @@ __global__ __launch_bounds__(256) void k_prompt_attention(PromptArgs a) {
       const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
       top = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
     }
+    // The maximum that the weights are taken from moves only where they would
+    // pass 2^kRise: O is seldom multiplied.
     top = fmaxf(m, top * scale);
-    const float at = top == -INFINITY ? 0.0f : top;
-    const float fade = __builtin_amdgcn_exp2f(m - at);
-    m = top;
-    sum *= fade;
-    if (__any(fade != 1.0f)) {
+    if (__any(top > m + kRise)) {
+      const float fade = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
+      m = top;
+      sum *= fade;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] *= fade;
     }
+    const float at = m == -INFINITY ? 0.0f : m;
     bf16x8 pb[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -196,70 +219,55 @@ __global__ __launch_bounds__(256) void k_prompt_attention(PromptArgs a) {
         bf16x8 v;
       } f;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t row = 16 * u + 8 * half + v_row;
-        const uint32_t piece = (4 * dt + v_piece) ^ swizzle<D>(row);
+      for (int half = 0; half < 2; ++half)
         f.x[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s16x4 *)(reinterpret_cast<const uint8_t *>(lv) + row * (2 * D) + piece * 16 + v_byte));
-      }
+            (lds_s16x4 *)(lv + v_at[dt % VA] + (16 * u + 8 * half) * (2 * D) + 64 * (dt - dt % VA)));
       return f.v;
     };
-    // An infinity or NaN in a V row that some rows must not see would reach
-    // them through 0 * inf: such values leave the product, and the rows that
-    // see them get them back from a count.
-    bool odd = false;
-    if (partial) {
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const u32x4 w = __builtin_bit_cast(u32x4, v_frag(dt, u));
-          odd |= (odd_halves(w[0]) | odd_halves(w[1]) | odd_halves(w[2]) | odd_halves(w[3])) != 0;
-        }
-    }
-    if (__any(odd)) {
-      u32x4 seen[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int32_t tok = b + 16 * u + 8 * (j / 2) + 4 * int32_t(h) + 2 * (j % 2);
-          seen[u][j] = (see(tok) ? 0x3f80u : 0u) | (see(tok + 1) ? 0x3f800000u : 0u);
-        }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        f32x16 up = {}, down = {};
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          u32x4 w = __builtin_bit_cast(u32x4, v_frag(dt, u)), pos_w, neg_w;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t clean = 0, pw = 0, nw = 0;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t x = (w[j] >> (16 * e)) & 0xffffu;
-              const bool fin = (x & 0x7f80u) != 0x7f80u, nan = !fin && (x & 0x7fu);
-              if (fin) clean |= x << (16 * e);
-              if (nan || x == 0x7f80u) pw |= 0x3f80u << (16 * e);
-              if (nan || x == 0xff80u) nw |= 0x3f80u << (16 * e);
-            }
-            w[j] = clean, pos_w[j] = pw, neg_w[j] = nw;
-          }
-          const bf16x8 sv = __builtin_bit_cast(bf16x8, seen[u]);
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb[u], o[dt], 0, 0, 0);
-          up = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, pos_w), sv, up, 0, 0, 0);
-          down = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, neg_w), sv, down, 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          o[dt][i] += (up[i] > 0.0f ? INFINITY : 0.0f) + (down[i] > 0.0f ? -INFINITY : 0.0f);
-      }
-    } else {
+    if (!partial) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int u = 0; u < U; ++u)
           o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_frag(dt, u), pb[u], o[dt], 0, 0, 0);
+    } else {
+      // An infinity or NaN in a V row that some rows must not see would reach
+      // them through 0 * inf: such values leave the product, and the rows that
+      // see them get them back below.
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          u32x4 w = __builtin_bit_cast(u32x4, v_frag(dt, u));
+          u32x4 t;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) t[j] = odd_halves(w[j]);
+          if (__any((t[0] | t[1] | t[2] | t[3]) != 0)) {
+            odd = true;
+            w &= ~(t | (t - (t >> 15)));  // 0x8000 in a half becomes 0xffff
+          }
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb[u], o[dt], 0, 0, 0);
+        }
+    }
+  }
+
+  if (odd) {  // uniform, and rare: one token after the other
+    for (int32_t b = lo; b <= wpos_hi; b += KT) {
+      if (b + KT - 1 <= wpos_lo && !(a.window && int64_t(b) <= int64_t(wpos_hi) - a.window)) continue;
+      for (int32_t j = b; j < min(b + KT, wpos_hi + 1); ++j) {
+        const uint16_t *row = vb + uint64_t(j) * a.v_token + 4 * h;
+        const bool in = see(j);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          f32x16 back;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float v = __uint_as_float(uint32_t(row[32 * dt + 8 * (i / 4) + i % 4]) << 16);
+            back[i] = (in & !(fabsf(v) < INFINITY)) ? v : 0.0f;
+          }
+          o[dt] += back;
+        }
+      }
     }
   }
 
