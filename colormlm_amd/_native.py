@@ -186,9 +186,10 @@ class LoadingReservationC(C.Structure):
     ]
 
 
-class Rows(C.Structure):
+class Rows(C.Structure):  # s14_rows, its s14_buffer's two members in place
     _fields_ = [
-        ("buf", Buffer),
+        ("ptr", C.c_void_p),
+        ("bytes", C.c_uint64),
         ("dtype", C.c_int),
         ("heads", C.c_uint32),
         ("token_stride", C.c_uint64),

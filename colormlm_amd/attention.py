@@ -31,18 +31,19 @@ from ._native import S14Error, check, lib
 from .s14 import Context
 
 PAGE_TOKENS = (16, 32, 64, 128)
-_DTYPES = {torch.float32: N.S14_X_F32, torch.bfloat16: N.S14_X_BF16}
+_DTYPES = {torch.float32: (N.S14_X_F32, 4), torch.bfloat16: (N.S14_X_BF16, 2)}
 _LAYOUTS = {"half": N.S14_ROPE_HALF, "interleaved": N.S14_ROPE_INTERLEAVED}
-_NO_BUFFER = N.Buffer(None, 0)
-_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_NO_BUFFER, _NO_ROWS = N.Buffer(None, 0), N.Rows()
 
 
-def _stream(ctx: Context, stream):
-    if stream is not None:
-        return stream
-    if _RAW_STREAM is not None:
-        return _RAW_STREAM(ctx.device)
-    return torch.cuda.current_stream(ctx.device).cuda_stream
+def _raw_stream():
+    """torch's current stream of a device, without the object where this torch
+    has the raw call."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw if raw is not None else lambda device: torch.cuda.current_stream(device).cuda_stream
+
+
+_RAW_STREAM = _raw_stream()
 
 
 def _refuse(code: int, message: str):
@@ -50,36 +51,42 @@ def _refuse(code: int, message: str):
 
 
 def _here(ctx: Context, t, label: str):
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.device.index != ctx.device:
+    if not isinstance(t, torch.Tensor) or t.get_device() != ctx.device:
         _refuse(N.S14_ERR_INVALID, f"{label} must be a tensor on the context's device {ctx.device}")
 
 
-def _rows(ctx: Context, t, label: str, dim: Optional[int] = None) -> N.Rows:
-    """The s14_rows of a [tokens, heads, dim] tensor."""
-    _here(ctx, t, label)
-    code = _DTYPES.get(t.dtype)
-    if code is None:
-        _refuse(N.S14_ERR_INVALID, f"{label} must be float32 or bfloat16, not {t.dtype}")
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 3 or (stride[2] != 1 and shape[2] > 1) or (dim is not None and shape[2] != dim):
+def _rows(ctx: Context, t, label: str, dim: Optional[int] = None):
+    """The s14_rows of a [tokens, heads, dim] tensor.  (On the path of a
+    single token's calls: each tensor is asked for each property once.)"""
+    try:
+        code, size = _DTYPES[t.dtype]
+        tokens, heads, width = t.shape
+        token_stride, head_stride, one = t.stride()
+        if t.get_device() != ctx.device or (one != 1 and width > 1) or (dim is not None and width != dim):
+            raise ValueError
+    except (AttributeError, KeyError, ValueError):
+        _here(ctx, t, label)
+        if t.dtype not in _DTYPES:
+            _refuse(N.S14_ERR_INVALID, f"{label} must be float32 or bfloat16, not {t.dtype}")
         _refuse(N.S14_ERR_SHAPE, f"{label} must be [tokens, heads, {dim or 'dim'}] with a contiguous last dimension")
-    tokens, heads, width = shape
     # strides of a dimension of one are not used; what torch gives there may be anything
-    token_stride = stride[0] if tokens > 1 else 0
-    head_stride = stride[1] if heads > 1 else 0
-    size = 4 if code == N.S14_X_F32 else 2
+    if tokens < 2:
+        token_stride = 0
+    if heads < 2:
+        head_stride = 0
     reach = ((tokens - 1) * token_stride + (heads - 1) * head_stride + width) * size if tokens and heads else 0
-    return N.Rows(N.Buffer(t.data_ptr(), reach), code, heads, token_stride, head_stride)
+    return N.Rows(t.data_ptr(), reach, code, heads, token_stride, head_stride)
 
 
-def _flat(ctx: Context, t, dtype, label: str, size: Optional[int] = None) -> N.Buffer:
+def _flat(ctx: Context, t, dtype, label: str, size: int = 0):
     """The buffer of a contiguous tensor of one dtype, of `size` values at least."""
     if t is None:
         return _NO_BUFFER
-    _here(ctx, t, label)
-    if t.dtype != dtype or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.get_device() != ctx.device:
+        _here(ctx, t, label)
+    if t.dtype is not dtype or not t.is_contiguous():
         _refuse(N.S14_ERR_INVALID, f"{label} must be a contiguous {dtype} tensor")
-    if size is not None and t.numel() < size:
+    if size and t.numel() < size:
         _refuse(N.S14_ERR_CAPACITY, f"{label} has {t.numel()} values, {size} are required")
     return N.Buffer(t.data_ptr(), t.nbytes)
 
@@ -104,7 +111,8 @@ class Rope:
 def _rope(ctx: Context, rope: Optional[Rope]):
     if rope is None:
         return None
-    _here(ctx, rope.table, "rotation table")
+    if rope.table.get_device() != ctx.device:
+        _here(ctx, rope.table, "rotation table")
     return C.byref(rope._c)
 
 
@@ -151,7 +159,8 @@ class KvCache:
 
 
 def _cache(ctx: Context, cache: KvCache):
-    _here(ctx, cache.k_pages, "cache")
+    if cache.k_pages.get_device() != ctx.device:
+        _here(ctx, cache.k_pages, "cache")
     return C.byref(cache._c)
 
 
@@ -165,7 +174,7 @@ def rope_table(ctx: Context, table, theta: float = 10000.0, scaling: Optional[Ro
     if scaling is not None:
         s = C.byref(N.RopeScaling(scaling.factor, scaling.original, scaling.beta_fast, scaling.beta_slow,
                                   scaling.amplitude))
-    check(lib().s14_rope_table(ctx.handle, _stream(ctx, stream), table.shape[0], table.shape[1], theta, s, buf))
+    check(lib().s14_rope_table(ctx._h, _RAW_STREAM(ctx.device) if stream is None else stream, table.shape[0], table.shape[1], theta, s, buf))
 
 
 def qk_norm_rope(ctx: Context, q, k, q_out, k_out, q_weight=None, k_weight=None, eps: float = 1e-6,
@@ -177,15 +186,14 @@ def qk_norm_rope(ctx: Context, q, k, q_out, k_out, q_weight=None, k_weight=None,
     tokens, _, dim = q.shape
     if q_out.shape != q.shape:
         _refuse(N.S14_ERR_SHAPE, "q output must have q's shape")
-    rk = ko = None
     if k is None:
-        rk, ko = N.Rows(), N.Rows()
+        rk = ko = _NO_ROWS
     else:
         rk, ko = _rows(ctx, k, "k", dim), _rows(ctx, k_out, "k output", dim)
         if k.shape[0] != tokens or k_out.shape != k.shape:
             _refuse(N.S14_ERR_SHAPE, "k must have q's tokens, and k output k's shape")
     check(lib().s14_qk_norm_rope(
-        ctx.handle, _stream(ctx, stream), tokens, dim, C.byref(rq), C.byref(rk), C.byref(ro), C.byref(ko),
+        ctx._h, _RAW_STREAM(ctx.device) if stream is None else stream, tokens, dim, C.byref(rq), C.byref(rk), C.byref(ro), C.byref(ko),
         _flat(ctx, q_weight, torch.float32, "q norm weight"), _flat(ctx, k_weight, torch.float32, "k norm weight"),
         eps, _rope(ctx, rope), _flat(ctx, positions, torch.int32, "positions")))
 
@@ -211,7 +219,7 @@ def kv_append(ctx: Context, cache: KvCache, k, v, page_table, cu, past, k_weight
     table, width, cub, lenb, seqs = _table(ctx, page_table, cu, past, "past")
     tokens = k.shape[0]
     check(lib().s14_kv_append(
-        ctx.handle, _stream(ctx, stream), _cache(ctx, cache), tokens, seqs, tokens if max_new is None else max_new,
+        ctx._h, _RAW_STREAM(ctx.device) if stream is None else stream, _cache(ctx, cache), tokens, seqs, tokens if max_new is None else max_new,
         C.byref(rk), C.byref(rv), table, width, cub, lenb, _flat(ctx, k_weight, torch.float32, "k norm weight"), eps,
         _rope(ctx, rope)))
 
@@ -230,7 +238,7 @@ def paged_attention(ctx: Context, q, cache: KvCache, page_table, cu, lens, out, 
         _refuse(N.S14_ERR_SHAPE, "out must have q's shape")
     table, width, cub, lenb, seqs = _table(ctx, page_table, cu, lens, "lens")
     check(lib().s14_paged_attention(
-        ctx.handle, _stream(ctx, stream), C.byref(rq), _cache(ctx, cache), tokens, seqs,
+        ctx._h, _RAW_STREAM(ctx.device) if stream is None else stream, C.byref(rq), _cache(ctx, cache), tokens, seqs,
         tokens if max_new is None else max_new, width * cache.page_tokens if max_len is None else max_len, table, width,
         cub, lenb, C.byref(ro), _flat(ctx, lse, torch.float32, "lse", tokens * heads),
         dim ** -0.5 if scale is None else scale, window))
@@ -248,7 +256,7 @@ def prompt_attention(ctx: Context, q, k, v, cu, out, lse=None, scale: Optional[f
         _refuse(N.S14_ERR_SHAPE, "out must have q's shape, v k's, and k q's tokens")
     cub = _flat(ctx, cu, torch.int32, "cu", 1)
     check(lib().s14_prompt_attention(
-        ctx.handle, _stream(ctx, stream), dim, C.byref(rq), C.byref(rk), C.byref(rv), tokens, cu.numel() - 1, cub,
+        ctx._h, _RAW_STREAM(ctx.device) if stream is None else stream, dim, C.byref(rq), C.byref(rk), C.byref(rv), tokens, cu.numel() - 1, cub,
         C.byref(ro), _flat(ctx, lse, torch.float32, "lse", tokens * heads), dim ** -0.5 if scale is None else scale,
         window))
 

@@ -264,10 +264,10 @@ extern "C" int s14_paged_attention(s14_ctx *ctx, void *stream, const s14_rows *q
   a.cu = static_cast<const int32_t *>(cu.ptr), a.len = static_cast<const int32_t *>(lens.ptr);
   a.out = out_of(out), a.lse = static_cast<float *>(lse.ptr);
   a.scale = scale, a.window = window;
-  a.status = s14::ctx_status(ctx);
   const s14::PagedPlan p = s14::paged_plan(a);
   if (p.blocks >= (1u << 24) || uint64_t(max_new) * q->heads >= (1ull << 31))
     return fail(S14_ERR_SHAPE, "%u new tokens of %u sequences exceed one launch", max_new, seqs);
+  a.status = s14::ctx_status(ctx);
   const OnDevice on(s14::ctx_device(ctx));
   if (on.error() != hipSuccess) return hip_fail(on.error(), "hipSetDevice");
   float *part = nullptr;

@@ -78,15 +78,18 @@ constexpr uint32_t kRecord = D + 4;
 __device__ __forceinline__ uint32_t nan_codes(uint32_t c) { return ((c & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
 template <int D, int NT, int T>
-__global__ __launch_bounds__(256) void k_paged_attention(PagedArgs a, PagedPlan p, float *part) {
+__global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(PagedArgs a, PagedPlan p, float *part) {
   constexpr int C = D / 64;   // 16-byte pieces of a K row a lane holds
   constexpr int DT = D / 16;  // 16-dimension tiles of O
   constexpr int W = T;        // 32-bit words of V codes a lane holds of one dimension
   const uint32_t kvh = a.cache.heads, group = a.heads / kvh;
-  // row tiles are the slowest index: those that read the same pages are a
-  // multiple of `items` apart
+  // Row tiles are the slowest index: those that read the same pages are a
+  // multiple of `items` apart.  Chunks come before them, so that the late
+  // chunks, which short sequences lack, are together: among the sequences the
+  // empty workgroups fell to the same compute units (128 ragged sequences of
+  // 8,192 tokens at most, 8 chunks: 228 us; so DECODE_US).
   const uint32_t items = kvh * p.chunks * a.seqs, tile = blockIdx.x / items, item = blockIdx.x % items;
-  const uint32_t head = item % kvh, chunk = item / kvh % p.chunks, seq = item / kvh / p.chunks;
+  const uint32_t head = item % kvh, seq = item / kvh % a.seqs, chunk = item / kvh / a.seqs;
   const uint32_t row0 = tile * 16 * NT;
   const Span sp = paged_span(a, p, seq, row0);
   if (int64_t(row0) >= sp.rows || (chunk && chunk >= sp.chunks)) return;
@@ -372,9 +375,9 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, PagedPlan p, co
   const Span sp = paged_span(a, p, seq, tile * per);
   if (int64_t(r) >= sp.rows || sp.chunks <= 1) return;
   const uint64_t rec = uint64_t(p.rec_rows) * kRecord<D>;
-  const float *row = part + (uint64_t(tile) * kvh * p.chunks * a.seqs + uint64_t(seq) * p.chunks * kvh + head) * rec +
+  const float *row = part + (uint64_t(tile) * kvh * p.chunks * a.seqs + uint64_t(seq) * kvh + head) * rec +
                      uint32_t(r % per) * kRecord<D>;
-  const uint64_t next = kvh * rec;  // the next chunk's record
+  const uint64_t next = uint64_t(kvh) * a.seqs * rec;  // the next chunk's record
   float top = -INFINITY;
   for (uint32_t c = tid & 63u; c < sp.chunks; c += 64) top = fmaxf(top, row[c * next + D]);
 #pragma unroll
@@ -450,17 +453,13 @@ PagedPlan paged_plan(const PagedArgs &a) {
   const uint64_t base = tiles * a.cache.heads * a.seqs;  // workgroups of an uncut launch
   uint64_t span = a.max_len;
   if (a.window && uint64_t(a.window) + a.max_new + 63 < span) span = uint64_t(a.window) + a.max_new + 63;
-  #ifndef KWANT
-#define KWANT 512
-#endif
-#ifndef KMOST
-#define KMOST 2048
-#endif
-  constexpr uint64_t kWant = KWANT, kLeast = 256, kMost = KMOST;
+    // workgroups that the card holds at once, by the registers of a wavefront
+  const uint32_t words = dim * p.row_tiles;
+  const uint64_t slots = 256 * (words <= 64 ? 3 : words <= 128 ? 2 : 1);
+  constexpr uint64_t kLeast = 256, kMost = 2048;
   p.rec_rows = uint32_t(rows < 16 * p.row_tiles ? rows : 16 * p.row_tiles);
   const uint64_t rec = uint64_t(p.rec_rows) * (dim + 4);
-  uint64_t chunks = (kWant + base - 1) / base;
-  if (chunks < (span + kMost - 1) / kMost) chunks = (span + kMost - 1) / kMost;
+  uint64_t chunks = base < slots ? slots / base : (span + kMost - 1) / kMost;
   const uint64_t fit = kPagedPartFloats / (rec * base);
   if (chunks > fit) chunks = fit;
   if (chunks > (span + kLeast - 1) / kLeast) chunks = (span + kLeast - 1) / kLeast;
