@@ -38,10 +38,10 @@ __device__ __forceinline__ bool find_block(const PromptArgs &a, uint32_t index, 
   uint32_t before = 0;
   for (uint32_t s0 = 0; s0 < a.seqs; s0 += 64) {
     const uint32_t s = s0 + l;
-    int64_t first = 0, len = 0;
+    int32_t first = 0, len = 0;  // packed rows fit 31 bits
     if (s < a.seqs) {
-      first = clamp_row(a.cu[s], a.tokens);
-      len = clamp_row(a.cu[s + 1], a.tokens) - first;
+      first = int32_t(clamp_row(a.cu[s], a.tokens));
+      len = int32_t(clamp_row(a.cu[s + 1], a.tokens)) - first;
     }
     const uint32_t blocks = len > 0 ? uint32_t((uint64_t(len) * group + kPromptRows - 1) / kPromptRows) : 0;
     uint32_t sum = blocks;
@@ -52,15 +52,14 @@ __device__ __forceinline__ bool find_block(const PromptArgs &a, uint32_t index, 
     }
     const uint64_t here = __ballot(index - before < sum);
     if (here) {
-      const int lane = __builtin_ctzll(here);
-      const uint32_t end = __shfl(sum, lane);
-      // packed rows fit 31 bits; a uniform block lets its descriptors and bounds stay scalar
-      out.first = __builtin_amdgcn_readfirstlane(int32_t(__shfl(int32_t(first), lane)));
-      out.len = __builtin_amdgcn_readfirstlane(int32_t(__shfl(int32_t(len), lane)));
-      out.row0 = __builtin_amdgcn_readfirstlane((end - 1 - (index - before)) * kPromptRows);
+      // one lane's values: the block is uniform, its descriptors and bounds scalar
+      const int lane = __builtin_amdgcn_readfirstlane(__builtin_ctzll(here));
+      out.first = __builtin_amdgcn_readlane(first, lane);
+      out.len = __builtin_amdgcn_readlane(len, lane);
+      out.row0 = (__builtin_amdgcn_readlane(sum, lane) - 1 - (index - before)) * kPromptRows;
       return true;
     }
-    before += __shfl(sum, 63);
+    before += __builtin_amdgcn_readlane(sum, 63);
   }
   return false;
 }
