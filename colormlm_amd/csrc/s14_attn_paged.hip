@@ -77,6 +77,9 @@ constexpr uint32_t kRecord = D + 4;
 // The top bit of each byte that is a NaN code (0x7f, 0xff).
 __device__ __forceinline__ uint32_t nan_codes(uint32_t c) { return ((c & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
+// Those bytes as zeros.
+__device__ __forceinline__ uint32_t no_nan(uint32_t c) { return c & ~((nan_codes(c) >> 7) * 0xffu); }
+
 template <int D, int NT, int T>
 __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(PagedArgs a, PagedPlan p, float *part) {
   constexpr int C = D / 64;   // 16-byte pieces of a K row a lane holds
@@ -204,14 +207,16 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
         top = fmaxf(top, x[i]);
       }
       top = fmaxf(m[nt], max_lane16(top));
-      const float at = top == -INFINITY ? 0.0f : top;  // no key seen yet: every weight 0
-      const float fade = __builtin_amdgcn_exp2f(m[nt] - at);
-      m[nt] = top;
-      sum[nt] *= fade;
-      if (__any(fade != 1.0f)) {
+      // the maximum that the weights are taken from moves only where they
+      // would pass 2^kRise: O is seldom multiplied
+      if (__any(top > m[nt] + kRise)) {
+        const float fade = __builtin_amdgcn_exp2f(m[nt] - (top == -INFINITY ? 0.0f : top));
+        m[nt] = top;
+        sum[nt] *= fade;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[nt][dt] *= fade;
       }
+      const float at = m[nt] == -INFINITY ? 0.0f : m[nt];  // no key seen yet: every weight 0
       u32x4 w[T / 2];
 #pragma unroll
       for (int t = 0; t < T; ++t) {
@@ -245,7 +250,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
 #pragma unroll
         for (int k = 0; k < W; ++k)
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) vv[dt][k] &= ~((nan_codes(vv[dt][k]) >> 7) * 0xffu);
+          for (int dt = 0; dt < DT; ++dt) vv[dt][k] = no_nan(vv[dt][k]);
       }
     }
 #pragma unroll
@@ -362,6 +367,253 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   }
 }
 
+// Heads of 512 (one wide key head for many query heads): 16 NT rows of Q and O
+// do not fit a wavefront, and rows in pieces of 16 would read every page again
+// for each.  Here a wavefront keeps a quarter of the head, 128 dimensions, of
+// all the workgroup's rows, and no byte of the cache goes to two wavefronts:
+// its part of S^T goes to LDS, wavefront w sums row tile w's parts and takes
+// the softmax, its P goes back through LDS in the operand layout, and each
+// wavefront's second product gives its quarter of O.
+template <int NT>
+__global__ __launch_bounds__(256, NT == 4 ? 1 : 2) void k_paged_wide(PagedArgs a, PagedPlan p, float *part) {
+  constexpr int D = 512, T = 4, C = 2, DT = 8;
+  const uint32_t kvh = a.cache.heads, group = a.heads / kvh;
+  const uint32_t items = kvh * p.chunks * a.seqs, tile = blockIdx.x / items, item = blockIdx.x % items;
+  const uint32_t head = item % kvh, seq = item / kvh % a.seqs, chunk = item / kvh / a.seqs;
+  const uint32_t row0 = tile * 16 * NT;
+  const Span sp = paged_span(a, p, seq, row0);
+  if (int64_t(row0) >= sp.rows || (chunk && chunk >= sp.chunks)) return;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63u, n = l & 15u, g = l >> 4;
+  const uint32_t P = a.cache.page, d0 = 128 * wave;
+  const int32_t *table = a.page_table + uint64_t(seq) * a.table_width;
+  const int32_t begin = sp.lo + int32_t(chunk * sp.chunk);
+  const int32_t end = min(sp.hi, begin + int32_t(sp.chunk));
+  const auto row_of = [&](int nt) {
+    const int64_t r = int64_t(row0) + 16 * nt + n;
+    return r < sp.rows ? r : sp.rows - 1;
+  };
+  const auto see_of = [&](int nt) { return Visible(sp.pos0 + int32_t(row_of(nt) / group), a.window); };
+
+  bf16x8 q[NT][2 * C];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int64_t rr = row_of(nt);
+    const uint16_t *row = a.q + uint64_t(sp.first + rr / group) * a.q_token +
+                          uint64_t(head * group + uint32_t(rr % group)) * a.q_head + d0;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) q[nt][2 * c + h] = *reinterpret_cast<const bf16x8 *>(row + 64 * c + 16 * g + 8 * h);
+  }
+  const int32_t pos_lo = sp.pos0 + int32_t(row0 / group), pos_hi = sp.hi - 1;
+  const bool softmax = wave < NT;  // wavefront w: row tile w
+  const Visible see = see_of(softmax ? int(wave) : 0);
+
+  __shared__ f32x4 s_part[4][NT][T][64];
+  __shared__ bf16x8 s_p[NT][T / 2][64];
+  __shared__ float s_fade[NT][16], s_m[NT][16], s_l[NT][16];
+
+  f32x4 o[NT][DT] = {};
+  float m = -INFINITY, sum = 0.0f;
+  bool bad = false, odd = false;
+  const float scale = a.scale * kLog2e;
+  const uint64_t page_bytes = uint64_t(P) * D;
+
+  uint4 kk[T][C], vv[DT];
+  uint32_t ksc = 0, vsc = 0;
+  int32_t idk = 0, idv = 0;
+  auto load_ids = [&](int32_t b) {
+    idk = page_of(a, table, b + 4 * T * int32_t(n / 4), sp.len, bad);
+    idv = page_of(a, table, b + 4 * T * int32_t(g), sp.len, bad);
+  };
+  auto load_k = [&](int32_t b) {
+    const uint32_t at = uint32_t(b + 4 * T * int32_t(n / 4)) % P + (n & 3u);
+    const uint8_t *kp = a.cache.k + (uint64_t(idk) * kvh + head) * page_bytes + at * uint32_t(D) + d0 + 16 * g;
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int c = 0; c < C; ++c) kk[t][c] = *reinterpret_cast<const uint4 *>(kp + 4 * t * D + 64 * c);
+    const uint64_t sat = uint64_t(idv) * kvh + head;
+    ksc = a.cache.ks[sat], vsc = a.cache.vs[sat];
+  };
+  auto load_v = [&](int32_t b) {
+    const uint8_t *vp = a.cache.v + (uint64_t(idv) * kvh + head) * page_bytes + (d0 + n) * P +
+                        uint32_t(b + 4 * T * int32_t(g)) % P;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) vv[dt] = *reinterpret_cast<const uint4 *>(vp + 16 * dt * P);
+  };
+  constexpr int32_t kStep = 16 * T;
+  if (begin < end) {
+    load_ids(begin);
+    load_k(begin);
+    load_v(begin);
+    if (begin + kStep < end) load_ids(begin + kStep);
+  }
+
+  for (int32_t b = begin; b < end; b += kStep) {
+    const int32_t tv = b + 4 * T * int32_t(g);
+    const bool more = b + kStep < end;
+    const float ks = scale * power_of_two(int(ksc) - 127);
+    const float vs = power_of_two(int(vsc) - 127);
+    const bool partial = b + kStep - 1 > pos_lo || (a.window && int64_t(b) <= int64_t(pos_hi) - a.window);
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      f32x4 s[NT] = {};
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const bf16x8 k0 = e4m3_bf16(kk[t][c].x, kk[t][c].y), k1 = e4m3_bf16(kk[t][c].z, kk[t][c].w);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          s[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q[nt][2 * c], s[nt], 0, 0, 0);
+          s[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q[nt][2 * c + 1], s[nt], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s_part[wave][nt][t][l] = s[nt];
+    }
+    if (more) load_k(b + kStep);
+    __syncthreads();
+    if (softmax) {
+      float x[4 * T];
+      float top = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const f32x4 s = s_part[0][wave][t][l] + s_part[1][wave][t][l] + s_part[2][wave][t][l] + s_part[3][wave][t][l];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[4 * t + i] = s[i] * ks;
+          if (partial) x[4 * t + i] = see(tv + 4 * t + i) ? x[4 * t + i] : -INFINITY;
+          top = fmaxf(top, x[4 * t + i]);
+        }
+      }
+      top = fmaxf(m, max_lane16(top));
+      float fade = 1.0f;
+      if (__any(top > m + kRise)) {
+        fade = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
+        m = top;
+        sum *= fade;
+      }
+      if (g == 0) s_fade[wave][n] = fade;
+      const float at = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int u = 0; u < T / 2; ++u) {
+        u32x4 w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float e0 = __builtin_amdgcn_exp2f(x[8 * u + 2 * j] - at), e1 = __builtin_amdgcn_exp2f(x[8 * u + 2 * j + 1] - at);
+          sum += e0;
+          sum += e1;
+          w[j] = bf16_pair(e0 * vs, e1 * vs);  // half a step of each weight: the matrix operand's type
+        }
+        s_p[wave][u][l] = __builtin_bit_cast(bf16x8, w);
+      }
+    }
+    __syncthreads();
+    if (partial) {  // as in k_paged_attention
+      uint32_t nan = 0;
+      uint32_t keep[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int32_t left = sp.len - (tv + 4 * k);
+        keep[k] = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        vv[dt].x &= keep[0], vv[dt].y &= keep[1], vv[dt].z &= keep[2], vv[dt].w &= keep[3];
+        nan |= nan_codes(vv[dt].x) | nan_codes(vv[dt].y) | nan_codes(vv[dt].z) | nan_codes(vv[dt].w);
+      }
+      if (__any(nan != 0)) {
+        odd = true;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          vv[dt].x = no_nan(vv[dt].x), vv[dt].y = no_nan(vv[dt].y);
+          vv[dt].z = no_nan(vv[dt].z), vv[dt].w = no_nan(vv[dt].w);
+        }
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float fade = s_fade[nt][n];
+      if (__any(fade != 1.0f)) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[nt][dt] *= fade;
+      }
+    }
+    bf16x8 pb[NT][T / 2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int u = 0; u < T / 2; ++u) pb[nt][u] = s_p[nt][u][l];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const bf16x8 v0 = e4m3_bf16(vv[dt].x, vv[dt].y), v1 = e4m3_bf16(vv[dt].z, vv[dt].w);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pb[nt][0], o[nt][dt], 0, 0, 0);
+        o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pb[nt][1], o[nt][dt], 0, 0, 0);
+      }
+    }
+    if (more) load_v(b + kStep);
+    if (b + 2 * kStep < end) load_ids(b + 2 * kStep);
+  }
+
+  if (odd) {  // uniform, and rare: one token after the other
+    for (int32_t b0 = begin; b0 < end; b0 += kStep) {
+      if (b0 + kStep - 1 <= pos_lo && !(a.window && int64_t(b0) <= int64_t(pos_hi) - a.window)) continue;
+      for (int32_t j = b0; j < min(b0 + kStep, sp.len); ++j) {
+        const int32_t id = page_of(a, table, j, sp.len, bad);
+        const uint8_t *vp = a.cache.v + (uint64_t(id) * kvh + head) * page_bytes + d0 * P + uint32_t(j) % P;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          f32x4 nan;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            nan[i] = (vp[(16 * dt + 4 * g + i) * P] & 0x7fu) == 0x7fu ? __uint_as_float(0x7fc00000u) : 0.0f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const bool in = see_of(nt)(j);
+            f32x4 back;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) back[i] = in ? nan[i] : 0.0f;
+            o[nt][dt] += back;
+          }
+        }
+      }
+    }
+  }
+  if (__any(bad)) {  // every wavefront has read the same ids
+    if (l == 0) atomicOr(a.status, kStatusBadCachePage);
+    sum = __uint_as_float(0x7fc00000u);
+  }
+  if (softmax) {
+    sum = sum_lane16(sum);
+    if (g == 0) s_m[wave][n] = m, s_l[wave][n] = sum;
+  }
+  __syncthreads();
+  float *rec = part + uint64_t(blockIdx.x) * (p.rec_rows * kRecord<D>);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int64_t r = int64_t(row0) + 16 * nt + n;
+    if (r >= sp.rows) continue;
+    const float top = s_m[nt][n], total = s_l[nt][n];
+    if (sp.chunks > 1) {
+      float *row = rec + (16 * nt + n) * kRecord<D>;
+      if (wave == 0 && g == 0) row[D] = top, row[D + 1] = total;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4 *>(row + d0 + 16 * dt + 4 * g) = o[nt][dt];
+      continue;
+    }
+    const uint64_t t = uint64_t(sp.first + r / group);
+    const uint32_t h = head * group + uint32_t(r % group);
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      store_out(a.out, t * a.out.token + uint64_t(h) * a.out.head + d0 + 16 * dt + 4 * g, o[nt][dt][0] * inv,
+                o[nt][dt][1] * inv, o[nt][dt][2] * inv, o[nt][dt][3] * inv);
+    if (a.lse && wave == 0 && g == 0) a.lse[t * a.heads + h] = total == 0.0f ? -INFINITY : top * kLn2 + __logf(total);
+  }
+}
+
 // Joins the chunks of one row a workgroup, in an order that its size alone
 // sets: the chunks' maxima in the lanes, then their rows in groups of
 // threads at once.
@@ -418,23 +670,28 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, PagedPlan p, co
   if (a.lse && lane == 0) a.lse[t * a.heads + h] = total == 0.0f ? -INFINITY : top * kLn2 + __logf(total);
 }
 
-template <int D, int NT, int T>
-hipError_t launch(hipStream_t s, const PagedArgs &a, const PagedPlan &p, float *part) {
-  k_paged_attention<D, NT, T><<<uint32_t(p.blocks), 256, 0, s>>>(a, p, part);
+template <class Kernel, class Join>
+hipError_t launch(hipStream_t s, const PagedArgs &a, const PagedPlan &p, float *part, Kernel kernel, Join join) {
+  kernel<<<uint32_t(p.blocks), 256, 0, s>>>(a, p, part);
   if (p.chunks > 1) {
     const uint32_t rows = uint32_t(a.max_new) * (a.heads / a.cache.heads);
-    k_paged_join<D><<<dim3(rows, a.seqs, a.cache.heads), 256, 0, s>>>(a, p, part);
+    join<<<dim3(rows, a.seqs, a.cache.heads), 256, 0, s>>>(a, p, part);
   }
   return hipGetLastError();
 }
 
 template <int D>
 hipError_t launch_dim(hipStream_t s, const PagedArgs &a, const PagedPlan &p, float *part) {
-  if constexpr (D <= 128)
-    if (p.row_tiles == 4) return launch<D, 4, 4>(s, a, p, part);
-  if constexpr (D <= 256)
-    if (p.row_tiles == 2) return launch<D, 2, D == 256 ? 2 : 4>(s, a, p, part);
-  return launch<D, 1, D == 512 ? 2 : 4>(s, a, p, part);
+  if constexpr (D == 512) {
+    if (p.row_tiles == 4) return launch(s, a, p, part, k_paged_wide<4>, k_paged_join<D>);
+    if (p.row_tiles == 2) return launch(s, a, p, part, k_paged_wide<2>, k_paged_join<D>);
+    return launch(s, a, p, part, k_paged_wide<1>, k_paged_join<D>);
+  } else {
+    if constexpr (D <= 128)
+      if (p.row_tiles == 4) return launch(s, a, p, part, k_paged_attention<D, 4, 4>, k_paged_join<D>);
+    if (p.row_tiles == 2) return launch(s, a, p, part, k_paged_attention<D, 2, D == 256 ? 2 : 4>, k_paged_join<D>);
+    return launch(s, a, p, part, k_paged_attention<D, 1, 4>, k_paged_join<D>);
+  }
 }
 
 }  // namespace
@@ -446,7 +703,7 @@ hipError_t launch_dim(hipStream_t s, const PagedArgs &a, const PagedPlan &p, flo
 PagedPlan paged_plan(const PagedArgs &a) {
   PagedPlan p{};
   const uint64_t rows = uint64_t(a.max_new) * (a.heads / a.cache.heads);
-  const uint32_t dim = a.cache.dim, most = dim <= 128 ? 4 : dim == 256 ? 2 : 1;
+  const uint32_t dim = a.cache.dim, most = dim == 256 ? 2 : 4;
   p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   if (p.row_tiles > most) p.row_tiles = most;
   const uint64_t tiles = (rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles);
@@ -454,7 +711,7 @@ PagedPlan paged_plan(const PagedArgs &a) {
   uint64_t span = a.max_len;
   if (a.window && uint64_t(a.window) + a.max_new + 63 < span) span = uint64_t(a.window) + a.max_new + 63;
     // workgroups that the card holds at once, by the registers of a wavefront
-  const uint32_t words = dim * p.row_tiles;
+  const uint32_t words = (dim == 512 ? 128 : dim) * p.row_tiles;
   const uint64_t slots = 256 * (words <= 64 ? 3 : words <= 128 ? 2 : 1);
   constexpr uint64_t kLeast = 256, kMost = 2048;
   p.rec_rows = uint32_t(rows < 16 * p.row_tiles ? rows : 16 * p.row_tiles);

@@ -23,7 +23,6 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr uint32_t kPromptRows = 128;
-constexpr float kRise = 8.0f;
 
 // Row block `index` of the packed sequences: its sequence's first token and
 // length, and the block within it.  Every sequence has its rows in whole

@@ -294,7 +294,7 @@ __device__ __forceinline__ bool find_page(const AppendArgs &a, uint32_t index, u
 //
 // A lane holds eight dimensions (Unit) of four neighbouring slots, kIt times
 // over: four V codes of a dimension are one word.
-template <int kDim, int kIt, bool kIn16>
+template <int kDim, int kIt, bool kTurn, bool kIn16>
 __device__ __forceinline__ void append_page(const AppendArgs &a, const Touched &t, uint32_t head, uint32_t side) {
   constexpr uint32_t kLanes = kDim / 8;
   const uint32_t P = a.cache.page;
@@ -307,8 +307,8 @@ __device__ __forceinline__ void append_page(const AppendArgs &a, const Touched &
   const uint32_t slot0 = kept / 4 * 4 + 4 * (threadIdx.x / kLanes);
   const AttnRows in = a.in[side];
   RopeArgs rope = a.rope;
-  if (side) rope.table = nullptr;
-  const float *weight = side ? nullptr : a.k_weight;
+  if (!kTurn || side) rope.table = nullptr;
+  const float *weight = !kTurn || side ? nullptr : a.k_weight;
   const Unit x = unit_of(lane, rope);
 
   Quad p[kIt][4], q[kIt][4];
@@ -333,18 +333,20 @@ __device__ __forceinline__ void append_page(const AppendArgs &a, const Touched &
   for (int it = 0; it < kIt; ++it) {
     if (kept / 4 * 4 + 4 * groups * it >= full) continue;  // uniform: past the last slot
     Angles n[4];
-    if (rope.table) {
+    const auto angles = [&](int j) {
+      const uint32_t slot = slot0 + 4 * groups * it + j;
+      const uint32_t s = slot < kept ? kept : slot < full ? slot : full - 1;
+      n[j] = load_angles(rope, x, int32_t(min(start + s, int64_t(INT_MAX))));
+    };
+    if (kIt == 1 && rope.table) {  // (kIt 2 has no registers for all at once)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t slot = slot0 + 4 * groups * it + j;
-        const uint32_t s = slot < kept ? kept : slot < full ? slot : full - 1;
-        n[j] = load_angles(rope, x, int32_t(min(start + s, int64_t(INT_MAX))));
-      }
+      for (int j = 0; j < 4; ++j) angles(j);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (weight) row_norm<kLanes>(p[it][j], q[it][j], w, a.eps);
       if (rope.table) {
+        if (kIt > 1) angles(j);
         row_rotate(p[it][j], q[it][j], rope, x, n[j]);
         if (!n[j].good && lane == 0) atomicOr(a.status, kStatusBadPosition);
       }
@@ -419,7 +421,8 @@ __device__ __forceinline__ void append_page(const AppendArgs &a, const Touched &
   }
 }
 
-template <int kDim, int kIt>
+// kTurn: K takes a norm or a rotation on the way.
+template <int kDim, int kIt, bool kTurn>
 __global__ __launch_bounds__(1024) void k_kv_append(AppendArgs a, uint32_t direct) {
   const uint32_t head = blockIdx.y >> 1, side = blockIdx.y & 1u;
   Touched t;
@@ -432,9 +435,9 @@ __global__ __launch_bounds__(1024) void k_kv_append(AppendArgs a, uint32_t direc
     return;
   }
   if (a.in[side].bf16)
-    append_page<kDim, kIt, true>(a, t, head, side);
+    append_page<kDim, kIt, kTurn, true>(a, t, head, side);
   else
-    append_page<kDim, kIt, false>(a, t, head, side);
+    append_page<kDim, kIt, kTurn, false>(a, t, head, side);
 }
 
 }  // namespace
@@ -478,15 +481,15 @@ static hipError_t kv_append(hipStream_t s, const AppendArgs &a) {
   // threads for the slot groups (of four) that a sequence can fill
   uint32_t groups = (a.max_new + 2) / 4 + 1;
   if (groups > P / 4) groups = P / 4;
-  uint32_t threads = (groups * kLanes + 63) / 64 * 64;
-  if constexpr (kDim == 512) {
-    if (threads > 1024) {
-      k_kv_append<kDim, 2><<<grid, 1024, 0, s>>>(a, direct);
-      return hipGetLastError();
-    }
-  }
-  k_kv_append<kDim, 1><<<grid, threads, 0, s>>>(a, direct);
-  return hipGetLastError();
+  const uint32_t threads = (groups * kLanes + 63) / 64 * 64;
+  const bool turn = a.k_weight || a.rope.table;
+  const auto launch = [&](auto kernel) {
+    kernel<<<grid, threads < 1024 ? threads : 1024, 0, s>>>(a, direct);
+    return hipGetLastError();
+  };
+  if constexpr (kDim == 512)
+    if (threads > 1024) return turn ? launch(k_kv_append<kDim, 2, true>) : launch(k_kv_append<kDim, 2, false>);
+  return turn ? launch(k_kv_append<kDim, 1, true>) : launch(k_kv_append<kDim, 1, false>);
 }
 
 hipError_t launch_kv_append(hipStream_t s, const AppendArgs &a) {

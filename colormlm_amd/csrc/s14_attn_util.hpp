@@ -17,6 +17,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kRise = 8.0f;  // how far (log2) a maximum may pass the one that weights are taken from
 
 // A row bound from device memory, held inside the packed rows.
 __device__ __forceinline__ int64_t clamp_row(int32_t r, uint32_t rows) {
