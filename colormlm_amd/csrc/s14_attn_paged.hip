@@ -61,14 +61,21 @@ __device__ __forceinline__ void store_out(const AttnOut &o, uint64_t at, float a
     *reinterpret_cast<float4 *>(static_cast<float *>(o.p) + at) = make_float4(a, b, c, d);
 }
 
-// The page of token group `tok` (held inside the sequence): its id, or -1.
-__device__ __forceinline__ int32_t page_of(const PagedArgs &a, const int32_t *table, int32_t tok, int32_t len,
-                                           bool &bad) {
-  const uint32_t t = uint32_t(tok < len ? tok : len - 1);
-  int32_t id = table[t / a.cache.page];
-  if (uint32_t(id) >= a.cache.pages) bad = true, id = 0;
-  return id;
-}
+// What a wavefront needs to find a step's pages.  A lane's tokens, 4 T
+// neighbours, lie in one page; tokens behind the sequence take its last page
+// (and are masked).  An id is looked at when it is used, a step after its
+// load: looking at once would wait for every load in flight.
+struct Pages {
+  const int32_t *table;
+  int32_t len;
+  uint32_t pages, shift;
+  __device__ __forceinline__ int32_t id(int32_t tok) const { return table[uint32_t(tok < len ? tok : len - 1) >> shift]; }
+  __device__ __forceinline__ uint32_t checked(int32_t id, bool &bad) const {
+    const bool out = uint32_t(id) >= pages;
+    bad |= out;
+    return out ? 0u : uint32_t(id);
+  }
+};
 
 // A row of a chunk's partial result: D sums, the maximum and the weights' sum.
 template <int D>
@@ -98,7 +105,8 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   if (int64_t(row0) >= sp.rows || (chunk && chunk >= sp.chunks)) return;
   const uint32_t wave = threadIdx.x / 64, l = threadIdx.x & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page;
-  const int32_t *table = a.page_table + uint64_t(seq) * a.table_width;
+  const uint32_t shift = __builtin_ctz(P);
+  const Pages pages{a.page_table + uint64_t(seq) * a.table_width, sp.len, a.cache.pages, shift};
   const int32_t begin = sp.lo + int32_t(chunk * sp.chunk);
   const int32_t end = min(sp.hi, begin + int32_t(sp.chunk));
 
@@ -134,24 +142,26 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   uint4 kk[T][C];
   uint32_t vv[DT][W];
   uint32_t ksc = 0, vsc = 0;
-  int32_t idk = 0, idv = 0;
-  auto load_ids = [&](int32_t b) {
-    idk = page_of(a, table, b + 4 * T * int32_t(n / 4), sp.len, bad);
-    idv = page_of(a, table, b + 4 * T * int32_t(g), sp.len, bad);
+  int32_t idk = 0, idv = 0;  // of the next step
+  uint32_t pagev = 0;
+  auto load_ids = [&](int32_t b, int32_t &k, int32_t &v) {
+    k = pages.id(b + 4 * T * int32_t(n / 4));
+    v = pages.id(b + 4 * T * int32_t(g));
   };
   auto load_k = [&](int32_t b) {
-    const uint32_t at = uint32_t(b + 4 * T * int32_t(n / 4)) % P + (n & 3u);
-    const uint8_t *kp = a.cache.k + (uint64_t(idk) * kvh + head) * page_bytes + at * uint32_t(D) + 16 * g;
+    const uint32_t at = (uint32_t(b + 4 * T * int32_t(n / 4)) & (P - 1)) + (n & 3u);
+    const uint8_t *kp = a.cache.k + (uint64_t(pages.checked(idk, bad)) * kvh + head) * page_bytes + at * uint32_t(D) + 16 * g;
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int c = 0; c < C; ++c) kk[t][c] = *reinterpret_cast<const uint4 *>(kp + 4 * t * D + 64 * c);
-    const uint64_t sat = uint64_t(idv) * kvh + head;
+    pagev = pages.checked(idv, bad);
+    const uint64_t sat = uint64_t(pagev) * kvh + head;
     ksc = a.cache.ks[sat], vsc = a.cache.vs[sat];
   };
   auto load_v = [&](int32_t b) {
-    const uint8_t *vp = a.cache.v + (uint64_t(idv) * kvh + head) * page_bytes + n * P +
-                        uint32_t(b + 4 * T * int32_t(g)) % P;
+    const uint8_t *vp = a.cache.v + (uint64_t(pagev) * kvh + head) * page_bytes + n * P +
+                        (uint32_t(b + 4 * T * int32_t(g)) & (P - 1));
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       if constexpr (T == 4) {
@@ -166,15 +176,17 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   constexpr int32_t kStride = 4 * 16 * T;  // the wavefronts' steps interleave
   int32_t b = begin + 16 * T * int32_t(wave);
   if (b < end) {
-    load_ids(b);
+    load_ids(b, idk, idv);
     load_k(b);
     load_v(b);
-    if (b + kStride < end) load_ids(b + kStride);
+    if (b + kStride < end) load_ids(b + kStride, idk, idv);
   }
 
   for (; b < end; b += kStride) {
     const int32_t tv = b + 4 * T * int32_t(g);
     const bool more = b + kStride < end;
+    int32_t idk2 = 0, idv2 = 0;  // ahead of the K and V loads below
+    if (b + 2 * kStride < end) load_ids(b + 2 * kStride, idk2, idv2);
     const float ks = scale * power_of_two(int(ksc) - 127);
     const float vs = power_of_two(int(vsc) - 127);
     f32x4 s[NT][T];
@@ -263,15 +275,14 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
           o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pb[nt][u], o[nt][dt], 0, 0, 0);
       }
     if (more) load_v(b + kStride);
-    if (b + 2 * kStride < end) load_ids(b + 2 * kStride);
+    idk = idk2, idv = idv2;
   }
 
   if (odd) {  // uniform, and rare: one token after the other
     for (int32_t b0 = begin + 16 * T * int32_t(wave); b0 < end; b0 += kStride) {
       if (b0 + 16 * T - 1 <= pos_lo && !(a.window && int64_t(b0) <= int64_t(pos_hi) - a.window)) continue;
       for (int32_t j = b0; j < min(b0 + 16 * T, sp.len); ++j) {
-        const int32_t id = page_of(a, table, j, sp.len, bad);
-        const uint8_t *vp = a.cache.v + (uint64_t(id) * kvh + head) * page_bytes + uint32_t(j) % P;
+        const uint8_t *vp = a.cache.v + (uint64_t(pages.checked(pages.id(j), bad)) * kvh + head) * page_bytes + (uint32_t(j) & (P - 1));
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           f32x4 nan;
@@ -385,7 +396,8 @@ __global__ __launch_bounds__(256, NT == 4 ? 1 : 2) void k_paged_wide(PagedArgs a
   if (int64_t(row0) >= sp.rows || (chunk && chunk >= sp.chunks)) return;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page, d0 = 128 * wave;
-  const int32_t *table = a.page_table + uint64_t(seq) * a.table_width;
+  const uint32_t shift = __builtin_ctz(P);
+  const Pages pages{a.page_table + uint64_t(seq) * a.table_width, sp.len, a.cache.pages, shift};
   const int32_t begin = sp.lo + int32_t(chunk * sp.chunk);
   const int32_t end = min(sp.hi, begin + int32_t(sp.chunk));
   const auto row_of = [&](int nt) {
@@ -421,38 +433,42 @@ __global__ __launch_bounds__(256, NT == 4 ? 1 : 2) void k_paged_wide(PagedArgs a
 
   uint4 kk[T][C], vv[DT];
   uint32_t ksc = 0, vsc = 0;
-  int32_t idk = 0, idv = 0;
-  auto load_ids = [&](int32_t b) {
-    idk = page_of(a, table, b + 4 * T * int32_t(n / 4), sp.len, bad);
-    idv = page_of(a, table, b + 4 * T * int32_t(g), sp.len, bad);
+  int32_t idk = 0, idv = 0;  // of the next step
+  uint32_t pagev = 0;
+  auto load_ids = [&](int32_t b, int32_t &k, int32_t &v) {
+    k = pages.id(b + 4 * T * int32_t(n / 4));
+    v = pages.id(b + 4 * T * int32_t(g));
   };
   auto load_k = [&](int32_t b) {
-    const uint32_t at = uint32_t(b + 4 * T * int32_t(n / 4)) % P + (n & 3u);
-    const uint8_t *kp = a.cache.k + (uint64_t(idk) * kvh + head) * page_bytes + at * uint32_t(D) + d0 + 16 * g;
+    const uint32_t at = (uint32_t(b + 4 * T * int32_t(n / 4)) & (P - 1)) + (n & 3u);
+    const uint8_t *kp = a.cache.k + (uint64_t(pages.checked(idk, bad)) * kvh + head) * page_bytes + at * uint32_t(D) + d0 + 16 * g;
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int c = 0; c < C; ++c) kk[t][c] = *reinterpret_cast<const uint4 *>(kp + 4 * t * D + 64 * c);
-    const uint64_t sat = uint64_t(idv) * kvh + head;
+    pagev = pages.checked(idv, bad);
+    const uint64_t sat = uint64_t(pagev) * kvh + head;
     ksc = a.cache.ks[sat], vsc = a.cache.vs[sat];
   };
   auto load_v = [&](int32_t b) {
-    const uint8_t *vp = a.cache.v + (uint64_t(idv) * kvh + head) * page_bytes + (d0 + n) * P +
-                        uint32_t(b + 4 * T * int32_t(g)) % P;
+    const uint8_t *vp = a.cache.v + (uint64_t(pagev) * kvh + head) * page_bytes + (d0 + n) * P +
+                        (uint32_t(b + 4 * T * int32_t(g)) & (P - 1));
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) vv[dt] = *reinterpret_cast<const uint4 *>(vp + 16 * dt * P);
   };
   constexpr int32_t kStep = 16 * T;
   if (begin < end) {
-    load_ids(begin);
+    load_ids(begin, idk, idv);
     load_k(begin);
     load_v(begin);
-    if (begin + kStep < end) load_ids(begin + kStep);
+    if (begin + kStep < end) load_ids(begin + kStep, idk, idv);
   }
 
   for (int32_t b = begin; b < end; b += kStep) {
     const int32_t tv = b + 4 * T * int32_t(g);
     const bool more = b + kStep < end;
+    int32_t idk2 = 0, idv2 = 0;  // ahead of the K and V loads below
+    if (b + 2 * kStep < end) load_ids(b + 2 * kStep, idk2, idv2);
     const float ks = scale * power_of_two(int(ksc) - 127);
     const float vs = power_of_two(int(vsc) - 127);
     const bool partial = b + kStep - 1 > pos_lo || (a.window && int64_t(b) <= int64_t(pos_hi) - a.window);
@@ -554,15 +570,14 @@ __global__ __launch_bounds__(256, NT == 4 ? 1 : 2) void k_paged_wide(PagedArgs a
       }
     }
     if (more) load_v(b + kStep);
-    if (b + 2 * kStep < end) load_ids(b + 2 * kStep);
+    idk = idk2, idv = idv2;
   }
 
   if (odd) {  // uniform, and rare: one token after the other
     for (int32_t b0 = begin; b0 < end; b0 += kStep) {
       if (b0 + kStep - 1 <= pos_lo && !(a.window && int64_t(b0) <= int64_t(pos_hi) - a.window)) continue;
       for (int32_t j = b0; j < min(b0 + kStep, sp.len); ++j) {
-        const int32_t id = page_of(a, table, j, sp.len, bad);
-        const uint8_t *vp = a.cache.v + (uint64_t(id) * kvh + head) * page_bytes + d0 * P + uint32_t(j) % P;
+        const uint8_t *vp = a.cache.v + (uint64_t(pages.checked(pages.id(j), bad)) * kvh + head) * page_bytes + d0 * P + (uint32_t(j) & (P - 1));
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           f32x4 nan;
@@ -699,7 +714,7 @@ hipError_t launch_dim(hipStream_t s, const PagedArgs &a, const PagedPlan &p, flo
 // Rows a wavefront holds: as many 16-row tiles as the longest new block fills
 // and the registers of the head size leave room for (64 rows of 128, 32 of
 // 256, 16 of 512).  Chunks: enough workgroups to fill the card where there
-// are few rows, none below one step a wavefront.
+// are few rows, none below a step.
 PagedPlan paged_plan(const PagedArgs &a) {
   PagedPlan p{};
   const uint64_t rows = uint64_t(a.max_new) * (a.heads / a.cache.heads);
@@ -713,15 +728,16 @@ PagedPlan paged_plan(const PagedArgs &a) {
     // workgroups that the card holds at once, by the registers of a wavefront
   const uint32_t words = (dim == 512 ? 128 : dim) * p.row_tiles;
   const uint64_t slots = 256 * (words <= 64 ? 3 : words <= 128 ? 2 : 1);
-  constexpr uint64_t kLeast = 256, kMost = 2048;
+  const uint64_t least = dim == 512 ? 64 : 256;  // a step of every wavefront
+  constexpr uint64_t kMost = 2048;
   p.rec_rows = uint32_t(rows < 16 * p.row_tiles ? rows : 16 * p.row_tiles);
   const uint64_t rec = uint64_t(p.rec_rows) * (dim + 4);
   uint64_t chunks = base < slots ? slots / base : (span + kMost - 1) / kMost;
   const uint64_t fit = kPagedPartFloats / (rec * base);
   if (chunks > fit) chunks = fit;
-  if (chunks > (span + kLeast - 1) / kLeast) chunks = (span + kLeast - 1) / kLeast;
+  if (chunks > (span + least - 1) / least) chunks = (span + least - 1) / least;
   if (chunks < 1) chunks = 1;
-  p.chunk = uint32_t(((span + chunks - 1) / chunks + kLeast - 1) / kLeast * kLeast);
+  p.chunk = uint32_t(((span + chunks - 1) / chunks + least - 1) / least * least);
   p.chunks = span ? uint32_t((span + p.chunk - 1) / p.chunk) : 1;
   p.blocks = base * p.chunks;
   return p;
