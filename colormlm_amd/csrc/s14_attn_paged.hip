@@ -26,7 +26,7 @@ namespace {
 // What a row tile of a sequence reads: tokens lo .. hi - 1 in chunks of
 // `chunk` (a multiple of 64, as lo is).
 struct Span {
-  int64_t first, rows;  // first packed token; (token, head) rows of the sequence
+  uint32_t first, rows;  // first packed token; (token, head) rows of the sequence
   int32_t len, pos0, lo, hi;
   uint32_t chunk, chunks;
 };
@@ -34,14 +34,15 @@ struct Span {
 __device__ __forceinline__ Span paged_span(const PagedArgs &a, const PagedPlan &p, uint32_t seq, uint32_t row0) {
   Span s;
   const uint32_t group = a.heads / a.cache.heads;
-  s.first = clamp_row(a.cu[seq], a.tokens);
-  const int64_t n = clamp_row(a.cu[seq + 1], a.tokens) - s.first;
-  s.rows = n > 0 ? n * group : 0;
+  s.first = uint32_t(clamp_row(a.cu[seq], a.tokens));
+  const int32_t n = int32_t(clamp_row(a.cu[seq + 1], a.tokens)) - int32_t(s.first);
+  // no more rows than the launch was planned for: below 2^31 in all
+  s.rows = n <= 0 ? 0u : (uint32_t(n) < a.max_new ? uint32_t(n) : a.max_new) * group;
   const int64_t room = int64_t(a.table_width) * a.cache.page;
   const int64_t len = a.len[seq] < 0 ? 0 : a.len[seq];
   s.len = int32_t(len < room ? len : room);
-  s.pos0 = int32_t(s.len - n);
-  const int64_t last = (row0 + 16 * p.row_tiles < s.rows ? row0 + 16 * p.row_tiles : s.rows) - 1;
+  s.pos0 = s.len - n;
+  const uint32_t last = (row0 + 16 * p.row_tiles < s.rows ? row0 + 16 * p.row_tiles : s.rows) - 1;
   const int32_t first_pos = s.pos0 + int32_t(row0 / group), last_pos = s.pos0 + int32_t(last / group);
   s.hi = last_pos + 1 < 0 ? 0 : last_pos + 1;
   int64_t lo = a.window ? int64_t(first_pos) - a.window + 1 : 0;
@@ -59,6 +60,29 @@ __device__ __forceinline__ void store_out(const AttnOut &o, uint64_t at, float a
     *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(o.p) + at) = make_uint2(bf16_pair(a, b), bf16_pair(c, d));
   else
     *reinterpret_cast<float4 *>(static_cast<float *>(o.p) + at) = make_float4(a, b, c, d);
+}
+
+// What a workgroup works on.  Row tiles are the slowest index: those that read
+// the same pages are a multiple of all items apart.  Chunks come before them,
+// so that the late chunks, which short sequences lack, are together: among the
+// sequences the empty workgroups fell to the same compute units (128 ragged
+// sequences of 8,192 tokens at most, 4 chunks: 228 us; so DECODE_US).
+// Workgroup i runs on XCD i % 8: where (sequence, key head) pairs are few, a
+// chunk's pairs are rotated each time their start comes back to the first XCD,
+// or one long sequence would have but some of the XCDs.
+struct Item {
+  uint32_t tile, chunk, seq, head;
+};
+__device__ __forceinline__ Item item_of(const PagedArgs &a, const PagedPlan &p, uint32_t kvh) {
+  const uint32_t pairs = kvh * a.seqs, items = pairs * p.chunks;
+  const uint32_t tile = blockIdx.x / items, item = blockIdx.x % items, chunk = item / pairs;
+  const uint32_t zeros = __builtin_ctz(pairs | 8u);
+  const uint32_t pair = (item % pairs + (chunk >> (3 - zeros))) % pairs;
+  return {tile, chunk, pair / kvh, pair % kvh};
+}
+
+__device__ __forceinline__ uint64_t record_of(const PagedArgs &a, const PagedPlan &p, const Item &i, uint32_t kvh) {
+  return ((uint64_t(i.tile) * p.chunks + i.chunk) * a.seqs + i.seq) * kvh + i.head;
 }
 
 // What a wavefront needs to find a step's pages.  A lane's tokens, 4 T
@@ -93,16 +117,11 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   constexpr int DT = D / 16;  // 16-dimension tiles of O
   constexpr int W = T;        // 32-bit words of V codes a lane holds of one dimension
   const uint32_t kvh = a.cache.heads, group = a.heads / kvh;
-  // Row tiles are the slowest index: those that read the same pages are a
-  // multiple of `items` apart.  Chunks come before them, so that the late
-  // chunks, which short sequences lack, are together: among the sequences the
-  // empty workgroups fell to the same compute units (128 ragged sequences of
-  // 8,192 tokens at most, 8 chunks: 228 us; so DECODE_US).
-  const uint32_t items = kvh * p.chunks * a.seqs, tile = blockIdx.x / items, item = blockIdx.x % items;
-  const uint32_t head = item % kvh, seq = item / kvh % a.seqs, chunk = item / kvh / a.seqs;
+  const Item it = item_of(a, p, kvh);
+  const uint32_t tile = it.tile, head = it.head, seq = it.seq, chunk = it.chunk;
   const uint32_t row0 = tile * 16 * NT;
   const Span sp = paged_span(a, p, seq, row0);
-  if (int64_t(row0) >= sp.rows || (chunk && chunk >= sp.chunks)) return;
+  if (row0 >= sp.rows || (chunk && chunk >= sp.chunks)) return;
   const uint32_t wave = threadIdx.x / 64, l = threadIdx.x & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page;
   const uint32_t shift = __builtin_ctz(P);
@@ -115,11 +134,11 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   bf16x8 q[NT][2 * C];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int64_t r = int64_t(row0) + 16 * nt + n;
-    const int64_t rr = r < sp.rows ? r : sp.rows - 1;
+    const uint32_t r = row0 + 16 * nt + n;
+    const uint32_t rr = r < sp.rows ? r : sp.rows - 1;
     see[nt] = Visible(sp.pos0 + int32_t(rr / group), a.window);
     const uint16_t *row = a.q + uint64_t(sp.first + rr / group) * a.q_token +
-                          uint64_t(head * group + uint32_t(rr % group)) * a.q_head;
+                          uint64_t(head * group + rr % group) * a.q_head;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -352,10 +371,10 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   if (sp.chunks <= 1) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int64_t r = int64_t(row0) + 16 * nt + n;
+      const uint32_t r = row0 + 16 * nt + n;
       if (r >= sp.rows) continue;
       const uint64_t t = uint64_t(sp.first + r / group);
-      const uint32_t h = head * group + uint32_t(r % group);
+      const uint32_t h = head * group + r % group;
       const float inv = sum[nt] == 0.0f ? 0.0f : 1.0f / sum[nt];
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
@@ -365,7 +384,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
     }
     return;
   }
-  float *rec = part + uint64_t(blockIdx.x) * (p.rec_rows * kRecord<D>);
+  float *rec = part + record_of(a, p, it, kvh) * (p.rec_rows * kRecord<D>);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     if (16 * nt + n >= p.rec_rows) continue;
@@ -386,14 +405,14 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
 // the softmax, its P goes back through LDS in the operand layout, and each
 // wavefront's second product gives its quarter of O.
 template <int NT>
-__global__ __launch_bounds__(256, NT == 4 ? 1 : 2) void k_paged_wide(PagedArgs a, PagedPlan p, float *part) {
+__global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p, float *part) {
   constexpr int D = 512, T = 4, C = 2, DT = 8;
   const uint32_t kvh = a.cache.heads, group = a.heads / kvh;
-  const uint32_t items = kvh * p.chunks * a.seqs, tile = blockIdx.x / items, item = blockIdx.x % items;
-  const uint32_t head = item % kvh, seq = item / kvh % a.seqs, chunk = item / kvh / a.seqs;
+  const Item it = item_of(a, p, kvh);
+  const uint32_t tile = it.tile, head = it.head, seq = it.seq, chunk = it.chunk;
   const uint32_t row0 = tile * 16 * NT;
   const Span sp = paged_span(a, p, seq, row0);
-  if (int64_t(row0) >= sp.rows || (chunk && chunk >= sp.chunks)) return;
+  if (row0 >= sp.rows || (chunk && chunk >= sp.chunks)) return;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page, d0 = 128 * wave;
   const uint32_t shift = __builtin_ctz(P);
@@ -401,7 +420,7 @@ __global__ __launch_bounds__(256, NT == 4 ? 1 : 2) void k_paged_wide(PagedArgs a
   const int32_t begin = sp.lo + int32_t(chunk * sp.chunk);
   const int32_t end = min(sp.hi, begin + int32_t(sp.chunk));
   const auto row_of = [&](int nt) {
-    const int64_t r = int64_t(row0) + 16 * nt + n;
+    const uint32_t r = row0 + 16 * nt + n;
     return r < sp.rows ? r : sp.rows - 1;
   };
   const auto see_of = [&](int nt) { return Visible(sp.pos0 + int32_t(row_of(nt) / group), a.window); };
@@ -409,9 +428,9 @@ __global__ __launch_bounds__(256, NT == 4 ? 1 : 2) void k_paged_wide(PagedArgs a
   bf16x8 q[NT][2 * C];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int64_t rr = row_of(nt);
+    const uint32_t rr = row_of(nt);
     const uint16_t *row = a.q + uint64_t(sp.first + rr / group) * a.q_token +
-                          uint64_t(head * group + uint32_t(rr % group)) * a.q_head + d0;
+                          uint64_t(head * group + rr % group) * a.q_head + d0;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -605,10 +624,10 @@ __global__ __launch_bounds__(256, NT == 4 ? 1 : 2) void k_paged_wide(PagedArgs a
     if (g == 0) s_m[wave][n] = m, s_l[wave][n] = sum;
   }
   __syncthreads();
-  float *rec = part + uint64_t(blockIdx.x) * (p.rec_rows * kRecord<D>);
+  float *rec = part + record_of(a, p, it, kvh) * (p.rec_rows * kRecord<D>);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int64_t r = int64_t(row0) + 16 * nt + n;
+    const uint32_t r = row0 + 16 * nt + n;
     if (r >= sp.rows) continue;
     const float top = s_m[nt][n], total = s_l[nt][n];
     if (sp.chunks > 1) {
@@ -619,7 +638,7 @@ __global__ __launch_bounds__(256, NT == 4 ? 1 : 2) void k_paged_wide(PagedArgs a
       continue;
     }
     const uint64_t t = uint64_t(sp.first + r / group);
-    const uint32_t h = head * group + uint32_t(r % group);
+    const uint32_t h = head * group + r % group;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -640,10 +659,9 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, PagedPlan p, co
   const uint32_t seq = blockIdx.y, head = blockIdx.z, r = blockIdx.x;
   const uint32_t per = 16 * p.row_tiles, tile = r / per;
   const Span sp = paged_span(a, p, seq, tile * per);
-  if (int64_t(r) >= sp.rows || sp.chunks <= 1) return;
+  if (r >= sp.rows || sp.chunks <= 1) return;
   const uint64_t rec = uint64_t(p.rec_rows) * kRecord<D>;
-  const float *row = part + (uint64_t(tile) * kvh * p.chunks * a.seqs + uint64_t(seq) * kvh + head) * rec +
-                     uint32_t(r % per) * kRecord<D>;
+  const float *row = part + record_of(a, p, Item{tile, 0, seq, head}, kvh) * rec + r % per * kRecord<D>;
   const uint64_t next = uint64_t(kvh) * a.seqs * rec;  // the next chunk's record
   float top = -INFINITY;
   for (uint32_t c = tid & 63u; c < sp.chunks; c += 64) top = fmaxf(top, row[c * next + D]);
@@ -698,7 +716,6 @@ hipError_t launch(hipStream_t s, const PagedArgs &a, const PagedPlan &p, float *
 template <int D>
 hipError_t launch_dim(hipStream_t s, const PagedArgs &a, const PagedPlan &p, float *part) {
   if constexpr (D == 512) {
-    if (p.row_tiles == 4) return launch(s, a, p, part, k_paged_wide<4>, k_paged_join<D>);
     if (p.row_tiles == 2) return launch(s, a, p, part, k_paged_wide<2>, k_paged_join<D>);
     return launch(s, a, p, part, k_paged_wide<1>, k_paged_join<D>);
   } else {
@@ -718,7 +735,7 @@ hipError_t launch_dim(hipStream_t s, const PagedArgs &a, const PagedPlan &p, flo
 PagedPlan paged_plan(const PagedArgs &a) {
   PagedPlan p{};
   const uint64_t rows = uint64_t(a.max_new) * (a.heads / a.cache.heads);
-  const uint32_t dim = a.cache.dim, most = dim == 256 ? 2 : 4;
+  const uint32_t dim = a.cache.dim, most = dim <= 128 ? 4 : 2;
   p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   if (p.row_tiles > most) p.row_tiles = most;
   const uint64_t tiles = (rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles);
@@ -727,12 +744,17 @@ PagedPlan paged_plan(const PagedArgs &a) {
   if (a.window && uint64_t(a.window) + a.max_new + 63 < span) span = uint64_t(a.window) + a.max_new + 63;
     // workgroups that the card holds at once, by the registers of a wavefront
   const uint32_t words = (dim == 512 ? 128 : dim) * p.row_tiles;
-  const uint64_t slots = 256 * (words <= 64 ? 3 : words <= 128 ? 2 : 1);
+  const uint64_t slots = 256 * (words <= 64 ? 3 : words <= 128 || dim == 512 ? 2 : 1);
+  uint64_t base_slots = slots;
   const uint64_t least = dim == 512 ? 64 : 256;  // a step of every wavefront
   constexpr uint64_t kMost = 2048;
   p.rec_rows = uint32_t(rows < 16 * p.row_tiles ? rows : 16 * p.row_tiles);
   const uint64_t rec = uint64_t(p.rec_rows) * (dim + 4);
-  uint64_t chunks = base < slots ? slots / base : (span + kMost - 1) / kMost;
+#ifndef KX
+#define KX 1
+#endif
+  if (a.seqs > 1) base_slots = slots * KX;
+  uint64_t chunks = base < slots ? base_slots / base : (span + kMost - 1) / kMost;
   const uint64_t fit = kPagedPartFloats / (rec * base);
   if (chunks > fit) chunks = fit;
   if (chunks > (span + least - 1) / least) chunks = (span + least - 1) / least;
