@@ -13,6 +13,7 @@
 #include <cstring>
 #include <new>
 
+#include "s14_attn.hpp"
 #include "s14_device.hpp"
 #include "s14_internal.hpp"
 #include "s14_linear.hpp"
@@ -126,8 +127,8 @@ extern "C" int s14_ctx_create(int device, s14_ctx **out) {
     s14_ctx_destroy(ctx);
     return hip_fail(e, "hipStreamCreate");
   }
-  // workspace: table | h | scores | biased | route counters | h windows
-  const size_t off = s14::kWorkspaceBytes;
+  // workspace: table | h | scores | biased | route counters | h windows ..., then the attention's counters
+  const size_t off = s14::kWorkspaceBytes + s14::kPagedCounters * sizeof(uint32_t);
   e = hipMalloc(&ctx->ws_base, off);
   if (e != hipSuccess) {
     s14_ctx_destroy(ctx);
@@ -174,6 +175,9 @@ extern "C" void s14_ctx_destroy(s14_ctx *ctx) {
 extern "C" void *s14_ctx_compute_stream(s14_ctx *ctx) { return ctx ? ctx->compute : nullptr; }
 int s14::ctx_device(const s14_ctx *ctx) { return ctx->device; }
 uint32_t *s14::ctx_status(const s14_ctx *ctx) { return status_word(ctx->ws); }
+uint32_t *s14::ctx_attn_counters(const s14_ctx *ctx) {
+  return reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(ctx->ws_base) + kWorkspaceBytes);
+}
 int s14::ctx_attn_workspace(s14_ctx *ctx, uint64_t bytes, float **out) {
   if (!ctx->attn_base) {
     // the call may be under capture, where this thread's mode forbids hipMalloc

@@ -73,7 +73,7 @@ struct PagedArgs {
   float *lse;  // [tokens][heads] or NULL
   float scale;
   uint32_t window;
-  uint32_t *status;
+  uint32_t *status, *count;  // count: kPagedCounters
 };
 
 struct PromptArgs {
@@ -100,9 +100,11 @@ struct PagedPlan {
   uint32_t rec_rows;   // rows of a chunk's partial result
   uint32_t chunk;      // tokens of one workgroup, a multiple of 64
   uint32_t chunks;     // of the longest sequence; above 1 the partial results go to the workspace
+  uint32_t fused;      // the last workgroup of a row tile joins its chunks; else a second launch
   uint64_t blocks;     // workgroups
 };
 constexpr uint64_t kPagedPartFloats = 16ull << 20;  // the workspace: 64 MiB
+constexpr uint32_t kPagedCounters = 16384;          // arrivals at a row tile, 0 between launches
 PagedPlan paged_plan(const PagedArgs &a);
 
 hipError_t launch_rope_table(hipStream_t s, const RopeTableArgs &a);

@@ -267,7 +267,7 @@ extern "C" int s14_paged_attention(s14_ctx *ctx, void *stream, const s14_rows *q
   const s14::PagedPlan p = s14::paged_plan(a);
   if (p.blocks >= (1u << 24) || uint64_t(max_new) * q->heads >= (1ull << 31))
     return fail(S14_ERR_SHAPE, "%u new tokens of %u sequences exceed one launch", max_new, seqs);
-  a.status = s14::ctx_status(ctx);
+  a.status = s14::ctx_status(ctx), a.count = s14::ctx_attn_counters(ctx);
   const OnDevice on(s14::ctx_device(ctx));
   if (on.error() != hipSuccess) return hip_fail(on.error(), "hipSetDevice");
   float *part = nullptr;

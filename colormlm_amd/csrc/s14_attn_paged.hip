@@ -105,6 +105,111 @@ struct Pages {
 template <int D>
 constexpr uint32_t kRecord = D + 4;
 
+// Where the chunks of a row are joined.  A second launch costs about 4 us, its
+// workgroups share the rows; the workgroup that arrives last at a (row tile,
+// sequence, key head) does it at once, but reads all its partial results
+// alone: the plan fuses where those are few (PagedPlan::fused).
+//
+// The last one sees the others' results, across the XCDs, because they are
+// written through to the device's coherence point (agent scope, sc1), each
+// wavefront waits for its stores before the barrier that precedes the count,
+// and they are read from there.  A release fence would write back the L2.
+constexpr int kAgent = 0x10;  // buffer cache policy: sc1
+
+struct PartStore {
+  __amdgpu_buffer_rsrc_t r;
+  uint32_t fused;
+  float *p;
+  __device__ __forceinline__ PartStore(float *rec, uint32_t floats, uint32_t fused) : fused(fused), p(rec) {
+    r = __builtin_amdgcn_make_buffer_rsrc(rec, 0, int(floats * 4), 0x00020000);
+  }
+  __device__ __forceinline__ void operator()(uint32_t at, f32x4 v) const {
+    if (fused)
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at * 4, 0, kAgent);
+    else
+      *reinterpret_cast<f32x4 *>(p + at) = v;
+  }
+};
+
+// Counts this workgroup's arrival; true in every thread of the last one.
+__device__ __forceinline__ bool arrived_last(uint32_t *count, uint32_t chunks) {
+  __shared__ uint32_t s_last;
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's stores are done
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const bool last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == chunks;
+    if (last) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
+    s_last = last;
+  }
+  __syncthreads();
+  return s_last != 0;
+}
+
+// A tile's rows from their partial results, a row a wavefront at a time: lane
+// c holds chunk c's maximum and sum (64 chunks at most), then the chunks' rows
+// in order.
+template <int D>
+__device__ __forceinline__ void join_tile(const PagedArgs &a, const PagedPlan &p, const Span &sp, const Item &it,
+                                          uint32_t row0, const float *part) {
+  constexpr uint32_t kLanes = D / 4 < 64 ? D / 4 : 64, kSpan = D / (4 * kLanes), kSets = 64 / kLanes;
+  const uint32_t kvh = a.cache.heads, group = a.heads / kvh, l = threadIdx.x & 63u;
+  const uint32_t lane = l % kLanes, set = l / kLanes;
+  const uint64_t rec = uint64_t(p.rec_rows) * kRecord<D>;
+  const uint32_t next = uint32_t(uint64_t(kvh) * a.seqs * rec * 4);  // bytes to the next chunk's record
+  const float *first = part + record_of(a, p, Item{it.tile, 0, it.seq, it.head}, kvh) * rec;
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(first), 0,
+                                                   int((sp.chunks - 1) * next + uint32_t(rec) * 4), 0x00020000);
+  for (uint32_t k = threadIdx.x / 64; k < p.rec_rows && row0 + k < sp.rows; k += 4) {
+    const uint32_t at = k * kRecord<D> * 4;
+    float m = -INFINITY, sum = 0.0f;
+    if (l < sp.chunks) {
+      const auto ml = __builtin_amdgcn_raw_buffer_load_b64(r, l * next + at + D * 4, 0, kAgent);
+      m = __uint_as_float(ml[0]), sum = __uint_as_float(ml[1]);
+    }
+    float top = m;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float w = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));  // 0 in lanes without a chunk
+    float total = sum * w;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
+    f32x4 o[kSpan] = {};
+    for (uint32_t c0 = 0; c0 < sp.chunks; c0 += 4 * kSets) {
+      u32x4 x[4][kSpan];
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j)
+#pragma unroll
+        for (uint32_t i = 0; i < kSpan; ++i)  // past the last chunk: zeros (descriptor range), weight 0
+          x[j][i] = __builtin_amdgcn_raw_buffer_load_b128(
+              r, (c0 + j * kSets + set) * next + at + 16 * (lane + kLanes * i), 0, kAgent);
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        const float f = __shfl(w, int((c0 + j * kSets + set) & 63u));
+#pragma unroll
+        for (uint32_t i = 0; i < kSpan; ++i) o[i] += __builtin_bit_cast(f32x4, x[j][i]) * f;
+      }
+    }
+#pragma unroll
+    for (uint32_t d = kLanes; d < 64; d <<= 1)
+#pragma unroll
+      for (uint32_t i = 0; i < kSpan; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] += __shfl_xor(o[i][e], int(d));
+    const uint32_t row = row0 + k;
+    const uint64_t t = uint64_t(sp.first + row / group);
+    const uint32_t h = it.head * group + row % group;
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    if (set == 0) {
+#pragma unroll
+      for (uint32_t i = 0; i < kSpan; ++i) {
+        const f32x4 y = o[i] * inv;
+        store_out(a.out, t * a.out.token + uint64_t(h) * a.out.head + 4 * (lane + kLanes * i), y[0], y[1], y[2], y[3]);
+      }
+    }
+    if (a.lse && l == 0) a.lse[t * a.heads + h] = total == 0.0f ? -INFINITY : top * kLn2 + __logf(total);
+  }
+}
+
 // The top bit of each byte that is a NaN code (0x7f, 0xff).
 __device__ __forceinline__ uint32_t nan_codes(uint32_t c) { return ((c & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
@@ -366,9 +471,8 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
     }
     __syncthreads();
   }
-  if (wave) return;
-
   if (sp.chunks <= 1) {
+    if (wave) return;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const uint32_t r = row0 + 16 * nt + n;
@@ -384,17 +488,20 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
     }
     return;
   }
-  float *rec = part + record_of(a, p, it, kvh) * (p.rec_rows * kRecord<D>);
+  if (wave == 0) {
+    const uint32_t floats = p.rec_rows * kRecord<D>;
+    const PartStore store(part + record_of(a, p, it, kvh) * floats, floats, p.fused);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    if (16 * nt + n >= p.rec_rows) continue;
-    float *row = rec + (16 * nt + n) * kRecord<D>;
-    if (g == 0) row[D] = m[nt], row[D + 1] = sum[nt];
+    for (int nt = 0; nt < NT; ++nt) {
+      if (16 * nt + n >= p.rec_rows) continue;
+      const uint32_t row = (16 * nt + n) * kRecord<D>;
+      if (g == 0) store(row + D, f32x4{m[nt], sum[nt], 0.0f, 0.0f});
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      *reinterpret_cast<f32x4 *>(row + 16 * dt + 4 * g) = o[nt][dt];
+      for (int dt = 0; dt < DT; ++dt) store(row + 16 * dt + 4 * g, o[nt][dt]);
     }
   }
+  if (!p.fused) return;
+  if (arrived_last(a.count + (tile * a.seqs + seq) * kvh + head, sp.chunks)) join_tile<D>(a, p, sp, it, row0, part);
 }
 
 // Heads of 512 (one wide key head for many query heads): 16 NT rows of Q and O
@@ -624,17 +731,18 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
     if (g == 0) s_m[wave][n] = m, s_l[wave][n] = sum;
   }
   __syncthreads();
-  float *rec = part + record_of(a, p, it, kvh) * (p.rec_rows * kRecord<D>);
+  const uint32_t floats = p.rec_rows * kRecord<D>;
+  const PartStore store(part + record_of(a, p, it, kvh) * floats, floats, p.fused);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const uint32_t r = row0 + 16 * nt + n;
     if (r >= sp.rows) continue;
     const float top = s_m[nt][n], total = s_l[nt][n];
     if (sp.chunks > 1) {
-      float *row = rec + (16 * nt + n) * kRecord<D>;
-      if (wave == 0 && g == 0) row[D] = top, row[D + 1] = total;
+      const uint32_t row = (16 * nt + n) * kRecord<D>;
+      if (wave == 0 && g == 0) store(row + D, f32x4{top, total, 0.0f, 0.0f});
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4 *>(row + d0 + 16 * dt + 4 * g) = o[nt][dt];
+      for (int dt = 0; dt < DT; ++dt) store(row + d0 + 16 * dt + 4 * g, o[nt][dt]);
       continue;
     }
     const uint64_t t = uint64_t(sp.first + r / group);
@@ -646,6 +754,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
                 o[nt][dt][1] * inv, o[nt][dt][2] * inv, o[nt][dt][3] * inv);
     if (a.lse && wave == 0 && g == 0) a.lse[t * a.heads + h] = total == 0.0f ? -INFINITY : top * kLn2 + __logf(total);
   }
+  if (sp.chunks <= 1 || !p.fused) return;
+  if (arrived_last(a.count + (tile * a.seqs + seq) * kvh + head, sp.chunks)) join_tile<D>(a, p, sp, it, row0, part);
 }
 
 // Joins the chunks of one row a workgroup, in an order that its size alone
@@ -706,7 +816,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, PagedPlan p, co
 template <class Kernel, class Join>
 hipError_t launch(hipStream_t s, const PagedArgs &a, const PagedPlan &p, float *part, Kernel kernel, Join join) {
   kernel<<<uint32_t(p.blocks), 256, 0, s>>>(a, p, part);
-  if (p.chunks > 1) {
+  if (p.chunks > 1 && !p.fused) {
     const uint32_t rows = uint32_t(a.max_new) * (a.heads / a.cache.heads);
     join<<<dim3(rows, a.seqs, a.cache.heads), 256, 0, s>>>(a, p, part);
   }
@@ -729,9 +839,19 @@ hipError_t launch_dim(hipStream_t s, const PagedArgs &a, const PagedPlan &p, flo
 }  // namespace
 
 // Rows a wavefront holds: as many 16-row tiles as the longest new block fills
-// and the registers of the head size leave room for (64 rows of 128, 32 of
-// 256, 16 of 512).  Chunks: enough workgroups to fill the card where there
-// are few rows, none below a step.
+// and the registers of the head size leave room for (64 rows of 128, 32 of 256,
+// and of 512 by quarters of the head).
+//
+// Chunks.  Where the launch alone would leave compute units idle: as many
+// workgroups as the card holds at once (a second round for a few of them costs
+// as much as the first), of several sequences twice as many, since their
+// lengths differ and short ones leave chunks empty (us, once / twice: 16
+// sequences of up to 8,192 tokens 36 / 29 ragged, 55 / 55 equal; 4 of up to
+// 9,000, 64 heads of 512, 49 / 37 and 56 / 72).  Where it fills the card:
+// chunks of 2,048 tokens, so that one long sequence does not outlast the rest.
+// A row tile whose partial results stay within 64 KB is joined by its last
+// workgroup (1 token of 4,097: 12.4 us with a second launch, 10.4 without; 32
+// rows of 31 chunks, 1 MB: 25 and 42).
 PagedPlan paged_plan(const PagedArgs &a) {
   PagedPlan p{};
   const uint64_t rows = uint64_t(a.max_new) * (a.heads / a.cache.heads);
@@ -745,16 +865,11 @@ PagedPlan paged_plan(const PagedArgs &a) {
     // workgroups that the card holds at once, by the registers of a wavefront
   const uint32_t words = (dim == 512 ? 128 : dim) * p.row_tiles;
   const uint64_t slots = 256 * (words <= 64 ? 3 : words <= 128 || dim == 512 ? 2 : 1);
-  uint64_t base_slots = slots;
   const uint64_t least = dim == 512 ? 64 : 256;  // a step of every wavefront
-  constexpr uint64_t kMost = 2048;
+  constexpr uint64_t kMost = 2048, kFuse = 64 * 1024;
   p.rec_rows = uint32_t(rows < 16 * p.row_tiles ? rows : 16 * p.row_tiles);
   const uint64_t rec = uint64_t(p.rec_rows) * (dim + 4);
-#ifndef KX
-#define KX 1
-#endif
-  if (a.seqs > 1) base_slots = slots * KX;
-  uint64_t chunks = base < slots ? base_slots / base : (span + kMost - 1) / kMost;
+  uint64_t chunks = base < slots ? slots * (a.seqs > 1 ? 2 : 1) / base : (span + kMost - 1) / kMost;
   const uint64_t fit = kPagedPartFloats / (rec * base);
   if (chunks > fit) chunks = fit;
   if (chunks > (span + least - 1) / least) chunks = (span + least - 1) / least;
@@ -762,6 +877,8 @@ PagedPlan paged_plan(const PagedArgs &a) {
   p.chunk = uint32_t(((span + chunks - 1) / chunks + least - 1) / least * least);
   p.chunks = span ? uint32_t((span + p.chunk - 1) / p.chunk) : 1;
   p.blocks = base * p.chunks;
+  p.fused = p.chunks > 1 && p.chunks <= 64 && base <= kPagedCounters && rec * 4 * p.chunks <= kFuse &&
+            rec * 4 * p.chunks * a.seqs * a.cache.heads < (1ull << 31);
   return p;
 }
 

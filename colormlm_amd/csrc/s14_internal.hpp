@@ -37,6 +37,9 @@ int read_launch_status(const Workspace &ws, int device);
 int ctx_device(const s14_ctx *ctx);
 // Its device status word (kStatus* bits).
 uint32_t *ctx_status(const s14_ctx *ctx);
+// Its arrival counters of split paged attentions (kPagedCounters), made and
+// zeroed with the context: a first call under capture finds them ready.
+uint32_t *ctx_attn_counters(const s14_ctx *ctx);
 // Its workspace for a split paged attention's partial results, allocated on
 // the first call (always the same `bytes`), on the current device.
 int ctx_attn_workspace(s14_ctx *ctx, uint64_t bytes, float **out);
