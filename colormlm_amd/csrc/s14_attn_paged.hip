@@ -335,13 +335,16 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float x[4 * T];
-      float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 4 * T; ++i) {
-        x[i] = s[nt][i / 4][i % 4] * ks;
-        if (partial) x[i] = see[nt](tv + i) ? x[i] : -INFINITY;
-        top = fmaxf(top, x[i]);
+      for (int i = 0; i < 4 * T; ++i) x[i] = s[nt][i / 4][i % 4] * ks;
+      if (partial) {
+        keep_branch();
+#pragma unroll
+        for (int i = 0; i < 4 * T; ++i) x[i] = see[nt](tv + i) ? x[i] : -INFINITY;
       }
+      float top = x[0];
+#pragma unroll
+      for (int i = 1; i < 4 * T; ++i) top = fmaxf(top, x[i]);
       top = fmaxf(m[nt], max_lane16(top));
       // the maximum that the weights are taken from moves only where they
       // would pass 2^kRise: O is seldom multiplied
@@ -617,17 +620,20 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
     __syncthreads();
     if (softmax) {
       float x[4 * T];
-      float top = -INFINITY;
 #pragma unroll
       for (int t = 0; t < T; ++t) {
         const f32x4 s = s_part[0][wave][t][l] + s_part[1][wave][t][l] + s_part[2][wave][t][l] + s_part[3][wave][t][l];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[4 * t + i] = s[i] * ks;
-          if (partial) x[4 * t + i] = see(tv + 4 * t + i) ? x[4 * t + i] : -INFINITY;
-          top = fmaxf(top, x[4 * t + i]);
-        }
+        for (int i = 0; i < 4; ++i) x[4 * t + i] = s[i] * ks;
       }
+      if (partial) {
+        keep_branch();
+#pragma unroll
+        for (int i = 0; i < 4 * T; ++i) x[i] = see(tv + i) ? x[i] : -INFINITY;
+      }
+      float top = x[0];
+#pragma unroll
+      for (int i = 1; i < 4 * T; ++i) top = fmaxf(top, x[i]);
       top = fmaxf(m, max_lane16(top));
       float fade = 1.0f;
       if (__any(top > m + kRise)) {

@@ -11,7 +11,7 @@
 // transposing LDS read gives: P stays in registers.
 //
 // LDS rows are D values in 16-byte pieces, piece c of row r at place c ^
-// swizzle(r), so that neither read of eight rows meets a bank twice.
+// swizzle(r), so that neither read meets a bank twice.
 #include "s14_attn.hpp"
 #include "s14_attn_util.hpp"
 
@@ -63,14 +63,18 @@ __device__ __forceinline__ bool find_block(const PromptArgs &a, uint32_t index, 
   return false;
 }
 
-template <int D>
+// K: sixteen neighbouring rows' pieces of one number, the first product's
+// read, are in different banks.  V: so are the pieces of four rows and 32
+// dimensions, which half a wavefront reads for the second.
+template <int D, bool kV>
 __device__ __forceinline__ uint32_t swizzle(uint32_t row) {
-  return D == 64 ? ((row >> 1) & 3u) * 2u : (row & 7u) * 2u;
+  if (kV) return D == 64 ? (row & 2u) * 2u : (row & 3u) * 4u;
+  return D == 64 ? (row >> 1) & 7u : row & 15u;
 }
 
 // KT rows of D values from `base` (rows `stride` >= 2 D bytes apart, `valid`
 // >= 1 of them there: the rest become zeros) into LDS.
-template <int D, int KT>
+template <int D, int KT, bool kV>
 __device__ __forceinline__ void stage(const uint16_t *base, uint32_t stride, int32_t valid, uint16_t *lds) {
   constexpr uint32_t kPieces = D / 8, kPasses = KT * kPieces / 256;
   const uint32_t rows = valid < KT ? uint32_t(valid) : uint32_t(KT);
@@ -82,7 +86,7 @@ __device__ __forceinline__ void stage(const uint16_t *base, uint32_t stride, int
   // them; the wait at the head of the next tile does.
 #pragma unroll
   for (uint32_t i = 0; i < kPasses; ++i) {
-    const uint32_t at = i * 256 + threadIdx.x, row = at / kPieces, piece = (at % kPieces) ^ swizzle<D>(row);
+    const uint32_t at = i * 256 + threadIdx.x, row = at / kPieces, piece = (at % kPieces) ^ swizzle<D, kV>(row);
     const uint32_t wave_at = __builtin_amdgcn_readfirstlane(to + (i * 256 + (threadIdx.x & ~63u)) * 16);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(wave_at),
                  "v"(row * stride + piece * 16), "s"(r)
@@ -143,21 +147,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(Prom
   constexpr int KA = KS < 8 ? KS : 8, VA = DT < 4 ? DT : 4;
   uint32_t k_at[KA], v_at[VA];
 #pragma unroll
-  for (int k = 0; k < KA; ++k) k_at[k] = n * (2 * D) + ((2 * k + h) ^ swizzle<D>(n)) * 16;
+  for (int k = 0; k < KA; ++k) k_at[k] = n * (2 * D) + ((2 * k + h) ^ swizzle<D, false>(n)) * 16;
   const uint32_t v_row = 4 * h + (l & 15u) / 4;
 #pragma unroll
   for (int dt = 0; dt < VA; ++dt)
-    v_at[dt] = v_row * (2 * D) + ((4 * dt + ((l >> 4) & 1u) * 2 + ((l & 3u) >> 1)) ^ swizzle<D>(v_row)) * 16 + (l & 1u) * 8;
+    v_at[dt] = v_row * (2 * D) + ((4 * dt + ((l >> 4) & 1u) * 2 + ((l & 3u) >> 1)) ^ swizzle<D, true>(v_row)) * 16 + (l & 1u) * 8;
 
-  stage<D, KT>(kb + uint64_t(lo) * a.k_token, ks, blk.len - lo, lds_k[0]);
-  stage<D, KT>(vb + uint64_t(lo) * a.v_token, vs, blk.len - lo, lds_v[0]);
+  stage<D, KT, false>(kb + uint64_t(lo) * a.k_token, ks, blk.len - lo, lds_k[0]);
+  stage<D, KT, true>(vb + uint64_t(lo) * a.v_token, vs, blk.len - lo, lds_v[0]);
   uint32_t buf = 0;
   for (int32_t b = lo; b < hi; b += KT, buf ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (b + KT < hi) {
-      stage<D, KT>(kb + uint64_t(b + KT) * a.k_token, ks, blk.len - b - KT, lds_k[buf ^ 1]);
-      stage<D, KT>(vb + uint64_t(b + KT) * a.v_token, vs, blk.len - b - KT, lds_v[buf ^ 1]);
+      stage<D, KT, false>(kb + uint64_t(b + KT) * a.k_token, ks, blk.len - b - KT, lds_k[buf ^ 1]);
+      stage<D, KT, true>(vb + uint64_t(b + KT) * a.v_token, vs, blk.len - b - KT, lds_v[buf ^ 1]);
     }
     if (b > wpos_hi || (a.window && int64_t(b) + KT - 1 <= int64_t(wpos_lo) - a.window)) continue;
     const auto *lk = (const __attribute__((address_space(3))) uint8_t *)lds_k[buf];
@@ -175,13 +179,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(Prom
     }
     const bool partial = b + KT - 1 > wpos_lo || (a.window && int64_t(b) <= int64_t(wpos_hi) - a.window);
     float x[16 * ST];
-    float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 16 * ST; ++i) {
-      x[i] = s[i / 16][i % 16];
-      if (partial) x[i] = see(b + 8 * (i / 4) + 4 * int32_t(h) + i % 4) ? x[i] : -INFINITY;
-      top = fmaxf(top, x[i]);
+    for (int i = 0; i < 16 * ST; ++i) x[i] = s[i / 16][i % 16];
+    if (partial) {
+      keep_branch();
+#pragma unroll
+      for (int i = 0; i < 16 * ST; ++i) x[i] = see(b + 8 * (i / 4) + 4 * int32_t(h) + i % 4) ? x[i] : -INFINITY;
     }
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < 16 * ST; ++i) top = fmaxf(top, x[i]);
     {
       const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
       top = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));

@@ -48,6 +48,10 @@ struct Visible {
   __device__ __forceinline__ bool operator()(int32_t j) const { return uint32_t(j - base) < count; }
 };
 
+// Inside a uniform branch: it stays one.  (A mask's selects are otherwise done
+// in every step, taken or not: a third of the softmax's instructions.)
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
+
 // The result of a max or sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float max_lane16(float v) {
   auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
