@@ -12,6 +12,8 @@
 //
 // LDS rows are D values in 16-byte pieces, piece c of row r at place c ^
 // swizzle(r), so that neither read meets a bank twice.
+#include <type_traits>
+
 #include "s14_attn.hpp"
 #include "s14_attn_util.hpp"
 
@@ -72,24 +74,27 @@ __device__ __forceinline__ uint32_t swizzle(uint32_t row) {
   return D == 64 ? (row >> 1) & 7u : row & 15u;
 }
 
+__device__ __forceinline__ uint32_t lds_at(const void *p) { return uint32_t(reinterpret_cast<uintptr_t>((lds_void *)p)); }
+
 // KT rows of D values from `base` (rows `stride` >= 2 D bytes apart, `valid`
 // >= 1 of them there: the rest become zeros) into LDS.
 template <int D, int KT, bool kV>
 __device__ __forceinline__ void stage(const uint16_t *base, uint32_t stride, int32_t valid, uint16_t *lds) {
-  constexpr uint32_t kPieces = D / 8, kPasses = KT * kPieces / 256;
+  constexpr uint32_t kPieces = D / 8, kPasses = KT * kPieces / 256, kRows = 256 / kPieces;  // rows a pass
   const uint32_t rows = valid < KT ? uint32_t(valid) : uint32_t(KT);
-  const uint64_t at0 = reinterpret_cast<uint64_t>(base);
-  const u32x4 r = {uint32_t(at0), uint32_t(at0 >> 32), (rows - 1) * stride + 2 * D, 0x00020000u};
-  const uint32_t to = uint32_t(reinterpret_cast<uintptr_t>((lds_void *)lds));
+  const uint32_t to = lds_at(lds) + (threadIdx.x & ~63u) * 16;
   // In asm: the compiler would let every LDS read wait for these loads, whose
   // halves of the double buffer it cannot tell apart.  No register waits for
   // them; the wait at the head of the next tile does.
 #pragma unroll
   for (uint32_t i = 0; i < kPasses; ++i) {
-    const uint32_t at = i * 256 + threadIdx.x, row = at / kPieces, piece = (at % kPieces) ^ swizzle<D, kV>(row);
-    const uint32_t wave_at = __builtin_amdgcn_readfirstlane(to + (i * 256 + (threadIdx.x & ~63u)) * 16);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(wave_at),
-                 "v"(row * stride + piece * 16), "s"(r)
+    const uint32_t in = threadIdx.x / kPieces, piece = (threadIdx.x % kPieces) ^ swizzle<D, kV>(i * kRows + in);
+    const uint64_t at = reinterpret_cast<uint64_t>(base) + uint64_t(i * kRows) * stride;
+    const u32x4 r = {uint32_t(at), uint32_t(at >> 32), rows > i * kRows ? (rows - i * kRows - 1) * stride + 2 * D : 0u,
+                     0x00020000u};
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
+                     __builtin_amdgcn_readfirstlane(to) + i * 4096),
+                 "v"(in * stride + piece * 16), "s"(r)
                  : "memory");
   }
 }
@@ -99,10 +104,10 @@ __device__ __forceinline__ uint32_t odd_halves(uint32_t w) {  // 0x8000 in each 
   return ((e + 0x00800080u) & 0x80008000u);
 }
 
-template <int D, int KT>
+template <int D, int KT, bool kWindow>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(PromptArgs a) {
   constexpr int KS = D / 16, DT = D / 32, ST = KT / 32, U = KT / 16;
-  __shared__ __align__(16) uint16_t lds_k[2][KT * D], lds_v[2][KT * D];
+  __shared__ __align__(1024) uint16_t lds_k[2][KT * D], lds_v[2][KT * D];
   const uint32_t group = a.heads / a.kv_heads, head = blockIdx.x % a.kv_heads;
   Block blk;
   if (!find_block(a, blockIdx.x / a.kv_heads, group, blk)) return;
@@ -112,7 +117,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(Prom
 
   const uint64_t r = wrow + n < rows ? wrow + n : rows - 1;
   const int32_t pos = int32_t(r / group);
-  const Visible see(pos, a.window);
+  const uint32_t window = kWindow ? a.window : 0u;
+  const Visible see(pos, window);
   bf16x8 q[KS];
   {
     const uint16_t *row = a.q + uint64_t(blk.first + pos) * a.q_token +
@@ -128,74 +134,94 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(Prom
   const uint64_t blk_last = (blk.row0 + kPromptRows < rows ? blk.row0 + kPromptRows : rows) - 1;
   const int32_t hi = int32_t(blk_last / group) + 1;
   const int32_t blk_first = int32_t(blk.row0 / group);
-  const int32_t lo = a.window && blk_first + 1 > int64_t(a.window) ? (blk_first + 1 - int32_t(a.window)) & ~(KT - 1) : 0;
+  const int32_t lo = kWindow && blk_first + 1 > int64_t(window) ? (blk_first + 1 - int32_t(window)) & ~(KT - 1) : 0;
   const bool live = wrow < rows;
   const int32_t wpos_lo = int32_t(wrow / group);
   const int32_t wpos_hi = live ? int32_t((wrow + 31 < rows ? wrow + 31 : rows - 1) / group) : -1;
 
+  const int32_t last = live ? wpos_hi & ~(KT - 1) : -1;  // this wavefront's last tile
+  const auto is_partial = [&](int32_t b) {
+    return b + KT - 1 > wpos_lo || (kWindow && int64_t(b) <= int64_t(wpos_hi) - window);
+  };
+
   f32x16 o[DT] = {};
-  float m = -INFINITY, sum = 0.0f;
   bool odd = false;
   const float scale = a.scale * kLog2e;
   const uint16_t *kb = a.k + uint64_t(blk.first) * a.k_token + uint64_t(head) * a.k_head;
   const uint16_t *vb = a.v + uint64_t(blk.first) * a.v_token + uint64_t(head) * a.v_head;
   const uint32_t ks = uint32_t(a.k_token * 2), vs = uint32_t(a.v_token * 2);
 
-  // This lane's places in an LDS tile, the rest of a read's address being a
-  // constant: the pieces of its K row (rows 32 apart have the same swizzle),
-  // and its part of a V row for the transposing read (rows 8 apart).
-  constexpr int KA = KS < 8 ? KS : 8, VA = DT < 4 ? DT : 4;
-  uint32_t k_at[KA], v_at[VA];
-#pragma unroll
-  for (int k = 0; k < KA; ++k) k_at[k] = n * (2 * D) + ((2 * k + h) ^ swizzle<D, false>(n)) * 16;
+  // This lane's places in an LDS tile: piece h of its K row, from which the
+  // others are an exclusive or away (rows 32 apart: a constant), and its part
+  // of a V row for the transposing read (dimensions 32 apart: an exclusive or,
+  // rows 8 apart: a constant).
+  const uint32_t k_at = n * (2 * D) + (h ^ swizzle<D, false>(n)) * 16;
   const uint32_t v_row = 4 * h + (l & 15u) / 4;
-#pragma unroll
-  for (int dt = 0; dt < VA; ++dt)
-    v_at[dt] = v_row * (2 * D) + ((4 * dt + ((l >> 4) & 1u) * 2 + ((l & 3u) >> 1)) ^ swizzle<D, true>(v_row)) * 16 + (l & 1u) * 8;
+  const uint32_t v_at = v_row * (2 * D) + ((((l >> 4) & 1u) * 2 + ((l & 3u) >> 1)) ^ swizzle<D, true>(v_row)) * 16 + (l & 1u) * 8;
 
-  stage<D, KT, false>(kb + uint64_t(lo) * a.k_token, ks, blk.len - lo, lds_k[0]);
-  stage<D, KT, true>(vb + uint64_t(lo) * a.v_token, vs, blk.len - lo, lds_v[0]);
-  uint32_t buf = 0;
-  for (int32_t b = lo; b < hi; b += KT, buf ^= 1) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (b + KT < hi) {
-      stage<D, KT, false>(kb + uint64_t(b + KT) * a.k_token, ks, blk.len - b - KT, lds_k[buf ^ 1]);
-      stage<D, KT, true>(vb + uint64_t(b + KT) * a.v_token, vs, blk.len - b - KT, lds_v[buf ^ 1]);
-    }
-    if (b > wpos_hi || (a.window && int64_t(b) + KT - 1 <= int64_t(wpos_lo) - a.window)) continue;
-    const auto *lk = (const __attribute__((address_space(3))) uint8_t *)lds_k[buf];
-    const auto *lv = (const __attribute__((address_space(3))) uint8_t *)lds_v[buf];
-
-    f32x16 s[ST];
+  // The scores of the tile to come are computed while this one's weights are:
+  // the first product's matrix instructions stand between the exponentials,
+  // in this order (left to itself the compiler puts one after the other).
+  float x[16 * ST];  // scores of the next tile to be weighted
+  bf16x8 pb[U];      // weights
+  float m = -INFINITY, sum = 0.0f;
+  constexpr int kAhead = 4;  // LDS reads this many matrix instructions ahead of their use
+  const auto step = [&](uint32_t buf, auto weigh, auto tail) {
+    constexpr int N = ST * KS, E = 16 * ST / N;  // matrix instructions, weights at each
+    const uint32_t lk = lds_at(lds_k[buf]) + k_at;
+    const auto k_frag = [&](int i) {
+      const int t = i % ST, k = i / ST;
+      return *(const __attribute__((address_space(3))) bf16x8 *)(uintptr_t)((lk ^ (32u * k)) + 64 * D * t);
+    };
+    f32x16 s[ST] = {};
+    bf16x8 kf[kAhead];
 #pragma unroll
-    for (int t = 0; t < ST; ++t) {
-      s[t] = f32x16{};
+    for (int i = 0; i < kAhead; ++i) kf[i] = k_frag(i);
+    const float at = m == -INFINITY ? 0.0f : m;
+    uint32_t w[4 * U];
+    float even = 0.0f;
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const bf16x8 kf = *(const __attribute__((address_space(3))) bf16x8 *)(lk + k_at[k % KA] + 64 * D * t + 32 * (k - k % KA));
-        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[k], s[t], 0, 0, 0);
+    for (int i = 0; i < N; ++i) {
+      s[i % ST] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % kAhead], q[i / ST], s[i % ST], 0, 0, 0);
+      if (i + kAhead < N)
+        kf[i % kAhead] = k_frag(i + kAhead);
+      else
+        tail(i + kAhead - N);
+      if constexpr (decltype(weigh)::value) {
+#pragma unroll
+        for (int e = i * E; e < (i + 1) * E; ++e) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], scale, -at));
+          sum += p;
+          if (e % 2) {
+            w[e / 2] = bf16_pair(even, p);  // half a step of each weight: the matrix operand's type
+            asm volatile("" : "+v"(w[e / 2]));
+          } else {
+            even = p;
+          }
+        }
+        asm volatile("" : "+v"(sum));  // here, not when it is needed: the weights' registers are
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-    const bool partial = b + KT - 1 > wpos_lo || (a.window && int64_t(b) <= int64_t(wpos_hi) - a.window);
-    float x[16 * ST];
+    if constexpr (decltype(weigh)::value) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) pb[u] = __builtin_bit_cast(bf16x8, u32x4{w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]});
+    }
 #pragma unroll
     for (int i = 0; i < 16 * ST; ++i) x[i] = s[i / 16][i % 16];
-    if (partial) {
+  };
+  // Hides what tile b's rows must not see.
+  const auto hide = [&](int32_t b) {
+    if (is_partial(b)) {
       keep_branch();
 #pragma unroll
       for (int i = 0; i < 16 * ST; ++i) x[i] = see(b + 8 * (i / 4) + 4 * int32_t(h) + i % 4) ? x[i] : -INFINITY;
     }
-    float top = x[0];
-#pragma unroll
-    for (int i = 1; i < 16 * ST; ++i) top = fmaxf(top, x[i]);
-    {
-      const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-      top = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
-    }
-    // The maximum that the weights are taken from moves only where they would
-    // pass 2^kRise: O is seldom multiplied.
-    top = fmaxf(m, top * scale);
+  };
+  // Moves the maximum, where the weights would pass 2^kRise: O is seldom multiplied.
+  const auto raise = [&](float top) {
+    const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+    top = fmaxf(m, fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])) * scale);
     if (__any(top > m + kRise)) {
       const float fade = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
       m = top;
@@ -203,47 +229,91 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(Prom
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] *= fade;
     }
-    const float at = m == -INFINITY ? 0.0f : m;
-    bf16x8 pb[U];
+  };
+  const auto largest = [&]() {
+    float top = x[0];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      u32x4 w;
+    for (int i = 1; i < 16 * ST; ++i) top = fmaxf(top, x[i]);
+    return top;
+  };
+
+  // At the head of tile b the LDS holds K of b + KT and V of b; K of b, whose
+  // scores are in registers, and V of b - KT give their places to the loads.
+  stage<D, KT, false>(kb + uint64_t(lo) * a.k_token, ks, blk.len - lo, lds_k[0]);
+  stage<D, KT, true>(vb + uint64_t(lo) * a.v_token, vs, blk.len - lo, lds_v[0]);
+  if (lo + KT < hi) stage<D, KT, false>(kb + uint64_t(lo + KT) * a.k_token, ks, blk.len - lo - KT, lds_k[1]);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (lo <= last) {
+    step(0, std::false_type{}, [](int) {});
+    hide(lo);
+    raise(largest());
+  }
+  uint32_t buf = 0;
+  int32_t b = lo;
+  const auto next_tile = [&]() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (b + 2 * KT < hi) stage<D, KT, false>(kb + uint64_t(b + 2 * KT) * a.k_token, ks, blk.len - b - 2 * KT, lds_k[buf]);
+    if (b + KT < hi) stage<D, KT, true>(vb + uint64_t(b + KT) * a.v_token, vs, blk.len - b - KT, lds_v[buf ^ 1]);
+  };
+  constexpr int N = DT * U;
+  bf16x8 vf[kAhead];
+  const auto v_frag = [&](int i) {
+    const int dt = i % DT, u = i / DT;
+    const uint32_t lv = lds_at(lds_v[buf]) + v_at;
+    union {
+      s16x4 x[2];
+      bf16x8 v;
+    } f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * u + 2 * j], scale, -at));
-        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * u + 2 * j + 1], scale, -at));
-        sum += e0;
-        sum += e1;
-        w[j] = bf16_pair(e0, e1);  // half a step of each weight: the matrix operand's type
-      }
-      pb[u] = __builtin_bit_cast(bf16x8, w);
+    for (int half = 0; half < 2; ++half)
+      f.x[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_s16x4 *)(uintptr_t)((lv ^ (64u * dt)) + (16 * u + 8 * half) * (2 * D)));
+    return f.v;
+  };
+  // (after the wavefront's last tile: scores of no tile, unused)
+  const auto weigh = [&]() { step(buf ^ 1, std::true_type{}, [&](int i) { vf[i] = v_frag(i); }); };
+  const auto add = [&]() {  // the second product; the largest of the next scores
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[i % kAhead], pb[i / DT], o[i % DT], 0, 0, 0);
+      if (i + kAhead < N) vf[i % kAhead] = v_frag(i + kAhead);
+#pragma unroll
+      for (int e = i * 16 * ST / N; e < (i + 1) * 16 * ST / N; e += 2) top[i % 2] = fmaxf(top[i % 2], fmaxf(x[e], x[e + 1]));
+      asm volatile("" : "+v"(top[i % 2]));
+      __builtin_amdgcn_sched_barrier(0);
     }
-    auto v_frag = [&](int dt, int u) {
-      union {
-        s16x4 x[2];
-        bf16x8 v;
-      } f;
+    return fmaxf(top[0], top[1]);
+  };
+  // Tiles that every row of the workgroup sees whole, and the next one too:
+  // the walk's bulk, without a branch, which would move O and x from registers
+  // to registers where its sides meet.
+  if constexpr (!kWindow) {
+    const int32_t whole = (blk_first + 1) & ~(KT - 1);  // tiles before this lie before every row
+    for (; b + 2 * KT <= whole; b += KT, buf ^= 1) {
+      next_tile();
+      weigh();
+      raise(add());
+    }
+  }
+  for (; b < hi; b += KT, buf ^= 1) {
+    next_tile();
+    if (b <= last) {
+      weigh();
+      hide(b + KT);
+      float top;
+      if (!is_partial(b)) {
+        top = add();
+      } else {
+        // An infinity or NaN in a V row that some rows must not see would reach
+        // them through 0 * inf: such values leave the product, and the rows that
+        // see them get them back below.
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
-        f.x[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s16x4 *)(lv + v_at[dt % VA] + (16 * u + 8 * half) * (2 * D) + 64 * (dt - dt % VA)));
-      return f.v;
-    };
-    if (!partial) {
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_frag(dt, u), pb[u], o[dt], 0, 0, 0);
-    } else {
-      // An infinity or NaN in a V row that some rows must not see would reach
-      // them through 0 * inf: such values leave the product, and the rows that
-      // see them get them back below.
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          u32x4 w = __builtin_bit_cast(u32x4, v_frag(dt, u));
+        for (int i = 0; i < N; ++i) {
+          u32x4 w = __builtin_bit_cast(u32x4, vf[i % kAhead]);
+          if (i + kAhead < N) vf[i % kAhead] = v_frag(i + kAhead);
           u32x4 t;
 #pragma unroll
           for (int j = 0; j < 4; ++j) t[j] = odd_halves(w[j]);
@@ -251,14 +321,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(Prom
             odd = true;
             w &= ~(t | (t - (t >> 15)));  // 0x8000 in a half becomes 0xffff
           }
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb[u], o[dt], 0, 0, 0);
+          o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb[i / DT], o[i % DT], 0, 0, 0);
         }
+        top = largest();
+      }
+      if (b < last) raise(top);
     }
   }
 
   if (odd) {  // uniform, and rare: one token after the other
     for (int32_t b = lo; b <= wpos_hi; b += KT) {
-      if (b + KT - 1 <= wpos_lo && !(a.window && int64_t(b) <= int64_t(wpos_hi) - a.window)) continue;
+      if (!is_partial(b)) continue;
       for (int32_t j = b; j < min(b + KT, wpos_hi + 1); ++j) {
         const uint16_t *row = vb + uint64_t(j) * a.v_token + 4 * h;
         const bool in = see(j);
@@ -306,10 +379,11 @@ hipError_t launch_prompt_attention(hipStream_t s, const PromptArgs &a) {
   const uint32_t group = a.heads / a.kv_heads;
   const uint64_t blocks = (uint64_t(a.tokens) * group + kPromptRows - 1) / kPromptRows + a.seqs;
   const uint32_t grid = uint32_t(blocks * a.kv_heads);
+  const auto launch = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(a); };
   switch (a.dim) {
-    case 64: k_prompt_attention<64, 64><<<grid, 256, 0, s>>>(a); break;
-    case 128: k_prompt_attention<128, 64><<<grid, 256, 0, s>>>(a); break;
-    case 256: k_prompt_attention<256, 32><<<grid, 256, 0, s>>>(a); break;
+    case 64: a.window ? launch(k_prompt_attention<64, 64, true>) : launch(k_prompt_attention<64, 64, false>); break;
+    case 128: a.window ? launch(k_prompt_attention<128, 64, true>) : launch(k_prompt_attention<128, 64, false>); break;
+    case 256: a.window ? launch(k_prompt_attention<256, 32, true>) : launch(k_prompt_attention<256, 32, false>); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
