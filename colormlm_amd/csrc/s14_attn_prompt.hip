@@ -119,27 +119,26 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(Prom
   const int32_t pos = int32_t(r / group);
   const uint32_t window = kWindow ? a.window : 0u;
   const Visible see(pos, window);
-  bf16x8 q[KS];
-  {
-    const uint16_t *row = a.q + uint64_t(blk.first + pos) * a.q_token +
-                          uint64_t(head * group + uint32_t(r % group)) * a.q_head;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const bf16x8 *>(row + 16 * k + 8 * h);
-    // Q is here before any tile is asked for: its first use, in the loop,
-    // would otherwise wait for every load in flight, each time round
-#pragma unroll
-    for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(q[k]));
-  }
   // tokens that the workgroup, and this wavefront, walk
   const uint64_t blk_last = (blk.row0 + kPromptRows < rows ? blk.row0 + kPromptRows : rows) - 1;
   const int32_t hi = int32_t(blk_last / group) + 1;
   const int32_t blk_first = int32_t(blk.row0 / group);
   const int32_t lo = kWindow && blk_first + 1 > int64_t(window) ? (blk_first + 1 - int32_t(window)) & ~(KT - 1) : 0;
-  const bool live = wrow < rows;
-  const int32_t wpos_lo = int32_t(wrow / group);
-  const int32_t wpos_hi = live ? int32_t((wrow + 31 < rows ? wrow + 31 : rows - 1) / group) : -1;
+  // (a wavefront without rows takes the last one's part, and stores nothing)
+  const int32_t wpos_lo = int32_t((wrow < rows ? wrow : rows - 1) / group);
+  const int32_t wpos_hi = int32_t((wrow + 31 < rows ? wrow + 31 : rows - 1) / group);
 
-  const int32_t last = live ? wpos_hi & ~(KT - 1) : -1;  // this wavefront's last tile
+  bf16x8 q[KS];
+  const auto load_q = [&]() {
+    const uint16_t *row = a.q + uint64_t(blk.first + pos) * a.q_token +
+                          uint64_t(head * group + uint32_t(r % group)) * a.q_head;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const bf16x8 *>(row + 16 * k + 8 * h);
+    // Q is here before the walk: its first use, in the loop, would otherwise
+    // wait for every load in flight, each time round
+#pragma unroll
+    for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(q[k]));
+  };
   const auto is_partial = [&](int32_t b) {
     return b + KT - 1 > wpos_lo || (kWindow && int64_t(b) <= int64_t(wpos_hi) - window);
   };
@@ -242,13 +241,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(Prom
   stage<D, KT, false>(kb + uint64_t(lo) * a.k_token, ks, blk.len - lo, lds_k[0]);
   stage<D, KT, true>(vb + uint64_t(lo) * a.v_token, vs, blk.len - lo, lds_v[0]);
   if (lo + KT < hi) stage<D, KT, false>(kb + uint64_t(lo + KT) * a.k_token, ks, blk.len - lo - KT, lds_k[1]);
+  load_q();
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (lo <= last) {
-    step(0, std::false_type{}, [](int) {});
-    hide(lo);
-    raise(largest());
-  }
+  step(0, std::false_type{}, [](int) {});
+  hide(lo);
+  raise(largest());
   uint32_t buf = 0;
   int32_t b = lo;
   const auto next_tile = [&]() {
@@ -287,9 +285,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(Prom
     }
     return fmaxf(top[0], top[1]);
   };
-  // Tiles that every row of the workgroup sees whole, and the next one too:
-  // the walk's bulk, without a branch, which would move O and x from registers
-  // to registers where its sides meet.
+  // Tiles that every row of the workgroup sees whole: the walk's bulk, without
+  // a branch, which would move O and x from registers to registers where its
+  // sides meet.  (A window's walk is short and has a branch.)
   if constexpr (!kWindow) {
     const int32_t whole = (blk_first + 1) & ~(KT - 1);  // tiles before this lie before every row
     for (; b + 2 * KT <= whole; b += KT, buf ^= 1) {
@@ -297,42 +295,48 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(Prom
       weigh();
       raise(add());
     }
-  }
-  for (; b < hi; b += KT, buf ^= 1) {
-    next_tile();
-    if (b <= last) {
+    if (b + KT <= whole) {  // the last of them
+      next_tile();
       weigh();
       hide(b + KT);
-      float top;
-      if (!is_partial(b)) {
-        top = add();
-      } else {
-        // An infinity or NaN in a V row that some rows must not see would reach
-        // them through 0 * inf: such values leave the product, and the rows that
-        // see them get them back below.
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          u32x4 w = __builtin_bit_cast(u32x4, vf[i % kAhead]);
-          if (i + kAhead < N) vf[i % kAhead] = v_frag(i + kAhead);
-          u32x4 t;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) t[j] = odd_halves(w[j]);
-          if (__any((t[0] | t[1] | t[2] | t[3]) != 0)) {
-            odd = true;
-            w &= ~(t | (t - (t >> 15)));  // 0x8000 in a half becomes 0xffff
-          }
-          o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb[i / DT], o[i % DT], 0, 0, 0);
-        }
-        top = largest();
-      }
-      if (b < last) raise(top);
+      raise(add());
+      b += KT, buf ^= 1;
     }
+  }
+  const int32_t careful = b;
+  for (; b < hi; b += KT, buf ^= 1) {
+    next_tile();
+    weigh();
+    hide(b + KT);
+    float top;
+    if (kWindow && !is_partial(b)) {
+      top = add();
+    } else {
+      // An infinity or NaN in a V row that some rows must not see would reach
+      // them through 0 * inf: such values leave the product, and the rows that
+      // see them get them back below.
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        u32x4 w = __builtin_bit_cast(u32x4, vf[i % kAhead]);
+        if (i + kAhead < N) vf[i % kAhead] = v_frag(i + kAhead);
+        u32x4 t;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = odd_halves(w[j]);
+        if (__any((t[0] | t[1] | t[2] | t[3]) != 0)) {
+          odd = true;
+          w &= ~(t | (t - (t >> 15)));  // 0x8000 in a half becomes 0xffff
+        }
+        o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb[i / DT], o[i % DT], 0, 0, 0);
+      }
+      top = largest();
+    }
+    if (b + KT < hi) raise(top);
   }
 
   if (odd) {  // uniform, and rare: one token after the other
-    for (int32_t b = lo; b <= wpos_hi; b += KT) {
-      if (!is_partial(b)) continue;
-      for (int32_t j = b; j < min(b + KT, wpos_hi + 1); ++j) {
+    for (b = careful; b < hi; b += KT) {
+      if (kWindow && !is_partial(b)) continue;
+      for (int32_t j = b; j < min(b + KT, hi); ++j) {
         const uint16_t *row = vb + uint64_t(j) * a.v_token + 4 * h;
         const bool in = see(j);
 #pragma unroll

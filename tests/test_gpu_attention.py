@@ -664,6 +664,22 @@ def test_prompt_special_values_in_hidden_places(ctx):
         check_attention(out, None, want, f"special values, window {window}")
 
 
+@pytest.mark.parametrize("heads,dim", [(2, 128), (3, 64), (2, 256)])
+@pytest.mark.parametrize("window", [0, 90])
+def test_prompt_special_values_one_head_a_key(ctx, heads, dim, window):
+    """One query head a key head: a workgroup's rows are 128 tokens, and its
+    wavefronts see different tiles whole.  An odd value before, in and behind
+    each of them."""
+    say(f"prompt: odd values, heads={heads} dim={dim} window={window}")
+    g = gen(19)
+    q, k, v = (rand(g, 300, heads, dim, dtype=BF16) for _ in range(3))
+    for i, (pos, val) in enumerate([(5, math.inf), (64, math.nan), (70, -math.inf), (127, math.inf), (128, -math.inf),
+                                    (190, math.nan), (191, math.inf), (255, -math.inf), (299, math.inf)]):
+        v[pos, 0, 2 * i + 1] = val
+    out, lse = run_prompt(ctx, q.cuda(), k.cuda(), v.cuda(), [300], window)
+    check_attention(out, lse, prompt_want(q, k, v, [300], window), "odd values")
+
+
 @pytest.mark.parametrize("heads,kv,dim", [(4, 1, 128), (2, 2, 64), (2, 1, 256)])
 def test_prompt_long(ctx, heads, kv, dim):
     say(f"prompt of 2,900 tokens heads={heads}/{kv} dim={dim}: late rows against 64 bits, all against the cut form")
