@@ -186,10 +186,9 @@ class LoadingReservationC(C.Structure):
     ]
 
 
-class Rows(C.Structure):  # s14_rows, its s14_buffer's two members in place
+class Rows(C.Structure):
     _fields_ = [
-        ("ptr", C.c_void_p),
-        ("bytes", C.c_uint64),
+        ("buf", Buffer),
         ("dtype", C.c_int),
         ("heads", C.c_uint32),
         ("token_stride", C.c_uint64),

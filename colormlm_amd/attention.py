@@ -21,6 +21,7 @@ no counterpart.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 from dataclasses import dataclass
 from typing import Optional
 
@@ -31,9 +32,7 @@ from ._native import S14Error, check, lib
 from .s14 import Context
 
 PAGE_TOKENS = (16, 32, 64, 128)
-_DTYPES = {torch.float32: (N.S14_X_F32, 4), torch.bfloat16: (N.S14_X_BF16, 2)}
 _LAYOUTS = {"half": N.S14_ROPE_HALF, "interleaved": N.S14_ROPE_INTERLEAVED}
-_NO_BUFFER, _NO_ROWS = N.Buffer(None, 0), N.Rows()
 
 
 def _raw_stream():
@@ -43,52 +42,30 @@ def _raw_stream():
     return raw if raw is not None else lambda device: torch.cuda.current_stream(device).cuda_stream
 
 
-_RAW_STREAM = _raw_stream()
-
-
 def _refuse(code: int, message: str):
     raise S14Error(code, message)
 
 
-def _here(ctx: Context, t, label: str):
-    if not isinstance(t, torch.Tensor) or t.get_device() != ctx.device:
-        _refuse(N.S14_ERR_INVALID, f"{label} must be a tensor on the context's device {ctx.device}")
+def _load():
+    """The calls' C side (csrc/s14_attn_py.c) with the library's entry points."""
+    path = N.LIB_DIR / "_s14attn.so"
+    if not path.exists():
+        raise ImportError(f"{path} is not built; run `python -m colormlm_amd.build` (there is no fallback path)")
+    spec = importlib.util.spec_from_file_location("_s14attn", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    names = ("s14_qk_norm_rope", "s14_kv_append", "s14_paged_attention", "s14_prompt_attention")
+    module.bind(tuple(C.cast(getattr(lib(), n), C.c_void_p).value for n in names),
+                (torch.float32, torch.bfloat16, torch.int32), _refuse, check, _raw_stream())
+    return module
 
 
-def _rows(ctx: Context, t, label: str, dim: Optional[int] = None):
-    """The s14_rows of a [tokens, heads, dim] tensor.  (On the path of a
-    single token's calls: each tensor is asked for each property once.)"""
-    try:
-        code, size = _DTYPES[t.dtype]
-        tokens, heads, width = t.shape
-        token_stride, head_stride, one = t.stride()
-        if t.get_device() != ctx.device or (one != 1 and width > 1) or (dim is not None and width != dim):
-            raise ValueError
-    except (AttributeError, KeyError, ValueError):
-        _here(ctx, t, label)
-        if t.dtype not in _DTYPES:
-            _refuse(N.S14_ERR_INVALID, f"{label} must be float32 or bfloat16, not {t.dtype}")
-        _refuse(N.S14_ERR_SHAPE, f"{label} must be [tokens, heads, {dim or 'dim'}] with a contiguous last dimension")
-    # strides of a dimension of one are not used; what torch gives there may be anything
-    if tokens < 2:
-        token_stride = 0
-    if heads < 2:
-        head_stride = 0
-    reach = ((tokens - 1) * token_stride + (heads - 1) * head_stride + width) * size if tokens and heads else 0
-    return N.Rows(t.data_ptr(), reach, code, heads, token_stride, head_stride)
+_call = _load()
 
 
-def _flat(ctx: Context, t, dtype, label: str, size: int = 0):
-    """The buffer of a contiguous tensor of one dtype, of `size` values at least."""
-    if t is None:
-        return _NO_BUFFER
-    if not isinstance(t, torch.Tensor) or t.get_device() != ctx.device:
-        _here(ctx, t, label)
-    if t.dtype is not dtype or not t.is_contiguous():
-        _refuse(N.S14_ERR_INVALID, f"{label} must be a contiguous {dtype} tensor")
-    if size and t.numel() < size:
-        _refuse(N.S14_ERR_CAPACITY, f"{label} has {t.numel()} values, {size} are required")
-    return N.Buffer(t.data_ptr(), t.nbytes)
+def _here(device: int, t, label: str):
+    if not isinstance(t, torch.Tensor) or t.get_device() != device:
+        _refuse(N.S14_ERR_INVALID, f"{label} must be a tensor on the context's device {device}")
 
 
 class Rope:
@@ -106,14 +83,16 @@ class Rope:
         self.table, self.layout, self.start = table, layout, start
         self._c = N.Rope(N.Buffer(table.data_ptr(), table.nbytes), table.shape[0], table.shape[1], start,
                          _LAYOUTS[layout])
+        self._at, self._device = C.addressof(self._c), table.get_device()
 
 
 def _rope(ctx: Context, rope: Optional[Rope]):
+    """The address of a rotation's s14_rope on the context's device."""
     if rope is None:
         return None
-    if rope.table.get_device() != ctx.device:
-        _here(ctx, rope.table, "rotation table")
-    return C.byref(rope._c)
+    if rope._device != ctx.device:
+        _here(ctx.device, rope.table, "rotation table")
+    return rope._at
 
 
 @dataclass(frozen=True)
@@ -149,6 +128,7 @@ class KvCache:
         self.pages, self.heads, self.page_tokens, self.dim = pages, heads, page, dim
         buf = [N.Buffer(t.data_ptr(), t.nbytes) for t in (k_pages, v_pages, k_scales, v_scales)]
         self._c = N.KvCache(*buf, pages, heads, page, dim)
+        self._at, self._device = C.addressof(self._c), k_pages.get_device()
 
     @classmethod
     def empty(cls, pages: int, heads: int, page_tokens: int, dim: int, device="cuda") -> "KvCache":
@@ -159,22 +139,24 @@ class KvCache:
 
 
 def _cache(ctx: Context, cache: KvCache):
-    if cache.k_pages.get_device() != ctx.device:
-        _here(ctx, cache.k_pages, "cache")
-    return C.byref(cache._c)
+    if cache._device != ctx.device:
+        _here(ctx.device, cache.k_pages, "cache")
+    return cache._at
 
 
 def rope_table(ctx: Context, table, theta: float = 10000.0, scaling: Optional[RopeScaling] = None, stream=None) -> None:
     """Fill table (f32 [positions, rot]) with cos | sin of each position's
     rot / 2 angles, computed in 64 bits."""
-    buf = _flat(ctx, table, torch.float32, "rotation table")
-    if table.dim() != 2:
-        _refuse(N.S14_ERR_SHAPE, "a rotation table is [positions, rot]")
+    _here(ctx.device, table, "rotation table")
+    if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
+        _refuse(N.S14_ERR_SHAPE, "a rotation table is contiguous float32 [positions, rot]")
     s = None
     if scaling is not None:
         s = C.byref(N.RopeScaling(scaling.factor, scaling.original, scaling.beta_fast, scaling.beta_slow,
                                   scaling.amplitude))
-    check(lib().s14_rope_table(ctx._h, _RAW_STREAM(ctx.device) if stream is None else stream, table.shape[0], table.shape[1], theta, s, buf))
+    stream = _raw_stream()(ctx.device) if stream is None else stream
+    check(lib().s14_rope_table(ctx.handle, stream, table.shape[0], table.shape[1], theta, s,
+                               N.Buffer(table.data_ptr(), table.nbytes)))
 
 
 def qk_norm_rope(ctx: Context, q, k, q_out, k_out, q_weight=None, k_weight=None, eps: float = 1e-6,
@@ -182,29 +164,8 @@ def qk_norm_rope(ctx: Context, q, k, q_out, k_out, q_weight=None, k_weight=None,
     """Per-head RMS norm (where a weight is given) and rotation (where `rope`
     is) of q [tokens, heads, dim] and k (or None) in one launch, in f32; f32 or
     bf16 in and out, outputs may be their inputs."""
-    rq, ro = _rows(ctx, q, "q"), _rows(ctx, q_out, "q output")
-    tokens, _, dim = q.shape
-    if q_out.shape != q.shape:
-        _refuse(N.S14_ERR_SHAPE, "q output must have q's shape")
-    if k is None:
-        rk = ko = _NO_ROWS
-    else:
-        rk, ko = _rows(ctx, k, "k", dim), _rows(ctx, k_out, "k output", dim)
-        if k.shape[0] != tokens or k_out.shape != k.shape:
-            _refuse(N.S14_ERR_SHAPE, "k must have q's tokens, and k output k's shape")
-    check(lib().s14_qk_norm_rope(
-        ctx._h, _RAW_STREAM(ctx.device) if stream is None else stream, tokens, dim, C.byref(rq), C.byref(rk), C.byref(ro), C.byref(ko),
-        _flat(ctx, q_weight, torch.float32, "q norm weight"), _flat(ctx, k_weight, torch.float32, "k norm weight"),
-        eps, _rope(ctx, rope), _flat(ctx, positions, torch.int32, "positions")))
-
-
-def _table(ctx: Context, page_table, cu, lens, label: str):
-    """Buffers of the index tensors, sequences and table width."""
-    table = _flat(ctx, page_table, torch.int32, "page table")
-    if page_table.dim() != 2:
-        _refuse(N.S14_ERR_SHAPE, "a page table is [sequences, pages]")
-    seqs, width = page_table.shape
-    return table, width, _flat(ctx, cu, torch.int32, "cu", seqs + 1), _flat(ctx, lens, torch.int32, label, seqs), seqs
+    _call.qk_norm_rope(ctx._h.value, ctx.device, stream, q, k, q_out, k_out, q_weight, k_weight, eps, _rope(ctx, rope),
+                       positions)
 
 
 def kv_append(ctx: Context, cache: KvCache, k, v, page_table, cu, past, k_weight=None, eps: float = 1e-6,
@@ -213,15 +174,8 @@ def kv_append(ctx: Context, cache: KvCache, k, v, page_table, cu, past, k_weight
     bf16) become positions past[i] .. of sequence i in the cache, K with the
     norm and rotation of ``qk_norm_rope`` on the way.  max_new: at least the
     most new tokens of a sequence (all of them if left out)."""
-    rk, rv = _rows(ctx, k, "k", cache.dim), _rows(ctx, v, "v", cache.dim)
-    if k.shape[0] != v.shape[0]:
-        _refuse(N.S14_ERR_SHAPE, "k and v have different token counts")
-    table, width, cub, lenb, seqs = _table(ctx, page_table, cu, past, "past")
-    tokens = k.shape[0]
-    check(lib().s14_kv_append(
-        ctx._h, _RAW_STREAM(ctx.device) if stream is None else stream, _cache(ctx, cache), tokens, seqs, tokens if max_new is None else max_new,
-        C.byref(rk), C.byref(rv), table, width, cub, lenb, _flat(ctx, k_weight, torch.float32, "k norm weight"), eps,
-        _rope(ctx, rope)))
+    _call.kv_append(ctx._h.value, ctx.device, stream, _cache(ctx, cache), cache.dim, k, v, page_table, cu, past, k_weight,
+                    eps, _rope(ctx, rope), max_new)
 
 
 def paged_attention(ctx: Context, q, cache: KvCache, page_table, cu, lens, out, lse=None, scale: Optional[float] = None,
@@ -232,16 +186,8 @@ def paged_attention(ctx: Context, q, cache: KvCache, page_table, cu, lens, out, 
     out: q's shape, bf16 or f32; lse: f32 [tokens, heads] or None.  max_new: at
     least the most rows of a sequence; max_len: about the longest sequence (it
     sets how the work is split; the page table's reach if left out)."""
-    rq, ro = _rows(ctx, q, "q", cache.dim), _rows(ctx, out, "out", cache.dim)
-    tokens, heads, dim = q.shape
-    if out.shape != q.shape:
-        _refuse(N.S14_ERR_SHAPE, "out must have q's shape")
-    table, width, cub, lenb, seqs = _table(ctx, page_table, cu, lens, "lens")
-    check(lib().s14_paged_attention(
-        ctx._h, _RAW_STREAM(ctx.device) if stream is None else stream, C.byref(rq), _cache(ctx, cache), tokens, seqs,
-        tokens if max_new is None else max_new, width * cache.page_tokens if max_len is None else max_len, table, width,
-        cub, lenb, C.byref(ro), _flat(ctx, lse, torch.float32, "lse", tokens * heads),
-        dim ** -0.5 if scale is None else scale, window))
+    _call.paged_attention(ctx._h.value, ctx.device, stream, q, _cache(ctx, cache), cache.dim, page_table, cu, lens, out,
+                          lse, scale, window, max_new, max_len, cache.page_tokens)
 
 
 def prompt_attention(ctx: Context, q, k, v, cu, out, lse=None, scale: Optional[float] = None, window: int = 0,
@@ -249,16 +195,7 @@ def prompt_attention(ctx: Context, q, k, v, cu, out, lse=None, scale: Optional[f
     """Causal attention over packed prompts, sequence i the rows cu[i] .. cu[i
     + 1] - 1 of q [tokens, heads, dim] and k, v [tokens, key heads, dim] (all
     bf16).  out, lse and window as in ``paged_attention``."""
-    rq, ro = _rows(ctx, q, "q"), _rows(ctx, out, "out")
-    tokens, heads, dim = q.shape
-    rk, rv = _rows(ctx, k, "k", dim), _rows(ctx, v, "v", dim)
-    if out.shape != q.shape or k.shape != v.shape or k.shape[0] != tokens:
-        _refuse(N.S14_ERR_SHAPE, "out must have q's shape, v k's, and k q's tokens")
-    cub = _flat(ctx, cu, torch.int32, "cu", 1)
-    check(lib().s14_prompt_attention(
-        ctx._h, _RAW_STREAM(ctx.device) if stream is None else stream, dim, C.byref(rq), C.byref(rk), C.byref(rv), tokens, cu.numel() - 1, cub,
-        C.byref(ro), _flat(ctx, lse, torch.float32, "lse", tokens * heads), dim ** -0.5 if scale is None else scale,
-        window))
+    _call.prompt_attention(ctx._h.value, ctx.device, stream, q, k, v, cu, out, lse, scale, window)
 
 
 __all__ = [

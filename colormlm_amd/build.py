@@ -13,6 +13,9 @@ into colormlm_amd/lib/libs14hip.so:
   know the feature; the device code objects are what the flag is for;
 - the host-only translation units (*.cpp: the C ABI, the pool and loader
   contracts) without that flag.
+
+Beside it lib/_s14attn.so, the attention calls' Python side (s14_attn_py.c, a
+plain CPython extension that links nothing).
 """
 
 from __future__ import annotations
@@ -21,6 +24,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -28,6 +32,7 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OUT = PKG / "lib" / "libs14hip.so"
+PY_OUT = PKG / "lib" / "_s14attn.so"
 OBJ = PKG / "lib" / "obj"
 DEVICE_SOURCES = ["s14_device.hip", "s14_block.hip", "s14_prefill.hip", "s14_static.hip", "s14_linear.hip",
                   "s14_attn_rows.hip", "s14_attn_paged.hip", "s14_attn_prompt.hip"]
@@ -66,13 +71,19 @@ def command(out: Path = OUT) -> list:
             *[str(CSRC / s) for s in SOURCES], "-o", str(out)]
 
 
+def python_command(out: Path = PY_OUT) -> list:
+    cc = os.environ.get("CC") or shutil.which("gcc") or shutil.which("cc") or str(Path(hipcc()).parent / "amdclang")
+    return [cc, "-O2", "-std=c11", "-fPIC", "-shared", "-Wall", f"-I{sysconfig.get_paths()['include']}", f"-I{ROOT / 'include'}",
+            str(CSRC / "s14_attn_py.c"), "-o", str(out)]
+
+
 def _run(cmd: list, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         sys.stderr.write(proc.stdout + proc.stderr)
-        raise RuntimeError(f"hipcc failed with status {proc.returncode}: {' '.join(cmd[-3:])}")
+        raise RuntimeError(f"{Path(cmd[0]).name} failed with status {proc.returncode}: {' '.join(cmd[-3:])}")
     notes = [ln for ln in (proc.stdout + proc.stderr).splitlines()
              if ln.strip() and "packed-fp32-ops' is not a recognized feature" not in ln]
     if notes:
@@ -89,6 +100,9 @@ def build(verbose: bool = False) -> Path:
     tmp = OUT.with_suffix(".so.tmp")
     _run(link_command(tmp), verbose)
     os.replace(tmp, OUT)
+    tmp = PY_OUT.with_suffix(".so.tmp")
+    _run(python_command(tmp), verbose)
+    os.replace(tmp, PY_OUT)
     return OUT
 
 

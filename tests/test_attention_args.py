@@ -21,7 +21,7 @@ NONE = N.Buffer(None, 0)
 
 
 def rows(heads=4, dtype=N.S14_X_BF16, token=512, head=128, buf=BIG):
-    return N.Rows(buf.ptr, buf.bytes, dtype, heads, token, head)
+    return N.Rows(buf, dtype, heads, token, head)
 
 
 def cache(pages=10, heads=2, page=64, dim=128, **bufs):
@@ -202,7 +202,7 @@ def test_rope_table_refusals(native, code, text, args):
 
 
 class FakeContext:
-    device, handle = 0, CTX
+    device, handle, _h = 0, CTX, CTX
 
 
 def test_python_layer_refuses_cpu_tensors_and_bad_caches():
