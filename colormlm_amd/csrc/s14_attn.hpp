@@ -96,7 +96,8 @@ struct RopeTableArgs {
 
 // Work split of a paged launch.
 struct PagedPlan {
-  uint32_t row_tiles;  // 16-row tiles a wavefront holds
+  uint32_t row_tiles;  // 16-row tiles of a workgroup
+  uint32_t staged;     // a row tile's K and V go through LDS (k_paged_rows)
   uint32_t rec_rows;   // rows of a chunk's partial result
   uint32_t chunk;      // tokens of one workgroup, a multiple of 64
   uint32_t chunks;     // of the longest sequence; above 1 the partial results go to the workspace

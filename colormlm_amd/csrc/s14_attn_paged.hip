@@ -11,11 +11,14 @@
 // scores (K) and the weights (V), and are one per lane, since the 4 T tokens
 // of a lane group lie in one page.
 //
-// A row is a (token, query head of the key head) pair: the group's heads
-// share the K and V that a wavefront loads.  The four wavefronts of a
-// workgroup take steps of 16 T tokens in turn and join through LDS; a long
-// sequence is cut into chunks of workgroups whose partial results a second
-// launch joins.
+// A row is a (token, query head of the key head) pair: the group's heads share
+// the K and V that are read.  Up to 16 rows (k_paged_attention), the four
+// wavefronts of a workgroup take steps of 16 T tokens in turn and join through
+// LDS; with more rows they share the tokens' codes through LDS (k_paged_rows),
+// or, with heads of 512, the dimensions (k_paged_wide).  A long sequence is cut
+// into chunks of workgroups, whose partial results are joined by the last of
+// them or by a second launch.  Few rows are bound by the cache's bytes: 128
+// sequences of up to 8,192 tokens, 8 key heads of 128, 160 us, 4.8 TB/s.
 #include "s14_attn.hpp"
 #include "s14_attn_util.hpp"
 #include "s14_device.hpp"
@@ -66,7 +69,7 @@ __device__ __forceinline__ void store_out(const AttnOut &o, uint64_t at, float a
 // the same pages are a multiple of all items apart.  Chunks come before them,
 // so that the late chunks, which short sequences lack, are together: among the
 // sequences the empty workgroups fell to the same compute units (128 ragged
-// sequences of 8,192 tokens at most, 4 chunks: 228 us; so DECODE_US).
+// sequences of 8,192 tokens at most, 4 chunks: 228 us; 160 now).
 // Workgroup i runs on XCD i % 8: where (sequence, key head) pairs are few, a
 // chunk's pairs are rotated each time their start comes back to the first XCD,
 // or one long sequence would have but some of the XCDs.
@@ -145,12 +148,12 @@ __device__ __forceinline__ bool arrived_last(uint32_t *count, uint32_t chunks) {
   return s_last != 0;
 }
 
-// A tile's rows from their partial results, a row a wavefront at a time: lane
-// c holds chunk c's maximum and sum (64 chunks at most), then the chunks' rows
-// in order.
-template <int D>
-__device__ __forceinline__ void join_tile(const PagedArgs &a, const PagedPlan &p, const Span &sp, const Item &it,
-                                          uint32_t row0, const float *part) {
+// Row row0 + k of a tile from its partial results, by one wavefront: lane c
+// holds chunk c's maximum and sum (64 chunks at most), then the chunks' rows in
+// order.
+template <int D, int kPolicy>
+__device__ __forceinline__ void join_row(const PagedArgs &a, const PagedPlan &p, const Span &sp, const Item &it,
+                                         uint32_t row0, uint32_t k, const float *part) {
   constexpr uint32_t kLanes = D / 4 < 64 ? D / 4 : 64, kSpan = D / (4 * kLanes), kSets = 64 / kLanes;
   const uint32_t kvh = a.cache.heads, group = a.heads / kvh, l = threadIdx.x & 63u;
   const uint32_t lane = l % kLanes, set = l / kLanes;
@@ -159,55 +162,61 @@ __device__ __forceinline__ void join_tile(const PagedArgs &a, const PagedPlan &p
   const float *first = part + record_of(a, p, Item{it.tile, 0, it.seq, it.head}, kvh) * rec;
   const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(first), 0,
                                                    int((sp.chunks - 1) * next + uint32_t(rec) * 4), 0x00020000);
-  for (uint32_t k = threadIdx.x / 64; k < p.rec_rows && row0 + k < sp.rows; k += 4) {
-    const uint32_t at = k * kRecord<D> * 4;
-    float m = -INFINITY, sum = 0.0f;
-    if (l < sp.chunks) {
-      const auto ml = __builtin_amdgcn_raw_buffer_load_b64(r, l * next + at + D * 4, 0, kAgent);
-      m = __uint_as_float(ml[0]), sum = __uint_as_float(ml[1]);
-    }
-    float top = m;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    const float w = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));  // 0 in lanes without a chunk
-    float total = sum * w;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
-    f32x4 o[kSpan] = {};
-    for (uint32_t c0 = 0; c0 < sp.chunks; c0 += 4 * kSets) {
-      u32x4 x[4][kSpan];
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j)
-#pragma unroll
-        for (uint32_t i = 0; i < kSpan; ++i)  // past the last chunk: zeros (descriptor range), weight 0
-          x[j][i] = __builtin_amdgcn_raw_buffer_load_b128(
-              r, (c0 + j * kSets + set) * next + at + 16 * (lane + kLanes * i), 0, kAgent);
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) {
-        const float f = __shfl(w, int((c0 + j * kSets + set) & 63u));
-#pragma unroll
-        for (uint32_t i = 0; i < kSpan; ++i) o[i] += __builtin_bit_cast(f32x4, x[j][i]) * f;
-      }
-    }
-#pragma unroll
-    for (uint32_t d = kLanes; d < 64; d <<= 1)
-#pragma unroll
-      for (uint32_t i = 0; i < kSpan; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] += __shfl_xor(o[i][e], int(d));
-    const uint32_t row = row0 + k;
-    const uint64_t t = uint64_t(sp.first + row / group);
-    const uint32_t h = it.head * group + row % group;
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    if (set == 0) {
-#pragma unroll
-      for (uint32_t i = 0; i < kSpan; ++i) {
-        const f32x4 y = o[i] * inv;
-        store_out(a.out, t * a.out.token + uint64_t(h) * a.out.head + 4 * (lane + kLanes * i), y[0], y[1], y[2], y[3]);
-      }
-    }
-    if (a.lse && l == 0) a.lse[t * a.heads + h] = total == 0.0f ? -INFINITY : top * kLn2 + __logf(total);
+  const uint32_t at = k * kRecord<D> * 4;
+  float m = -INFINITY, sum = 0.0f;
+  if (l < sp.chunks) {
+    const auto ml = __builtin_amdgcn_raw_buffer_load_b64(r, l * next + at + D * 4, 0, kPolicy);
+    m = __uint_as_float(ml[0]), sum = __uint_as_float(ml[1]);
   }
+  float top = m;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  const float w = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));  // 0 in lanes without a chunk
+  float total = sum * w;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
+  f32x4 o[kSpan] = {};
+  for (uint32_t c0 = 0; c0 < sp.chunks; c0 += 4 * kSets) {
+    u32x4 x[4][kSpan];
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j)
+#pragma unroll
+      for (uint32_t i = 0; i < kSpan; ++i)  // past the last chunk: zeros (descriptor range), weight 0
+        x[j][i] = __builtin_amdgcn_raw_buffer_load_b128(
+            r, (c0 + j * kSets + set) * next + at + 16 * (lane + kLanes * i), 0, kPolicy);
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+      const float f = __shfl(w, int((c0 + j * kSets + set) & 63u));
+#pragma unroll
+      for (uint32_t i = 0; i < kSpan; ++i) o[i] += __builtin_bit_cast(f32x4, x[j][i]) * f;
+    }
+  }
+#pragma unroll
+  for (uint32_t d = kLanes; d < 64; d <<= 1)
+#pragma unroll
+    for (uint32_t i = 0; i < kSpan; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] += __shfl_xor(o[i][e], int(d));
+  const uint32_t row = row0 + k;
+  const uint64_t t = uint64_t(sp.first + row / group);
+  const uint32_t h = it.head * group + row % group;
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  if (set == 0) {
+#pragma unroll
+    for (uint32_t i = 0; i < kSpan; ++i) {
+      const f32x4 y = o[i] * inv;
+      store_out(a.out, t * a.out.token + uint64_t(h) * a.out.head + 4 * (lane + kLanes * i), y[0], y[1], y[2], y[3]);
+    }
+  }
+  if (a.lse && l == 0) a.lse[t * a.heads + h] = total == 0.0f ? -INFINITY : top * kLn2 + __logf(total);
+}
+
+// All rows of a tile, by its last workgroup.
+template <int D>
+__device__ __forceinline__ void join_tile(const PagedArgs &a, const PagedPlan &p, const Span &sp, const Item &it,
+                                          uint32_t row0, const float *part) {
+  for (uint32_t k = threadIdx.x / 64; k < p.rec_rows && row0 + k < sp.rows; k += 4)
+    join_row<D, kAgent>(a, p, sp, it, row0, k, part);
 }
 
 // The top bit of each byte that is a NaN code (0x7f, 0xff).
@@ -216,8 +225,9 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t c) { return ((c & 0x7f7f7
 // Those bytes as zeros.
 __device__ __forceinline__ uint32_t no_nan(uint32_t c) { return c & ~((nan_codes(c) >> 7) * 0xffu); }
 
-template <int D, int NT, int T>
+template <int D, int NT>
 __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(PagedArgs a, PagedPlan p, float *part) {
+  constexpr int T = 4;        // 16-token tiles a step
   constexpr int C = D / 64;   // 16-byte pieces of a K row a lane holds
   constexpr int DT = D / 16;  // 16-dimension tiles of O
   constexpr int W = T;        // 32-bit words of V codes a lane holds of one dimension
@@ -288,13 +298,8 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
                         (uint32_t(b + 4 * T * int32_t(g)) & (P - 1));
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      if constexpr (T == 4) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(vp + 16 * dt * P);
-        vv[dt][0] = x.x, vv[dt][1] = x.y, vv[dt][2] = x.z, vv[dt][3] = x.w;
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2 *>(vp + 16 * dt * P);
-        vv[dt][0] = x.x, vv[dt][1] = x.y;
-      }
+      const uint4 x = *reinterpret_cast<const uint4 *>(vp + 16 * dt * P);
+      vv[dt][0] = x.x, vv[dt][1] = x.y, vv[dt][2] = x.z, vv[dt][3] = x.w;
     }
   };
   constexpr int32_t kStride = 4 * 16 * T;  // the wavefronts' steps interleave
@@ -764,6 +769,317 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
   if (arrived_last(a.count + (tile * a.seqs + seq) * kvh + head, sp.chunks)) join_tile<D>(a, p, sp, it, row0, part);
 }
 
+// Where a row's 16-byte piece of K or V lies in LDS: piece ^ turn(row), so that
+// the 16 lanes of a read, one piece of each of 16 rows, meet no bank twice (64
+// banks of 4 bytes).  K: a row is a token of D values, and a lane's token is
+// 8 (n / 4) + n % 4 of its 32.  V: a row is a dimension of TK values.
+template <int D>
+__device__ __forceinline__ uint32_t turn_k(uint32_t tok) {
+  return D == 64 ? ((tok >> 1) & 1u) | ((tok >> 2) & 6u) : (tok & 3u) | ((tok >> 1) & 12u);
+}
+template <int TK>
+__device__ __forceinline__ uint32_t turn_v(uint32_t dim) {
+  return TK == 64 ? (dim >> 1) & 7u : (dim >> 2) & 3u;
+}
+
+// More rows: each wavefront has 16 NT of its own (of two row tiles, two
+// wavefronts share one, half the tokens each), and all read the same TK tokens
+// from LDS, where the workgroup has put them as bf16 with their page's scale,
+// once for all its rows.  In registers 64 rows of 128 leave one wavefront a
+// SIMD, with spills, and their four partial sums to join: 8 sequences of 64 new
+// tokens of 3,000 104 us so, 59 here (420 TFLOP/s); 32 of 8 of 4,000 73 and 66
+// (4.1 TB/s); 74 of 17 of 67 75 and 21.  Short ones are bound by the chain of
+// loads before their first product, long ones by LDS reads (2 bytes a multiply,
+// half the matrix rate at NT = 1) and the softmax beside them.
+template <int D, int NT, int RW>
+__global__ __launch_bounds__(256, D * NT <= 128 ? 3 : 2) void k_paged_rows(PagedArgs a, PagedPlan p, float *part) {
+  constexpr int TK = D <= 128 ? 64 : 32;  // tokens a step
+  constexpr int TW = 4 / RW;              // wavefronts that share a row tile's tokens
+  constexpr int U = TK / 32 / TW, T = 2 * U, DT = D / 16, C = D / 32;
+  constexpr int R = D * TK / 4096;                // 16-code pieces of K, and of V, a thread
+  constexpr int kTokens = 4096 / D;               // of K in 256 pieces
+  constexpr int I = kTokens >= 16 ? R : TK / 16;  // pages of a thread's K pieces
+  const uint32_t kvh = a.cache.heads, group = a.heads / kvh;
+  const Item it = item_of(a, p, kvh);
+  const uint32_t tile = it.tile, head = it.head, seq = it.seq, chunk = it.chunk;
+  const uint32_t row0 = tile * 16 * NT * RW;
+  const Span sp = paged_span(a, p, seq, row0);
+  if (row0 >= sp.rows || (chunk && chunk >= sp.chunks)) return;
+  const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid & 63u, n = l & 15u, g = l >> 4;
+  const uint32_t P = a.cache.page;
+  const Pages pages{a.page_table + uint64_t(seq) * a.table_width, sp.len, a.cache.pages, uint32_t(__builtin_ctz(P))};
+  const int32_t begin = sp.lo + int32_t(chunk * sp.chunk);
+  const int32_t end = min(sp.hi, begin + int32_t(sp.chunk));
+  const uint32_t mine = row0 + 16 * NT * (wave % RW), u0 = U * (wave / RW);  // the wavefront's rows and 32-token parts
+  const bool active = mine < sp.rows;
+
+  Visible see[NT];
+  bf16x8 q[NT][C];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const uint32_t r = mine + 16 * nt + n;
+    const uint32_t rr = r < sp.rows ? r : sp.rows - 1;
+    see[nt] = Visible(sp.pos0 + int32_t(rr / group), a.window);
+    const uint16_t *row = a.q + uint64_t(sp.first + rr / group) * a.q_token +
+                          uint64_t(head * group + rr % group) * a.q_head;
+#pragma unroll
+    for (int c = 0; c < C; ++c) q[nt][c] = *reinterpret_cast<const bf16x8 *>(row + 32 * c + 8 * g);
+  }
+  const int32_t pos_lo = sp.pos0 + int32_t(row0 / group), pos_hi = sp.hi - 1;
+  const auto partial_at = [&](int32_t b) {
+    return b + TK - 1 > pos_lo || (a.window && int64_t(b) <= int64_t(pos_hi) - a.window);
+  };
+
+  constexpr uint32_t kPieces = TK * D / 8;
+  __shared__ u32x4 s_rows[2 * kPieces];  // K, V
+  __shared__ uint32_t s_flags;
+  if (tid == 0) s_flags = 0;
+
+  f32x4 o[NT][DT] = {};
+  float m[NT], sum[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) m[nt] = -INFINITY, sum[nt] = 0.0f;
+  bool bad = false, odd = false;
+  const float scale = a.scale * kLog2e;
+  const uint64_t page_bytes = uint64_t(P) * D;
+
+  // A step's pieces: K piece i of a thread is 16 dimensions of token 4096 / D *
+  // i + tid / (D / 16), V piece i 16 tokens of dimension 4096 / TK * i + tid /
+  // (TK / 16).  Loaded two steps ahead of their use, turned into bf16 one
+  // ahead (a step more in flight measured no better); their pages' ids are
+  // loaded another step ahead.
+  const uint32_t k_tok = tid / (D / 16), k_dim = tid % (D / 16) * 16;
+  const uint32_t v_dim = tid / (TK / 16), v_tok = tid % (TK / 16) * 16;
+  uint4 kk[R], vv[R];
+  uint32_t ksc[I], vsc;
+  int32_t idk[I], idv = 0;
+  auto load_ids = [&](int32_t b) {
+#pragma unroll
+    for (int i = 0; i < I; ++i) idk[i] = pages.id(b + int32_t(k_tok) + (kTokens >= 16 ? kTokens : 16) * i);
+    idv = pages.id(b + int32_t(v_tok));
+  };
+  auto load = [&](int32_t b) {
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const uint64_t at = uint64_t(pages.checked(idk[i], bad)) * kvh + head;
+      ksc[i] = a.cache.ks[at];
+#pragma unroll
+      for (int j = 0; j < R / I; ++j) {
+        const uint32_t slot = uint32_t(b + int32_t(k_tok) + kTokens * (R / I * i + j)) & (P - 1);
+        kk[R / I * i + j] = *reinterpret_cast<const uint4 *>(a.cache.k + at * page_bytes + slot * uint32_t(D) + k_dim);
+      }
+    }
+    const uint64_t at = uint64_t(pages.checked(idv, bad)) * kvh + head;
+    vsc = a.cache.vs[at];
+    const uint8_t *vp = a.cache.v + at * page_bytes + v_dim * P + (uint32_t(b + int32_t(v_tok)) & (P - 1));
+#pragma unroll
+    for (int i = 0; i < R; ++i) vv[i] = *reinterpret_cast<const uint4 *>(vp + 4096 / TK * i * P);
+  };
+  auto put = [&](u32x4 *to, uint32_t row, uint32_t pieces, uint32_t piece, uint32_t turn, uint4 x, float f) {
+    to[row * pieces + (piece ^ turn)] = __builtin_bit_cast(u32x4, e4m3_bf16(x.x, x.y, f));
+    to[row * pieces + ((piece + 1) ^ turn)] = __builtin_bit_cast(u32x4, e4m3_bf16(x.z, x.w, f));
+  };
+  auto stage = [&](int32_t b, u32x4 *to) {
+    if (partial_at(b)) {
+      // as in k_paged_attention: nothing from behind the sequence, and no NaN
+      // code that some row must not see
+      uint32_t nan = 0;
+      uint32_t keep[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int32_t left = sp.len - (b + int32_t(v_tok) + 4 * k);
+        keep[k] = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+      }
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        vv[i].x &= keep[0], vv[i].y &= keep[1], vv[i].z &= keep[2], vv[i].w &= keep[3];
+        nan |= nan_codes(vv[i].x) | nan_codes(vv[i].y) | nan_codes(vv[i].z) | nan_codes(vv[i].w);
+      }
+      if (__any(nan != 0)) {
+        odd = true;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          vv[i].x = no_nan(vv[i].x), vv[i].y = no_nan(vv[i].y), vv[i].z = no_nan(vv[i].z), vv[i].w = no_nan(vv[i].w);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const uint32_t tok = k_tok + kTokens * i;
+      put(to, tok, D / 8, k_dim / 8, turn_k<D>(tok), kk[i], power_of_two(int(ksc[i / (R / I)]) - 127));
+    }
+    const float vs = power_of_two(int(vsc) - 127);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const uint32_t dim = v_dim + 4096 / TK * i;
+      put(to + kPieces, dim, TK / 8, v_tok / 8, turn_v<TK>(dim), vv[i], vs);
+    }
+  };
+  const uint32_t k_row = 8 * (n / 4) + n % 4, k_turn = turn_k<D>(k_row), v_turn = turn_v<TK>(n);
+
+  if (begin < end) load_ids(begin);
+  // Q is waited for here, with the ids, or it would be in every step
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < C; ++c) asm volatile("" : "+v"(q[nt][c]));
+  if (begin < end) {
+    load(begin);
+    if (begin + TK < end) load_ids(begin + TK);
+    stage(begin, s_rows);
+    if (begin + TK < end) load(begin + TK);
+    if (begin + 2 * TK < end) load_ids(begin + 2 * TK);
+  }
+  __syncthreads();
+
+  for (int32_t b = begin; b < end; b += TK) {
+    const u32x4 *sk = s_rows, *sv = sk + kPieces;
+    bf16x8 pb[NT][U];
+    if (active) {
+      f32x4 s[NT][T] = {};
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const uint32_t row = 32 * (u0 + t / 2) + 4 * (t & 1) + k_row;
+          const bf16x8 k = __builtin_bit_cast(bf16x8, sk[row * (D / 8) + ((4 * c + g) ^ k_turn)]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) s[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[nt][c], s[nt][t], 0, 0, 0);
+        }
+      const bool partial = partial_at(b);
+      const int32_t tv = b + 32 * int32_t(u0) + 8 * int32_t(g);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float x[4 * T];
+#pragma unroll
+        for (int i = 0; i < 4 * T; ++i) x[i] = s[nt][i / 4][i % 4] * scale;
+        if (partial) {
+          keep_branch();
+#pragma unroll
+          for (int i = 0; i < 4 * T; ++i) x[i] = see[nt](tv + 32 * (i / 8) + i % 8) ? x[i] : -INFINITY;
+        }
+        float top = x[0];
+#pragma unroll
+        for (int i = 1; i < 4 * T; ++i) top = fmaxf(top, x[i]);
+        top = fmaxf(m[nt], max_lane16(top));
+        if (__any(top > m[nt] + kRise)) {
+          const float fade = __builtin_amdgcn_exp2f(m[nt] - (top == -INFINITY ? 0.0f : top));
+          m[nt] = top;
+          sum[nt] *= fade;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[nt][dt] *= fade;
+        }
+        const float at = m[nt] == -INFINITY ? 0.0f : m[nt];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          u32x4 w;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float e0 = __builtin_amdgcn_exp2f(x[8 * u + 2 * j] - at), e1 = __builtin_amdgcn_exp2f(x[8 * u + 2 * j + 1] - at);
+            sum[nt] += e0;
+            sum[nt] += e1;
+            w[j] = bf16_pair(e0, e1);  // half a step of each weight: the matrix operand's type
+          }
+          pb[nt][u] = __builtin_bit_cast(bf16x8, w);
+        }
+      }
+    }
+    if (active) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const bf16x8 v = __builtin_bit_cast(bf16x8, sv[(16 * dt + n) * (TK / 8) + ((4 * (u0 + u) + g) ^ v_turn)]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pb[nt][u], o[nt][dt], 0, 0, 0);
+        }
+    }
+    __syncthreads();
+    if (b + TK < end) {
+      stage(b + TK, s_rows);
+      if (b + 2 * TK < end) load(b + 2 * TK);
+      if (b + 3 * TK < end) load_ids(b + 3 * TK);
+      __syncthreads();
+    }
+  }
+
+  if (bad || odd) atomicOr(&s_flags, (bad ? 1u : 0u) | (odd ? 2u : 0u));
+  __syncthreads();
+  const uint32_t flags = s_flags;
+  if constexpr (TW == 2) {  // the token parts' sums: part 1 into 0, both taken from the larger maximum
+    float *x = reinterpret_cast<float *>(s_rows) + (wave % RW) * (64 * NT * (4 * DT + 2));
+    if (u0) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float *y = x + nt * 64 * (4 * DT + 2);
+        y[l] = m[nt], y[64 + l] = sum[nt];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) reinterpret_cast<f32x4 *>(y + 128)[64 * dt + l] = o[nt][dt];
+      }
+    }
+    __syncthreads();
+    if (!u0) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float *y = x + nt * 64 * (4 * DT + 2);
+        const float other = y[l], top = fmaxf(m[nt], other), at = top == -INFINITY ? 0.0f : top;
+        const float f0 = __builtin_amdgcn_exp2f(m[nt] - at), f1 = __builtin_amdgcn_exp2f(other - at);
+        m[nt] = top, sum[nt] = sum[nt] * f0 + y[64 + l] * f1;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[nt][dt] = o[nt][dt] * f0 + reinterpret_cast<const f32x4 *>(y + 128)[64 * dt + l] * f1;
+      }
+    }
+  }
+  if ((flags & 2u) && !u0) {  // rare: one token after the other
+    for (int32_t b0 = begin; b0 < end; b0 += TK) {
+      if (!partial_at(b0)) continue;
+      for (int32_t j = b0; j < min(b0 + TK, sp.len); ++j) {
+        const uint8_t *vp = a.cache.v + (uint64_t(pages.checked(pages.id(j), bad)) * kvh + head) * page_bytes + (uint32_t(j) & (P - 1));
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          f32x4 nan;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            nan[i] = (vp[(16 * dt + 4 * g + i) * P] & 0x7fu) == 0x7fu ? __uint_as_float(0x7fc00000u) : 0.0f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const bool in = see[nt](j);
+            f32x4 back;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) back[i] = in ? nan[i] : 0.0f;
+            o[nt][dt] += back;
+          }
+        }
+      }
+    }
+  }
+  if ((flags & 1u) && tid == 0) atomicOr(a.status, kStatusBadCachePage);
+  const uint32_t floats = p.rec_rows * kRecord<D>;
+  const PartStore store(part + record_of(a, p, it, kvh) * floats, floats, p.fused);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const float total = flags & 1u ? __uint_as_float(0x7fc00000u) : sum_lane16(sum[nt]);
+    const uint32_t r = mine + 16 * nt + n;
+    if (r >= sp.rows || u0) continue;
+    if (sp.chunks > 1) {
+      const uint32_t row = (r - row0) * kRecord<D>;
+      if (g == 0) store(row + D, f32x4{m[nt], total, 0.0f, 0.0f});
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) store(row + 16 * dt + 4 * g, o[nt][dt]);
+      continue;
+    }
+    const uint64_t t = uint64_t(sp.first + r / group);
+    const uint32_t h = head * group + r % group;
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      store_out(a.out, t * a.out.token + uint64_t(h) * a.out.head + 16 * dt + 4 * g, o[nt][dt][0] * inv,
+                o[nt][dt][1] * inv, o[nt][dt][2] * inv, o[nt][dt][3] * inv);
+    if (a.lse && g == 0) a.lse[t * a.heads + h] = total == 0.0f ? -INFINITY : m[nt] * kLn2 + __logf(total);
+  }
+  if (sp.chunks <= 1 || !p.fused) return;
+  if (arrived_last(a.count + (tile * a.seqs + seq) * kvh + head, sp.chunks)) join_tile<D>(a, p, sp, it, row0, part);
+}
+
 // Joins the chunks of one row a workgroup, in an order that its size alone
 // sets: the chunks' maxima in the lanes, then their rows in groups of
 // threads at once.
@@ -819,12 +1135,27 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, PagedPlan p, co
   if (a.lse && lane == 0) a.lse[t * a.heads + h] = total == 0.0f ? -INFINITY : top * kLn2 + __logf(total);
 }
 
-template <class Kernel, class Join>
-hipError_t launch(hipStream_t s, const PagedArgs &a, const PagedPlan &p, float *part, Kernel kernel, Join join) {
+// Up to 16 chunks of a row: a row a wavefront, which reads them at once (128
+// rows of 8 sequences, 8 key heads, 8 chunks, 69 MB: 78 us with the attention,
+// a row a workgroup 98).
+template <int D>
+__global__ __launch_bounds__(256) void k_paged_join_rows(PagedArgs a, PagedPlan p, const float *part) {
+  const uint32_t r = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / 64), per = 16 * p.row_tiles;
+  const Item it{r / per, 0, blockIdx.y, blockIdx.z};
+  const Span sp = paged_span(a, p, it.seq, it.tile * per);
+  if (r >= sp.rows || sp.chunks <= 1) return;
+  join_row<D, 0>(a, p, sp, it, it.tile * per, r % per, part);
+}
+
+template <int D, class Kernel>
+hipError_t launch(hipStream_t s, const PagedArgs &a, const PagedPlan &p, float *part, Kernel kernel) {
   kernel<<<uint32_t(p.blocks), 256, 0, s>>>(a, p, part);
   if (p.chunks > 1 && !p.fused) {
     const uint32_t rows = uint32_t(a.max_new) * (a.heads / a.cache.heads);
-    join<<<dim3(rows, a.seqs, a.cache.heads), 256, 0, s>>>(a, p, part);
+    if (p.chunks <= 16)
+      k_paged_join_rows<D><<<dim3((rows + 3) / 4, a.seqs, a.cache.heads), 256, 0, s>>>(a, p, part);
+    else
+      k_paged_join<D><<<dim3(rows, a.seqs, a.cache.heads), 256, 0, s>>>(a, p, part);
   }
   return hipGetLastError();
 }
@@ -832,46 +1163,68 @@ hipError_t launch(hipStream_t s, const PagedArgs &a, const PagedPlan &p, float *
 template <int D>
 hipError_t launch_dim(hipStream_t s, const PagedArgs &a, const PagedPlan &p, float *part) {
   if constexpr (D == 512) {
-    if (p.row_tiles == 2) return launch(s, a, p, part, k_paged_wide<2>, k_paged_join<D>);
-    return launch(s, a, p, part, k_paged_wide<1>, k_paged_join<D>);
+    if (p.row_tiles == 2) return launch<D>(s, a, p, part, k_paged_wide<2>);
+    return launch<D>(s, a, p, part, k_paged_wide<1>);
   } else {
-    if constexpr (D <= 128)
-      if (p.row_tiles == 4) return launch(s, a, p, part, k_paged_attention<D, 4, 4>, k_paged_join<D>);
-    if (p.row_tiles == 2) return launch(s, a, p, part, k_paged_attention<D, 2, D == 256 ? 2 : 4>, k_paged_join<D>);
-    return launch(s, a, p, part, k_paged_attention<D, 1, 4>, k_paged_join<D>);
+    if constexpr (D <= 128) {
+      if (p.row_tiles == 8) return launch<D>(s, a, p, part, k_paged_rows<D, 2, 4>);
+      if (p.row_tiles == 2 && p.staged) return launch<D>(s, a, p, part, k_paged_rows<D, 1, 2>);
+      if (p.row_tiles == 2) return launch<D>(s, a, p, part, k_paged_attention<D, 2>);
+    }
+    if (p.row_tiles == 4) return launch<D>(s, a, p, part, k_paged_rows<D, 1, 4>);
+    return launch<D>(s, a, p, part, k_paged_attention<D, 1>);
   }
 }
 
 }  // namespace
 
-// Rows a wavefront holds: as many 16-row tiles as the longest new block fills
-// and the registers of the head size leave room for (64 rows of 128, 32 of 256,
-// and of 512 by quarters of the head).
+// Rows of a workgroup: all of the longest new block's up to 64 (of 32 of
+// heads of 512), or K and V are read and turned into bf16 again for each row
+// tile; 128 where there are more, at heads of 128, and more than 256 at heads
+// of 64 (8 sequences of 64 new tokens of 3,000: 59 us, with tiles of 64 rows
+// 64; 6 of 24 of up to 5,000, heads of 64: 27, with tiles of 128 38).  Up to
+// 16 rows a wavefront reads K and V for itself; more go through LDS, but for
+// one sequence of 32 rows, where a compute unit so has more bytes in flight
+// (us, direct / staged: one of 40,000 tokens 24 / 28, 32 of 4,000 73 / 66, 3 of
+// up to 51,525 40 / 30, 38 of up to 422, window 161, 18 / 12).
 //
 // Chunks.  Where the launch alone would leave compute units idle: as many
 // workgroups as the card holds at once (a second round for a few of them costs
 // as much as the first), of several sequences twice as many, since their
 // lengths differ and short ones leave chunks empty (us, once / twice: 16
 // sequences of up to 8,192 tokens 36 / 29 ragged, 55 / 55 equal; 4 of up to
-// 9,000, 64 heads of 512, 49 / 37 and 56 / 72).  Where it fills the card:
-// chunks of 2,048 tokens, so that one long sequence does not outlast the rest.
-// A row tile whose partial results stay within 64 KB is joined by its last
-// workgroup (1 token of 4,097: 12.4 us with a second launch, 10.4 without; 32
-// rows of 31 chunks, 1 MB: 25 and 42).
+// 9,000, 64 heads of 512, 49 / 37 and 56 / 72; 3 of 200 new of up to 6,000 96 /
+// 80; 8 of 64 new of 3,000 51 / 59).  Where it fills the card: chunks of 2,048
+// tokens, so that one long sequence does not outlast the rest.
+//
+// A row tile of 4 rows whose partial results stay within 64 KB is joined by its
+// last workgroup, a row a wavefront (1 token of 4,097: 12.4 us with a second
+// launch, 10.4 without; 32 rows of 2 chunks take it 9 us longer than a launch).
+// Where a second launch would join them, a sequence of few steps is left whole
+// (20 sequences of 300 tokens, 32 rows: 10 us, in two chunks 21; one of 500
+// tokens and 8 of them 11, 20), and small chunks start at shorter ones (4 of 48
+// rows of 300 tokens, heads of 256: 12 us in chunks of 64, 19 of 256).
 PagedPlan paged_plan(const PagedArgs &a) {
   PagedPlan p{};
   const uint64_t rows = uint64_t(a.max_new) * (a.heads / a.cache.heads);
-  const uint32_t dim = a.cache.dim, most = dim <= 128 ? 4 : 2;
-  p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  if (p.row_tiles > most) p.row_tiles = most;
+  const uint32_t dim = a.cache.dim;
+  p.row_tiles = rows <= 16                          ? 1
+                : dim == 512                        ? 2
+                : rows <= 32 && dim <= 128          ? 2
+                : rows > 64 && dim == 128           ? 8
+                : rows > 256 && dim == 64           ? 8
+                                                    : 4;
+  p.staged = dim < 512 && (p.row_tiles >= 4 || (p.row_tiles == 2 && a.seqs > 1));
   const uint64_t tiles = (rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles);
   const uint64_t base = tiles * a.cache.heads * a.seqs;  // workgroups of an uncut launch
   uint64_t span = a.max_len;
   if (a.window && uint64_t(a.window) + a.max_new + 63 < span) span = uint64_t(a.window) + a.max_new + 63;
-    // workgroups that the card holds at once, by the registers of a wavefront
+  // workgroups that the card holds at once, by a wavefront's registers and by LDS
   const uint32_t words = (dim == 512 ? 128 : dim) * p.row_tiles;
-  const uint64_t slots = 256 * (words <= 64 ? 3 : words <= 128 || dim == 512 ? 2 : 1);
-  const uint64_t least = dim == 512 ? 64 : 256;  // a step of every wavefront
+  const uint64_t per_cu = p.staged ? (dim == 256 ? 2 : (dim == 64 ? 4 : 3) - p.row_tiles / 8)
+                                   : (words <= 64 ? 3 : words <= 128 || dim == 512 ? 2 : 1);
+  const uint64_t slots = 256 * per_cu;
+  const uint64_t least = dim == 512 ? 64 : !p.staged ? 256 : span <= 512 ? 64 : span <= 1024 ? 128 : 256;
   constexpr uint64_t kMost = 2048, kFuse = 64 * 1024;
   p.rec_rows = uint32_t(rows < 16 * p.row_tiles ? rows : 16 * p.row_tiles);
   const uint64_t rec = uint64_t(p.rec_rows) * (dim + 4);
@@ -880,11 +1233,11 @@ PagedPlan paged_plan(const PagedArgs &a) {
   if (chunks > fit) chunks = fit;
   if (chunks > (span + least - 1) / least) chunks = (span + least - 1) / least;
   if (chunks < 1) chunks = 1;
+  p.fused = chunks <= 64 && base <= kPagedCounters && p.rec_rows <= 4 && rec * 4 * chunks <= kFuse;
+  if (!p.fused && span <= (dim == 512 ? 128 : dim == 256 ? 256 : 512)) chunks = 1;
   p.chunk = uint32_t(((span + chunks - 1) / chunks + least - 1) / least * least);
   p.chunks = span ? uint32_t((span + p.chunk - 1) / p.chunk) : 1;
   p.blocks = base * p.chunks;
-  p.fused = p.chunks > 1 && p.chunks <= 64 && base <= kPagedCounters && rec * 4 * p.chunks <= kFuse &&
-            rec * 4 * p.chunks * a.seqs * a.cache.heads < (1ull << 31);
   return p;
 }
 

@@ -66,12 +66,13 @@ __device__ __forceinline__ float sum_lane16(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Eight E4M3 codes as bf16, exactly (a NaN code gives NaN).
-__device__ __forceinline__ bf16x8 e4m3_bf16(uint32_t lo, uint32_t hi) {
-  const u32x4 v = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true))};
+// Eight E4M3 codes times a power of two as bf16, exactly within bf16's range (a
+// NaN code gives NaN).
+__device__ __forceinline__ bf16x8 e4m3_bf16(uint32_t lo, uint32_t hi, float scale = 1.0f) {
+  const u32x4 v = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true))};
   return __builtin_bit_cast(bf16x8, v);
 }
 

@@ -560,6 +560,82 @@ def test_paged_special_values_in_hidden_places(ctx, page):
         assert torch.equal(out.isnan().cpu(), want.isnan()) and not bool(want[:, 0].isnan().all())
 
 
+ROWS = [  # lengths, new counts, heads, kv, dim, page: rows (token, query head of the key head) of each count a workgroup takes
+    ([300, 65, 1], [3, 2, 1], 8, 1, 64, 16), ([200, 130], [5, 5], 8, 1, 64, 64), ([500, 70], [40, 33], 16, 2, 64, 32),
+    ([330], [17], 48, 3, 64, 128), ([100, 700, 64], [8, 8, 7], 8, 2, 128, 64), ([129, 40], [2, 1], 24, 1, 128, 16),
+    ([900], [12], 4, 1, 128, 128), ([260, 31], [16, 16], 8, 2, 128, 32), ([300, 64, 5], [33, 64, 2], 4, 2, 128, 64),
+    ([400, 90], [90, 3], 6, 2, 128, 16), ([257], [3], 6, 1, 256, 64), ([70, 600], [20, 9], 8, 2, 256, 16),
+    ([333, 12, 64], [70, 12, 1], 2, 1, 256, 128)]
+
+
+@pytest.mark.parametrize("lengths,new,heads,kv,dim,page", ROWS)
+@pytest.mark.parametrize("window,dtype", [(0, F32), (90, BF16), (1, BF16)])
+def test_paged_rows(ctx, lengths, new, heads, kv, dim, page, window, dtype):
+    say(f"paged rows lens={lengths} new={new} heads={heads}/{kv} dim={dim} page={page} window={window} {dtype}")
+    p = Paged(sum(lengths) + 3 * dim, lengths, kv, dim, page, lo=112, hi=124)
+    q = rand(gen(13), sum(new), heads, dim, dtype=BF16).cuda()
+    out, lse = run_paged(ctx, p, q, new, heads, dim, window, dtype)
+    want = paged_want(p, q, new, window)
+    check_attention(out, lse, want, "paged rows")
+    ctx.launch_status()
+    # planned for shorter ones: larger pieces of the same sequences
+    out, lse = run_paged(ctx, p, q, new, heads, dim, window, dtype, max_len=1)
+    check_attention(out, lse, want, "paged rows, uncut")
+
+
+@pytest.mark.parametrize("heads,dim,new", [(4, 64, 6), (4, 64, 80), (4, 128, 7), (4, 128, 12), (4, 128, 60), (2, 256, 11)])
+def test_paged_rows_special_values_and_bad_pages(ctx, heads, dim, new):
+    say(f"paged rows: NaN codes that some rows see, rubbish behind the sequences, a bad page; {heads} heads of {dim}, {new} new")
+    lengths, page = [150, 90], 32
+    p = Paged(7, lengths, 1, dim, page)
+    seen = (lengths[0] - new + 3, 20, lengths[0] - 1)  # by some rows; before some windows; by the last row
+    for side, codes in ((0, p.k), (1, p.v.transpose(2, 3))):
+        for pos in seen:
+            codes[p.table[0, pos // page].long(), 0, pos % page, 7] = 0x7F if side else 0xFF
+        for i, n in enumerate(lengths):
+            for pos in range(n, -(-n // page) * page):
+                codes[p.table[i, pos // page].long(), :, pos % page] = 0xFF
+    p.upload()
+    q = rand(gen(4), 2 * new, heads, dim, dtype=BF16).cuda()
+    for keys in (True, False):
+        if not keys:  # the values alone
+            for pos in seen:
+                p.k[p.table[0, pos // page].long(), 0, pos % page, 7] = 0x10
+            p.upload()
+        for w in (0, 50):
+            out, _ = run_paged(ctx, p, q, [new, new], heads, dim, window=w)
+            want = paged_want(p, q, [new, new], w)
+            assert torch.equal(out.isnan().cpu(), want[0].isnan())
+            assert bool(want[0].isnan().any()) and not bool(out[new:].isnan().any())
+            tol = 2.0 ** -8 * 17 / 16 * want[2] + 2.0 ** -8 * want[0].abs()
+            ok = ~want[0].isnan()
+            assert bool(((out.cpu().double() - want[0]).abs() <= tol)[ok].all())
+    ctx.launch_status()
+    p.table[0, 1] = 10_000
+    p.upload()
+    out, lse = run_paged(ctx, p, q, [new, new], heads, dim)
+    assert bool(out[:new].isnan().all()) and bool(lse[:new].isnan().all()) and bool(out[new:].isfinite().all())
+    with pytest.raises(s14.S14Error, match="cache page"):
+        ctx.launch_status()
+
+
+@pytest.mark.parametrize("heads,kv,dim,new", [(8, 2, 128, 1), (8, 1, 128, 3), (8, 1, 64, 7), (4, 1, 256, 9), (16, 1, 512, 2)])
+@pytest.mark.parametrize("lo", [40, 200])
+def test_paged_far_scales(ctx, heads, kv, dim, new, lo):
+    """Page scales far from 1 on the values' side, and on the keys' with queries
+    that undo them."""
+    say(f"paged: scales near 2^{lo - 127}, heads={heads}/{kv} dim={dim} new={new}")
+    p = Paged(5, [200, 70], kv, dim, 32, lo=lo, hi=lo + 6)
+    q = (rand(gen(4), 2 * new, heads, dim) * 2.0 ** (120 - lo)).to(BF16).cuda()
+    out, _ = run_paged(ctx, p, q, [new, new], heads, dim, dtype=F32, lse=False)
+    o, _, mass, _ = paged_want(p, q, [new, new])
+    # Below 2^-126 a bf16 weight or an f32 product may count as zero.  A weight
+    # stands beside a code (448 at most), a product beside none, and the weights'
+    # sum is at least 1: 200 tokens lose at most 200 * 448 * 2^-126.
+    tol = 2.0 ** -8 * 17 / 16 * mass + 200 * 448 * 2.0 ** -126
+    assert bool(((out.cpu().double() - o).abs() <= tol).all())
+
+
 def test_paged_strides_scale_and_extreme_scores(ctx):
     say("paged: a slice of a projection as q, output in a wider row, large scores")
     p = Paged(3, [70, 200], 2, 128, 32, lo=124, hi=127)
