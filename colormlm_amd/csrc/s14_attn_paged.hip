@@ -65,11 +65,13 @@ __device__ __forceinline__ void store_out(const AttnOut &o, uint64_t at, float a
     *reinterpret_cast<float4 *>(static_cast<float *>(o.p) + at) = make_float4(a, b, c, d);
 }
 
-// What a workgroup works on.  Row tiles are the slowest index: those that read
-// the same pages are a multiple of all items apart.  Chunks come before them,
-// so that the late chunks, which short sequences lack, are together: among the
-// sequences the empty workgroups fell to the same compute units (128 ragged
-// sequences of 8,192 tokens at most, 4 chunks: 228 us; 160 now).
+// What a workgroup works on.  Row tiles, which read the same pages, are 8
+// workgroups apart, on one XCD at about the same time (64 sequences of 4,000
+// tokens, 64 heads of 512 in two row tiles: 118 us a whole launch apart, 105 so;
+// 4 of 100 new of up to 4,000: 63 and 48).  Chunks are the slowest index of the
+// others, so that the late chunks, which short sequences lack, are together:
+// among the sequences the empty workgroups fell to the same compute units (128
+// ragged sequences of 8,192 tokens at most, 4 chunks: 228 us; 160 now).
 // Workgroup i runs on XCD i % 8: where (sequence, key head) pairs are few, a
 // chunk's pairs are rotated each time their start comes back to the first XCD,
 // or one long sequence would have but some of the XCDs.
@@ -78,7 +80,14 @@ struct Item {
 };
 __device__ __forceinline__ Item item_of(const PagedArgs &a, const PagedPlan &p, uint32_t kvh) {
   const uint32_t pairs = kvh * a.seqs, items = pairs * p.chunks;
-  const uint32_t tile = blockIdx.x / items, item = blockIdx.x % items, chunk = item / pairs;
+  const uint32_t tiles = gridDim.x / items, whole = items & ~7u, i = blockIdx.x;
+  uint32_t tile, item;
+  if (i < whole * tiles) {
+    tile = i / 8 % tiles, item = i / (8 * tiles) * 8 + i % 8;
+  } else {
+    tile = (i - whole * tiles) / (items - whole), item = whole + (i - whole * tiles) % (items - whole);
+  }
+  const uint32_t chunk = item / pairs;
   const uint32_t zeros = __builtin_ctz(pairs | 8u);
   const uint32_t pair = (item % pairs + (chunk >> (3 - zeros))) % pairs;
   return {tile, chunk, pair / kvh, pair % kvh};
