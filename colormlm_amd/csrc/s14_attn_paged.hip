@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   const uint32_t row0 = tile * 16 * NT;
   const Span sp = paged_span(a, p, seq, row0);
   if (row0 >= sp.rows || (chunk && chunk >= sp.chunks)) return;
-  const uint32_t wave = threadIdx.x / 64, l = threadIdx.x & 63u, n = l & 15u, g = l >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page;
   const uint32_t shift = __builtin_ctz(P);
   const Pages pages{a.page_table + uint64_t(seq) * a.table_width, sp.len, a.cache.pages, shift};
@@ -293,14 +293,14 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   };
   auto load_k = [&](int32_t b) {
     const uint32_t at = (uint32_t(b + 4 * T * int32_t(n / 4)) & (P - 1)) + (n & 3u);
+    pagev = pages.checked(idv, bad);
+    const uint64_t sat = uint64_t(pagev) * kvh + head;
+    ksc = a.cache.ks[sat], vsc = a.cache.vs[sat];  // first: they are waited for before K
     const uint8_t *kp = a.cache.k + (uint64_t(pages.checked(idk, bad)) * kvh + head) * page_bytes + at * uint32_t(D) + 16 * g;
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int c = 0; c < C; ++c) kk[t][c] = *reinterpret_cast<const uint4 *>(kp + 4 * t * D + 64 * c);
-    pagev = pages.checked(idv, bad);
-    const uint64_t sat = uint64_t(pagev) * kvh + head;
-    ksc = a.cache.ks[sat], vsc = a.cache.vs[sat];
   };
   auto load_v = [&](int32_t b) {
     const uint8_t *vp = a.cache.v + (uint64_t(pagev) * kvh + head) * page_bytes + n * P +
@@ -313,18 +313,34 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   };
   constexpr int32_t kStride = 4 * 16 * T;  // the wavefronts' steps interleave
   int32_t b = begin + 16 * T * int32_t(wave);
+  const int32_t last = b + (end - 1 - b) / kStride * kStride;
   if (b < end) {
+    int32_t idk1, idv1;
     load_ids(b, idk, idv);
+    load_ids(min(b + kStride, last), idk1, idv1);
     load_k(b);
     load_v(b);
-    if (b + kStride < end) load_ids(b + kStride, idk, idv);
+    // waited for here and not, with K and V, in every step
+    asm volatile("" : "+v"(idk1), "+v"(idv1));
+    idk = idk1, idv = idv1;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2 * C; ++c) asm volatile("; a step's operands" : "+v"(q[nt][c]));
+  } else {  // on this way to the loop too; in other words, or both would be done where the ways meet
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2 * C; ++c) asm volatile("; no step" : "+v"(q[nt][c]));
   }
 
   for (; b < end; b += kStride) {
     const int32_t tv = b + 4 * T * int32_t(g);
-    const bool more = b + kStride < end;
-    int32_t idk2 = 0, idv2 = 0;  // ahead of the K and V loads below
-    if (b + 2 * kStride < end) load_ids(b + 2 * kStride, idk2, idv2);
+    // past the last step that step's again: a load behind a branch makes every
+    // later wait one for all loads
+    const int32_t next = min(b + kStride, last);
+    int32_t idk2, idv2;  // ahead of the K and V loads below
+    load_ids(min(b + 2 * kStride, last), idk2, idv2);
     const float ks = scale * power_of_two(int(ksc) - 127);
     const float vs = power_of_two(int(vsc) - 127);
     f32x4 s[NT][T];
@@ -343,7 +359,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
           s[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q[nt][2 * c + 1], s[nt][t], 0, 0, 0);
         }
       }
-    if (more) load_k(b + kStride);
+    load_k(next);
     const bool partial = b + 16 * T - 1 > pos_lo || (a.window && int64_t(b) <= int64_t(pos_hi) - a.window);
     bf16x8 pb[NT][T / 2];
 #pragma unroll
@@ -415,7 +431,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
         for (int nt = 0; nt < NT; ++nt)
           o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pb[nt][u], o[nt][dt], 0, 0, 0);
       }
-    if (more) load_v(b + kStride);
+    load_v(next);
     idk = idk2, idv = idv2;
   }
 
@@ -523,14 +539,17 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
 
 // Heads of 512 (one wide key head for many query heads): 16 NT rows of Q and O
 // do not fit a wavefront, and rows in pieces of 16 would read every page again
-// for each.  Here a wavefront keeps a quarter of the head, 128 dimensions, of
-// all the workgroup's rows, and no byte of the cache goes to two wavefronts:
-// its part of S^T goes to LDS, wavefront w sums row tile w's parts and takes
-// the softmax, its P goes back through LDS in the operand layout, and each
-// wavefront's second product gives its quarter of O.
+// for each.  Here no byte of the cache goes to two wavefronts.  Of a step's 64
+// tokens a wavefront takes 16 for the first product, all dimensions of them,
+// against Q from LDS; the wavefronts' maxima meet there, each weights its own
+// scores, and P goes through LDS for the second product, of which a wavefront
+// takes 128 dimensions, all tokens.  Two workgroups a compute unit: with 64
+// rows, one of them, 64 sequences of 4,000 tokens of 64 heads took 109 us, 97
+// here (2.8 TB/s, 346 TFLOP/s).  Instruction issue bounds it, two wavefronts a
+// SIMD, about 900 instructions a step beside 1,024 clocks of the matrix unit.
 template <int NT>
 __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p, float *part) {
-  constexpr int D = 512, T = 4, C = 2, DT = 8;
+  constexpr int D = 512, C = 8, DT = 8;
   const uint32_t kvh = a.cache.heads, group = a.heads / kvh;
   const Item it = item_of(a, p, kvh);
   const uint32_t tile = it.tile, head = it.head, seq = it.seq, chunk = it.chunk;
@@ -547,128 +566,128 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
     const uint32_t r = row0 + 16 * nt + n;
     return r < sp.rows ? r : sp.rows - 1;
   };
-  const auto see_of = [&](int nt) { return Visible(sp.pos0 + int32_t(row_of(nt) / group), a.window); };
+  Visible see[NT];
 
-  bf16x8 q[NT][2 * C];
+  __shared__ bf16x8 s_q[NT][2 * C][64];  // the first product's operands
+  __shared__ bf16x8 s_p[NT][2][64];      // the second's
+  __shared__ float s_m[4][NT][16], s_l[4][NT][16];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const uint32_t rr = row_of(nt);
+    see[nt] = Visible(sp.pos0 + int32_t(rr / group), a.window);
     const uint16_t *row = a.q + uint64_t(sp.first + rr / group) * a.q_token +
-                          uint64_t(head * group + rr % group) * a.q_head + d0;
+                          uint64_t(head * group + rr % group) * a.q_head;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C / 4; ++c)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) q[nt][2 * c + h] = *reinterpret_cast<const bf16x8 *>(row + 64 * c + 16 * g + 8 * h);
+      for (int h = 0; h < 2; ++h)
+        s_q[nt][2 * (2 * wave + c) + h][l] = *reinterpret_cast<const bf16x8 *>(row + 64 * (2 * wave + c) + 16 * g + 8 * h);
   }
   const int32_t pos_lo = sp.pos0 + int32_t(row0 / group), pos_hi = sp.hi - 1;
-  const bool softmax = wave < NT;  // wavefront w: row tile w
-  const Visible see = see_of(softmax ? int(wave) : 0);
-
-  __shared__ f32x4 s_part[4][NT][T][64];
-  __shared__ bf16x8 s_p[NT][T / 2][64];
-  __shared__ float s_fade[NT][16], s_m[NT][16], s_l[NT][16];
 
   f32x4 o[NT][DT] = {};
-  float m = -INFINITY, sum = 0.0f;
+  float m[NT], sum[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) m[nt] = -INFINITY, sum[nt] = 0.0f;
   bool bad = false, odd = false;
   const float scale = a.scale * kLog2e;
   const uint64_t page_bytes = uint64_t(P) * D;
 
-  uint4 kk[T][C], vv[DT];
+  // K: 16 dimensions of token 16 wave + n eight times; V: 16 tokens from 16 g of
+  // dimensions d0 + 16 dt + n.  (The K tokens' page is one for the wavefront,
+  // but not said so: a scalar id or scale would be waited for where it is
+  // loaded, with all loads before it.)
+  constexpr int32_t kStep = 64;
+  const uint32_t k_tok = threadIdx.x / 64 * 16;
+  uint4 kk[C], vv[DT];
   uint32_t ksc = 0, vsc = 0;
   int32_t idk = 0, idv = 0;  // of the next step
-  uint32_t pagev = 0;
   auto load_ids = [&](int32_t b, int32_t &k, int32_t &v) {
-    k = pages.id(b + 4 * T * int32_t(n / 4));
-    v = pages.id(b + 4 * T * int32_t(g));
+    k = pages.id(b + int32_t(k_tok));
+    v = pages.id(b + 16 * int32_t(g));
   };
+  uint32_t pagev = 0;
   auto load_k = [&](int32_t b) {
-    const uint32_t at = (uint32_t(b + 4 * T * int32_t(n / 4)) & (P - 1)) + (n & 3u);
-    const uint8_t *kp = a.cache.k + (uint64_t(pages.checked(idk, bad)) * kvh + head) * page_bytes + at * uint32_t(D) + d0 + 16 * g;
+    const uint64_t at = uint64_t(pages.checked(idk, bad)) * kvh + head;
+    ksc = a.cache.ks[at], vsc = a.cache.vs[at];  // first: they are waited for before K
+    const uint8_t *kp = a.cache.k + at * page_bytes + ((uint32_t(b + int32_t(k_tok)) & (P - 1)) + n) * uint32_t(D) + 16 * g;
 #pragma unroll
-    for (int t = 0; t < T; ++t)
-#pragma unroll
-      for (int c = 0; c < C; ++c) kk[t][c] = *reinterpret_cast<const uint4 *>(kp + 4 * t * D + 64 * c);
+    for (int c = 0; c < C; ++c) kk[c] = *reinterpret_cast<const uint4 *>(kp + 64 * c);
     pagev = pages.checked(idv, bad);
-    const uint64_t sat = uint64_t(pagev) * kvh + head;
-    ksc = a.cache.ks[sat], vsc = a.cache.vs[sat];
   };
   auto load_v = [&](int32_t b) {
     const uint8_t *vp = a.cache.v + (uint64_t(pagev) * kvh + head) * page_bytes + (d0 + n) * P +
-                        (uint32_t(b + 4 * T * int32_t(g)) & (P - 1));
+                        (uint32_t(b + 16 * int32_t(g)) & (P - 1));
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) vv[dt] = *reinterpret_cast<const uint4 *>(vp + 16 * dt * P);
   };
-  constexpr int32_t kStep = 16 * T;
+  const int32_t last = begin + (end - 1 - begin) / kStep * kStep;
   if (begin < end) {
+    int32_t idk1, idv1;
     load_ids(begin, idk, idv);
+    load_ids(min(begin + kStep, last), idk1, idv1);
     load_k(begin);
     load_v(begin);
-    if (begin + kStep < end) load_ids(begin + kStep, idk, idv);
+    asm volatile("" : "+v"(idk1), "+v"(idv1));  // waited for here and not, with K and V, in every step
+    idk = idk1, idv = idv1;
   }
+  __syncthreads();
 
   for (int32_t b = begin; b < end; b += kStep) {
-    const int32_t tv = b + 4 * T * int32_t(g);
-    const bool more = b + kStep < end;
-    int32_t idk2 = 0, idv2 = 0;  // ahead of the K and V loads below
-    if (b + 2 * kStep < end) load_ids(b + 2 * kStep, idk2, idv2);
+    const int32_t tv = b + 16 * int32_t(g), tk = b + int32_t(k_tok) + 4 * int32_t(g);
+    // past the last step that step's again: a load behind a branch makes every
+    // later wait one for all loads
+    const int32_t next = min(b + kStep, last);
+    int32_t idk2, idv2;  // ahead of the K and V loads below
+    load_ids(min(b + 2 * kStep, last), idk2, idv2);
     const float ks = scale * power_of_two(int(ksc) - 127);
     const float vs = power_of_two(int(vsc) - 127);
     const bool partial = b + kStep - 1 > pos_lo || (a.window && int64_t(b) <= int64_t(pos_hi) - a.window);
+    f32x4 s[NT][2] = {};
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-      f32x4 s[NT] = {};
+    for (int c = 0; c < C; ++c) {
+      const bf16x8 k0 = e4m3_bf16(kk[c].x, kk[c].y), k1 = e4m3_bf16(kk[c].z, kk[c].w);
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const bf16x8 k0 = e4m3_bf16(kk[t][c].x, kk[t][c].y), k1 = e4m3_bf16(kk[t][c].z, kk[t][c].w);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          s[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q[nt][2 * c], s[nt], 0, 0, 0);
-          s[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q[nt][2 * c + 1], s[nt], 0, 0, 0);
-        }
+      for (int nt = 0; nt < NT; ++nt) {
+        s[nt][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, s_q[nt][2 * c][l], s[nt][0], 0, 0, 0);
+        s[nt][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, s_q[nt][2 * c + 1][l], s[nt][1], 0, 0, 0);
       }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s_part[wave][nt][t][l] = s[nt];
     }
-    if (more) load_k(b + kStep);
-    __syncthreads();
-    if (softmax) {
-      float x[4 * T];
+    load_k(next);
+    float x[NT][4];
 #pragma unroll
-      for (int t = 0; t < T; ++t) {
-        const f32x4 s = s_part[0][wave][t][l] + s_part[1][wave][t][l] + s_part[2][wave][t][l] + s_part[3][wave][t][l];
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[4 * t + i] = s[i] * ks;
-      }
+      for (int i = 0; i < 4; ++i) x[nt][i] = (s[nt][0][i] + s[nt][1][i]) * ks;
       if (partial) {
         keep_branch();
 #pragma unroll
-        for (int i = 0; i < 4 * T; ++i) x[i] = see(tv + i) ? x[i] : -INFINITY;
+        for (int i = 0; i < 4; ++i) x[nt][i] = see[nt](tk + i) ? x[nt][i] : -INFINITY;
       }
-      float top = x[0];
+      const float top = max_lane16(fmaxf(fmaxf(x[nt][0], x[nt][1]), fmaxf(x[nt][2], x[nt][3])));
+      if (g == 0) s_m[wave][nt][n] = top;
+    }
+    __syncthreads();
 #pragma unroll
-      for (int i = 1; i < 4 * T; ++i) top = fmaxf(top, x[i]);
-      top = fmaxf(m, max_lane16(top));
-      float fade = 1.0f;
-      if (__any(top > m + kRise)) {
-        fade = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
-        m = top;
-        sum *= fade;
+    for (int nt = 0; nt < NT; ++nt) {
+      const float top = fmaxf(fmaxf(fmaxf(s_m[0][nt][n], s_m[1][nt][n]), fmaxf(s_m[2][nt][n], s_m[3][nt][n])), m[nt]);
+      if (__any(top > m[nt] + kRise)) {  // the same in every wavefront
+        const float fade = __builtin_amdgcn_exp2f(m[nt] - (top == -INFINITY ? 0.0f : top));
+        m[nt] = top;
+        sum[nt] *= fade;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[nt][dt] *= fade;
       }
-      if (g == 0) s_fade[wave][n] = fade;
-      const float at = m == -INFINITY ? 0.0f : m;
+      const float at = m[nt] == -INFINITY ? 0.0f : m[nt];
+      float e[4];
 #pragma unroll
-      for (int u = 0; u < T / 2; ++u) {
-        u32x4 w;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float e0 = __builtin_amdgcn_exp2f(x[8 * u + 2 * j] - at), e1 = __builtin_amdgcn_exp2f(x[8 * u + 2 * j + 1] - at);
-          sum += e0;
-          sum += e1;
-          w[j] = bf16_pair(e0 * vs, e1 * vs);  // half a step of each weight: the matrix operand's type
-        }
-        s_p[wave][u][l] = __builtin_bit_cast(bf16x8, w);
+      for (int i = 0; i < 4; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(x[nt][i] - at);
+        sum[nt] += e[i];
       }
+      // half a step of each weight: the matrix operand's type
+      reinterpret_cast<uint2 *>(&s_p[nt][g / 2][16 * wave + n])[g & 1] =
+          make_uint2(bf16_pair(e[0] * vs, e[1] * vs), bf16_pair(e[2] * vs, e[3] * vs));
     }
     __syncthreads();
     if (partial) {  // as in k_paged_attention
@@ -693,19 +712,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
         }
       }
     }
+    bf16x8 pb[NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const float fade = s_fade[nt][n];
-      if (__any(fade != 1.0f)) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[nt][dt] *= fade;
-      }
-    }
-    bf16x8 pb[NT][T / 2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int u = 0; u < T / 2; ++u) pb[nt][u] = s_p[nt][u][l];
+    for (int nt = 0; nt < NT; ++nt) pb[nt][0] = s_p[nt][0][l], pb[nt][1] = s_p[nt][1][l];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const bf16x8 v0 = e4m3_bf16(vv[dt].x, vv[dt].y), v1 = e4m3_bf16(vv[dt].z, vv[dt].w);
@@ -715,7 +724,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
         o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pb[nt][1], o[nt][dt], 0, 0, 0);
       }
     }
-    if (more) load_v(b + kStep);
+    load_v(next);
     idk = idk2, idv = idv2;
   }
 
@@ -732,7 +741,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
             nan[i] = (vp[(16 * dt + 4 * g + i) * P] & 0x7fu) == 0x7fu ? __uint_as_float(0x7fc00000u) : 0.0f;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const bool in = see_of(nt)(j);
+            const bool in = see[nt](j);
             f32x4 back;
 #pragma unroll
             for (int i = 0; i < 4; ++i) back[i] = in ? nan[i] : 0.0f;
@@ -742,13 +751,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
       }
     }
   }
-  if (__any(bad)) {  // every wavefront has read the same ids
+  if (__any(bad)) {  // every wavefront has read the same V ids
     if (l == 0) atomicOr(a.status, kStatusBadCachePage);
-    sum = __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) sum[nt] = __uint_as_float(0x7fc00000u);
   }
-  if (softmax) {
-    sum = sum_lane16(sum);
-    if (g == 0) s_m[wave][n] = m, s_l[wave][n] = sum;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    sum[nt] = sum_lane16(sum[nt]);
+    if (g == 0) s_l[wave][nt][n] = sum[nt];
   }
   __syncthreads();
   const uint32_t floats = p.rec_rows * kRecord<D>;
@@ -757,7 +768,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
   for (int nt = 0; nt < NT; ++nt) {
     const uint32_t r = row0 + 16 * nt + n;
     if (r >= sp.rows) continue;
-    const float top = s_m[nt][n], total = s_l[nt][n];
+    const float top = m[nt], total = s_l[0][nt][n] + s_l[1][nt][n] + s_l[2][nt][n] + s_l[3][nt][n];
     if (sp.chunks > 1) {
       const uint32_t row = (16 * nt + n) * kRecord<D>;
       if (wave == 0 && g == 0) store(row + D, f32x4{top, total, 0.0f, 0.0f});
