@@ -80,10 +80,12 @@ class Rope:
             _refuse(N.S14_ERR_SHAPE, "a rotation table is contiguous float32 [positions, rot]")
         if start < 0:
             _refuse(N.S14_ERR_SHAPE, f"rotation start {start}")
-        self.table, self.layout, self.start = table, layout, start
+        self._table, self.layout, self.start = table, layout, start
         self._c = N.Rope(N.Buffer(table.data_ptr(), table.nbytes), table.shape[0], table.shape[1], start,
                          _LAYOUTS[layout])
         self._at, self._device = C.addressof(self._c), table.get_device()
+
+    table = property(lambda self: self._table)  # its address is held: not to be replaced
 
 
 def _rope(ctx: Context, rope: Optional[Rope]):
@@ -124,11 +126,17 @@ class KvCache:
             _refuse(N.S14_ERR_SHAPE, f"v codes must be [{pages}, {heads}, {dim}, {page}]")
         if tuple(k_scales.shape) != (pages, heads) or tuple(v_scales.shape) != (pages, heads):
             _refuse(N.S14_ERR_SHAPE, f"scales must be [{pages}, {heads}]")
-        self.k_pages, self.k_scales, self.v_pages, self.v_scales = k_pages, k_scales, v_pages, v_scales
+        self._tensors = (k_pages, k_scales, v_pages, v_scales)
         self.pages, self.heads, self.page_tokens, self.dim = pages, heads, page, dim
         buf = [N.Buffer(t.data_ptr(), t.nbytes) for t in (k_pages, v_pages, k_scales, v_scales)]
         self._c = N.KvCache(*buf, pages, heads, page, dim)
         self._at, self._device = C.addressof(self._c), k_pages.get_device()
+
+    # their addresses are held: not to be replaced
+    k_pages = property(lambda self: self._tensors[0])
+    k_scales = property(lambda self: self._tensors[1])
+    v_pages = property(lambda self: self._tensors[2])
+    v_scales = property(lambda self: self._tensors[3])
 
     @classmethod
     def empty(cls, pages: int, heads: int, page_tokens: int, dim: int, device="cuda") -> "KvCache":

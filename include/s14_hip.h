@@ -511,7 +511,7 @@ typedef struct {
  * nearest even.  Slots past the last new token stay as they were.  A NaN is
  * stored as NaN (it sets no scale), an infinity as the largest value of the
  * largest scale.  A page outside the cache or past the table takes nothing.
- * Pages written by one call belong to one sequence each. */
+ * A page that one call writes stands in one place of one sequence's row. */
 int s14_kv_append(s14_ctx *ctx, void *stream, const s14_kv_cache *cache, uint32_t tokens,
                   uint32_t seqs, uint32_t max_new, const s14_rows *k, const s14_rows *v,
                   s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer past,
