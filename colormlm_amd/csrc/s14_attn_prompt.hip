@@ -112,15 +112,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(Prom
   Block blk;
   if (!find_block(a, blockIdx.x / a.kv_heads, group, blk)) return;
   const uint32_t wave = threadIdx.x / 64, l = threadIdx.x & 63u, n = l & 31u, h = l >> 5;
-  const uint64_t rows = uint64_t(blk.len) * group;
+  const uint32_t rows = uint32_t(blk.len) * group;  // below 2^31 in all: so the launch is checked
   const uint32_t wrow = blk.row0 + 32 * wave;
 
-  const uint64_t r = wrow + n < rows ? wrow + n : rows - 1;
+  const uint32_t r = wrow + n < rows ? wrow + n : rows - 1;
   const int32_t pos = int32_t(r / group);
   const uint32_t window = kWindow ? a.window : 0u;
   const Visible see(pos, window);
   // tokens that the workgroup, and this wavefront, walk
-  const uint64_t blk_last = (blk.row0 + kPromptRows < rows ? blk.row0 + kPromptRows : rows) - 1;
+  const uint32_t blk_last = (blk.row0 + kPromptRows < rows ? blk.row0 + kPromptRows : rows) - 1;
   const int32_t hi = int32_t(blk_last / group) + 1;
   const int32_t blk_first = int32_t(blk.row0 / group);
   const int32_t lo = kWindow && blk_first + 1 > int64_t(window) ? (blk_first + 1 - int32_t(window)) & ~(KT - 1) : 0;
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(Prom
   bf16x8 q[KS];
   const auto load_q = [&]() {
     const uint16_t *row = a.q + uint64_t(blk.first + pos) * a.q_token +
-                          uint64_t(head * group + uint32_t(r % group)) * a.q_head;
+                          uint64_t(head * group + r % group) * a.q_head;
 #pragma unroll
     for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const bf16x8 *>(row + 16 * k + 8 * h);
     // Q is here before the walk: its first use, in the loop, would otherwise
@@ -357,23 +357,36 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(Prom
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
     sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
   }
-  if (wrow + n >= rows) return;
+  const bool mine = wrow + n < rows;
   const uint64_t t = uint64_t(blk.first + pos);
-  const uint32_t qh = head * group + uint32_t(r % group);
+  const uint32_t qh = head * group + r % group;
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const uint64_t to = t * a.out.token + uint64_t(qh) * a.out.head + 4 * h;
+  const uint64_t to = t * a.out.token + uint64_t(qh) * a.out.head;
+  if (a.out.bf16) {
+    // lanes l and l + 32 have the halves of a row's eight values; after the
+    // swap one has the first eight, the other the next
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const uint64_t at = to + 32 * dt + 2 * i;
-      if (a.out.bf16)
-        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out.p) + at) =
-            make_uint2(bf16_pair(o[dt][i] * inv, o[dt][i + 1] * inv), bf16_pair(o[dt][i + 2] * inv, o[dt][i + 3] * inv));
-      else
-        *reinterpret_cast<float4 *>(static_cast<float *>(a.out.p) + at) =
+      for (int i = 0; i < 16; i += 8) {
+        const auto y = __builtin_amdgcn_permlane32_swap(bf16_pair(o[dt][i] * inv, o[dt][i + 1] * inv),
+                                                        bf16_pair(o[dt][i + 4] * inv, o[dt][i + 5] * inv), false, false);
+        const auto z = __builtin_amdgcn_permlane32_swap(bf16_pair(o[dt][i + 2] * inv, o[dt][i + 3] * inv),
+                                                        bf16_pair(o[dt][i + 6] * inv, o[dt][i + 7] * inv), false, false);
+        if (mine) {
+          const u32x4 w = {y[0], z[0], y[1], z[1]};
+          *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.out.p) + to + 32 * dt + 2 * i + 8 * h) = w;
+        }
+      }
+  } else if (mine) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4 *>(static_cast<float *>(a.out.p) + to + 32 * dt + 2 * i + 4 * h) =
             make_float4(o[dt][i] * inv, o[dt][i + 1] * inv, o[dt][i + 2] * inv, o[dt][i + 3] * inv);
-    }
+  }
+  if (!mine) return;
   if (a.lse && h == 0) a.lse[t * a.heads + qh] = sum == 0.0f ? -INFINITY : m * kLn2 + __logf(sum);
 }
 
