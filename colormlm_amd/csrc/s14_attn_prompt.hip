@@ -16,6 +16,7 @@
 
 #include "s14_attn.hpp"
 #include "s14_attn_util.hpp"
+#include "s14_device_util.hpp"
 
 namespace s14 {
 namespace {
@@ -28,12 +29,43 @@ constexpr uint32_t kPromptRows = 128;
 
 // Row block `index` of the packed sequences: its sequence's first token and
 // length, and the block within it.  Every sequence has its rows in whole
-// blocks, the last ones first (the longest work leads).
+// blocks, its last ones, with the most keys to walk, first.  kMixed (up to 64
+// sequences, of 8 blocks in the mean): of each sequence the blocks 8 q .. 8 q +
+// 7, which share its tiles in L2, from the highest q down, so that no long
+// block is left for the end (us, one sequence after the other / mixed: 12 of
+// up to 2,749 tokens 130 / 120, 7 of up to 2,977 142 / 135, 64 of up to 1,000 89
+// / 90: finding the block takes a little longer).  A window's blocks are alike.
 struct Block {
   int64_t first;
   int32_t len;
   uint32_t row0;
 };
+constexpr uint32_t kTogether = 8;
+
+// The sum of v over the wavefront, in each lane.
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0xb1, 0xf, 0xf, false));   // quad_perm [1,0,3,2]
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x4e, 0xf, 0xf, false));   // quad_perm [2,3,0,1]
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x141, 0xf, 0xf, false));  // row_half_mirror
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x140, 0xf, 0xf, false));  // row_mirror
+  auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = r[0] + r[1];
+  r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return r[0] + r[1];
+}
+
+// The sums of v over the lanes up to each.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  const uint32_t l = threadIdx.x & 63u;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t o = __shfl_up(v, d);
+    if (l >= uint32_t(d)) v += o;
+  }
+  return v;
+}
+
+template <bool kMixed>
 __device__ __forceinline__ bool find_block(const PromptArgs &a, uint32_t index, uint32_t group, Block &out) {
   const uint32_t l = threadIdx.x & 63u;
   uint32_t before = 0;
@@ -45,19 +77,32 @@ __device__ __forceinline__ bool find_block(const PromptArgs &a, uint32_t index, 
       len = int32_t(clamp_row(a.cu[s + 1], a.tokens)) - first;
     }
     const uint32_t blocks = len > 0 ? uint32_t((uint64_t(len) * group + kPromptRows - 1) / kPromptRows) : 0;
-    uint32_t sum = blocks;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t o = __shfl_up(sum, d);
-      if (l >= uint32_t(d)) sum += o;
+    // of every sequence, the blocks from number `low` on, `most` at the most
+    uint32_t low = 0, most = ~0u;
+    if constexpr (kMixed) {
+      const auto above = [&](uint32_t q) {  // blocks from number 8 q on
+        const uint32_t from = kTogether * q;
+        return uint32_t(__builtin_amdgcn_readfirstlane(wave_sum(blocks > from ? blocks - from : 0)));
+      };
+      uint32_t q = 0, end = (wave_max_u32(blocks) + kTogether - 1) / kTogether;
+      while (end - q > 1) {
+        const uint32_t mid = (q + end) / 2, n = above(mid);
+        if (index < n)
+          q = mid;
+        else
+          end = mid, before = n;
+      }
+      low = kTogether * q, most = kTogether;
     }
+    const uint32_t here_blocks = blocks > low ? (blocks - low < most ? blocks - low : most) : 0;
+    const uint32_t sum = wave_scan(here_blocks);
     const uint64_t here = __ballot(index - before < sum);
     if (here) {
       // one lane's values: the block is uniform, its descriptors and bounds scalar
       const int lane = __builtin_amdgcn_readfirstlane(__builtin_ctzll(here));
       out.first = __builtin_amdgcn_readlane(first, lane);
       out.len = __builtin_amdgcn_readlane(len, lane);
-      out.row0 = (__builtin_amdgcn_readlane(sum, lane) - 1 - (index - before)) * kPromptRows;
+      out.row0 = (low + __builtin_amdgcn_readlane(sum, lane) - 1 - (index - before)) * kPromptRows;
       return true;
     }
     before += __builtin_amdgcn_readlane(sum, 63);
@@ -104,13 +149,13 @@ __device__ __forceinline__ uint32_t odd_halves(uint32_t w) {  // 0x8000 in each 
   return ((e + 0x00800080u) & 0x80008000u);
 }
 
-template <int D, int KT, bool kWindow>
+template <int D, int KT, bool kWindow, bool kMixed>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(PromptArgs a) {
   constexpr int KS = D / 16, DT = D / 32, ST = KT / 32, U = KT / 16;
   __shared__ __align__(1024) uint16_t lds_k[2][KT * D], lds_v[2][KT * D];
   const uint32_t group = a.heads / a.kv_heads, head = blockIdx.x % a.kv_heads;
   Block blk;
-  if (!find_block(a, blockIdx.x / a.kv_heads, group, blk)) return;
+  if (!find_block<kMixed>(a, blockIdx.x / a.kv_heads, group, blk)) return;
   const uint32_t wave = threadIdx.x / 64, l = threadIdx.x & 63u, n = l & 31u, h = l >> 5;
   const uint32_t rows = uint32_t(blk.len) * group;  // below 2^31 in all: so the launch is checked
   const uint32_t wrow = blk.row0 + 32 * wave;
@@ -396,11 +441,22 @@ hipError_t launch_prompt_attention(hipStream_t s, const PromptArgs &a) {
   const uint32_t group = a.heads / a.kv_heads;
   const uint64_t blocks = (uint64_t(a.tokens) * group + kPromptRows - 1) / kPromptRows + a.seqs;
   const uint32_t grid = uint32_t(blocks * a.kv_heads);
-  const auto launch = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(a); };
+  const bool mixed = !a.window && a.seqs > 1 && a.seqs <= 64 && uint64_t(a.tokens) * group / kPromptRows >= 8ull * a.seqs;
+  const auto launch = [&](auto dim, auto keys) {
+    constexpr int D = decltype(dim)::value, KT = decltype(keys)::value;
+    const auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(a); };
+    if (a.window)
+      go(k_prompt_attention<D, KT, true, false>);
+    else if (mixed)
+      go(k_prompt_attention<D, KT, false, true>);
+    else
+      go(k_prompt_attention<D, KT, false, false>);
+  };
+  using std::integral_constant;
   switch (a.dim) {
-    case 64: a.window ? launch(k_prompt_attention<64, 64, true>) : launch(k_prompt_attention<64, 64, false>); break;
-    case 128: a.window ? launch(k_prompt_attention<128, 64, true>) : launch(k_prompt_attention<128, 64, false>); break;
-    case 256: a.window ? launch(k_prompt_attention<256, 32, true>) : launch(k_prompt_attention<256, 32, false>); break;
+    case 64: launch(integral_constant<int, 64>{}, integral_constant<int, 64>{}); break;
+    case 128: launch(integral_constant<int, 128>{}, integral_constant<int, 64>{}); break;
+    case 256: launch(integral_constant<int, 256>{}, integral_constant<int, 32>{}); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();

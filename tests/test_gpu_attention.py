@@ -756,6 +756,26 @@ def test_prompt_special_values_one_head_a_key(ctx, heads, dim, window):
     check_attention(out, lse, prompt_want(q, k, v, [300], window), "odd values")
 
 
+@pytest.mark.parametrize("lengths", [[130, 0, 70, 1, 200, 90], [300, 2], [1, 129, 64] * 21 + [257], [64] * 64, [70, 60] * 40])
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(64, 1, 64, BF16), (64, 2, 128, F32), (40, 1, 256, BF16)])
+def test_prompt_blocks_of_several_sequences(ctx, lengths, heads, kv, dim, dtype):
+    """Whatever order the sequences' blocks are taken in, each sequence has the
+    bits that it has alone."""
+    say(f"prompt: {len(lengths)} sequences {lengths[:4]} heads={heads}/{kv} dim={dim} {dtype}")
+    g, t = gen(len(lengths)), sum(lengths)
+    q, k, v = (rand(g, t, h, dim, dtype=BF16).cuda() for h in (heads, kv, kv))
+    out, lse = run_prompt(ctx, q, k, v, lengths, dtype=dtype)
+    at = 0
+    for n in lengths:
+        if n:
+            s = slice(at, at + n)
+            alone, alone_lse = run_prompt(ctx, q[s], k[s], v[s], [n], dtype=dtype)
+            assert torch.equal(out[s], alone) and torch.equal(lse[s], alone_lse)
+        at += n
+    s = slice(0, lengths[0])
+    check_attention(out[s], lse[s], attention64(q[s].cpu(), k[s].cpu(), v[s].cpu(), dim ** -0.5, 0), "the first sequence")
+
+
 @pytest.mark.parametrize("heads,kv,dim", [(4, 1, 128), (2, 2, 64), (2, 1, 256)])
 def test_prompt_long(ctx, heads, kv, dim):
     say(f"prompt of 2,900 tokens heads={heads}/{kv} dim={dim}: late rows against 64 bits, all against the cut form")
