@@ -47,7 +47,7 @@ def _refuse(code: int, message: str):
 
 
 def _load():
-    """The calls' C side (csrc/s14_attn_py.c) with the library's entry points."""
+    """The calls' C side (csrc/s14_attn_py.cpp) with the library's entry points."""
     path = N.LIB_DIR / "_s14attn.so"
     if not path.exists():
         raise ImportError(f"{path} is not built; run `python -m colormlm_amd.build` (there is no fallback path)")
@@ -55,8 +55,7 @@ def _load():
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
     names = ("s14_qk_norm_rope", "s14_kv_append", "s14_paged_attention", "s14_prompt_attention")
-    module.bind(tuple(C.cast(getattr(lib(), n), C.c_void_p).value for n in names),
-                (torch.float32, torch.bfloat16, torch.int32), _refuse, check, _raw_stream())
+    module.bind(tuple(C.cast(getattr(lib(), n), C.c_void_p).value for n in names), _refuse, check, _raw_stream())
     return module
 
 

@@ -14,8 +14,8 @@ into colormlm_amd/lib/libs14hip.so:
 - the host-only translation units (*.cpp: the C ABI, the pool and loader
   contracts) without that flag.
 
-Beside it lib/_s14attn.so, the attention calls' Python side (s14_attn_py.c, a
-plain CPython extension that links nothing).
+Beside it lib/_s14attn.so, the attention calls' Python side (s14_attn_py.cpp, a
+CPython extension over torch's headers and libraries, which are loaded before it).
 """
 
 from __future__ import annotations
@@ -72,9 +72,14 @@ def command(out: Path = OUT) -> list:
 
 
 def python_command(out: Path = PY_OUT) -> list:
-    cc = os.environ.get("CC") or shutil.which("gcc") or shutil.which("cc") or str(Path(hipcc()).parent / "amdclang")
-    return [cc, "-O2", "-std=c11", "-fPIC", "-shared", "-Wall", f"-I{sysconfig.get_paths()['include']}", f"-I{ROOT / 'include'}",
-            str(CSRC / "s14_attn_py.c"), "-o", str(out)]
+    import torch
+
+    cxx = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++") or str(Path(hipcc()).parent / "amdclang++")
+    home = Path(torch.__file__).resolve().parent
+    inc = home / "include"
+    return [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            f"-I{sysconfig.get_paths()['include']}", f"-I{ROOT / 'include'}", "-isystem", str(inc), "-isystem",
+            str(inc / "torch/csrc/api/include"), str(CSRC / "s14_attn_py.cpp"), f"-L{home / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", str(out)]
 
 
 def _run(cmd: list, verbose: bool) -> None:
