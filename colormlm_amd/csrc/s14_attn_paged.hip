@@ -159,7 +159,7 @@ __device__ __forceinline__ bool arrived_last(uint32_t *count, uint32_t chunks) {
 
 // Row row0 + k of a tile from its partial results, by one wavefront: lane c
 // holds chunk c's maximum and sum (64 chunks at most), then the chunks' rows in
-// order.
+// order, the first of them loaded with the maxima.
 template <int D, int kPolicy>
 __device__ __forceinline__ void join_row(const PagedArgs &a, const PagedPlan &p, const Span &sp, const Item &it,
                                          uint32_t row0, uint32_t k, const float *part) {
@@ -172,11 +172,20 @@ __device__ __forceinline__ void join_row(const PagedArgs &a, const PagedPlan &p,
   const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(first), 0,
                                                    int((sp.chunks - 1) * next + uint32_t(rec) * 4), 0x00020000);
   const uint32_t at = k * kRecord<D> * 4;
-  float m = -INFINITY, sum = 0.0f;
-  if (l < sp.chunks) {
-    const auto ml = __builtin_amdgcn_raw_buffer_load_b64(r, l * next + at + D * 4, 0, kPolicy);
-    m = __uint_as_float(ml[0]), sum = __uint_as_float(ml[1]);
-  }
+  constexpr uint32_t kAt = D == 512 ? 4 : 8;  // loads of each lane at once
+  u32x4 x[kAt][kSpan];
+  const auto load = [&](uint32_t c0) {
+#pragma unroll
+    for (uint32_t j = 0; j < kAt; ++j)
+#pragma unroll
+      for (uint32_t i = 0; i < kSpan; ++i)  // past the last chunk: zeros (descriptor range), weight 0
+        x[j][i] = __builtin_amdgcn_raw_buffer_load_b128(
+            r, (c0 + j * kSets + set) * next + at + 16 * (lane + kLanes * i), 0, kPolicy);
+  };
+  // lanes without a chunk: past the range too
+  const auto ml = __builtin_amdgcn_raw_buffer_load_b64(r, l * next + at + D * 4, 0, kPolicy);
+  load(0);
+  const float m = l < sp.chunks ? __uint_as_float(ml[0]) : -INFINITY, sum = l < sp.chunks ? __uint_as_float(ml[1]) : 0.0f;
   float top = m;
 #pragma unroll
   for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
@@ -185,20 +194,17 @@ __device__ __forceinline__ void join_row(const PagedArgs &a, const PagedPlan &p,
 #pragma unroll
   for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
   f32x4 o[kSpan] = {};
-  for (uint32_t c0 = 0; c0 < sp.chunks; c0 += 4 * kSets) {
-    u32x4 x[4][kSpan];
+  for (uint32_t c0 = 0;;) {
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j)
-#pragma unroll
-      for (uint32_t i = 0; i < kSpan; ++i)  // past the last chunk: zeros (descriptor range), weight 0
-        x[j][i] = __builtin_amdgcn_raw_buffer_load_b128(
-            r, (c0 + j * kSets + set) * next + at + 16 * (lane + kLanes * i), 0, kPolicy);
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
+    for (uint32_t j = 0; j < kAt; ++j) {
       const float f = __shfl(w, int((c0 + j * kSets + set) & 63u));
+      const bool in = c0 + j * kSets + set < sp.chunks;
 #pragma unroll
-      for (uint32_t i = 0; i < kSpan; ++i) o[i] += __builtin_bit_cast(f32x4, x[j][i]) * f;
+      for (uint32_t i = 0; i < kSpan; ++i) o[i] += __builtin_bit_cast(f32x4, x[j][i]) * (in ? f : 0.0f);
     }
+    c0 += kAt * kSets;
+    if (c0 >= sp.chunks) break;
+    load(c0);
   }
 #pragma unroll
   for (uint32_t d = kLanes; d < 64; d <<= 1)
