@@ -347,7 +347,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
     const int32_t next = min(b + kStride, last);
     int32_t idk2, idv2;  // ahead of the K and V loads below
     load_ids(min(b + 2 * kStride, last), idk2, idv2);
-    const float ks = scale * power_of_two(int(ksc) - 127);
+    const float ks = fmaxf(scale * power_of_two(int(ksc) - 127), 0x1p-126f);  // above 0: a masked score stays -inf
     const float vs = power_of_two(int(vsc) - 127);
     f32x4 s[NT][T];
 #pragma unroll
@@ -372,7 +372,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
     for (int nt = 0; nt < NT; ++nt) {
       float x[4 * T];
 #pragma unroll
-      for (int i = 0; i < 4 * T; ++i) x[i] = s[nt][i / 4][i % 4] * ks;
+      for (int i = 0; i < 4 * T; ++i) x[i] = s[nt][i / 4][i % 4];
       if (partial) {
         keep_branch();
 #pragma unroll
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
       float top = x[0];
 #pragma unroll
       for (int i = 1; i < 4 * T; ++i) top = fmaxf(top, x[i]);
-      top = fmaxf(m[nt], max_lane16(top));
+      top = fmaxf(m[nt], max_lane16(top * ks));
       // the maximum that the weights are taken from moves only where they
       // would pass 2^kRise: O is seldom multiplied
       if (__any(top > m[nt] + kRise)) {
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
         float e[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          e[i] = __builtin_amdgcn_exp2f(x[4 * t + i] - at);
+          e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[4 * t + i], ks, -at));
           sum[nt] += e[i];
         }
         // rounded to bf16, half a step of each weight: the matrix operand's type
@@ -818,7 +818,7 @@ __device__ __forceinline__ uint32_t turn_v(uint32_t dim) {
 // loads before their first product, long ones by LDS reads (2 bytes a multiply,
 // half the matrix rate at NT = 1) and the softmax beside them.
 template <int D, int NT, int RW>
-__global__ __launch_bounds__(256, D * NT <= 128 ? 3 : 2) void k_paged_rows(PagedArgs a, PagedPlan p, float *part) {
+__global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 ? 4 : 3) void k_paged_rows(PagedArgs a, PagedPlan p, float *part) {
   constexpr int TK = D <= 128 ? 64 : 32;  // tokens a step
   constexpr int TW = 4 / RW;              // wavefronts that share a row tile's tokens
   constexpr int U = TK / 32 / TW, T = 2 * U, DT = D / 16, C = D / 32;
@@ -977,7 +977,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 3 : 2) void k_paged_rows(Paged
       for (int nt = 0; nt < NT; ++nt) {
         float x[4 * T];
 #pragma unroll
-        for (int i = 0; i < 4 * T; ++i) x[i] = s[nt][i / 4][i % 4] * scale;
+        for (int i = 0; i < 4 * T; ++i) x[i] = s[nt][i / 4][i % 4];
         if (partial) {
           keep_branch();
 #pragma unroll
@@ -986,7 +986,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 3 : 2) void k_paged_rows(Paged
         float top = x[0];
 #pragma unroll
         for (int i = 1; i < 4 * T; ++i) top = fmaxf(top, x[i]);
-        top = fmaxf(m[nt], max_lane16(top));
+        top = fmaxf(m[nt], max_lane16(top) * scale);
         if (__any(top > m[nt] + kRise)) {
           const float fade = __builtin_amdgcn_exp2f(m[nt] - (top == -INFINITY ? 0.0f : top));
           m[nt] = top;
@@ -1000,7 +1000,8 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 3 : 2) void k_paged_rows(Paged
           u32x4 w;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float e0 = __builtin_amdgcn_exp2f(x[8 * u + 2 * j] - at), e1 = __builtin_amdgcn_exp2f(x[8 * u + 2 * j + 1] - at);
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * u + 2 * j], scale, -at));
+            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * u + 2 * j + 1], scale, -at));
             sum[nt] += e0;
             sum[nt] += e1;
             w[j] = bf16_pair(e0, e1);  // half a step of each weight: the matrix operand's type
