@@ -257,6 +257,10 @@ extern "C" int s14_paged_attention(s14_ctx *ctx, void *stream, const s14_rows *q
   if (max_len > uint32_t(INT32_MAX)) return fail(S14_ERR_SHAPE, "longest sequence of %u tokens", max_len);
   if (!tokens || !seqs || !max_new) return S14_OK;
   if (int rc = check_table(cu, lens, page_table, seqs, table_width, "lens")) return rc;
+  // positions, and those of the steps ahead, stay in 31 bits
+  if (uint64_t(table_width) * cache->page_tokens > (1ull << 31) - (1u << 16))
+    return fail(S14_ERR_SHAPE, "page table of %u pages of %u tokens: past %llu positions", table_width, cache->page_tokens,
+                (1ull << 31) - (1u << 16));
   a.tokens = tokens, a.seqs = seqs, a.heads = q->heads, a.max_new = max_new, a.max_len = max_len;
   a.table_width = table_width;
   a.q = static_cast<const uint16_t *>(q->buf.ptr), a.q_token = q->token_stride, a.q_head = q->head_stride;

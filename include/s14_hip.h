@@ -526,7 +526,7 @@ int s14_kv_append(s14_ctx *ctx, void *stream, const s14_kv_cache *cache, uint32_
  * [tokens][heads], or ptr NULL) the natural log of the weights' sum.  A row
  * that sees nothing is 0 with lse -inf.  max_new and max_len: at least the
  * largest count of rows, and about the longest sequence (it only sets how the
- * work is split). */
+ * work is split).  table_width * page_tokens is at most 2^31 - 2^16. */
 int s14_paged_attention(s14_ctx *ctx, void *stream, const s14_rows *q, const s14_kv_cache *cache,
                         uint32_t tokens, uint32_t seqs, uint32_t max_new, uint32_t max_len,
                         s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer lens,

@@ -150,6 +150,7 @@ def paged(native, ctx=CTX, q=rows(), c=cache(), tokens=5, seqs=2, most=3, length
     (N.S14_ERR_SHAPE, "longest", dict(length=1 << 31)),
     (N.S14_ERR_INVALID, "longest", dict(most=6)),
     (N.S14_ERR_CAPACITY, "lens", dict(lens=N.Buffer(AT, 4))),
+    (N.S14_ERR_SHAPE, "positions", dict(width=1 << 24, c=cache(page=128))),
     (N.S14_ERR_SHAPE, "one launch", dict(tokens=1 << 29, most=1 << 29, q=rows(32, token=4096), out=rows(32, token=4096),
                                          seqs=64)),
 ])
