@@ -8,6 +8,7 @@
 
 #include <cstdint>
 
+#include "s14_attn_plan.h"
 #include "s14_hip.h"
 
 namespace s14 {
@@ -93,20 +94,6 @@ struct RopeTableArgs {
   double theta, factor, original, fast, slow, amplitude;
   float *out;
 };
-
-// Work split of a paged launch.
-struct PagedPlan {
-  uint32_t row_tiles;  // 16-row tiles of a workgroup
-  uint32_t staged;     // a row tile's K and V go through LDS (k_paged_rows)
-  uint32_t rec_rows;   // rows of a chunk's partial result
-  uint32_t chunk;      // tokens of one workgroup, a multiple of 64
-  uint32_t chunks;     // of the longest sequence; above 1 the partial results go to the workspace
-  uint32_t fused;      // the last workgroup of a row tile joins its chunks; else a second launch
-  uint64_t blocks;     // workgroups
-};
-constexpr uint64_t kPagedPartFloats = 16ull << 20;  // the workspace: 64 MiB
-constexpr uint32_t kPagedCounters = 16384;          // arrivals at a row tile, 0 between launches
-PagedPlan paged_plan(const PagedArgs &a);
 
 hipError_t launch_rope_table(hipStream_t s, const RopeTableArgs &a);
 hipError_t launch_norm_rope(hipStream_t s, const NormRopeArgs &a);

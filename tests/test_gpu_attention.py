@@ -498,6 +498,24 @@ def test_paged_rows_that_see_nothing(ctx):
     ctx_status(ctx)
 
 
+@pytest.mark.parametrize("heads,kv,dim,new", [(4, 1, 128, 1), (32, 8, 128, 8), (8, 1, 64, 5), (8, 2, 128, 40), (16, 1, 512, 1),
+                                              (64, 1, 512, 3), (12, 2, 256, 9)])
+@pytest.mark.parametrize("window", [0, 70])
+def test_paged_without_cached_tokens(ctx, heads, kv, dim, new, window):
+    """max_len 0, the longest of empty sequences."""
+    say(f"paged: nothing cached, max_len 0, heads={heads}/{kv} dim={dim} new={new} window={window}")
+    p = Paged(2, [0, 0], kv, dim, 16)
+    q = rand(gen(4), 2 * new, heads, dim, dtype=BF16).cuda()
+    out, lse = run_paged(ctx, p, q, [new, new], heads, dim, window=window, max_len=0)
+    assert not out.any() and bool((lse == -math.inf).all())
+    ctx.launch_status()
+    # beside one that the promise left out
+    p = Paged(2, [0, 90], kv, dim, 16)
+    out, lse = run_paged(ctx, p, q, [new, new], heads, dim, window=window, max_len=0)
+    check_attention(out, lse, paged_want(p, q, [new, new], window), "more than promised")
+    ctx.launch_status()
+
+
 def ctx_status(ctx):
     try:
         ctx.launch_status()
