@@ -268,7 +268,8 @@ extern "C" int s14_paged_attention(s14_ctx *ctx, void *stream, const s14_rows *q
   a.cu = static_cast<const int32_t *>(cu.ptr), a.len = static_cast<const int32_t *>(lens.ptr);
   a.out = out_of(out), a.lse = static_cast<float *>(lse.ptr);
   a.scale = scale, a.window = window;
-  const s14::PagedPlan p = s14::paged_plan({seqs, a.heads, cache->heads, cache->dim, max_new, max_len, window});
+  const s14::PagedPlan p = s14::paged_plan(
+      {seqs, a.heads, cache->heads, cache->dim, max_new, max_len, window, table_width * cache->page_tokens});
   if (p.blocks >= (1u << 24) || uint64_t(max_new) * q->heads >= (1ull << 31))
     return fail(S14_ERR_SHAPE, "%u new tokens of %u sequences exceed one launch", max_new, seqs);
   a.status = s14::ctx_status(ctx), a.count = s14::ctx_attn_counters(ctx);

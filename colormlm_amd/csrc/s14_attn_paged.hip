@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   const uint32_t shift = __builtin_ctz(P);
   const Pages pages{a.page_table + uint64_t(seq) * a.table_width, sp.len, a.cache.pages, shift};
   const int32_t begin = sp.lo + int32_t(chunk * sp.chunk);
-  const int32_t end = min(sp.hi, begin + int32_t(sp.chunk));
+  const int32_t end = paged_end(begin, sp.hi, sp.chunk);
 
   // each lane's row of every tile: its position, and Q in the operand layout
   Visible see[NT];
@@ -565,7 +565,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
   const uint32_t shift = __builtin_ctz(P);
   const Pages pages{a.page_table + uint64_t(seq) * a.table_width, sp.len, a.cache.pages, shift};
   const int32_t begin = sp.lo + int32_t(chunk * sp.chunk);
-  const int32_t end = min(sp.hi, begin + int32_t(sp.chunk));
+  const int32_t end = paged_end(begin, sp.hi, sp.chunk);
   const auto row_of = [&](int nt) {
     const uint32_t r = row0 + 16 * nt + n;
     return r < sp.rows ? r : sp.rows - 1;
@@ -833,7 +833,7 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
   const uint32_t P = a.cache.page;
   const Pages pages{a.page_table + uint64_t(seq) * a.table_width, sp.len, a.cache.pages, uint32_t(__builtin_ctz(P))};
   const int32_t begin = sp.lo + int32_t(chunk * sp.chunk);
-  const int32_t end = min(sp.hi, begin + int32_t(sp.chunk));
+  const int32_t end = paged_end(begin, sp.hi, sp.chunk);
   const uint32_t mine = row0 + 16 * NT * (wave % RW), u0 = U * (wave / RW);  // the wavefront's rows and 32-token parts
   const bool active = mine < sp.rows;
 

@@ -7,9 +7,10 @@
 
 namespace s14 {
 
-// What a launch is planned by.
+// What a launch is planned by.  reach: the positions that the page table can
+// hold, 2^31 - 2^16 at most; a promise (max_len) past it is one of that.
 struct PagedShape {
-  uint32_t seqs, heads, kv_heads, dim, max_new, max_len, window;
+  uint32_t seqs, heads, kv_heads, dim, max_new, max_len, window, reach;
 };
 
 // Work split of a paged launch.
@@ -34,6 +35,12 @@ constexpr PagedCut paged_cut(uint32_t span, uint32_t chunk, uint32_t chunks) {
   const uint32_t least = ((span + chunks - 1) / chunks + 63u) & ~63u;
   const uint32_t c = chunk > least ? chunk : least;
   return {c, (span + c - 1) / c};
+}
+
+// The end of the chunk that starts at begin <= hi, in 31 bits whatever the two
+// and the chunk are.
+constexpr int32_t paged_end(int32_t begin, int32_t hi, uint32_t chunk) {
+  return uint32_t(hi - begin) > chunk ? begin + int32_t(chunk) : hi;
 }
 
 // Rows of a workgroup: all of the longest new block's up to 64 (of 32 of
@@ -75,7 +82,8 @@ inline PagedPlan paged_plan(const PagedShape &a) {
   p.staged = dim < 512 && (p.row_tiles >= 4 || (p.row_tiles == 2 && a.seqs > 1));
   const uint64_t tiles = (rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles);
   const uint64_t base = tiles * a.kv_heads * a.seqs;  // workgroups of an uncut launch
-  uint64_t span = a.max_len ? a.max_len : 1;  // a chunk is never of no tokens: the kernels divide by it
+  uint64_t span = a.max_len < a.reach ? a.max_len : a.reach;
+  if (!span) span = 1;  // a chunk is never of no tokens: the kernels divide by it
   if (a.window && uint64_t(a.window) + a.max_new + 63 < span) span = uint64_t(a.window) + a.max_new + 63;
   // workgroups that the card holds at once, by a wavefront's registers and by LDS
   const uint32_t words = (dim == 512 ? 128 : dim) * p.row_tiles;

@@ -43,9 +43,9 @@ def lib(tmp_path_factory):
     return C.CDLL(str(out))
 
 
-def plan(lib, seqs, heads, kv, dim, max_new, max_len, window=0):
+def plan(lib, seqs, heads, kv, dim, max_new, max_len, window=0, reach=REACH):
     out = (C.c_uint64 * 6)()
-    lib.attn_plan((C.c_uint32 * 7)(seqs, heads, kv, dim, max_new, max_len, window), out)
+    lib.attn_plan((C.c_uint32 * 8)(seqs, heads, kv, dim, max_new, max_len, window, reach), out)
     return Plan(*out)
 
 
@@ -58,8 +58,8 @@ def cut(lib, p, span):
 LAYOUTS = [(32, 8, 128), (64, 8, 64), (16, 16, 64), (12, 2, 256), (64, 1, 512), (7, 1, 64), (128, 1, 512)]
 
 
-def check(lib, seqs, heads, kv, dim, max_new, max_len, window=0):
-    p = plan(lib, seqs, heads, kv, dim, max_new, max_len, window)
+def check(lib, seqs, heads, kv, dim, max_new, max_len, window=0, reach=REACH):
+    p = plan(lib, seqs, heads, kv, dim, max_new, max_len, window, reach)
     part, counters = C.c_uint64(), C.c_uint32()
     lib.attn_limits(C.byref(part), C.byref(counters))
     what = (seqs, heads, kv, dim, max_new, max_len, window, p)
@@ -77,6 +77,11 @@ def check(lib, seqs, heads, kv, dim, max_new, max_len, window=0):
         chunk, chunks = cut(lib, p, span)
         assert chunk >= 64 and chunk % 64 == 0 and chunks <= p.chunks, (what, span)
         assert chunks * chunk >= span and (chunks - 1) * chunk < max(span, 1), (what, span)
+        # each chunk's end, in the kernels' 31 bits, where the span starts at position 0 and as late as it may
+        for lo in (0, (REACH - span) & ~63):
+            for i in {0, chunks - 1} if chunks else ():
+                begin = lo + i * chunk
+                assert lib.attn_end(begin, lo + span, C.c_uint32(chunk)) == min(lo + span, begin + chunk), (what, span, lo)
     return p
 
 
@@ -96,3 +101,15 @@ def test_split_without_cached_tokens(lib, heads, kv, dim, window):
     for seqs, new in itertools.product((1, 3, 128), (1, 4, 8, 40)):
         p = check(lib, seqs, heads, kv, dim, new, 0, window)
         assert p.chunks == 1 and cut(lib, p, 0)[1] <= 1
+
+
+@pytest.mark.parametrize("heads,kv,dim", LAYOUTS)
+@pytest.mark.parametrize("max_len", [REACH, (1 << 31) - 256, (1 << 31) - 255, (1 << 31) - 1])
+@pytest.mark.parametrize("window", [0, 1 << 30])
+def test_split_of_the_longest_promise(lib, heads, kv, dim, max_len, window):
+    """A max_len that promises nothing, up to the largest that is accepted: the
+    page table's reach sets the split, and no chunk passes 31 bits."""
+    for seqs, new, reach in itertools.product((1, 4, 96, 256), (1, 8, 64, 512, 2048, 1 << 20), (64, 12_000, REACH)):
+        p = check(lib, seqs, heads, kv, dim, new, max_len, window, reach)
+        assert p.chunk < 1 << 31 and p.chunk * p.chunks < reach + 256 * p.chunks
+        assert p == plan(lib, seqs, heads, kv, dim, new, reach, window, reach)

@@ -516,6 +516,21 @@ def test_paged_without_cached_tokens(ctx, heads, kv, dim, new, window):
     ctx.launch_status()
 
 
+@pytest.mark.parametrize("seqs,new,heads,kv,dim", [(40, 33, 32, 8, 128), (96, 8, 32, 8, 64), (2, 1, 32, 8, 128), (40, 4, 64, 1, 512),
+                                                   (200, 8, 12, 2, 256)])
+def test_paged_longest_promise(ctx, seqs, new, heads, kv, dim):
+    """max_len up to the largest that is accepted: planned by the page table's reach."""
+    say(f"paged: max_len 2^31 - 1, {seqs} x {new} heads={heads}/{kv} dim={dim}")
+    p = Paged(3, [70 + i % 5 for i in range(seqs)], kv, dim, 16)
+    q = rand(gen(4), seqs * new, heads, dim, dtype=BF16).cuda()
+    out, lse = run_paged(ctx, p, q, [new] * seqs, heads, dim)
+    k, v = p.rows(seqs - 1)
+    check_attention(out[-new:], lse[-new:], attention64(q[-new:].cpu(), k, v, dim ** -0.5, 0), "the last sequence")
+    for most in ((1 << 31) - 1, (1 << 31) - 255, 1 << 20):
+        again, lse2 = run_paged(ctx, p, q, [new] * seqs, heads, dim, max_len=most)
+        assert torch.equal(again, out) and torch.equal(lse2, lse)
+
+
 def ctx_status(ctx):
     try:
         ctx.launch_status()
