@@ -27,10 +27,10 @@ namespace s14 {
 namespace {
 
 // What a row tile of a sequence reads: tokens lo .. hi - 1 in chunks of
-// `chunk` (a multiple of 64, as lo is).
+// `chunk` (a multiple of 64, as lo is).  Its rows see none before `seen`.
 struct Span {
   uint32_t first, rows;  // first packed token; (token, head) rows of the sequence
-  int32_t len, pos0, lo, hi;
+  int32_t len, pos0, seen, lo, hi;
   uint32_t chunk, chunks;
 };
 
@@ -48,8 +48,9 @@ __device__ __forceinline__ Span paged_span(const PagedArgs &a, const PagedPlan &
   const uint32_t last = (row0 + 16 * p.row_tiles < s.rows ? row0 + 16 * p.row_tiles : s.rows) - 1;
   const int32_t first_pos = s.pos0 + int32_t(row0 / group), last_pos = s.pos0 + int32_t(last / group);
   s.hi = last_pos + 1 < 0 ? 0 : last_pos + 1;
-  int64_t lo = a.window ? int64_t(first_pos) - a.window + 1 : 0;
-  s.lo = int32_t(lo < 0 ? 0 : lo) & ~63;
+  const int64_t lo = a.window ? int64_t(first_pos) - a.window + 1 : 0;
+  s.seen = int32_t(lo < 0 ? 0 : lo);
+  s.lo = s.seen & ~63;
   const uint32_t span = s.hi > s.lo ? s.hi - s.lo : 0;
   const PagedCut cut = paged_cut(span, p.chunk, p.chunks);
   s.chunk = cut.chunk, s.chunks = cut.chunks;
@@ -96,14 +97,16 @@ __device__ __forceinline__ uint64_t record_of(const PagedArgs &a, const PagedPla
 }
 
 // What a wavefront needs to find a step's pages.  A lane's tokens, 4 T
-// neighbours, lie in one page; tokens behind the sequence take its last page
-// (and are masked).  An id is looked at when it is used, a step after its
-// load: looking at once would wait for every load in flight.
+// neighbours, lie in one page; tokens behind the sequence take its last page,
+// tokens of the first 64 before the window its first one (both are masked: what
+// a table holds for pages that nobody sees is not looked at).  An id is looked
+// at when it is used, a step after its load: looking at once would wait for
+// every load in flight.
 struct Pages {
   const int32_t *table;
-  int32_t len;
+  int32_t seen, last;
   uint32_t pages, shift;
-  __device__ __forceinline__ int32_t id(int32_t tok) const { return table[uint32_t(tok < len ? tok : len - 1) >> shift]; }
+  __device__ __forceinline__ int32_t id(int32_t tok) const { return table[uint32_t(min(max(tok, seen), last)) >> shift]; }
   __device__ __forceinline__ uint32_t checked(int32_t id, bool &bad) const {
     const bool out = uint32_t(id) >= pages;
     bad |= out;
@@ -253,7 +256,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page;
   const uint32_t shift = __builtin_ctz(P);
-  const Pages pages{a.page_table + uint64_t(seq) * a.table_width, sp.len, a.cache.pages, shift};
+  const Pages pages{a.page_table + uint64_t(seq) * a.table_width, sp.seen, sp.len - 1, a.cache.pages, shift};
   const int32_t begin = sp.lo + int32_t(chunk * sp.chunk);
   const int32_t end = paged_end(begin, sp.hi, sp.chunk);
 
@@ -563,7 +566,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page, d0 = 128 * wave;
   const uint32_t shift = __builtin_ctz(P);
-  const Pages pages{a.page_table + uint64_t(seq) * a.table_width, sp.len, a.cache.pages, shift};
+  const Pages pages{a.page_table + uint64_t(seq) * a.table_width, sp.seen, sp.len - 1, a.cache.pages, shift};
   const int32_t begin = sp.lo + int32_t(chunk * sp.chunk);
   const int32_t end = paged_end(begin, sp.hi, sp.chunk);
   const auto row_of = [&](int nt) {
@@ -831,7 +834,7 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
   if (row0 >= sp.rows || (chunk && chunk >= sp.chunks)) return;
   const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page;
-  const Pages pages{a.page_table + uint64_t(seq) * a.table_width, sp.len, a.cache.pages, uint32_t(__builtin_ctz(P))};
+  const Pages pages{a.page_table + uint64_t(seq) * a.table_width, sp.seen, sp.len - 1, a.cache.pages, uint32_t(__builtin_ctz(P))};
   const int32_t begin = sp.lo + int32_t(chunk * sp.chunk);
   const int32_t end = paged_end(begin, sp.hi, sp.chunk);
   const uint32_t mine = row0 + 16 * NT * (wave % RW), u0 = U * (wave / RW);  // the wavefront's rows and 32-token parts

@@ -531,6 +531,29 @@ def test_paged_longest_promise(ctx, seqs, new, heads, kv, dim):
         assert torch.equal(again, out) and torch.equal(lse2, lse)
 
 
+@pytest.mark.parametrize("heads,kv,dim,new", [(4, 2, 128, 1), (8, 2, 128, 8), (8, 1, 64, 6), (4, 1, 128, 40), (16, 1, 512, 1),
+                                              (32, 1, 512, 3), (12, 2, 256, 2), (6, 1, 256, 9)])
+@pytest.mark.parametrize("page", [16, 32])
+def test_paged_pages_behind_the_window_may_be_gone(ctx, heads, kv, dim, new, page):
+    """Pages that lie wholly before the window of a sequence's first row are not
+    looked up, wherever in 64 tokens the window starts."""
+    say(f"paged: pages before the window given back, heads={heads}/{kv} dim={dim} new={new} page={page}")
+    window, lengths = 40, [300 + 16 * i + i % 3 for i in range(5)]
+    p = Paged(6, lengths, kv, dim, page)
+    q = rand(gen(4), new * len(lengths), heads, dim, dtype=BF16).cuda()
+    want = paged_want(p, q, [new] * len(lengths), window)
+    gone = 0
+    for i, n in enumerate(lengths):
+        first = (n - new - window + 1) // page  # the first page that a row sees
+        p.table[i, :first] = -1 if i % 2 else 0x7FFFFFFF
+        gone = max(gone, first * page - ((n - new - window + 1) & ~63))
+    assert gone >= page  # some page is gone that lies behind a multiple of 64
+    p.upload()
+    out, lse = run_paged(ctx, p, q, [new] * len(lengths), heads, dim, window=window)
+    check_attention(out, lse, want, "windowed")
+    ctx.launch_status()
+
+
 def ctx_status(ctx):
     try:
         ctx.launch_status()
