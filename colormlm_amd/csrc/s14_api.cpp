@@ -659,6 +659,10 @@ int read_launch_status(const Workspace &ws, int device) {
                 "and its outputs are NaN");
   if (bits & kStatusBadPosition)
     return fail(S14_ERR_INVALID, "a position lies outside the rotation table; its rows are NaN");
+  if (bits & kStatusBadCounts)
+    return fail(S14_ERR_INVALID,
+                "a sequence has a length below 0 or past its page table (it was held to them) or more new rows than "
+                "max_new (the first max_new were taken)");
   return fail(S14_ERR_ROUTE,
               "a token's route failed RouteDecision::validate_for (expert id out of range or repeated, weight "
               "not finite or negative, or weight sum off route_scale by more than 1e-4); its outputs are NaN");

@@ -32,6 +32,7 @@ struct Span {
   uint32_t first, rows;  // first packed token; (token, head) rows of the sequence
   int32_t len, pos0, seen, lo, hi;
   uint32_t chunk, chunks;
+  bool wrong;  // its length is outside the table, or it has rows that no workgroup takes
 };
 
 __device__ __forceinline__ Span paged_span(const PagedArgs &a, const PagedPlan &p, uint32_t seq, uint32_t row0) {
@@ -42,8 +43,9 @@ __device__ __forceinline__ Span paged_span(const PagedArgs &a, const PagedPlan &
   // no more rows than the launch was planned for: below 2^31 in all
   s.rows = n <= 0 ? 0u : (uint32_t(n) < a.max_new ? uint32_t(n) : a.max_new) * group;
   const int64_t room = int64_t(a.table_width) * a.cache.page;
-  const int64_t len = a.len[seq] < 0 ? 0 : a.len[seq];
-  s.len = int32_t(len < room ? len : room);
+  const int64_t len = a.len[seq];
+  s.len = int32_t(len < 0 ? 0 : len < room ? len : room);
+  s.wrong = n > 0 && (len != s.len || uint32_t(n) > a.max_new);
   s.pos0 = s.len - n;
   const uint32_t last = (row0 + 16 * p.row_tiles < s.rows ? row0 + 16 * p.row_tiles : s.rows) - 1;
   const int32_t first_pos = s.pos0 + int32_t(row0 / group), last_pos = s.pos0 + int32_t(last / group);
@@ -55,6 +57,11 @@ __device__ __forceinline__ Span paged_span(const PagedArgs &a, const PagedPlan &
   const PagedCut cut = paged_cut(span, p.chunk, p.chunks);
   s.chunk = cut.chunk, s.chunks = cut.chunks;
   return s;
+}
+
+// Once a sequence.
+__device__ __forceinline__ void report_counts(const PagedArgs &a, const Span &s, uint32_t tile, uint32_t chunk, uint32_t head) {
+  if (s.wrong && !tile && !chunk && !head && threadIdx.x == 0) atomicOr(a.status, kStatusBadCounts);
 }
 
 __device__ __forceinline__ void store_out(const AttnOut &o, uint64_t at, float a, float b, float c, float d) {
@@ -253,6 +260,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   const uint32_t row0 = tile * 16 * NT;
   const Span sp = paged_span(a, p, seq, row0);
   if (row0 >= sp.rows || (chunk && chunk >= sp.chunks)) return;
+  report_counts(a, sp, tile, chunk, head);
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page;
   const uint32_t shift = __builtin_ctz(P);
@@ -563,6 +571,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
   const uint32_t row0 = tile * 16 * NT;
   const Span sp = paged_span(a, p, seq, row0);
   if (row0 >= sp.rows || (chunk && chunk >= sp.chunks)) return;
+  report_counts(a, sp, tile, chunk, head);
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page, d0 = 128 * wave;
   const uint32_t shift = __builtin_ctz(P);
@@ -832,6 +841,7 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
   const uint32_t row0 = tile * 16 * NT * RW;
   const Span sp = paged_span(a, p, seq, row0);
   if (row0 >= sp.rows || (chunk && chunk >= sp.chunks)) return;
+  report_counts(a, sp, tile, chunk, head);
   const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page;
   const Pages pages{a.page_table + uint64_t(seq) * a.table_width, sp.seen, sp.len - 1, a.cache.pages, uint32_t(__builtin_ctz(P))};

@@ -101,7 +101,13 @@ constexpr uint32_t kSyncStatusLine = kSyncLines - 1;  // the status word's line
 inline uint32_t *status_word(const Workspace &ws) { return ws.sync + kSyncStatusLine * kRouteCounterStride; }
 // Status bits a launch leaves in the status line of ws.sync (sticky until
 // read by s14_launch_status).
-enum : uint32_t { kStatusNullPage = 1u, kStatusBadRoute = 2u, kStatusBadCachePage = 4u, kStatusBadPosition = 8u };
+enum : uint32_t {
+  kStatusNullPage = 1u,
+  kStatusBadRoute = 2u,
+  kStatusBadCachePage = 4u,
+  kStatusBadPosition = 8u,
+  kStatusBadCounts = 16u
+};
 
 // Layout of the workspace in one device allocation (each region 256-byte
 // aligned): table | h | scores | biased | route counters | h windows | x

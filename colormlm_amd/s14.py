@@ -128,8 +128,9 @@ class Context:
         return [float(ms[i]) for i in range(n.value)]
 
     def launch_status(self) -> None:
-        """Raises S14Error if a routed launch since the last call found a
-        page address of 0 (synchronises)."""
+        """Raises S14Error if a routed launch since the last call found a page
+        address of 0 or a bad route, or an attention launch a page, position,
+        length or count outside what it was given (synchronises)."""
         check(lib().s14_launch_status(self._h))
 
     def destroy(self) -> None:

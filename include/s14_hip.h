@@ -317,7 +317,8 @@ uint64_t s14_noalloc_scratch_bytes(void);
  * on each token's device-chosen route: expert ids inside [0, n_experts) and
  * distinct, weights finite and >= 0, their f32 sum within 1e-4 of
  * route_scale.  A token whose route fails them gets NaN outputs and this
- * call reports S14_ERR_ROUTE. */
+ * call reports S14_ERR_ROUTE.  The attention launches leave their statuses here
+ * too (S14_ERR_INVALID). */
 int s14_launch_status(s14_ctx *ctx);
 
 /* Router only (scores f32 [n_experts], ids u16 [topk], weights f32 [topk]). */
@@ -440,9 +441,13 @@ int s14_fp8_linear(s14_ctx *ctx, void *stream, uint32_t m, uint32_t n, uint32_t 
  * Token t, head h of a packed [tokens][heads][dim] operand starts at element
  * t * token_stride + h * head_stride; a row's dim values are contiguous.  dim
  * is 64, 128, 256 or 512 (prompt: to 256).  Operands start on 16 bytes and
- * have strides that are multiples of 8 elements.  Device index arrays (cu, past, lens, page tables, positions) are
- * checked on the device: no value makes a launch read or write outside its
- * operands, and one that is wrong is reported by s14_launch_status.
+ * have strides that are multiples of 8 elements.  Device index arrays (cu, past,
+ * lens, page tables, positions) are checked on the device: no value makes a
+ * launch read or write outside its operands.  s14_launch_status reports pages
+ * outside the cache, positions outside the rotation table, lengths below 0 or
+ * past the page table (they are held to them) and more new rows of a sequence
+ * than max_new.  Bounds in cu are held inside the packed rows and not reported:
+ * a sequence whose bounds run backwards is empty.
  * Launches of one context share its workspace and must not overlap.
  * ====================================================================== */
 typedef struct {
@@ -526,9 +531,9 @@ int s14_kv_append(s14_ctx *ctx, void *stream, const s14_kv_cache *cache, uint32_
  * [tokens][heads], or ptr NULL) the natural log of the weights' sum.  A row
  * that sees nothing is 0 with lse -inf.  Table entries of pages that no row
  * sees, behind the length or wholly before the window of the sequence's first
- * row, may hold anything.  max_new and max_len: at least the
- * largest count of rows, and about the longest sequence (it only sets how the
- * work is split).  table_width * page_tokens is at most 2^31 - 2^16. */
+ * row, may hold anything.  max_new and max_len: at least the largest count of
+ * rows (a sequence's rows past it are not computed), and about the longest
+ * sequence (it only sets how the work is split).  table_width * page_tokens is at most 2^31 - 2^16. */
 int s14_paged_attention(s14_ctx *ctx, void *stream, const s14_rows *q, const s14_kv_cache *cache,
                         uint32_t tokens, uint32_t seqs, uint32_t max_new, uint32_t max_len,
                         s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer lens,

@@ -554,6 +554,54 @@ def test_paged_pages_behind_the_window_may_be_gone(ctx, heads, kv, dim, new, pag
     ctx.launch_status()
 
 
+def test_paged_lengths_outside_the_page_table(ctx):
+    """A length past the table is that of the table's reach, one below 0 is 0;
+    the outputs are those, and the status says so."""
+    say("paged: lengths past the page table and below 0")
+    for new, dim, heads, kv in ((2, 128, 4, 2), (9, 64, 8, 1), (3, 512, 16, 1)):
+        p = Paged(2, [48, 48, 20], kv, dim, 16)
+        q = rand(gen(4), 3 * new, heads, dim, dtype=BF16).cuda()
+        want = paged_want(p, q, [new] * 3)
+        p.lens = ints([1 << 30, 48, 20])
+        out, lse = run_paged(ctx, p, q, [new] * 3, heads, dim)
+        check_attention(out, lse, want, "held to 48 positions")
+        with pytest.raises(s14.S14Error, match="length"):
+            ctx.launch_status()
+        p.lens = ints([48, -5, 20])
+        out, lse = run_paged(ctx, p, q, [new] * 3, heads, dim)
+        assert not out[new:2 * new].any() and bool((lse[new:2 * new] == -math.inf).all())
+        check_attention(out[:new], lse[:new], [x[:new] for x in want], "the sequence before")
+        with pytest.raises(s14.S14Error, match="length"):
+            ctx.launch_status()
+        # a sequence without new tokens: its length is not asked for
+        p.lens = ints([48, -5, 20])
+        cu = cumulative([new, 0, new])
+        out = torch.full((2 * new, heads, dim), 7.0, device="cuda")
+        A.paged_attention(ctx, torch.cat([q[:new], q[2 * new:]]), p.cache, p.dev_table, cu, p.lens, out, max_new=new, max_len=48)
+        check_attention(out, None, [torch.cat([x[:new], x[2 * new:]]) for x in want], "the others")
+        ctx.launch_status()
+
+
+@pytest.mark.parametrize("heads,kv,dim,counts,most", [(4, 2, 128, [3, 1], 1), (8, 1, 64, [2, 9], 8), (4, 1, 128, [50, 3], 40),
+                                                      (16, 1, 512, [1, 4], 2)])
+def test_paged_more_rows_than_planned(ctx, heads, kv, dim, counts, most):
+    """Rows past max_new of a sequence stay as they were, and the status says so."""
+    say(f"paged: {counts} rows, planned for {most}")
+    p = Paged(2, [100, 70], kv, dim, 16)
+    q = rand(gen(4), sum(counts), heads, dim, dtype=BF16).cuda()
+    want = paged_want(p, q, counts)
+    out = torch.full((sum(counts), heads, dim), 7.0, device="cuda")
+    A.paged_attention(ctx, q, p.cache, p.dev_table, cumulative(counts), p.lens, out, max_new=most, max_len=100)
+    at = 0
+    for n in counts:
+        s = slice(at, at + min(n, most))
+        check_attention(out[s], None, [x[s] for x in want], "the first rows")
+        assert bool((out[s.stop:at + n] == 7).all())
+        at += n
+    with pytest.raises(s14.S14Error, match="max_new"):
+        ctx.launch_status()
+
+
 def ctx_status(ctx):
     try:
         ctx.launch_status()
