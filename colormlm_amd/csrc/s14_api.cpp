@@ -12,6 +12,7 @@
 #include <cmath>
 #include <cstring>
 #include <new>
+#include <string>
 
 #include "s14_attn.hpp"
 #include "s14_device.hpp"
@@ -651,21 +652,29 @@ int read_launch_status(const Workspace &ws, int device) {
   if (!bits) return S14_OK;
   const uint32_t zero = 0;
   S14_HIP(hipMemcpy(word, &zero, sizeof(zero), hipMemcpyHostToDevice), "hipMemcpy(status clear)");
-  if (bits & kStatusNullPage)
-    return fail(S14_ERR_INVALID, "a routed expert's page address was 0 (page not resident); outputs are NaN");
-  if (bits & kStatusBadCachePage)
-    return fail(S14_ERR_INVALID,
-                "a sequence's cache page lies outside the cache or past its page table; its new rows are not stored "
-                "and its outputs are NaN");
-  if (bits & kStatusBadPosition)
-    return fail(S14_ERR_INVALID, "a position lies outside the rotation table; its rows are NaN");
-  if (bits & kStatusBadCounts)
-    return fail(S14_ERR_INVALID,
-                "a sequence has a length below 0 or past its page table (it was held to them) or more new rows than "
-                "max_new (the first max_new were taken)");
-  return fail(S14_ERR_ROUTE,
-              "a token's route failed RouteDecision::validate_for (expert id out of range or repeated, weight "
-              "not finite or negative, or weight sum off route_scale by more than 1e-4); its outputs are NaN");
+  // Every cause is named: reading clears them all.  The code is that of the
+  // routed launches, where they have one.
+  const struct {
+    uint32_t bit;
+    const char *what;
+  } causes[] = {
+      {kStatusNullPage, "a routed expert's page address was 0 (page not resident); outputs are NaN"},
+      {kStatusBadRoute,
+       "a token's route failed RouteDecision::validate_for (expert id out of range or repeated, weight not finite or "
+       "negative, or weight sum off route_scale by more than 1e-4); its outputs are NaN"},
+      {kStatusBadCachePage,
+       "a sequence's cache page lies outside the cache or past its page table; its new rows are not stored and its "
+       "outputs are NaN"},
+      {kStatusBadPosition, "a position lies outside the rotation table; its rows are NaN"},
+      {kStatusBadCounts,
+       "a sequence has a length below 0 or past its page table (it was held to them) or more new rows than max_new (the "
+       "first max_new were taken)"},
+  };
+  std::string all;
+  for (const auto &c : causes)
+    if (bits & c.bit) all += (all.empty() ? "" : "; ") + std::string(c.what);
+  const bool route = (bits & kStatusBadRoute) && !(bits & kStatusNullPage);
+  return fail(route ? S14_ERR_ROUTE : S14_ERR_INVALID, "%s", all.c_str());
 }
 }  // namespace s14
 

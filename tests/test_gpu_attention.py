@@ -602,6 +602,25 @@ def test_paged_more_rows_than_planned(ctx, heads, kv, dim, counts, most):
         ctx.launch_status()
 
 
+def test_status_names_every_cause(ctx):
+    say("one launch status for a page, a position and a length that are wrong")
+    p = Paged(2, [100, 100], 2, 128, 16)
+    p.table[0, 3] = -1
+    p.upload()
+    p.lens = ints([100, 1 << 20])
+    q = rand(gen(4), 2, 4, 128, dtype=BF16).cuda()
+    run_paged(ctx, p, q, [1, 1], 4, 128)
+    x = torch.zeros(1, 1, 128, device="cuda")
+    rope = A.Rope(torch.zeros(4, 128, device="cuda"))
+    A.qk_norm_rope(ctx, x, None, x.clone(), None, rope=rope, positions=ints([4]))
+    with pytest.raises(s14.S14Error) as e:
+        ctx.launch_status()
+    assert e.value.code == N.S14_ERR_INVALID
+    for cause in ("cache page", "rotation table", "length"):
+        assert cause in str(e.value)
+    ctx.launch_status()
+
+
 def ctx_status(ctx):
     try:
         ctx.launch_status()
