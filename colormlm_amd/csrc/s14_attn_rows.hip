@@ -246,7 +246,8 @@ __global__ __launch_bounds__(256) void k_rope_table(RopeTableArgs a) {
 // ---------------------------------------------------------------------------
 
 // The page that workgroup `index` of a (head, side) writes: pages of the first
-// sequence first.  A sequence has the pages that its new tokens touch.
+// sequence first.  A sequence has the pages that its new tokens touch, the
+// first max_new of them: the grid and the workgroups are made for these.
 struct Touched {
   uint32_t seq;
   int64_t first, last, past, page;  // packed rows, and the page of the sequence
@@ -254,8 +255,10 @@ struct Touched {
 // Page `k` of those that the sequence of rows first .. last - 1 touches.
 __device__ __forceinline__ bool sequence_page(const AppendArgs &a, uint32_t seq, int64_t first, int64_t last,
                                               int64_t past, uint32_t k, Touched &t) {
-  t = Touched{seq, first, last, past, past / a.cache.page + k};
-  return past >= 0 && last > first && t.page * a.cache.page < past + (last - first);
+  const int64_t end = min(last, first + int64_t(a.max_new));
+  if (past >= 0 && last > end && k == 0 && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(a.status, kStatusBadCounts);
+  t = Touched{seq, first, end, past, past / a.cache.page + k};
+  return past >= 0 && end > first && t.page * a.cache.page < past + (end - first);
 }
 __device__ __forceinline__ bool find_page(const AppendArgs &a, uint32_t index, uint32_t lane, Touched &t) {
   const uint32_t P = a.cache.page;
@@ -267,7 +270,8 @@ __device__ __forceinline__ bool find_page(const AppendArgs &a, uint32_t index, u
       first = int32_t(clamp_row(a.cu[s], a.tokens)), last = int32_t(clamp_row(a.cu[s + 1], a.tokens));
       past = a.past[s];
     }
-    const uint32_t pages = last > first ? (uint32_t(past) % P + uint32_t(last - first) + P - 1) / P : 0;
+    const uint32_t count = last > first ? min(uint32_t(last - first), a.max_new) : 0;
+    const uint32_t pages = count ? (uint32_t(past) % P + count + P - 1) / P : 0;
     uint32_t sum = pages;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {

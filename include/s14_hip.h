@@ -445,9 +445,10 @@ int s14_fp8_linear(s14_ctx *ctx, void *stream, uint32_t m, uint32_t n, uint32_t 
  * lens, page tables, positions) are checked on the device: no value makes a
  * launch read or write outside its operands.  s14_launch_status reports pages
  * outside the cache, positions outside the rotation table, lengths below 0 or
- * past the page table (they are held to them) and more new rows of a sequence
- * than max_new.  Bounds in cu are held inside the packed rows and not reported:
- * a sequence whose bounds run backwards is empty.
+ * past the page table (they are held to them) and more new rows
+ * of a sequence than max_new.  Bounds in cu run upwards; they are held inside
+ * the packed rows and not reported: a sequence whose bounds run backwards is
+ * empty, and those behind it may not be worked on.
  * Launches of one context share its workspace and must not overlap.
  * ====================================================================== */
 typedef struct {
@@ -508,7 +509,8 @@ typedef struct {
 
 /* Rows cu[i] .. cu[i + 1] - 1 of k and v become positions past[i] .. of
  * sequence i (cu, past: device int32 [seqs + 1], [seqs]; page_table device
- * int32 [seqs][table_width]; max_new >= the largest count).  K takes the norm
+ * int32 [seqs][table_width]; max_new >= the largest count, a sequence's rows
+ * past it are not stored).  K takes the norm
  * and rotation of s14_qk_norm_rope on the way, at those positions.
  * A page's scale is 2^ceil(log2(max(amax, 1e-4) / 448)) of the values put in,
  * never less than the one that its earlier tokens have (slots below past[i]):

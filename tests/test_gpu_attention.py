@@ -440,6 +440,30 @@ def test_append_special_values(ctx):
     ctx.launch_status()
 
 
+@pytest.mark.parametrize("dim,kv,page", [(64, 2, 16), (128, 1, 64), (512, 1, 128)])
+@pytest.mark.parametrize("past,counts,most", [([5, 0], [40, 3], 3), ([0, 15], [2, 1], 1), ([100, 7], [130, 200], 129),
+                                              ([3] * 9, [20, 1, 0, 1, 1, 1, 1, 1, 1], 17)])
+def test_append_more_rows_than_planned(ctx, dim, kv, page, past, counts, most):
+    """Rows past max_new of a sequence are not stored: the cache is that of the
+    first max_new, and the status says so."""
+    say(f"append: {counts} rows, planned for {most}, dim={dim} page={page}")
+    g = gen(5)
+    lengths = [a + b for a, b in zip(past, counts)]
+    p, w = Paged(4, lengths, kv, dim, page), Paged(4, lengths, kv, dim, page)
+    k, v = (rand(g, sum(counts), kv, dim).cuda() for _ in range(2))
+    k[::3] *= 50
+    A.kv_append(ctx, p.cache, k, v, p.dev_table, cumulative(counts), ints(past), max_new=most)
+    with pytest.raises(s14.S14Error, match="max_new"):
+        ctx.launch_status()
+    start = np.cumsum([0, *counts])
+    rows = torch.cat([torch.arange(a, a + min(n, most)) for a, n in zip(start, counts)]).cuda()
+    kept = [min(n, most) for n in counts]
+    A.kv_append(ctx, w.cache, k[rows], v[rows], w.dev_table, cumulative(kept), ints(past), max_new=most)
+    ctx.launch_status()
+    for x in ("k_pages", "v_pages", "k_scales", "v_scales"):
+        assert torch.equal(getattr(p.cache, x), getattr(w.cache, x)), x
+
+
 # ---------------------------------------------------------------------------
 # attention over the cache
 # ---------------------------------------------------------------------------
