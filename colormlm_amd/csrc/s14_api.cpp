@@ -669,6 +669,7 @@ int read_launch_status(const Workspace &ws, int device) {
       {kStatusBadCounts,
        "a sequence has a length below 0 or past its page table (it was held to them) or more new rows than max_new (the "
        "first max_new were taken)"},
+      {kStatusBadPast, "a sequence's past is below 0; its new rows are not stored"},
   };
   std::string all;
   for (const auto &c : causes)

@@ -256,7 +256,8 @@ struct Touched {
 __device__ __forceinline__ bool sequence_page(const AppendArgs &a, uint32_t seq, int64_t first, int64_t last,
                                               int64_t past, uint32_t k, Touched &t) {
   const int64_t end = min(last, first + int64_t(a.max_new));
-  if (past >= 0 && last > end && k == 0 && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(a.status, kStatusBadCounts);
+  if (last > first && (past < 0 || last > end) && k == 0 && blockIdx.y == 0 && threadIdx.x == 0)
+    atomicOr(a.status, past < 0 ? kStatusBadPast : kStatusBadCounts);
   t = Touched{seq, first, end, past, past / a.cache.page + k};
   return past >= 0 && end > first && t.page * a.cache.page < past + (end - first);
 }

@@ -106,7 +106,8 @@ enum : uint32_t {
   kStatusBadRoute = 2u,
   kStatusBadCachePage = 4u,
   kStatusBadPosition = 8u,
-  kStatusBadCounts = 16u
+  kStatusBadCounts = 16u,
+  kStatusBadPast = 32u
 };
 
 // Layout of the workspace in one device allocation (each region 256-byte

@@ -445,7 +445,7 @@ int s14_fp8_linear(s14_ctx *ctx, void *stream, uint32_t m, uint32_t n, uint32_t 
  * lens, page tables, positions) are checked on the device: no value makes a
  * launch read or write outside its operands.  s14_launch_status reports pages
  * outside the cache, positions outside the rotation table, lengths below 0 or
- * past the page table (they are held to them) and more new rows
+ * past the page table (they are held to them), a past below 0 and more new rows
  * of a sequence than max_new.  Bounds in cu run upwards; they are held inside
  * the packed rows and not reported: a sequence whose bounds run backwards is
  * empty, and those behind it may not be worked on.
@@ -517,7 +517,8 @@ typedef struct {
  * where it grows their codes are divided by the power of two, rounded to
  * nearest even.  Slots past the last new token stay as they were.  A NaN is
  * stored as NaN (it sets no scale), an infinity as the largest value of the
- * largest scale.  A page outside the cache or past the table takes nothing.
+ * largest scale.  A page outside the cache or past the table takes nothing, nor
+ * does a sequence whose past is below 0.
  * A page that one call writes stands in one place of one sequence's row. */
 int s14_kv_append(s14_ctx *ctx, void *stream, const s14_kv_cache *cache, uint32_t tokens,
                   uint32_t seqs, uint32_t max_new, const s14_rows *k, const s14_rows *v,

@@ -464,6 +464,23 @@ def test_append_more_rows_than_planned(ctx, dim, kv, page, past, counts, most):
         assert torch.equal(getattr(p.cache, x), getattr(w.cache, x)), x
 
 
+def test_append_before_the_first_position(ctx):
+    """A past below 0 stores nothing of its sequence, and the status says so."""
+    say("append: a past below 0")
+    x = rand(gen(5), 5, 1, 64).cuda()
+    for counts, past in (([1, 4], [-4, 0]), ([4, 1], [-1, 0]), ([5, 0], [-(1 << 31), 0]), ([0, 5], [-3, 2])):
+        p, w = Paged(4, [20, 20], 1, 64, 16), Paged(4, [20, 20], 1, 64, 16)
+        A.kv_append(ctx, p.cache, x, x, p.dev_table, cumulative(counts), ints(past))
+        if counts[0]:
+            with pytest.raises(s14.S14Error, match="past"):
+                ctx.launch_status()
+        ctx.launch_status()  # (of a sequence without new tokens it is not asked for)
+        y = x[counts[0]:]
+        A.kv_append(ctx, w.cache, y, y, w.dev_table, cumulative([0, counts[1]]), ints([0, past[1]]))
+        for t in ("k_pages", "v_pages", "k_scales", "v_scales"):
+            assert torch.equal(getattr(p.cache, t), getattr(w.cache, t)), t
+
+
 # ---------------------------------------------------------------------------
 # attention over the cache
 # ---------------------------------------------------------------------------
