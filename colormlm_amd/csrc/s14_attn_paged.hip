@@ -242,11 +242,28 @@ __device__ __forceinline__ void join_tile(const PagedArgs &a, const PagedPlan &p
     join_row<D, kAgent>(a, p, sp, it, row0, k, part);
 }
 
-// The top bit of each byte that is a NaN code (0x7f, 0xff).
-__device__ __forceinline__ uint32_t nan_codes(uint32_t c) { return ((c & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// The least code that is no finite bf16 value at a page's scale: the NaN code,
+// and at scales from 2^120 on, which an infinity's page has, large ones.
+__device__ __forceinline__ uint32_t odd_code(uint32_t scale) { return scale < 247u ? 0x7fu : 0x78u - 8u * (scale - 247u); }
+
+// The top bit of each byte whose code is `from` (0x7f at the most) or larger in magnitude.
+__device__ __forceinline__ uint32_t odd_codes(uint32_t c, uint32_t from) {
+  return ((c & 0x7f7f7f7fu) + (0x80u - from) * 0x01010101u) & 0x80808080u;
+}
 
 // Those bytes as zeros.
-__device__ __forceinline__ uint32_t no_nan(uint32_t c) { return c & ~((nan_codes(c) >> 7) * 0xffu); }
+__device__ __forceinline__ uint32_t no_odd(uint32_t c, uint32_t from) { return c & ~((odd_codes(c, from) >> 7) * 0xffu); }
+
+// What such a code stands for: NaN or an infinity; of another 0.
+__device__ __forceinline__ float odd_value(uint32_t c, uint32_t from) {
+  return (c & 0x7fu) < from ? 0.0f : __uint_as_float((c & 0x7fu) == 0x7fu ? 0x7fc00000u : 0x7f800000u | ((c & 0x80u) << 24));
+}
+
+// The top bit of each byte that is a NaN code (0x7f, 0xff).
+__device__ __forceinline__ uint32_t nan_codes(uint32_t c) { return odd_codes(c, 0x7fu); }
+
+// Those bytes as zeros.
+__device__ __forceinline__ uint32_t no_nan(uint32_t c) { return no_odd(c, 0x7fu); }
 
 template <int D, int NT>
 __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(PagedArgs a, PagedPlan p, float *part) {
@@ -918,9 +935,10 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
   };
   auto stage = [&](int32_t b, u32x4 *to) {
     if (partial_at(b)) {
-      // as in k_paged_attention: nothing from behind the sequence, and no NaN
-      // code that some row must not see
-      uint32_t nan = 0;
+      // as in k_paged_attention: nothing from behind the sequence, and no NaN or
+      // infinity that some row must not see
+      uint32_t found = 0;
+      const uint32_t from = odd_code(vsc);
       uint32_t keep[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -930,13 +948,14 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
 #pragma unroll
       for (int i = 0; i < R; ++i) {
         vv[i].x &= keep[0], vv[i].y &= keep[1], vv[i].z &= keep[2], vv[i].w &= keep[3];
-        nan |= nan_codes(vv[i].x) | nan_codes(vv[i].y) | nan_codes(vv[i].z) | nan_codes(vv[i].w);
+        found |= odd_codes(vv[i].x, from) | odd_codes(vv[i].y, from) | odd_codes(vv[i].z, from) | odd_codes(vv[i].w, from);
       }
-      if (__any(nan != 0)) {
+      if (__any(found != 0)) {
         odd = true;
 #pragma unroll
         for (int i = 0; i < R; ++i)
-          vv[i].x = no_nan(vv[i].x), vv[i].y = no_nan(vv[i].y), vv[i].z = no_nan(vv[i].z), vv[i].w = no_nan(vv[i].w);
+          vv[i].x = no_odd(vv[i].x, from), vv[i].y = no_odd(vv[i].y, from), vv[i].z = no_odd(vv[i].z, from),
+          vv[i].w = no_odd(vv[i].w, from);
       }
     }
 #pragma unroll
@@ -1071,19 +1090,20 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
     for (int32_t b0 = begin; b0 < end; b0 += TK) {
       if (!partial_at(b0)) continue;
       for (int32_t j = b0; j < min(b0 + TK, sp.len); ++j) {
-        const uint8_t *vp = a.cache.v + (uint64_t(pages.checked(pages.id(j), bad)) * kvh + head) * page_bytes + (uint32_t(j) & (P - 1));
+        const uint64_t at = uint64_t(pages.checked(pages.id(j), bad)) * kvh + head;
+        const uint32_t from = odd_code(a.cache.vs[at]);
+        const uint8_t *vp = a.cache.v + at * page_bytes + (uint32_t(j) & (P - 1));
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          f32x4 nan;
+          f32x4 odds;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            nan[i] = (vp[(16 * dt + 4 * g + i) * P] & 0x7fu) == 0x7fu ? __uint_as_float(0x7fc00000u) : 0.0f;
+          for (int i = 0; i < 4; ++i) odds[i] = odd_value(vp[(16 * dt + 4 * g + i) * P], from);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const bool in = see[nt](j);
             f32x4 back;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) back[i] = in ? nan[i] : 0.0f;
+            for (int i = 0; i < 4; ++i) back[i] = in ? odds[i] : 0.0f;
             o[nt][dt] += back;
           }
         }

@@ -662,6 +662,63 @@ def test_status_names_every_cause(ctx):
     ctx.launch_status()
 
 
+# query heads, key heads, head size, new tokens: rows of one wavefront, of one
+# workgroup through LDS in each tile size, and wide heads
+EVERY_TILE = [(4, 1, 128, 1), (4, 1, 128, 4), (8, 1, 64, 2), (4, 1, 256, 3), (4, 1, 128, 7), (4, 1, 64, 6), (4, 1, 64, 12),
+              (4, 1, 128, 12), (4, 1, 128, 30), (2, 1, 256, 11), (8, 1, 64, 40), (16, 1, 512, 1), (16, 1, 512, 3)]
+
+
+@pytest.mark.parametrize("heads,kv,dim,new", EVERY_TILE)
+@pytest.mark.parametrize("seqs", [1, 2])
+def test_paged_stored_infinities(ctx, heads, kv, dim, new, seqs):
+    """A value past f32's range, which is how an infinity is stored, is infinite
+    in its dimension of the rows that see it, and nowhere else."""
+    say(f"paged: infinities among the values, heads={heads}/{kv} dim={dim} new={new} seqs={seqs}")
+    length, page = 90, 16
+    for window in (0, 50):
+        first = length - new
+        # the first row's own; the last row's; of a whole tile of every row; one before some rows' windows
+        for pos, sign in ((first, 1), (length - 1, -1), (10, 1), (first - 45, -1)):
+            p = Paged(7, [length] * seqs, kv, dim, page)
+            q = (rand(gen(4), new * seqs, heads, dim) * 0.01).to(BF16).cuda()  # about equal weights
+            pid, slot = int(p.table[0, pos // page]), pos % page
+            p.vs[pid, 0] = 254
+            p.v[pid, 0] = 0
+            p.v[pid, 0, 7, slot] = 0x7E if sign > 0 else 0xFE
+            p.v[pid, 0, 9] = 0x01  # 2^118: a value of the same page within the range
+            p.upload()
+            out, lse = run_paged(ctx, p, q, [new] * seqs, heads, dim, window=window, dtype=F32)
+            o, l, mass, big = paged_want(p, q, [new] * seqs, window)
+            over = o.abs() > torch.finfo(F32).max
+            got = out.cpu().double()
+            assert torch.equal(got.isinf(), over) and not bool(got.isnan().any()), (window, pos)
+            assert bool((got[over] == sign * math.inf).all())
+            hidden = [i for i in range(new) if pos > first + i or (window and pos <= first + i - window)]
+            assert not bool(over[hidden].any()) and bool(over[:new, :, 7].any()) == (len(hidden) < new)
+            o[over] = got[over] = 0.0
+            assert bool(((got - o).abs() <= 2.0 ** -8 * 17 / 16 * mass + 1e-30)[~over].all())
+            ctx.launch_status()
+
+
+@pytest.mark.parametrize("heads,kv,dim,new", EVERY_TILE)
+def test_paged_append_of_infinities(ctx, heads, kv, dim, new):
+    """The same through kv_append, the last token's value infinite."""
+    say(f"append of an infinite value, then attention: heads={heads}/{kv} dim={dim} new={new}")
+    g = gen(8)
+    length, page = 70 + new, 32
+    k, v = rand(g, length, kv, dim), rand(g, length, kv, dim)
+    v[length - 1, 0, 3] = math.inf
+    q = (rand(g, new, heads, dim) * 0.1).to(BF16).cuda()
+    p = Paged(7, [length], kv, dim, page)
+    A.kv_append(ctx, p.cache, k.cuda(), v.cuda(), p.dev_table, ints([0, length]), ints([0]))
+    pid, slot = int(p.table[0, (length - 1) // page]), (length - 1) % page
+    assert int(p.cache.v_pages[pid, 0, 3, slot]) == 0x7E and int(p.cache.v_scales[pid, 0]) == 254
+    out = run_paged(ctx, p, q, [new], heads, dim, dtype=F32)[0].cpu()
+    assert bool((out[-1, :, 3] == math.inf).all())
+    out[-1, :, 3] = 0.0
+    assert bool(out.isfinite().all())
+
+
 def ctx_status(ctx):
     try:
         ctx.launch_status()
