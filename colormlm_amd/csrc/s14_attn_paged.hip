@@ -8,8 +8,9 @@
 // registers.  A lane's V operand is then 4 T neighbouring tokens of one
 // dimension, which is why V pages lie [dim][slot].  E4M3 codes become bf16
 // exactly, so the products are of the stored values; page scales multiply the
-// scores (K) and the weights (V), and are one per lane, since the 4 T tokens
-// of a lane group lie in one page.
+// scores (K) and the codes as they become bf16 (V; on the weights the scale of
+// an infinity's page would pass bf16's range), and are one per lane, since the
+// 4 T tokens of a lane group lie in one page.
 //
 // A row is a (token, query head of the key head) pair: the group's heads share
 // the K and V that are read.  Up to 16 rows (k_paged_attention), the four
@@ -259,12 +260,6 @@ __device__ __forceinline__ float odd_value(uint32_t c, uint32_t from) {
   return (c & 0x7fu) < from ? 0.0f : __uint_as_float((c & 0x7fu) == 0x7fu ? 0x7fc00000u : 0x7f800000u | ((c & 0x80u) << 24));
 }
 
-// The top bit of each byte that is a NaN code (0x7f, 0xff).
-__device__ __forceinline__ uint32_t nan_codes(uint32_t c) { return odd_codes(c, 0x7fu); }
-
-// Those bytes as zeros.
-__device__ __forceinline__ uint32_t no_nan(uint32_t c) { return no_odd(c, 0x7fu); }
-
 template <int D, int NT>
 __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(PagedArgs a, PagedPlan p, float *part) {
   constexpr int T = 4;        // 16-token tiles a step
@@ -374,7 +369,8 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
     int32_t idk2, idv2;  // ahead of the K and V loads below
     load_ids(min(b + 2 * kStride, last), idk2, idv2);
     const float ks = fmaxf(scale * power_of_two(int(ksc) - 127), 0x1p-126f);  // above 0: a masked score stays -inf
-    const float vs = power_of_two(int(vsc) - 127);
+    const uint32_t vcode = vsc;  // of this step, whose V is read after the next one's scales
+    const float vs = power_of_two(int(vcode) - 127);
     f32x4 s[NT][T];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -428,37 +424,38 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
           sum[nt] += e[i];
         }
         // rounded to bf16, half a step of each weight: the matrix operand's type
-        w[t / 2][2 * (t & 1)] = bf16_pair(e[0] * vs, e[1] * vs);
-        w[t / 2][2 * (t & 1) + 1] = bf16_pair(e[2] * vs, e[3] * vs);
+        w[t / 2][2 * (t & 1)] = bf16_pair(e[0], e[1]);
+        w[t / 2][2 * (t & 1) + 1] = bf16_pair(e[2], e[3]);
       }
 #pragma unroll
       for (int u = 0; u < T / 2; ++u) pb[nt][u] = __builtin_bit_cast(bf16x8, w[u]);
     }
     if (partial) {
-      // what lies behind the sequence is not read; a NaN code that some row
-      // must not see leaves the product (0 * NaN is NaN), and the rows that see
-      // it get it back below
-      uint32_t nan = 0;
+      // what lies behind the sequence is not read; a NaN or infinity that some
+      // row must not see leaves the product (0 times it is NaN), and the rows
+      // that see it get it back below
+      uint32_t found = 0;
+      const uint32_t from = odd_code(vcode);
 #pragma unroll
       for (int k = 0; k < W; ++k) {
         const int32_t left = sp.len - (tv + 4 * k);
         const uint32_t keep = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) vv[dt][k] &= keep, nan |= nan_codes(vv[dt][k]);
+        for (int dt = 0; dt < DT; ++dt) vv[dt][k] &= keep, found |= odd_codes(vv[dt][k], from);
       }
-      if (__any(nan != 0)) {
+      if (__any(found != 0)) {
         odd = true;
 #pragma unroll
         for (int k = 0; k < W; ++k)
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) vv[dt][k] = no_nan(vv[dt][k]);
+          for (int dt = 0; dt < DT; ++dt) vv[dt][k] = no_odd(vv[dt][k], from);
       }
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int u = 0; u < T / 2; ++u) {
-        const bf16x8 v = e4m3_bf16(vv[dt][2 * u], vv[dt][2 * u + 1]);
+        const bf16x8 v = e4m3_bf16(vv[dt][2 * u], vv[dt][2 * u + 1], vs);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pb[nt][u], o[nt][dt], 0, 0, 0);
@@ -471,19 +468,20 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
     for (int32_t b0 = begin + 16 * T * int32_t(wave); b0 < end; b0 += kStride) {
       if (b0 + 16 * T - 1 <= pos_lo && !(a.window && int64_t(b0) <= int64_t(pos_hi) - a.window)) continue;
       for (int32_t j = b0; j < min(b0 + 16 * T, sp.len); ++j) {
-        const uint8_t *vp = a.cache.v + (uint64_t(pages.checked(pages.id(j), bad)) * kvh + head) * page_bytes + (uint32_t(j) & (P - 1));
+        const uint64_t at = uint64_t(pages.checked(pages.id(j), bad)) * kvh + head;
+        const uint32_t from = odd_code(a.cache.vs[at]);
+        const uint8_t *vp = a.cache.v + at * page_bytes + (uint32_t(j) & (P - 1));
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          f32x4 nan;
+          f32x4 odds;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            nan[i] = (vp[(16 * dt + 4 * g + i) * P] & 0x7fu) == 0x7fu ? __uint_as_float(0x7fc00000u) : 0.0f;
+          for (int i = 0; i < 4; ++i) odds[i] = odd_value(vp[(16 * dt + 4 * g + i) * P], from);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const bool in = see[nt](j);
             f32x4 back;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) back[i] = in ? nan[i] : 0.0f;
+            for (int i = 0; i < 4; ++i) back[i] = in ? odds[i] : 0.0f;
             o[nt][dt] += back;
           }
         }
@@ -642,11 +640,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
   uint32_t pagev = 0;
   auto load_k = [&](int32_t b) {
     const uint64_t at = uint64_t(pages.checked(idk, bad)) * kvh + head;
-    ksc = a.cache.ks[at], vsc = a.cache.vs[at];  // first: they are waited for before K
+    pagev = pages.checked(idv, bad);
+    ksc = a.cache.ks[at], vsc = a.cache.vs[uint64_t(pagev) * kvh + head];  // first: they are waited for before K
     const uint8_t *kp = a.cache.k + at * page_bytes + ((uint32_t(b + int32_t(k_tok)) & (P - 1)) + n) * uint32_t(D) + 16 * g;
 #pragma unroll
     for (int c = 0; c < C; ++c) kk[c] = *reinterpret_cast<const uint4 *>(kp + 64 * c);
-    pagev = pages.checked(idv, bad);
   };
   auto load_v = [&](int32_t b) {
     const uint8_t *vp = a.cache.v + (uint64_t(pagev) * kvh + head) * page_bytes + (d0 + n) * P +
@@ -674,7 +672,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
     int32_t idk2, idv2;  // ahead of the K and V loads below
     load_ids(min(b + 2 * kStep, last), idk2, idv2);
     const float ks = scale * power_of_two(int(ksc) - 127);
-    const float vs = power_of_two(int(vsc) - 127);
+    const uint32_t vcode = vsc;  // of this step, whose V is read after the next one's scales
+    const float vs = power_of_two(int(vcode) - 127);
     const bool partial = b + kStep - 1 > pos_lo || (a.window && int64_t(b) <= int64_t(pos_hi) - a.window);
     f32x4 s[NT][2] = {};
 #pragma unroll
@@ -720,11 +719,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
       }
       // half a step of each weight: the matrix operand's type
       reinterpret_cast<uint2 *>(&s_p[nt][g / 2][16 * wave + n])[g & 1] =
-          make_uint2(bf16_pair(e[0] * vs, e[1] * vs), bf16_pair(e[2] * vs, e[3] * vs));
+          make_uint2(bf16_pair(e[0], e[1]), bf16_pair(e[2], e[3]));
     }
     __syncthreads();
     if (partial) {  // as in k_paged_attention
-      uint32_t nan = 0;
+      uint32_t found = 0;
+      const uint32_t from = odd_code(vcode);
       uint32_t keep[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -734,14 +734,14 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         vv[dt].x &= keep[0], vv[dt].y &= keep[1], vv[dt].z &= keep[2], vv[dt].w &= keep[3];
-        nan |= nan_codes(vv[dt].x) | nan_codes(vv[dt].y) | nan_codes(vv[dt].z) | nan_codes(vv[dt].w);
+        found |= odd_codes(vv[dt].x, from) | odd_codes(vv[dt].y, from) | odd_codes(vv[dt].z, from) | odd_codes(vv[dt].w, from);
       }
-      if (__any(nan != 0)) {
+      if (__any(found != 0)) {
         odd = true;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          vv[dt].x = no_nan(vv[dt].x), vv[dt].y = no_nan(vv[dt].y);
-          vv[dt].z = no_nan(vv[dt].z), vv[dt].w = no_nan(vv[dt].w);
+          vv[dt].x = no_odd(vv[dt].x, from), vv[dt].y = no_odd(vv[dt].y, from);
+          vv[dt].z = no_odd(vv[dt].z, from), vv[dt].w = no_odd(vv[dt].w, from);
         }
       }
     }
@@ -750,7 +750,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
     for (int nt = 0; nt < NT; ++nt) pb[nt][0] = s_p[nt][0][l], pb[nt][1] = s_p[nt][1][l];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const bf16x8 v0 = e4m3_bf16(vv[dt].x, vv[dt].y), v1 = e4m3_bf16(vv[dt].z, vv[dt].w);
+      const bf16x8 v0 = e4m3_bf16(vv[dt].x, vv[dt].y, vs), v1 = e4m3_bf16(vv[dt].z, vv[dt].w, vs);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pb[nt][0], o[nt][dt], 0, 0, 0);
@@ -765,19 +765,20 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
     for (int32_t b0 = begin; b0 < end; b0 += kStep) {
       if (b0 + kStep - 1 <= pos_lo && !(a.window && int64_t(b0) <= int64_t(pos_hi) - a.window)) continue;
       for (int32_t j = b0; j < min(b0 + kStep, sp.len); ++j) {
-        const uint8_t *vp = a.cache.v + (uint64_t(pages.checked(pages.id(j), bad)) * kvh + head) * page_bytes + d0 * P + (uint32_t(j) & (P - 1));
+        const uint64_t at = uint64_t(pages.checked(pages.id(j), bad)) * kvh + head;
+        const uint32_t from = odd_code(a.cache.vs[at]);
+        const uint8_t *vp = a.cache.v + at * page_bytes + d0 * P + (uint32_t(j) & (P - 1));
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          f32x4 nan;
+          f32x4 odds;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            nan[i] = (vp[(16 * dt + 4 * g + i) * P] & 0x7fu) == 0x7fu ? __uint_as_float(0x7fc00000u) : 0.0f;
+          for (int i = 0; i < 4; ++i) odds[i] = odd_value(vp[(16 * dt + 4 * g + i) * P], from);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const bool in = see[nt](j);
             f32x4 back;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) back[i] = in ? nan[i] : 0.0f;
+            for (int i = 0; i < 4; ++i) back[i] = in ? odds[i] : 0.0f;
             o[nt][dt] += back;
           }
         }

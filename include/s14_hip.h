@@ -532,7 +532,9 @@ int s14_kv_append(s14_ctx *ctx, void *stream, const s14_kv_cache *cache, uint32_
  * heads / cache heads.  out (bf16 or f32) = softmax(scale q.k) v (scale > 0), the
  * softmax in f32, its weights rounded to bf16 for the second product; lse (f32
  * [tokens][heads], or ptr NULL) the natural log of the weights' sum.  A row
- * that sees nothing is 0 with lse -inf.  Table entries of pages that no row
+ * that sees nothing is 0 with lse -inf.  A value past f32's range, as which an
+ * infinity is stored, makes its dimension of the rows that see it infinite (NaN
+ * where its weight is 0), and nothing else.  Table entries of pages that no row
  * sees, behind the length or wholly before the window of the sequence's first
  * row, may hold anything.  max_new and max_len: at least the largest count of
  * rows (a sequence's rows past it are not computed), and about the longest

@@ -719,6 +719,34 @@ def test_paged_append_of_infinities(ctx, heads, kv, dim, new):
     assert bool(out.isfinite().all())
 
 
+@pytest.mark.parametrize("heads,kv,dim,new", EVERY_TILE)
+def test_paged_stored_infinities_under_rising_scores(ctx, heads, kv, dim, new):
+    """Weights above 1, which later, larger scores have, beside a page of the
+    largest scale: the infinity stays in its dimension."""
+    say(f"paged: an infinity at a weight of 2^4, heads={heads}/{kv} dim={dim} new={new}")
+    length, page = 330, 16
+    p = Paged(7, [length], kv, dim, page)
+    p.ks.fill_(127)
+    p.k.zero_()
+    for pos in range(256, length):
+        p.k[int(p.table[0, pos // page]), :, pos % page, 0] = 0x38
+    pid = int(p.table[0, 260 // page])
+    p.vs[pid, 0] = 254
+    p.v[pid, 0] = 0
+    p.v[pid, 0, 7, 260 % page] = 0xFE
+    p.upload()
+    q = torch.zeros(new, heads, dim)
+    q[:, :, 0] = 4 * math.log(2) * dim ** 0.5  # 2^4 times the first tokens' weights
+    q = q.to(BF16).cuda()
+    for max_len in (length, 1):  # cut, and in one piece
+        out, _ = run_paged(ctx, p, q, [new], heads, dim, dtype=F32, max_len=max_len)
+        o, _, mass, _ = paged_want(p, q, [new])
+        got = out.cpu().double()
+        assert bool((got[:, :, 7] == -math.inf).all())
+        o[:, :, 7] = got[:, :, 7] = mass[:, :, 7] = 0.0
+        assert bool(((got - o).abs() <= 2.0 ** -8 * 17 / 16 * mass + 1e-30).all())
+
+
 def ctx_status(ctx):
     try:
         ctx.launch_status()
