@@ -33,7 +33,7 @@ struct Span {
   uint32_t first, rows;  // first packed token; (token, head) rows of the sequence
   int32_t len, pos0, seen, lo, hi;
   uint32_t chunk, chunks;
-  bool wrong;  // its length is outside the table, or it has rows that no workgroup takes
+  uint32_t wrong;  // status: its length is outside the table, or it has rows that no workgroup takes
 };
 
 __device__ __forceinline__ Span paged_span(const PagedArgs &a, const PagedPlan &p, uint32_t seq, uint32_t row0) {
@@ -46,7 +46,7 @@ __device__ __forceinline__ Span paged_span(const PagedArgs &a, const PagedPlan &
   const int64_t room = int64_t(a.table_width) * a.cache.page;
   const int64_t len = a.len[seq];
   s.len = int32_t(len < 0 ? 0 : len < room ? len : room);
-  s.wrong = n > 0 && (len != s.len || uint32_t(n) > a.max_new);
+  s.wrong = n > 0 && (len != s.len || uint32_t(n) > a.max_new) ? kStatusBadCounts : 0u;
   s.pos0 = s.len - n;
   const uint32_t last = (row0 + 16 * p.row_tiles < s.rows ? row0 + 16 * p.row_tiles : s.rows) - 1;
   const int32_t first_pos = s.pos0 + int32_t(row0 / group), last_pos = s.pos0 + int32_t(last / group);
@@ -58,11 +58,6 @@ __device__ __forceinline__ Span paged_span(const PagedArgs &a, const PagedPlan &
   const PagedCut cut = paged_cut(span, p.chunk, p.chunks);
   s.chunk = cut.chunk, s.chunks = cut.chunks;
   return s;
-}
-
-// Once a sequence.
-__device__ __forceinline__ void report_counts(const PagedArgs &a, const Span &s, uint32_t tile, uint32_t chunk, uint32_t head) {
-  if (s.wrong && !tile && !chunk && !head && threadIdx.x == 0) atomicOr(a.status, kStatusBadCounts);
 }
 
 __device__ __forceinline__ void store_out(const AttnOut &o, uint64_t at, float a, float b, float c, float d) {
@@ -272,7 +267,6 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   const uint32_t row0 = tile * 16 * NT;
   const Span sp = paged_span(a, p, seq, row0);
   if (row0 >= sp.rows || (chunk && chunk >= sp.chunks)) return;
-  report_counts(a, sp, tile, chunk, head);
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page;
   const uint32_t shift = __builtin_ctz(P);
@@ -311,7 +305,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   // pages' ids another step ahead.
   uint4 kk[T][C];
   uint32_t vv[DT][W];
-  uint32_t ksc = 0, vsc = 0;
+  uint8_t ksc = 0, vsc = 0;  // (as loaded: widened where they are used, not while in flight)
   int32_t idk = 0, idv = 0;  // of the next step
   uint32_t pagev = 0;
   auto load_ids = [&](int32_t b, int32_t &k, int32_t &v) {
@@ -369,8 +363,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
     int32_t idk2, idv2;  // ahead of the K and V loads below
     load_ids(min(b + 2 * kStride, last), idk2, idv2);
     const float ks = fmaxf(scale * power_of_two(int(ksc) - 127), 0x1p-126f);  // above 0: a masked score stays -inf
-    const uint32_t vcode = vsc;  // of this step, whose V is read after the next one's scales
-    const float vs = power_of_two(int(vcode) - 127);
+    const float vs = power_of_two(int(vsc) - 127);
     f32x4 s[NT][T];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -435,7 +428,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
       // row must not see leaves the product (0 times it is NaN), and the rows
       // that see it get it back below
       uint32_t found = 0;
-      const uint32_t from = odd_code(vcode);
+      const uint32_t from = odd_code(__float_as_uint(vs) >> 23);  // (vsc is the next step's)
 #pragma unroll
       for (int k = 0; k < W; ++k) {
         const int32_t left = sp.len - (tv + 4 * k);
@@ -492,8 +485,9 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   // join the four wavefronts: 2 and 3 into 0 and 1, then 1 into 0
   __shared__ float s_m[4][NT][16], s_l[4][NT][16];
   __shared__ f32x4 s_o[2][NT * DT][64];
-  if (__any(bad)) {
-    if (l == 0) atomicOr(a.status, kStatusBadCachePage);
+  const bool bad_page = __any(bad);
+  if (const uint32_t status = sp.wrong | (bad_page ? kStatusBadCachePage : 0u); status && l == 0) atomicOr(a.status, status);
+  if (bad_page) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) sum[nt] = __uint_as_float(0x7fc00000u);
   }
@@ -586,7 +580,6 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
   const uint32_t row0 = tile * 16 * NT;
   const Span sp = paged_span(a, p, seq, row0);
   if (row0 >= sp.rows || (chunk && chunk >= sp.chunks)) return;
-  report_counts(a, sp, tile, chunk, head);
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page, d0 = 128 * wave;
   const uint32_t shift = __builtin_ctz(P);
@@ -631,7 +624,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
   constexpr int32_t kStep = 64;
   const uint32_t k_tok = threadIdx.x / 64 * 16;
   uint4 kk[C], vv[DT];
-  uint32_t ksc = 0, vsc = 0;
+  uint8_t ksc = 0, vsc = 0;  // (as loaded: widened where they are used, not while in flight)
   int32_t idk = 0, idv = 0;  // of the next step
   auto load_ids = [&](int32_t b, int32_t &k, int32_t &v) {
     k = pages.id(b + int32_t(k_tok));
@@ -672,17 +665,26 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
     int32_t idk2, idv2;  // ahead of the K and V loads below
     load_ids(min(b + 2 * kStep, last), idk2, idv2);
     const float ks = scale * power_of_two(int(ksc) - 127);
-    const uint32_t vcode = vsc;  // of this step, whose V is read after the next one's scales
-    const float vs = power_of_two(int(vcode) - 127);
+    const float vs = power_of_two(int(vsc) - 127);
     const bool partial = b + kStep - 1 > pos_lo || (a.window && int64_t(b) <= int64_t(pos_hi) - a.window);
     f32x4 s[NT][2] = {};
+    // Q a piece ahead of its use (left to itself the compiler reads it right before:
+    // 4 x 4 of up to 9,000 tokens 34.5 us so, 35.1)
+    bf16x8 qa[2][NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) qa[0][nt][0] = s_q[nt][0][l], qa[0][nt][1] = s_q[nt][1][l];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
+      if (c + 1 < C) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) qa[(c + 1) & 1][nt][0] = s_q[nt][2 * c + 2][l], qa[(c + 1) & 1][nt][1] = s_q[nt][2 * c + 3][l];
+      }
       const bf16x8 k0 = e4m3_bf16(kk[c].x, kk[c].y), k1 = e4m3_bf16(kk[c].z, kk[c].w);
+      __builtin_amdgcn_sched_barrier(0x1 | 0x2 | 0x4 | 0x8);  // LDS reads stay ahead
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        s[nt][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, s_q[nt][2 * c][l], s[nt][0], 0, 0, 0);
-        s[nt][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, s_q[nt][2 * c + 1][l], s[nt][1], 0, 0, 0);
+        s[nt][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qa[c & 1][nt][0], s[nt][0], 0, 0, 0);
+        s[nt][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qa[c & 1][nt][1], s[nt][1], 0, 0, 0);
       }
     }
     load_k(next);
@@ -724,7 +726,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
     __syncthreads();
     if (partial) {  // as in k_paged_attention
       uint32_t found = 0;
-      const uint32_t from = odd_code(vcode);
+      const uint32_t from = odd_code(__float_as_uint(vs) >> 23);  // (vsc is the next step's)
       uint32_t keep[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -785,8 +787,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
       }
     }
   }
-  if (__any(bad)) {  // every wavefront has read the same V ids
-    if (l == 0) atomicOr(a.status, kStatusBadCachePage);
+  const bool bad_page = __any(bad);  // every wavefront has read the same V ids
+  if (const uint32_t status = sp.wrong | (bad_page ? kStatusBadCachePage : 0u); status && l == 0) atomicOr(a.status, status);
+  if (bad_page) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) sum[nt] = __uint_as_float(0x7fc00000u);
   }
@@ -859,7 +862,6 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
   const uint32_t row0 = tile * 16 * NT * RW;
   const Span sp = paged_span(a, p, seq, row0);
   if (row0 >= sp.rows || (chunk && chunk >= sp.chunks)) return;
-  report_counts(a, sp, tile, chunk, head);
   const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page;
   const Pages pages{a.page_table + uint64_t(seq) * a.table_width, sp.seen, sp.len - 1, a.cache.pages, uint32_t(__builtin_ctz(P))};
@@ -1111,7 +1113,7 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
       }
     }
   }
-  if ((flags & 1u) && tid == 0) atomicOr(a.status, kStatusBadCachePage);
+  if (const uint32_t status = sp.wrong | (flags & 1u ? kStatusBadCachePage : 0u); status && tid == 0) atomicOr(a.status, status);
   const uint32_t floats = p.rec_rows * kRecord<D>;
   const PartStore store(part + record_of(a, p, it, kvh) * floats, floats, p.fused);
 #pragma unroll
