@@ -400,7 +400,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
       // the maximum that the weights are taken from moves only where they
       // would pass 2^kRise: O is seldom multiplied
       if (__any(top > m[nt] + kRise)) {
-        const float fade = __builtin_amdgcn_exp2f(m[nt] - (top == -INFINITY ? 0.0f : top));
+        const float fade = fade_of(m[nt], top);
         m[nt] = top;
         sum[nt] *= fade;
 #pragma unroll
@@ -706,7 +706,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
     for (int nt = 0; nt < NT; ++nt) {
       const float top = fmaxf(fmaxf(fmaxf(s_m[0][nt][n], s_m[1][nt][n]), fmaxf(s_m[2][nt][n], s_m[3][nt][n])), m[nt]);
       if (__any(top > m[nt] + kRise)) {  // the same in every wavefront
-        const float fade = __builtin_amdgcn_exp2f(m[nt] - (top == -INFINITY ? 0.0f : top));
+        const float fade = fade_of(m[nt], top);
         m[nt] = top;
         sum[nt] *= fade;
 #pragma unroll
@@ -1021,7 +1021,7 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
         for (int i = 1; i < 4 * T; ++i) top = fmaxf(top, x[i]);
         top = fmaxf(m[nt], max_lane16(top) * scale);
         if (__any(top > m[nt] + kRise)) {
-          const float fade = __builtin_amdgcn_exp2f(m[nt] - (top == -INFINITY ? 0.0f : top));
+          const float fade = fade_of(m[nt], top);
           m[nt] = top;
           sum[nt] *= fade;
 #pragma unroll

@@ -534,7 +534,8 @@ int s14_kv_append(s14_ctx *ctx, void *stream, const s14_kv_cache *cache, uint32_
  * [tokens][heads], or ptr NULL) the natural log of the weights' sum.  A row
  * that sees nothing is 0 with lse -inf.  A value past f32's range, as which an
  * infinity is stored, makes its dimension of the rows that see it infinite (NaN
- * where its weight is 0), and nothing else.  Table entries of pages that no row
+ * where its weight is 0), and nothing else.  A row that sees a score past 2^28
+ * in magnitude, an infinity or a NaN among them, may be NaN.  Table entries of pages that no row
  * sees, behind the length or wholly before the window of the sequence's first
  * row, may hold anything.  max_new and max_len: at least the largest count of
  * rows (a sequence's rows past it are not computed), and about the longest

@@ -747,6 +747,72 @@ def test_paged_stored_infinities_under_rising_scores(ctx, heads, kv, dim, new):
         assert bool(((got - o).abs() <= 2.0 ** -8 * 17 / 16 * mass + 1e-30).all())
 
 
+@pytest.mark.parametrize("heads,kv,dim,new", [(4, 1, 128, 1), (4, 1, 128, 4), (8, 1, 64, 2), (4, 1, 256, 3), (4, 1, 128, 7),
+                                              (4, 1, 64, 12), (4, 1, 128, 30), (2, 1, 256, 11), (16, 1, 512, 1), (16, 1, 512, 3)])
+@pytest.mark.parametrize("seqs", [1, 2])
+def test_paged_infinite_scores(ctx, heads, kv, dim, new, seqs):
+    """A key past f32's range: a row that sees it is NaN where their product is
+    positive, as if it were not there where it is negative; a row that does not
+    see it has what it has without it."""
+    say(f"paged: infinities among the keys, heads={heads}/{kv} dim={dim} new={new} seqs={seqs}")
+    length, page = 90, 16
+    first = length - new
+    for pos in (length - 1, 10, first):
+        p = Paged(7, [length] * seqs, kv, dim, page)
+        q = rand(gen(4), new * seqs, heads, dim)
+        q[:, ::2, 7], q[:, 1::2, 7] = 1.0, -1.0
+        q = q.to(BF16).cuda()
+        pid, slot = int(p.table[0, pos // page]), pos % page
+        p.ks[pid, 0] = 254
+        p.k[pid, 0] = 0
+        p.k[pid, 0, slot, 7] = 0x7E
+        p.upload()
+        out, lse = run_paged(ctx, p, q, [new] * seqs, heads, dim, dtype=F32)
+        o, l, mass, _ = paged_want(p, q, [new] * seqs)
+        sees = torch.zeros(new * seqs, heads, dtype=torch.bool)
+        sees[[i for i in range(new) if pos <= first + i], ::2] = True
+        got = out.cpu().double()
+        assert torch.equal(got.isnan().all(-1), sees) and torch.equal(got.isnan().any(-1), sees), pos
+        assert torch.equal(lse.cpu().isnan(), sees)
+        assert bool(((got - o).abs() <= 2.0 ** -8 * 17 / 16 * mass + 1e-30)[~sees].all())
+
+
+@pytest.mark.parametrize("heads,kv,dim,n", [(4, 1, 64, 70), (2, 2, 128, 300), (4, 2, 256, 90)])
+def test_scores_near_and_past_the_range(ctx, heads, kv, dim, n):
+    """Scores of 2^27 pick their key; past the range, here by the scale alone, the
+    rows that see them are NaN: in the prompt and through the cache."""
+    say(f"scores of 2^27 and 2^128: heads={heads}/{kv} dim={dim}")
+    g = gen(12)
+    q, k, v = (rand(g, n, h, dim, dtype=BF16).cuda() for h in (heads, kv, kv))
+    late = (torch.arange(n) >= 40)[:, None].expand(n, heads)
+    for q0, k0, scale in ((2.0 ** 13, 2.0 ** 14, 1.0), (2.0 ** 60, 2.0 ** 60, 256.0), (-(2.0 ** 13), 2.0 ** 14, 1.0)):
+        q[:, :, 0], k[:, :, 0] = q0, 0.0
+        k[40, :, 0] = k0
+        out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+        A.prompt_attention(ctx, q, k, v, ints([0, n]), out, lse=lse, scale=scale)
+        p = Paged(7, [n], kv, dim, 32)
+        A.kv_append(ctx, p.cache, k, v, p.dev_table, ints([0, n]), ints([0]))
+        p.k, p.v, p.ks, p.vs = (x.cpu() for x in (p.cache.k_pages, p.cache.v_pages, p.cache.k_scales, p.cache.v_scales))
+        cut = []
+        for new in (1, 20):
+            o, l = torch.empty_like(q[:new]), torch.empty(new, heads, device="cuda")
+            A.paged_attention(ctx, q[n - new:], p.cache, p.dev_table, ints([0, new]), p.lens, o, lse=l, scale=scale)
+            cut.append((new, o, l))
+        if scale > 1.0:
+            assert torch.equal(out.isnan().all(-1).cpu(), late) and torch.equal(out.isnan().any(-1).cpu(), late)
+            assert torch.equal(lse.isnan().cpu(), late)
+            assert all(bool(o.isnan().all()) and bool(l.isnan().all()) for _, o, l in cut)
+            continue
+        o, _, mass, _ = attention64(q.cpu(), k.cpu(), v.cpu(), scale, 0)
+        # the other scores' f32 sums: 2^27 takes no part in them
+        tol = 2.0 ** -8 * 17 / 16 * mass + 2.0 ** -8 * o.abs() + 1e-30
+        assert bool(((out.cpu().double() - o).abs() <= tol).all())
+        kk, vv = p.rows(0)
+        for new, o, l in cut:
+            want = attention64(q[n - new:].cpu(), kk, vv, scale, 0)
+            assert bool(((o.cpu().double() - want[0]).abs() <= 2.0 ** -8 * 17 / 16 * want[2] + 2.0 ** -8 * want[0].abs() + 1e-30).all())
+
+
 def ctx_status(ctx):
     try:
         ctx.launch_status()
