@@ -196,7 +196,7 @@ extern "C" int s14_qk_norm_rope(s14_ctx *ctx, void *stream, uint32_t tokens, uin
   if (int rc = check_weight(k_weight, dim, eps, "k norm weight")) return rc;
   s14::NormRopeArgs a{};
   if (int rc = check_rope(rope, dim, &a.rope)) return rc;
-  if (a.rope.table)
+  if (a.rope.table && tokens)
     if (int rc = require(positions, 4ull * tokens, 4, "positions")) return rc;
   if (uint64_t(tokens) * (uint64_t(q->heads) + k->heads) > (1ull << 31))
     return fail(S14_ERR_SHAPE, "%u tokens of %u heads exceed one launch", tokens, q->heads + k->heads);

@@ -88,6 +88,11 @@ def test_norm_rope_without_tokens_is_no_launch(native):
     assert norm_rope(native, tokens=0) == N.S14_OK
 
 
+def test_norm_rope_without_tokens_asks_for_no_positions(native):
+    """An empty tensor has no address."""
+    assert norm_rope(native, tokens=0, rp=rope(), pos=NONE) == N.S14_OK
+
+
 def append(native, ctx=CTX, c=cache(), tokens=5, seqs=2, most=3, k=rows(2, token=256), v=rows(2, token=256), table=BIG,
            width=4, cu=BIG, past=BIG, kw=NONE, eps=1e-6, rp=None):
     return native.s14_kv_append(ctx, None, ref(c), tokens, seqs, most, ref(k), ref(v), table, width, cu, past, kw, eps,

@@ -1279,6 +1279,20 @@ def test_another_stream(ctx):
     check_attention(out, None, want, "given stream")
 
 
+def test_calls_without_tokens(ctx):
+    say("no tokens: every call returns, a rotation's positions and the tables as empty as the rows")
+    x, none = torch.empty(0, 4, 64, device="cuda"), torch.empty(0, dtype=I32, device="cuda")
+    rope = A.Rope(torch.empty(8, 64, device="cuda"))
+    A.qk_norm_rope(ctx, x, x, x, x, rope=rope, positions=none)
+    cache = A.KvCache.empty(2, 4, 16, 64)
+    table = torch.empty(0, 1, dtype=I32, device="cuda")
+    A.kv_append(ctx, cache, x, x, table, ints([0]), none, rope=rope)
+    y = x.to(BF16)
+    A.paged_attention(ctx, y, cache, table, ints([0]), none, y)
+    A.prompt_attention(ctx, y, y, y, ints([0]), y)
+    torch.cuda.synchronize()
+
+
 def test_refusals_of_tensors(ctx):
     say("tensors that the Python layer refuses")
     x = torch.empty(4, 2, 128, device="cuda")
