@@ -813,6 +813,27 @@ def test_scores_near_and_past_the_range(ctx, heads, kv, dim, n):
             assert bool(((o.cpu().double() - want[0]).abs() <= 2.0 ** -8 * 17 / 16 * want[2] + 2.0 ** -8 * want[0].abs() + 1e-30).all())
 
 
+CUT = [  # lengths, new counts, heads, kv, dim, page, window: chunks that start behind the first token
+    ([5000, 1200], [1, 1], 8, 2, 128, 16, 1500), ([4000], [8], 8, 2, 128, 64, 1900), ([6000, 300], [4, 4], 4, 1, 64, 32, 1000),
+    ([5000, 2000], [9, 3], 8, 2, 128, 16, 700), ([4000, 900], [30, 12], 4, 1, 128, 64, 1200), ([3000], [60], 8, 2, 64, 32, 800),
+    ([4000, 77], [2, 1], 12, 2, 256, 64, 1500), ([3500], [20], 6, 2, 256, 16, 900), ([5000, 640], [1, 1], 16, 1, 512, 16, 1100),
+    ([3000], [4], 32, 1, 512, 64, 1300), ([3000, 2000], [60, 60], 4, 1, 128, 64, 0), ([3000, 2000], [60, 41], 4, 1, 128, 16, 900),
+    ([2500], [70], 8, 2, 64, 64, 0), ([2500, 1000], [70, 66], 8, 2, 64, 16, 700)]
+
+
+@pytest.mark.parametrize("lengths,new,heads,kv,dim,page,window", CUT)
+def test_paged_cut_windows_and_large_tiles(ctx, lengths, new, heads, kv, dim, page, window):
+    """Chunks that start at a window, some before some rows' own; chunks of tiles of 128 rows."""
+    say(f"paged cut: lens={lengths} new={new} heads={heads}/{kv} dim={dim} page={page} window={window}")
+    p = Paged(sum(lengths), lengths, kv, dim, page)
+    q = rand(gen(14), sum(new), heads, dim, dtype=BF16).cuda()
+    want = paged_want(p, q, new, window)
+    for max_len in (max(lengths), 64, 1 << 24):
+        out, lse = run_paged(ctx, p, q, new, heads, dim, window, F32, max_len=max_len)
+        check_attention(out, lse, want, f"max_len {max_len}")
+    ctx.launch_status()
+
+
 def ctx_status(ctx):
     try:
         ctx.launch_status()
@@ -1100,6 +1121,51 @@ def test_prompt_long(ctx, heads, kv, dim):
     out, lse = run_prompt(ctx, q, k, v, [2900])
     want = attention64(q[-3:].cpu(), k.cpu(), v.cpu(), dim ** -0.5, 0)
     check_attention(out[-3:], lse[-3:], want, "last rows")
+
+
+def test_prompt_counts_that_lie(ctx):
+    """Bounds are held inside the rows: one that runs backwards is an empty
+    sequence, one past the rows ends there."""
+    say("prompt: counts outside the rows, each sequence against its own run")
+    g = gen(8)
+    q, k, v = (rand(g, 90, h, 128, dtype=BF16).cuda() for h in (8, 2, 2))
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+    A.prompt_attention(ctx, q, k, v, ints([-3, 40, 20, 1 << 30]), out, lse=lse)
+    first = run_prompt(ctx, q[:40], k[:40], v[:40], [40])
+    last = run_prompt(ctx, q[20:], k[20:], v[20:], [70])
+    # rows 20 to 39 stand in both: either's
+    assert torch.equal(out[:20], first[0][:20]) and torch.equal(lse[:20], first[1][:20])
+    assert torch.equal(out[40:], last[0][20:]) and torch.equal(lse[40:], last[1][20:])
+    both = (out[20:40] == first[0][20:]) | (out[20:40] == last[0][:20])
+    assert bool(both.all())
+
+
+@pytest.mark.parametrize("heads,kv,dim,lengths,window", [(4, 1, 128, [2900], 0), (2, 2, 64, [1500, 700], 0), (2, 1, 256, [1300], 0),
+                                                         (4, 4, 128, [1100, 64, 900], 700), (3, 1, 64, [1700], 1000)])
+def test_prompt_every_row_of_long_ones(ctx, heads, kv, dim, lengths, window):
+    """Every row of prompts whose tiles are mostly walked without a mask."""
+    say(f"prompt {lengths} heads={heads}/{kv} dim={dim} window={window}: every row")
+    g, t = gen(31), sum(lengths)
+    q, k, v = (rand(g, t, h, dim, dtype=BF16).cuda() for h in (heads, kv, kv))
+    q *= 2
+    out, lse = run_prompt(ctx, q, k, v, lengths, window, F32)
+    at = 0
+    for n in lengths:
+        i = torch.arange(n)
+        hidden = i[None] > i[:, None]
+        if window:
+            hidden |= i[None] <= i[:, None] - window
+        for h in range(heads):
+            qd, kd, vd = (x[at:at + n, j].cpu().double() for x, j in ((q, h), (k, h // (heads // kv)), (v, h // (heads // kv))))
+            s = (qd @ kd.T * dim ** -0.5).masked_fill(hidden, -math.inf)
+            l = s.logsumexp(-1)
+            w = (s - l[:, None]).exp()
+            big = (qd.abs() @ kd.abs().T * dim ** -0.5).masked_fill(hidden, 0.0).amax(-1)
+            o, mass = w @ vd, w @ vd.abs()
+            assert bool(((out[at:at + n, h].cpu().double() - o).abs() <= 2.0 ** -8 * 17 / 16 * mass + 1e-30).all()), (at, h)
+            tol = (dim + 8) * 2.0 ** -24 * big + 2.0 ** -20 * (1 + l.abs())
+            assert bool(((lse[at:at + n, h].cpu().double() - l).abs() <= tol).all()), (at, h)
+        at += n
 
 
 # ---------------------------------------------------------------------------
