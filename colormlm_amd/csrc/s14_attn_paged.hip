@@ -124,7 +124,7 @@ constexpr uint32_t kRecord = D + 4;
 // Where the chunks of a row are joined.  A second launch costs about 4 us, its
 // workgroups share the rows; the workgroup that arrives last at a (row tile,
 // sequence, key head) does it at once, but reads all its partial results
-// alone: the plan fuses where those are few (PagedPlan::fused).
+// alone: the plan fuses where those are few (PagedPlan::fused: 4 rows at the most).
 //
 // The last one sees the others' results, across the XCDs, because they are
 // written through to the device's coherence point (agent scope, sc1), each
@@ -132,6 +132,8 @@ constexpr uint32_t kRecord = D + 4;
 // and they are read from there.  A release fence would write back the L2.
 constexpr int kAgent = 0x10;  // buffer cache policy: sc1
 
+// kFuse: the kernel has plans that fuse (those of one row tile).
+template <bool kFuse>
 struct PartStore {
   __amdgpu_buffer_rsrc_t r;
   uint32_t fused;
@@ -140,7 +142,7 @@ struct PartStore {
     r = __builtin_amdgcn_make_buffer_rsrc(rec, 0, int(floats * 4), 0x00020000);
   }
   __device__ __forceinline__ void operator()(uint32_t at, f32x4 v) const {
-    if (fused)
+    if (kFuse && fused)
       __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at * 4, 0, kAgent);
     else
       *reinterpret_cast<f32x4 *>(p + at) = v;
@@ -547,7 +549,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
   }
   if (wave == 0) {
     const uint32_t floats = p.rec_rows * kRecord<D>;
-    const PartStore store(part + record_of(a, p, it, kvh) * floats, floats, p.fused);
+    const PartStore<NT == 1> store(part + record_of(a, p, it, kvh) * floats, floats, p.fused);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       if (16 * nt + n >= p.rec_rows) continue;
@@ -557,8 +559,10 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
       for (int dt = 0; dt < DT; ++dt) store(row + 16 * dt + 4 * g, o[nt][dt]);
     }
   }
-  if (!p.fused) return;
-  if (arrived_last(a.count + (tile * a.seqs + seq) * kvh + head, sp.chunks)) join_tile<D>(a, p, sp, it, row0, part);
+  if constexpr (NT == 1) {
+    if (!p.fused) return;
+    if (arrived_last(a.count + (tile * a.seqs + seq) * kvh + head, sp.chunks)) join_tile<D>(a, p, sp, it, row0, part);
+  }
 }
 
 // Heads of 512 (one wide key head for many query heads): 16 NT rows of Q and O
@@ -800,7 +804,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
   }
   __syncthreads();
   const uint32_t floats = p.rec_rows * kRecord<D>;
-  const PartStore store(part + record_of(a, p, it, kvh) * floats, floats, p.fused);
+  const PartStore<NT == 1> store(part + record_of(a, p, it, kvh) * floats, floats, p.fused);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const uint32_t r = row0 + 16 * nt + n;
@@ -822,8 +826,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
                 o[nt][dt][1] * inv, o[nt][dt][2] * inv, o[nt][dt][3] * inv);
     if (a.lse && wave == 0 && g == 0) a.lse[t * a.heads + h] = total == 0.0f ? -INFINITY : top * kLn2 + __logf(total);
   }
-  if (sp.chunks <= 1 || !p.fused) return;
-  if (arrived_last(a.count + (tile * a.seqs + seq) * kvh + head, sp.chunks)) join_tile<D>(a, p, sp, it, row0, part);
+  if constexpr (NT == 1) {
+    if (sp.chunks <= 1 || !p.fused) return;
+    if (arrived_last(a.count + (tile * a.seqs + seq) * kvh + head, sp.chunks)) join_tile<D>(a, p, sp, it, row0, part);
+  }
 }
 
 // Where a row's 16-byte piece of K or V lies in LDS: piece ^ turn(row), so that
@@ -1115,7 +1121,7 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
   }
   if (const uint32_t status = sp.wrong | (flags & 1u ? kStatusBadCachePage : 0u); status && tid == 0) atomicOr(a.status, status);
   const uint32_t floats = p.rec_rows * kRecord<D>;
-  const PartStore store(part + record_of(a, p, it, kvh) * floats, floats, p.fused);
+  const PartStore<false> store(part + record_of(a, p, it, kvh) * floats, floats, 0);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const float total = flags & 1u ? __uint_as_float(0x7fc00000u) : sum_lane16(sum[nt]);
@@ -1137,8 +1143,6 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
                 o[nt][dt][1] * inv, o[nt][dt][2] * inv, o[nt][dt][3] * inv);
     if (a.lse && g == 0) a.lse[t * a.heads + h] = total == 0.0f ? -INFINITY : m[nt] * kLn2 + __logf(total);
   }
-  if (sp.chunks <= 1 || !p.fused) return;
-  if (arrived_last(a.count + (tile * a.seqs + seq) * kvh + head, sp.chunks)) join_tile<D>(a, p, sp, it, row0, part);
 }
 
 // Joins the chunks of one row a workgroup, in an order that its size alone

@@ -69,7 +69,8 @@ def check(lib, seqs, heads, kv, dim, max_new, max_len, window=0, reach=REACH):
     assert p.blocks == tiles * kv * seqs * p.chunks, what
     if p.chunks > 1:
         assert p.blocks * p.rec_rows * (dim + 4) <= part.value, what
-        if p.fused:
+        if p.fused:  # only the kernels of one row tile join their own chunks
+            assert p.row_tiles == 1 and p.rec_rows <= 4, what
             assert p.chunks <= 64 and tiles * kv * seqs <= counters.value, what
     for span in (0, 1, 63, 64, 65, max_len, 5 * max_len, p.chunk, p.chunk * p.chunks, 1_000_003, REACH):
         if span > REACH:
