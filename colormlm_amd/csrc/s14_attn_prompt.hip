@@ -140,7 +140,7 @@ __device__ __forceinline__ void stage(const uint16_t *base, uint32_t stride, int
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
                      __builtin_amdgcn_readfirstlane(to) + i * 4096),
                  "v"(in * stride + piece * 16), "s"(r)
-                 : "memory", "m0");
+                 : "memory");
   }
 }
 
