@@ -131,6 +131,8 @@ __device__ __forceinline__ void stage(const uint16_t *base, uint32_t stride, int
   // In asm: the compiler would let every LDS read wait for these loads, whose
   // halves of the double buffer it cannot tell apart.  No register waits for
   // them; the wait at the head of the next tile does.
+  // m0 cannot be named as changed (the compiler reserves it, and warns); nothing
+  // else in these kernels reads it: gfx950's other LDS instructions do not.
 #pragma unroll
   for (uint32_t i = 0; i < kPasses; ++i) {
     const uint32_t in = threadIdx.x / kPieces, piece = (threadIdx.x % kPieces) ^ swizzle<D, kV>(i * kRows + in);
