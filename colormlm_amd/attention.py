@@ -79,12 +79,13 @@ class Rope:
             _refuse(N.S14_ERR_SHAPE, "a rotation table is contiguous float32 [positions, rot]")
         if start < 0:
             _refuse(N.S14_ERR_SHAPE, f"rotation start {start}")
-        self._table, self.layout, self.start = table, layout, start
+        self._tensors, self.layout, self.start = (table,), layout, start
         self._c = N.Rope(N.Buffer(table.data_ptr(), table.nbytes), table.shape[0], table.shape[1], start,
                          _LAYOUTS[layout])
         self._at, self._device = C.addressof(self._c), table.get_device()
 
-    table = property(lambda self: self._table)  # its address is held: not to be replaced
+    # its address is held: not to be replaced, and a call refuses other memory behind it
+    table = property(lambda self: self._tensors[0])
 
 
 def _rope(ctx: Context, rope: Optional[Rope]):
@@ -131,7 +132,7 @@ class KvCache:
         self._c = N.KvCache(*buf, pages, heads, page, dim)
         self._at, self._device = C.addressof(self._c), k_pages.get_device()
 
-    # their addresses are held: not to be replaced
+    # their addresses are held: not to be replaced, and a call refuses other memory behind them
     k_pages = property(lambda self: self._tensors[0])
     k_scales = property(lambda self: self._tensors[1])
     v_pages = property(lambda self: self._tensors[2])
@@ -172,7 +173,7 @@ def qk_norm_rope(ctx: Context, q, k, q_out, k_out, q_weight=None, k_weight=None,
     is) of q [tokens, heads, dim] and k (or None) in one launch, in f32; f32 or
     bf16 in and out, outputs may be their inputs."""
     _call.qk_norm_rope(ctx._h.value, ctx.device, stream, q, k, q_out, k_out, q_weight, k_weight, eps, _rope(ctx, rope),
-                       positions)
+                       positions, None if rope is None else rope._tensors)
 
 
 def kv_append(ctx: Context, cache: KvCache, k, v, page_table, cu, past, k_weight=None, eps: float = 1e-6,
@@ -182,7 +183,7 @@ def kv_append(ctx: Context, cache: KvCache, k, v, page_table, cu, past, k_weight
     norm and rotation of ``qk_norm_rope`` on the way.  max_new: at least the
     most new tokens of a sequence (all of them if left out)."""
     _call.kv_append(ctx._h.value, ctx.device, stream, _cache(ctx, cache), cache.dim, k, v, page_table, cu, past, k_weight,
-                    eps, _rope(ctx, rope), max_new)
+                    eps, _rope(ctx, rope), max_new, cache._tensors, None if rope is None else rope._tensors)
 
 
 def paged_attention(ctx: Context, q, cache: KvCache, page_table, cu, lens, out, lse=None, scale: Optional[float] = None,
@@ -194,7 +195,7 @@ def paged_attention(ctx: Context, q, cache: KvCache, page_table, cu, lens, out, 
     least the most rows of a sequence; max_len: about the longest sequence (it
     sets how the work is split; the page table's reach if left out)."""
     _call.paged_attention(ctx._h.value, ctx.device, stream, q, _cache(ctx, cache), cache.dim, page_table, cu, lens, out,
-                          lse, scale, window, max_new, max_len, cache.page_tokens)
+                          lse, scale, window, max_new, max_len, cache.page_tokens, cache._tensors)
 
 
 def prompt_attention(ctx: Context, q, k, v, cu, out, lse=None, scale: Optional[float] = None, window: int = 0,

@@ -130,6 +130,31 @@ static int u32_of(PyObject *v, const char *label, uint32_t *out) {
 
 static void *pointer_of(PyObject *v) { return v == Py_None ? nullptr : PyLong_AsVoidPtr(v); }
 
+// A KvCache or Rope holds the addresses that its tensors had when it was made:
+// refused where one has other memory since (resize_, set_, .data).
+static int held(PyObject *tensors, const s14_buffer *const *bufs, Py_ssize_t n, const char *what) {
+  if (!PyTuple_Check(tensors) || PyTuple_GET_SIZE(tensors) != n) return refuse(S14_ERR_INVALID, "%s has no tensors", what);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject *t = PyTuple_GET_ITEM(tensors, i);
+    if (!THPVariable_Check(t) || THPVariable_Unpack(t).data_ptr() != bufs[i]->ptr ||
+        THPVariable_Unpack(t).nbytes() < bufs[i]->bytes)
+      return refuse(S14_ERR_INVALID, "%s was made of other memory than its tensors have now", what);
+  }
+  return 0;
+}
+static int cache_of(PyObject *at, PyObject *tensors, const s14_kv_cache **out) {
+  const s14_kv_cache *c = *out = (const s14_kv_cache *)pointer_of(at);
+  if (!c) return refuse(S14_ERR_INVALID, "a cache is required");
+  const s14_buffer *const bufs[4] = {&c->k, &c->k_scale, &c->v, &c->v_scale};
+  return held(tensors, bufs, 4, "the cache");
+}
+static int rope_of(PyObject *at, PyObject *tensors, const s14_rope **out) {
+  const s14_rope *r = *out = (const s14_rope *)pointer_of(at);
+  if (!r) return 0;
+  const s14_buffer *const buf = &r->table;
+  return held(tensors, &buf, 1, "the rotation");
+}
+
 static PyObject *done(int rc) {
   if (!rc) Py_RETURN_NONE;
   PyObject *r = PyObject_CallFunction(p_check, "i", rc);
@@ -145,18 +170,18 @@ static int same(const long long a[3], const long long b[3]) { return a[0] == b[0
     if (argc != (n)) return PyErr_Format(PyExc_TypeError, "%d arguments, not %zd", (n), argc);    \
   } while (0)
 
-// handle, device, stream, q, k, q_out, k_out, q_weight, k_weight, eps, rope, positions
+// handle, device, stream, q, k, q_out, k_out, q_weight, k_weight, eps, rope, positions, the rotation's tensors
 static PyObject *qk_norm_rope(PyObject *, PyObject *const *v, Py_ssize_t argc) {
-  ARGUMENTS(12);
+  ARGUMENTS(13);
   s14_ctx *ctx = (s14_ctx *)pointer_of(v[0]);
   const long device = PyLong_AsLong(v[1]);
   const double eps = PyFloat_AsDouble(v[9]);
-  const s14_rope *rope = (const s14_rope *)pointer_of(v[10]);
+  const s14_rope *rope;
   void *stream;
   s14_rows q, qo, k, ko;
   s14_buffer qw, kw, pos;
   long long shape[3], other[3], ks[3];
-  if (PyErr_Occurred()) return nullptr;
+  if (PyErr_Occurred() || rope_of(v[10], v[12], &rope)) return nullptr;
   if (rows_of(v[3], "q", device, 0, &q, shape) || rows_of(v[5], "q output", device, shape[2], &qo, other)) return nullptr;
   if (!same(shape, other)) return refuse(S14_ERR_SHAPE, "q output must have q's shape"), nullptr;
   if (v[4] == Py_None) {
@@ -177,22 +202,22 @@ static PyObject *qk_norm_rope(PyObject *, PyObject *const *v, Py_ssize_t argc) {
   return done(rc);
 }
 
-// handle, device, stream, cache, dim, k, v, page_table, cu, past, k_weight, eps, rope, max_new
+// handle, device, stream, cache, dim, k, v, page_table, cu, past, k_weight, eps, rope, max_new, the cache's and the rotation's tensors
 static PyObject *kv_append(PyObject *, PyObject *const *v, Py_ssize_t argc) {
-  ARGUMENTS(14);
+  ARGUMENTS(16);
   s14_ctx *ctx = (s14_ctx *)pointer_of(v[0]);
   const long device = PyLong_AsLong(v[1]);
-  const s14_kv_cache *cache = (const s14_kv_cache *)pointer_of(v[3]);
+  const s14_kv_cache *cache;
   const long long dim = PyLong_AsLongLong(v[4]);
   const double eps = PyFloat_AsDouble(v[11]);
-  const s14_rope *rope = (const s14_rope *)pointer_of(v[12]);
+  const s14_rope *rope;
   void *stream;
   s14_rows k, x;
   s14_buffer kw;
   index_rows at;
   long long shape[3], other[3];
   uint32_t most;
-  if (PyErr_Occurred()) return nullptr;
+  if (PyErr_Occurred() || cache_of(v[3], v[14], &cache) || rope_of(v[12], v[15], &rope)) return nullptr;
   if (rows_of(v[5], "k", device, dim, &k, shape) || rows_of(v[6], "v", device, dim, &x, other)) return nullptr;
   if (shape[0] != other[0]) return refuse(S14_ERR_SHAPE, "k and v have different token counts"), nullptr;
   if (index_of(v[7], v[8], v[9], "past", device, &at) || flat_of(v[10], "k norm weight", device, at::kFloat, 0, &kw)) return nullptr;
@@ -214,12 +239,12 @@ static int scale_of(PyObject *v, long long dim, float *out) {
   return PyErr_Occurred() ? -1 : 0;
 }
 
-// handle, device, stream, q, cache, dim, page_table, cu, lens, out, lse, scale, window, max_new, max_len, reach of the table's pages
+// handle, device, stream, q, cache, dim, page_table, cu, lens, out, lse, scale, window, max_new, max_len, tokens a page, the cache's tensors
 static PyObject *paged_attention(PyObject *, PyObject *const *v, Py_ssize_t argc) {
-  ARGUMENTS(16);
+  ARGUMENTS(17);
   s14_ctx *ctx = (s14_ctx *)pointer_of(v[0]);
   const long device = PyLong_AsLong(v[1]);
-  const s14_kv_cache *cache = (const s14_kv_cache *)pointer_of(v[4]);
+  const s14_kv_cache *cache;
   const long long dim = PyLong_AsLongLong(v[5]);
   const long long page = PyLong_AsLongLong(v[15]);
   void *stream;
@@ -229,7 +254,7 @@ static PyObject *paged_attention(PyObject *, PyObject *const *v, Py_ssize_t argc
   long long shape[3], other[3];
   uint32_t window = 0, most, length;
   float scale;
-  if (PyErr_Occurred()) return nullptr;
+  if (PyErr_Occurred() || cache_of(v[4], v[16], &cache)) return nullptr;
   if (rows_of(v[3], "q", device, dim, &q, shape) || rows_of(v[9], "out", device, dim, &out, other)) return nullptr;
   if (!same(shape, other)) return refuse(S14_ERR_SHAPE, "out must have q's shape"), nullptr;
   if (index_of(v[6], v[7], v[8], "lens", device, &at)) return nullptr;

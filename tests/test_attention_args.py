@@ -229,3 +229,32 @@ def test_python_layer_refuses_cpu_tensors_and_bad_caches():
         A.qk_norm_rope(FakeContext(), x, None, x, None)
     with pytest.raises(N.S14Error, match="context's device"):
         A.prompt_attention(FakeContext(), x, x, x, torch.zeros(2, dtype=torch.int32), x)
+
+
+class CpuContext:
+    """A context of no GPU: its calls end at the tensors' checks."""
+
+    device, handle, _h = -1, CTX, CTX
+
+
+@pytest.mark.parametrize("swap", [lambda t: t.resize_(2 * t.shape[0], *t.shape[1:]), lambda t: t.set_(torch.zeros_like(t)),
+                                  lambda t: setattr(t, "data", torch.zeros_like(t))])
+@pytest.mark.parametrize("which", range(5))
+def test_other_memory_behind_a_cache_or_rotation_is_refused(swap, which):
+    """A cache and a rotation are made of addresses: a tensor that has other
+    memory since would leave calls writing to what was freed."""
+    u8 = lambda *s: torch.zeros(s, dtype=torch.uint8)  # noqa: E731
+    tensors = [u8(3, 2, 16, 64), u8(3, 2), u8(3, 2, 64, 16), u8(3, 2)]
+    cache, table = A.KvCache(*tensors), torch.zeros(4, 64)
+    rope = A.Rope(table)
+    swap([*tensors, table][which])
+    x, i = torch.zeros(2, 2, 64), torch.zeros(2, dtype=torch.int32)
+    ctx, pages = CpuContext(), torch.zeros(1, 1, dtype=torch.int32)
+    what = "rotation" if which == 4 else "cache"
+    with pytest.raises(N.S14Error, match=f"the {what} was made of other memory"):
+        A.kv_append(ctx, cache, x, x, pages, i, i, rope=rope)
+    with pytest.raises(N.S14Error, match=f"the {what} was made of other memory"):
+        if which == 4:
+            A.qk_norm_rope(ctx, x, None, x, None, rope=rope, positions=i)
+        else:
+            A.paged_attention(ctx, x.bfloat16(), cache, pages, i, i, x)
