@@ -251,14 +251,14 @@ __global__ __launch_bounds__(256) void k_rope_table(RopeTableArgs a) {
 struct Touched {
   uint32_t seq;
   int64_t first, last, past, page;  // packed rows, and the page of the sequence
+  uint32_t wrong;                   // status of the sequence's counts
 };
 // Page `k` of those that the sequence of rows first .. last - 1 touches.
 __device__ __forceinline__ bool sequence_page(const AppendArgs &a, uint32_t seq, int64_t first, int64_t last,
                                               int64_t past, uint32_t k, Touched &t) {
   const int64_t end = min(last, first + int64_t(a.max_new));
-  if (last > first && (past < 0 || last > end) && k == 0 && blockIdx.y == 0 && threadIdx.x == 0)
-    atomicOr(a.status, past < 0 ? kStatusBadPast : kStatusBadCounts);
-  t = Touched{seq, first, end, past, past / a.cache.page + k};
+  t = Touched{seq, first, end, past, past / a.cache.page + k, 0};
+  if (last > first) t.wrong = past < 0 ? kStatusBadPast : last > end ? kStatusBadCounts : 0u;
   return past >= 0 && end > first && t.page * a.cache.page < past + (end - first);
 }
 __device__ __forceinline__ bool find_page(const AppendArgs &a, uint32_t index, uint32_t lane, Touched &t) {
@@ -430,19 +430,22 @@ __device__ __forceinline__ void append_page(const AppendArgs &a, const Touched &
 template <int kDim, int kIt, bool kTurn>
 __global__ __launch_bounds__(1024) void k_kv_append(AppendArgs a, uint32_t direct) {
   const uint32_t head = blockIdx.y >> 1, side = blockIdx.y & 1u;
-  Touched t;
+  Touched t{};
+  bool any;
   if (direct) {
     const uint32_t seq = blockIdx.x / direct;
-    if (!sequence_page(a, seq, clamp_row(a.cu[seq], a.tokens), clamp_row(a.cu[seq + 1], a.tokens), a.past[seq],
-                       blockIdx.x % direct, t))
-      return;
-  } else if (!find_page(a, blockIdx.x, threadIdx.x & 63u, t)) {
-    return;
+    any = sequence_page(a, seq, clamp_row(a.cu[seq], a.tokens), clamp_row(a.cu[seq + 1], a.tokens), a.past[seq],
+                        blockIdx.x % direct, t);
+  } else {
+    any = find_page(a, blockIdx.x, threadIdx.x & 63u, t);
   }
-  if (a.in[side].bf16)
-    append_page<kDim, kIt, kTurn, true>(a, t, head, side);
-  else
-    append_page<kDim, kIt, kTurn, false>(a, t, head, side);
+  if (any) {
+    if (a.in[side].bf16)
+      append_page<kDim, kIt, kTurn, true>(a, t, head, side);
+    else
+      append_page<kDim, kIt, kTurn, false>(a, t, head, side);
+  }
+  if (t.wrong && threadIdx.x == 0) atomicOr(a.status, t.wrong);
 }
 
 }  // namespace
