@@ -77,7 +77,7 @@ class Rope:
             _refuse(N.S14_ERR_INVALID, f"unknown rotation layout {layout!r}")
         if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
             _refuse(N.S14_ERR_SHAPE, "a rotation table is contiguous float32 [positions, rot]")
-        if start < 0:
+        if not 0 <= start < 1 << 32:
             _refuse(N.S14_ERR_SHAPE, f"rotation start {start}")
         self._tensors, self.layout, self.start = (table,), layout, start
         self._c = N.Rope(N.Buffer(table.data_ptr(), table.nbytes), table.shape[0], table.shape[1], start,

@@ -258,3 +258,10 @@ def test_other_memory_behind_a_cache_or_rotation_is_refused(swap, which):
             A.qk_norm_rope(ctx, x, None, x, None, rope=rope, positions=i)
         else:
             A.paged_attention(ctx, x.bfloat16(), cache, pages, i, i, x)
+
+
+@pytest.mark.parametrize("start", [1 << 32, (1 << 32) + 8, 1 << 40, -(1 << 32)])
+def test_rotation_start_past_32_bits_is_refused(start):
+    """It would be another one in the call's 32 bits."""
+    with pytest.raises(N.S14Error, match="start"):
+        A.Rope(torch.zeros(4, 8), start=start)
