@@ -50,6 +50,7 @@ bool head_dim(uint32_t dim) { return dim == 64 || dim == 128 || dim == 256 || di
 
 constexpr uint64_t kMaxStride = 1ull << 24;  // elements; a key tile's rows stay inside 32-bit offsets
 constexpr uint32_t kMaxTokens = 1u << 30, kMaxGrid = 65535;
+constexpr uint64_t kMaxBlocks = 1u << 24;  // of 256 threads: a launch has below 2^32 in one dimension
 
 // A packed [tokens][heads][dim] operand: dtype, strides, and that its last
 // value lies inside the buffer.
@@ -173,6 +174,8 @@ extern "C" int s14_rope_table(s14_ctx *ctx, void *stream, uint32_t positions, ui
     a.factor = s.factor, a.original = s.original, a.fast = s.beta_fast, a.slow = s.beta_slow, a.amplitude = s.amplitude;
   }
   if (int rc = require(table, uint64_t(positions) * rot * 4, 16, "rotation table")) return rc;
+  if ((uint64_t(positions) * (rot / 2) + 255) / 256 >= kMaxBlocks)
+    return fail(S14_ERR_SHAPE, "rotation table of %u positions and %u dimensions exceeds one launch", positions, rot);
   const OnDevice on(s14::ctx_device(ctx));
   if (on.error() != hipSuccess) return hip_fail(on.error(), "hipSetDevice");
   const hipError_t e = s14::launch_rope_table(reinterpret_cast<hipStream_t>(stream), a);
@@ -198,7 +201,8 @@ extern "C" int s14_qk_norm_rope(s14_ctx *ctx, void *stream, uint32_t tokens, uin
   if (int rc = check_rope(rope, dim, &a.rope)) return rc;
   if (a.rope.table && tokens)
     if (int rc = require(positions, 4ull * tokens, 4, "positions")) return rc;
-  if (uint64_t(tokens) * (uint64_t(q->heads) + k->heads) > (1ull << 31))
+  const uint64_t per = 2048 / dim;  // rows of a workgroup
+  if ((uint64_t(tokens) * q->heads + per - 1) / per + (uint64_t(tokens) * k->heads + per - 1) / per >= kMaxBlocks)
     return fail(S14_ERR_SHAPE, "%u tokens of %u heads exceed one launch", tokens, q->heads + k->heads);
   if (!tokens) return S14_OK;
   a.tokens = tokens, a.dim = dim;
@@ -270,7 +274,7 @@ extern "C" int s14_paged_attention(s14_ctx *ctx, void *stream, const s14_rows *q
   a.scale = scale, a.window = window;
   const s14::PagedPlan p = s14::paged_plan(
       {seqs, a.heads, cache->heads, cache->dim, max_new, max_len, window, table_width * cache->page_tokens});
-  if (p.blocks >= (1u << 24) || uint64_t(max_new) * q->heads >= (1ull << 31))
+  if (p.blocks >= kMaxBlocks || uint64_t(max_new) * q->heads >= (1ull << 31))
     return fail(S14_ERR_SHAPE, "%u new tokens of %u sequences exceed one launch", max_new, seqs);
   a.status = s14::ctx_status(ctx), a.count = s14::ctx_attn_counters(ctx);
   const OnDevice on(s14::ctx_device(ctx));
@@ -297,7 +301,7 @@ extern "C" int s14_prompt_attention(s14_ctx *ctx, void *stream, uint32_t dim, co
   if (int rc = check_scale(scale)) return rc;
   if (!tokens || !seqs) return S14_OK;
   if (int rc = require(cu, 4 * (uint64_t(seqs) + 1), 4, "cu")) return rc;
-  if ((uint64_t(tokens) * (q->heads / k->heads) / 128 + seqs + 1) * k->heads >= (1u << 24))
+  if ((uint64_t(tokens) * (q->heads / k->heads) / 128 + seqs + 1) * k->heads >= kMaxBlocks)
     return fail(S14_ERR_SHAPE, "%u tokens of %u heads exceed one launch", tokens, q->heads);
   s14::PromptArgs a{};
   a.tokens = tokens, a.seqs = seqs, a.heads = q->heads, a.kv_heads = k->heads, a.dim = dim;

@@ -265,3 +265,13 @@ def test_rotation_start_past_32_bits_is_refused(start):
     """It would be another one in the call's 32 bits."""
     with pytest.raises(N.S14Error, match="start"):
         A.Rope(torch.zeros(4, 8), start=start)
+
+
+@pytest.mark.parametrize("dim,tokens,heads", [(512, 1 << 26, 1), (256, 1 << 27, 1), (64, 1 << 23, 64), (128, 1 << 23, 32)])
+def test_more_rows_than_a_launch_has_threads_are_refused(native, dim, tokens, heads):
+    x = rows(heads, token=heads * dim, head=dim)
+    refused(N.S14_ERR_SHAPE, norm_rope(native, tokens=tokens, dim=dim, q=x, k=rows(0), qo=x, ko=rows(0)), "one launch")
+
+
+def test_a_table_past_a_launch_is_refused(native):
+    refused(N.S14_ERR_SHAPE, native.s14_rope_table(CTX, None, 1 << 27, 64, 1e4, None, BIG), "one launch")
