@@ -65,11 +65,11 @@ static int rows_of(PyObject *t, const char *label, long device, long long dim, s
   const at::IntArrayRef size = x->sizes(), stride = x->strides();
   if (size.size() != 3 || (stride[2] != 1 && size[2] > 1) || (dim && size[2] != dim))
     return refuse(S14_ERR_SHAPE, "%s must be [tokens, heads, dim] of the call's dim, its last dimension contiguous", label);
-  if (size[0] > UINT32_MAX || size[1] > UINT32_MAX || size[2] > UINT32_MAX || stride[1] > UINT32_MAX)
-    return refuse(S14_ERR_SHAPE, "%s is too large", label);
-  for (int i = 0; i < 3; ++i) shape[i] = size[i];
   // strides of a dimension of one are not used; what torch gives there may be anything
   const uint64_t token = size[0] < 2 ? 0 : uint64_t(stride[0]), head = size[1] < 2 ? 0 : uint64_t(stride[1]);
+  if (size[0] > UINT32_MAX || size[1] > UINT32_MAX || size[2] > UINT32_MAX || head > UINT32_MAX)
+    return refuse(S14_ERR_SHAPE, "%s is too large", label);
+  for (int i = 0; i < 3; ++i) shape[i] = size[i];
   r->buf.ptr = x->data_ptr();
   r->buf.bytes = size[0] && size[1] ? ((size[0] - 1) * token + (size[1] - 1) * head + size[2]) * (f32 ? 4 : 2) : 0;
   r->dtype = f32 ? S14_X_F32 : S14_X_BF16;

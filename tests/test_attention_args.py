@@ -275,3 +275,11 @@ def test_more_rows_than_a_launch_has_threads_are_refused(native, dim, tokens, he
 
 def test_a_table_past_a_launch_is_refused(native):
     refused(N.S14_ERR_SHAPE, native.s14_rope_table(CTX, None, 1 << 27, 64, 1e4, None, BIG), "one launch")
+
+
+def test_strides_of_single_heads_are_not_asked_for():
+    """torch may give a dimension of one any stride: such a call ends at the next
+    thing that is wrong with it, here its eps."""
+    x = torch.zeros(2, 64).as_strided((2, 1, 64), (64, 1 << 33, 1))
+    with pytest.raises(N.S14Error, match="eps"):
+        A.qk_norm_rope(CpuContext(), x, None, x, None, q_weight=torch.ones(64), eps=-1.0)
