@@ -282,4 +282,4 @@ def test_strides_of_single_heads_are_not_asked_for():
     thing that is wrong with it, here its eps."""
     x = torch.zeros(2, 64).as_strided((2, 1, 64), (64, 1 << 33, 1))
     with pytest.raises(N.S14Error, match="eps"):
-        A.qk_norm_rope(CpuContext(), x, None, x, None, q_weight=torch.ones(64), eps=-1.0)
+        A.qk_norm_rope(CpuContext(), x, None, x, None, q_weight=torch.ones(64), eps=-1.0, stream=0)
