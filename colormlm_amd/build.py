@@ -15,11 +15,13 @@ into colormlm_amd/lib/libs14hip.so:
   contracts) without that flag.
 
 Beside it lib/_s14attn.so, the attention calls' Python side (s14_attn_py.cpp, a
-CPython extension over torch's headers and libraries, which are loaded before it).
+CPython extension over torch's headers and libraries, which are loaded before it;
+left out where there is no torch).
 """
 
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -105,6 +107,9 @@ def build(verbose: bool = False) -> Path:
     tmp = OUT.with_suffix(".so.tmp")
     _run(link_command(tmp), verbose)
     os.replace(tmp, OUT)
+    if importlib.util.find_spec("torch") is None:
+        print(f"{PY_OUT.name} is not built: there is no torch (colormlm_amd.attention needs both)", file=sys.stderr)
+        return OUT
     tmp = PY_OUT.with_suffix(".so.tmp")
     _run(python_command(tmp), verbose)
     os.replace(tmp, PY_OUT)
