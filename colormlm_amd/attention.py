@@ -171,7 +171,8 @@ def qk_norm_rope(ctx: Context, q, k, q_out, k_out, q_weight=None, k_weight=None,
                  rope: Optional[Rope] = None, positions=None, stream=None) -> None:
     """Per-head RMS norm (where a weight is given) and rotation (where `rope`
     is) of q [tokens, heads, dim] and k (or None) in one launch, in f32; f32 or
-    bf16 in and out, outputs may be their inputs."""
+    bf16 in and out.  An output may be its own input; outputs that share memory
+    with other rows are refused, here and below."""
     _call.qk_norm_rope(ctx._h.value, ctx.device, stream, q, k, q_out, k_out, q_weight, k_weight, eps, _rope(ctx, rope),
                        positions, None if rope is None else rope._tensors)
 

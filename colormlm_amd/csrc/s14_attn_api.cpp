@@ -6,6 +6,7 @@
 #include <cmath>
 
 #include "s14_attn.hpp"
+#include "s14_attn_share.h"
 #include "s14_internal.hpp"
 
 using s14::fail;
@@ -83,6 +84,18 @@ int check_out(const s14_rows *out, const s14_rows *like, uint32_t tokens, uint32
                   out->head_stride);
   }
   return S14_OK;
+}
+
+s14::RowBytes bytes_of(const s14_rows *r, uint32_t dim) {
+  const uint64_t size = r->dtype == S14_X_F32 ? 4 : 2;
+  return {reinterpret_cast<uintptr_t>(r->buf.ptr), r->token_stride * size, r->head_stride * size, dim * size, r->heads};
+}
+
+// An output's rows lie apart from another operand's, but for each its own
+// input's place: workgroups write while others read.
+int check_apart(const s14_rows *out, const s14_rows *other, uint32_t tokens, uint32_t dim, bool own, const char *label) {
+  if (!tokens || !s14::rows_share(bytes_of(out, dim), bytes_of(other, dim), tokens, own)) return S14_OK;
+  return fail(S14_ERR_INVALID, "%s shares memory with %s rows", label, own ? "other" : "another operand's");
 }
 
 int check_rope(const s14_rope *r, uint32_t dim, s14::RopeArgs *out) {
@@ -205,6 +218,14 @@ extern "C" int s14_qk_norm_rope(s14_ctx *ctx, void *stream, uint32_t tokens, uin
   if ((uint64_t(tokens) * q->heads + per - 1) / per + (uint64_t(tokens) * k->heads + per - 1) / per >= kMaxBlocks)
     return fail(S14_ERR_SHAPE, "%u tokens of %u heads exceed one launch", tokens, q->heads + k->heads);
   if (!tokens) return S14_OK;
+  if (int rc = check_apart(q_out, q, tokens, dim, true, "q output")) return rc;
+  if (k->heads) {
+    if (int rc = check_apart(k_out, k, tokens, dim, true, "k output")) return rc;
+    if (int rc = check_apart(q_out, k, tokens, dim, false, "q output")) return rc;
+    if (int rc = check_apart(k_out, q, tokens, dim, false, "k output")) return rc;
+    if (s14::rows_share(bytes_of(q_out, dim), bytes_of(k_out, dim), tokens, false))
+      return fail(S14_ERR_INVALID, "the q and k outputs share memory");
+  }
   a.tokens = tokens, a.dim = dim;
   a.in[0] = rows_of(q), a.out[0] = out_of(q_out);
   if (k->heads) a.in[1] = rows_of(k), a.out[1] = out_of(k_out);
@@ -276,6 +297,7 @@ extern "C" int s14_paged_attention(s14_ctx *ctx, void *stream, const s14_rows *q
       {seqs, a.heads, cache->heads, cache->dim, max_new, max_len, window, table_width * cache->page_tokens});
   if (p.blocks >= kMaxBlocks || uint64_t(max_new) * q->heads >= (1ull << 31))
     return fail(S14_ERR_SHAPE, "%u new tokens of %u sequences exceed one launch", max_new, seqs);
+  if (int rc = check_apart(out, q, tokens, cache->dim, true, "out")) return rc;
   a.status = s14::ctx_status(ctx), a.count = s14::ctx_attn_counters(ctx);
   const OnDevice on(s14::ctx_device(ctx));
   if (on.error() != hipSuccess) return hip_fail(on.error(), "hipSetDevice");
@@ -303,6 +325,9 @@ extern "C" int s14_prompt_attention(s14_ctx *ctx, void *stream, uint32_t dim, co
   if (int rc = require(cu, 4 * (uint64_t(seqs) + 1), 4, "cu")) return rc;
   if ((uint64_t(tokens) * (q->heads / k->heads) / 128 + seqs + 1) * k->heads >= kMaxBlocks)
     return fail(S14_ERR_SHAPE, "%u tokens of %u heads exceed one launch", tokens, q->heads);
+  if (int rc = check_apart(out, q, tokens, dim, true, "out")) return rc;
+  if (int rc = check_apart(out, k, tokens, dim, false, "out")) return rc;
+  if (int rc = check_apart(out, v, tokens, dim, false, "out")) return rc;
   s14::PromptArgs a{};
   a.tokens = tokens, a.seqs = seqs, a.heads = q->heads, a.kv_heads = k->heads, a.dim = dim;
   a.q = static_cast<const uint16_t *>(q->buf.ptr), a.q_token = q->token_stride, a.q_head = q->head_stride;

@@ -489,8 +489,9 @@ int s14_rope_table(s14_ctx *ctx, void *stream, uint32_t positions, uint32_t rot,
 /* Per-head RMS norm x * rsqrt(mean(x^2) + eps) * weight of queries and keys,
  * then the rotation at positions[t] (device int32 [tokens]), f32 throughout,
  * each output rounded once to its dtype.  A weight (f32 [dim]) of NULL leaves that side's norm out; rope
- * NULL leaves the rotation out; k.heads 0 leaves the keys out.  Outputs may be
- * their inputs.  A position outside the table gives NaN rows. */
+ * NULL leaves the rotation out; k.heads 0 leaves the keys out.  An output may
+ * lie in its own input's place, row on row; outputs that share memory with
+ * other rows are refused, here and below.  A position outside the table gives NaN rows. */
 int s14_qk_norm_rope(s14_ctx *ctx, void *stream, uint32_t tokens, uint32_t dim, const s14_rows *q,
                      const s14_rows *k, const s14_rows *q_out, const s14_rows *k_out,
                      s14_buffer q_weight, s14_buffer k_weight, float eps, const s14_rope *rope,
@@ -529,7 +530,7 @@ int s14_kv_append(s14_ctx *ctx, void *stream, const s14_kv_cache *cache, uint32_
  * sequence i, over its lens[i] cached tokens (these rows' own among them:
  * append first).  Row j of n sees positions <= lens[i] - n + j, with window >
  * 0 only the last `window` of them; heads of q share a key head in groups of
- * heads / cache heads.  out (bf16 or f32) = softmax(scale q.k) v (scale > 0), the
+ * heads / cache heads.  out (bf16 or f32; it may be q) = softmax(scale q.k) v (scale > 0), the
  * softmax in f32, its weights rounded to bf16 for the second product; lse (f32
  * [tokens][heads], or ptr NULL) the natural log of the weights' sum.  A row
  * that sees nothing is 0 with lse -inf.  A value past f32's range, as which an

@@ -1359,6 +1359,37 @@ def test_calls_without_tokens(ctx):
     torch.cuda.synchronize()
 
 
+def test_outputs_in_their_inputs_place(ctx):
+    say("outputs in the place of their inputs: q and k interleaved, prompts, every tile of the cache's attention")
+    g = gen(17)
+    rope, pos, w = A.Rope(table64(64, 128).float().cuda()), torch.arange(40, dtype=I32).cuda(), rand(g, 128).cuda()
+    fused = rand(g, 40, 4, 3, 128).cuda()  # q, k and v of a head side by side
+    q, k = fused[:, :, 0], fused[:, :, 1]
+    before = fused.clone()
+    want = [torch.empty(40, 4, 128, device="cuda") for _ in range(2)]
+    A.qk_norm_rope(ctx, q, k, *want, q_weight=w, k_weight=w, rope=rope, positions=pos)
+    A.qk_norm_rope(ctx, q, k, q, k, q_weight=w, k_weight=w, rope=rope, positions=pos)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(fused[:, :, 2], before[:, :, 2])
+    with pytest.raises(s14.S14Error, match="shares memory"):
+        A.qk_norm_rope(ctx, q, k, k, q)
+    packed = rand(g, 300, 12 * 128, dtype=BF16).cuda()
+    q, k, v = (packed[:, a * 128:b * 128].view(300, -1, 128) for a, b in ((0, 8), (8, 10), (10, 12)))
+    for window in (0, 70):
+        mine = packed.clone()
+        mq, mk, mv = (mine[:, a * 128:b * 128].view(300, -1, 128) for a, b in ((0, 8), (8, 10), (10, 12)))
+        out, _ = run_prompt(ctx, q, k, v, [170, 130], window)
+        A.prompt_attention(ctx, mq, mk, mv, cumulative([170, 130]), mq, window=window)
+        assert torch.equal(mq, out) and torch.equal(mine[:, 1024:], packed[:, 1024:])
+    with pytest.raises(s14.S14Error, match="shares memory"):
+        A.prompt_attention(ctx, q[:, :2], k, v, cumulative([170, 130]), v)
+    for heads, kv, dim, new in EVERY_TILE:
+        p = Paged(7, [700, 150], kv, dim, 32)
+        q = rand(gen(4), 2 * new, heads, dim, dtype=BF16).cuda()
+        out, _ = run_paged(ctx, p, q, [new, new], heads, dim)
+        A.paged_attention(ctx, q, p.cache, p.dev_table, cumulative([new, new]), p.lens, q, max_new=new, max_len=700)
+        assert torch.equal(q, out), (heads, kv, dim, new)
+
+
 def test_refusals_of_tensors(ctx):
     say("tensors that the Python layer refuses")
     x = torch.empty(4, 2, 128, device="cuda")
