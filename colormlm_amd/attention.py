@@ -182,7 +182,8 @@ def kv_append(ctx: Context, cache: KvCache, k, v, page_table, cu, past, k_weight
     """Rows cu[i] .. cu[i + 1] - 1 of k and v [tokens, heads, dim] (f32 or
     bf16) become positions past[i] .. of sequence i in the cache, K with the
     norm and rotation of ``qk_norm_rope`` on the way.  max_new: at least the
-    most new tokens of a sequence (all of them if left out)."""
+    most new tokens of a sequence, and at most the call's (which it is if left
+    out); rows past it are not stored."""
     _call.kv_append(ctx._h.value, ctx.device, stream, _cache(ctx, cache), cache.dim, k, v, page_table, cu, past, k_weight,
                     eps, _rope(ctx, rope), max_new, cache._tensors, None if rope is None else rope._tensors)
 
@@ -192,8 +193,10 @@ def paged_attention(ctx: Context, q, cache: KvCache, page_table, cu, lens, out, 
     """Attention of q's rows (bf16 [tokens, heads, dim]; cu[i] .. cu[i + 1] - 1
     are the last tokens of sequence i) over the sequences' lens[i] cached
     tokens, causal, with `window` > 0 over the last `window` positions only.
-    out: q's shape, bf16 or f32; lse: f32 [tokens, heads] or None.  max_new: at
-    least the most rows of a sequence; max_len: about the longest sequence (it
+    out: q's shape, bf16 or f32, q itself at will; lse: f32 [tokens, heads] or
+    None.  max_new: at least the most rows of a sequence, and at most the call's
+    tokens, which it is if left out (the work is split for one sequence that has
+    them all: give it for a batch); max_len: about the longest sequence (it
     sets how the work is split; the page table's reach if left out)."""
     _call.paged_attention(ctx._h.value, ctx.device, stream, q, _cache(ctx, cache), cache.dim, page_table, cu, lens, out,
                           lse, scale, window, max_new, max_len, cache.page_tokens, cache._tensors)

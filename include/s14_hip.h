@@ -510,8 +510,8 @@ typedef struct {
 
 /* Rows cu[i] .. cu[i + 1] - 1 of k and v become positions past[i] .. of
  * sequence i (cu, past: device int32 [seqs + 1], [seqs]; page_table device
- * int32 [seqs][table_width]; max_new >= the largest count, a sequence's rows
- * past it are not stored).  K takes the norm
+ * int32 [seqs][table_width]; tokens >= max_new >= the largest count, a
+ * sequence's rows past it are not stored).  K takes the norm
  * and rotation of s14_qk_norm_rope on the way, at those positions.
  * A page's scale is 2^ceil(log2(max(amax, 1e-4) / 448)) of the values put in,
  * never less than the one that its earlier tokens have (slots below past[i]):
@@ -539,8 +539,8 @@ int s14_kv_append(s14_ctx *ctx, void *stream, const s14_kv_cache *cache, uint32_
  * in magnitude, an infinity or a NaN among them, may be NaN.  Table entries of pages that no row
  * sees, behind the length or wholly before the window of the sequence's first
  * row, may hold anything.  max_new and max_len: at least the largest count of
- * rows (a sequence's rows past it are not computed), and about the longest
- * sequence (it only sets how the work is split).  table_width * page_tokens is at most 2^31 - 2^16. */
+ * rows and at most tokens (a sequence's rows past it are not computed), and
+ * about the longest sequence (it only sets how the work is split).  table_width * page_tokens is at most 2^31 - 2^16. */
 int s14_paged_attention(s14_ctx *ctx, void *stream, const s14_rows *q, const s14_kv_cache *cache,
                         uint32_t tokens, uint32_t seqs, uint32_t max_new, uint32_t max_len,
                         s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer lens,
