@@ -511,16 +511,15 @@ typedef struct {
 /* Rows cu[i] .. cu[i + 1] - 1 of k and v become positions past[i] .. of
  * sequence i (cu, past: device int32 [seqs + 1], [seqs]; page_table device
  * int32 [seqs][table_width]; tokens >= max_new >= the largest count, a
- * sequence's rows past it are not stored).  K takes the norm
- * and rotation of s14_qk_norm_rope on the way, at those positions.
+ * sequence's rows past it are not stored).  K takes the norm and rotation of
+ * s14_qk_norm_rope on the way, at those positions.
  * A page's scale is 2^ceil(log2(max(amax, 1e-4) / 448)) of the values put in,
  * never less than the one that its earlier tokens have (slots below past[i]):
  * where it grows their codes are divided by the power of two, rounded to
  * nearest even.  Slots past the last new token stay as they were.  A NaN is
  * stored as NaN (it sets no scale), an infinity as the largest value of the
  * largest scale.  A page outside the cache or past the table takes nothing, nor
- * does a sequence whose past is below 0.
- * A page that one call writes stands in one place of one sequence's row. */
+ * does a sequence whose past is below 0.  A page that one call writes stands in one place of one sequence's row. */
 int s14_kv_append(s14_ctx *ctx, void *stream, const s14_kv_cache *cache, uint32_t tokens,
                   uint32_t seqs, uint32_t max_new, const s14_rows *k, const s14_rows *v,
                   s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer past,
@@ -530,17 +529,19 @@ int s14_kv_append(s14_ctx *ctx, void *stream, const s14_kv_cache *cache, uint32_
  * sequence i, over its lens[i] cached tokens (these rows' own among them:
  * append first).  Row j of n sees positions <= lens[i] - n + j, with window >
  * 0 only the last `window` of them; heads of q share a key head in groups of
- * heads / cache heads.  out (bf16 or f32; it may be q) = softmax(scale q.k) v (scale > 0), the
- * softmax in f32, its weights rounded to bf16 for the second product; lse (f32
- * [tokens][heads], or ptr NULL) the natural log of the weights' sum.  A row
- * that sees nothing is 0 with lse -inf.  A value past f32's range, as which an
- * infinity is stored, makes its dimension of the rows that see it infinite (NaN
- * where its weight is 0), and nothing else.  A row that sees a score past 2^28
- * in magnitude, an infinity or a NaN among them, may be NaN.  Table entries of pages that no row
- * sees, behind the length or wholly before the window of the sequence's first
- * row, may hold anything.  max_new and max_len: at least the largest count of
- * rows and at most tokens (a sequence's rows past it are not computed), and
- * about the longest sequence (it only sets how the work is split).  table_width * page_tokens is at most 2^31 - 2^16. */
+ * heads / cache heads.  out (bf16 or f32; it may be q) = softmax(scale q.k) v
+ * (scale > 0), the softmax in f32, its weights rounded to bf16 for the second
+ * product; lse (f32 [tokens][heads], or ptr NULL) the natural log of the
+ * weights' sum.  A row that sees nothing is 0 with lse -inf.  A value past f32's
+ * range, as which an infinity is stored, makes its dimension of the rows that
+ * see it infinite (NaN where its weight is 0), and nothing else.  A row that
+ * sees a score past 2^28 in magnitude, an infinity or a NaN among them, may be
+ * NaN.  Table entries of pages that no row sees, behind the length or wholly
+ * before the window of the sequence's first row, may hold anything.
+ * max_new: at least the largest count of rows and at most tokens (a sequence's
+ * rows past it are not computed).  max_len: about the longest sequence (it only
+ * sets how the work is split).  table_width * page_tokens is at most 2^31 -
+ * 2^16. */
 int s14_paged_attention(s14_ctx *ctx, void *stream, const s14_rows *q, const s14_kv_cache *cache,
                         uint32_t tokens, uint32_t seqs, uint32_t max_new, uint32_t max_len,
                         s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer lens,
