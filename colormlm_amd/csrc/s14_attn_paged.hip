@@ -710,7 +710,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
     for (int nt = 0; nt < NT; ++nt) {
       const float top = fmaxf(fmaxf(fmaxf(s_m[0][nt][n], s_m[1][nt][n]), fmaxf(s_m[2][nt][n], s_m[3][nt][n])), m[nt]);
       if (__any(top > m[nt] + kRise)) {  // the same in every wavefront
-        const float fade = fade_of(m[nt], top);
+        const float fade = __builtin_amdgcn_exp2f(m[nt] - (top == -INFINITY ? 0.0f : top));  // (x is rounded as top is)
         m[nt] = top;
         sum[nt] *= fade;
 #pragma unroll

@@ -834,6 +834,25 @@ def test_paged_cut_windows_and_large_tiles(ctx, lengths, new, heads, kv, dim, pa
     ctx.launch_status()
 
 
+@pytest.mark.parametrize("heads,new", [(16, 1), (16, 3)])
+def test_wide_heads_keep_large_scores(ctx, heads, new):
+    """At heads of 512 scores are scaled before their maximum is taken: any finite one picks its key."""
+    say(f"paged: scores of 2^60 at heads of 512, {heads} x {new}")
+    g = gen(12)
+    n = 200
+    k, v = rand(g, n, 1, 512).cuda(), rand(g, n, 1, 512).cuda()
+    k[:, :, 0] = 0.0
+    k[40, :, 0] = 2.0 ** 30
+    q = rand(g, new, heads, 512, dtype=BF16)
+    q[:, :, 0] = 2.0 ** 30
+    p = Paged(7, [n], 1, 512, 32)
+    A.kv_append(ctx, p.cache, k, v, p.dev_table, ints([0, n]), ints([0]))
+    p.v, p.vs = p.cache.v_pages.cpu(), p.cache.v_scales.cpu()
+    out, lse = run_paged(ctx, p, q.cuda(), [new], heads, 512, dtype=F32)
+    _, vv = p.rows(0)
+    assert torch.equal(out.cpu().double(), vv[40].expand(new, heads, 512)) and bool((lse > 2.0 ** 55).all())
+
+
 def ctx_status(ctx):
     try:
         ctx.launch_status()
