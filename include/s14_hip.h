@@ -446,7 +446,7 @@ int s14_fp8_linear(s14_ctx *ctx, void *stream, uint32_t m, uint32_t n, uint32_t 
  * launch read or write outside its operands.  s14_launch_status reports pages
  * outside the cache, positions outside the rotation table, lengths below 0 or
  * past the page table (they are held to them), a past below 0 and more new rows
- * of a sequence than max_new.  Bounds in cu run upwards; they are held inside
+ * of a sequence than max_new (max_new 0: nothing is launched, nor reported).  Bounds in cu run upwards; they are held inside
  * the packed rows and not reported: a sequence whose bounds run backwards is
  * empty, and those behind it may not be worked on.
  * Launches of one context share its workspace and must not overlap.

@@ -1409,6 +1409,72 @@ def test_outputs_in_their_inputs_place(ctx):
         assert torch.equal(q, out), (heads, kv, dim, new)
 
 
+def test_operands_of_different_types(ctx):
+    say("q f32 to bf16 beside k bf16 to f32; f32 keys with bf16 values")
+    g = gen(41)
+    q, k = rand(g, 33, 6, 128), rand(g, 33, 2, 128, dtype=BF16)
+    w, table, pos = rand(g, 128), table64(64, 64).float(), torch.arange(33, dtype=I32)
+    outs = torch.empty(33, 6, 128, dtype=BF16, device="cuda"), torch.empty(33, 2, 128, device="cuda")
+    A.qk_norm_rope(ctx, q.cuda(), k.cuda(), *outs, k_weight=w.cuda(), rope=A.Rope(table.cuda()), positions=pos.cuda())
+    for x, weight, got in ((q, None, outs[0]), (k, w, outs[1])):
+        y, mag = norm_rope64(x, weight, 1e-6, table, pos, "half", 0)
+        tol = 144 * 2.0 ** -24 * mag + (2.0 ** -8 * y.abs() if got.dtype == BF16 else 0) + 1e-30
+        assert bool(((got.cpu().double() - y).abs() <= tol).all())
+    k, v = rand(g, 50, 2, 64), rand(g, 50, 2, 64, dtype=BF16)
+    a, b = (Paged(4, [50], 2, 64, 16) for _ in range(2))
+    A.kv_append(ctx, a.cache, k.cuda(), v.cuda(), a.dev_table, ints([0, 50]), ints([0]))
+    A.kv_append(ctx, b.cache, k.cuda(), v.float().cuda(), b.dev_table, ints([0, 50]), ints([0]))
+    for t in ("k_pages", "v_pages", "k_scales", "v_scales"):
+        assert torch.equal(getattr(a.cache, t), getattr(b.cache, t)), t
+
+
+def test_two_contexts_at_once(ctx):
+    """Each context has its own partial results and counters: their launches may overlap."""
+    say("paged: two contexts on two streams, cut sequences, joined in the launch and after it")
+    other = s14.Context(0)
+    p = Paged(9, [9000, 4000], 8, 128, 64)
+    for new in (1, 8):
+        q = [rand(gen(s), 2 * new, 32, 128, dtype=BF16).cuda() for s in (4, 5)]
+        want = [run_paged(ctx, p, x, [new, new], 32, 128)[0] for x in q]
+        cu, streams = cumulative([new, new]), [torch.cuda.Stream() for _ in q]
+        outs = [[torch.empty_like(x) for _ in range(20)] for x in q]
+        torch.cuda.synchronize()
+        for i in range(20):
+            for c, s, x, o in zip((ctx, other), streams, q, outs):
+                A.paged_attention(c, x, p.cache, p.dev_table, cu, p.lens, o[i], max_new=new, max_len=9000, stream=s.cuda_stream)
+        torch.cuda.synchronize()
+        for w, o in zip(want, outs):
+            assert all(torch.equal(x, w) for x in o)
+    other.destroy()
+
+
+def test_most_sequences_of_a_call(ctx):
+    """65,535 sequences, the last ones among them."""
+    say("65,535 sequences: append, attention, prompts")
+    n, kv, dim = 65535, 1, 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k, v, q = (torch.randn(n, kv, dim, generator=g, device="cuda") for _ in range(3))
+    cache = A.KvCache.empty(n, kv, 16, dim)
+    table, cu = torch.randperm(n, generator=g, device="cuda").int()[:, None], torch.arange(n + 1, dtype=I32, device="cuda")
+    zero, one = torch.zeros(n, dtype=I32, device="cuda"), torch.ones(n, dtype=I32, device="cuda")
+    A.kv_append(ctx, cache, k, v, table.contiguous(), cu, zero, max_new=1)
+    out = torch.full((n, kv, dim), 7.0, device="cuda")
+    A.paged_attention(ctx, q.to(BF16), cache, table.contiguous(), cu, one, out, max_new=1, max_len=1)
+    stored = cache.v_pages[table[:, 0].long(), :, :, 0].view(E4M3).double() * (cache.v_scales[table[:, 0].long()].double() - 127).exp2()[..., None]
+    # One visible token: its own value.  Its weight is 2^r, r the rounding of its
+    # score: below 2^-24 * 64 where |q| |k| / 8 * log2(e) is below 64.  As bf16 that is 1,
+    # the sum of weights is 2^r itself, and two roundings of 2^-24 follow: 2^-17 in all.
+    assert float((q.norm(dim=-1) * k.norm(dim=-1)).max()) / 8 * 1.4427 * 1.1 < 64
+    assert bool(((out.double() - stored).abs() <= 2.0 ** -17 * stored.abs()).all())
+    assert bool(((stored - v.double()).abs() <= v.abs().amax(-1, keepdim=True) * 2.0 ** -4).all())
+    ctx.launch_status()
+    vb = v.to(BF16)
+    A.prompt_attention(ctx, q.to(BF16), k.to(BF16), vb, cu, out)
+    assert bool(((out - vb.float()).abs() <= 2.0 ** -17 * vb.float().abs()).all())
+    with pytest.raises(s14.S14Error, match="sequences"):
+        A.prompt_attention(ctx, q.to(BF16), k.to(BF16), vb, torch.zeros(n + 2, dtype=I32, device="cuda"), out)
+
+
 def test_refusals_of_tensors(ctx):
     say("tensors that the Python layer refuses")
     x = torch.empty(4, 2, 128, device="cuda")
