@@ -221,6 +221,7 @@ __device__ __forceinline__ void join_row(const PagedArgs &a, const PagedPlan &p,
   const uint32_t row = row0 + k;
   const uint64_t t = uint64_t(sp.first + row / group);
   const uint32_t h = it.head * group + row % group;
+  if constexpr (D < 512) total = checked_sum(total, top);  // (k_paged_wide scales its scores before it compares them)
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   if (set == 0) {
 #pragma unroll
@@ -258,7 +259,7 @@ __device__ __forceinline__ float odd_value(uint32_t c, uint32_t from) {
 }
 
 template <int D, int NT>
-__global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(PagedArgs a, PagedPlan p, float *part) {
+__global__ __launch_bounds__(256, D * NT <= 64 ? 4 : D * NT <= 128 ? 2 : 1) void k_paged_attention(PagedArgs a, PagedPlan p, float *part) {
   constexpr int T = 4;        // 16-token tiles a step
   constexpr int C = D / 64;   // 16-byte pieces of a K row a lane holds
   constexpr int DT = D / 16;  // 16-dimension tiles of O
@@ -402,7 +403,7 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
       // the maximum that the weights are taken from moves only where they
       // would pass 2^kRise: O is seldom multiplied
       if (__any(top > m[nt] + kRise)) {
-        const float fade = fade_of(m[nt], top);
+        const float fade = __builtin_amdgcn_exp2f(m[nt] - (top == -INFINITY ? 0.0f : top));
         m[nt] = top;
         sum[nt] *= fade;
 #pragma unroll
@@ -538,12 +539,12 @@ __global__ __launch_bounds__(256, D * NT <= 128 ? 2 : 1) void k_paged_attention(
       if (r >= sp.rows) continue;
       const uint64_t t = uint64_t(sp.first + r / group);
       const uint32_t h = head * group + r % group;
-      const float inv = sum[nt] == 0.0f ? 0.0f : 1.0f / sum[nt];
+      const float total = checked_sum(sum[nt], m[nt]), inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
         store_out(a.out, t * a.out.token + uint64_t(h) * a.out.head + 16 * dt + 4 * g, o[nt][dt][0] * inv,
                   o[nt][dt][1] * inv, o[nt][dt][2] * inv, o[nt][dt][3] * inv);
-      if (a.lse && g == 0) a.lse[t * a.heads + h] = sum[nt] == 0.0f ? -INFINITY : m[nt] * kLn2 + __logf(sum[nt]);
+      if (a.lse && g == 0) a.lse[t * a.heads + h] = total == 0.0f ? -INFINITY : m[nt] * kLn2 + __logf(total);
     }
     return;
   }
@@ -710,7 +711,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_wide(PagedArgs a, PagedPlan p,
     for (int nt = 0; nt < NT; ++nt) {
       const float top = fmaxf(fmaxf(fmaxf(s_m[0][nt][n], s_m[1][nt][n]), fmaxf(s_m[2][nt][n], s_m[3][nt][n])), m[nt]);
       if (__any(top > m[nt] + kRise)) {  // the same in every wavefront
-        const float fade = __builtin_amdgcn_exp2f(m[nt] - (top == -INFINITY ? 0.0f : top));  // (x is rounded as top is)
+        const float fade = __builtin_amdgcn_exp2f(m[nt] - (top == -INFINITY ? 0.0f : top));
         m[nt] = top;
         sum[nt] *= fade;
 #pragma unroll
@@ -1027,7 +1028,7 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
         for (int i = 1; i < 4 * T; ++i) top = fmaxf(top, x[i]);
         top = fmaxf(m[nt], max_lane16(top) * scale);
         if (__any(top > m[nt] + kRise)) {
-          const float fade = fade_of(m[nt], top);
+          const float fade = __builtin_amdgcn_exp2f(m[nt] - (top == -INFINITY ? 0.0f : top));
           m[nt] = top;
           sum[nt] *= fade;
 #pragma unroll
@@ -1068,6 +1069,11 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
     }
   }
 
+  // the lane's place again from the thread's number: kept over the loop it was
+  // spilled (32 of 8 new and 300 tokens 9.8 us, 9.6 so)
+  uint32_t lane = tid & 63u;
+  asm volatile("" : "+v"(lane));
+  const uint32_t group4 = lane >> 4;
   if (bad || odd) atomicOr(&s_flags, (bad ? 1u : 0u) | (odd ? 2u : 0u));
   __syncthreads();
   const uint32_t flags = s_flags;
@@ -1077,9 +1083,9 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float *y = x + nt * 64 * (4 * DT + 2);
-        y[l] = m[nt], y[64 + l] = sum[nt];
+        y[lane] = m[nt], y[64 + lane] = sum[nt];
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) reinterpret_cast<f32x4 *>(y + 128)[64 * dt + l] = o[nt][dt];
+        for (int dt = 0; dt < DT; ++dt) reinterpret_cast<f32x4 *>(y + 128)[64 * dt + lane] = o[nt][dt];
       }
     }
     __syncthreads();
@@ -1087,11 +1093,11 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float *y = x + nt * 64 * (4 * DT + 2);
-        const float other = y[l], top = fmaxf(m[nt], other), at = top == -INFINITY ? 0.0f : top;
+        const float other = y[lane], top = fmaxf(m[nt], other), at = top == -INFINITY ? 0.0f : top;
         const float f0 = __builtin_amdgcn_exp2f(m[nt] - at), f1 = __builtin_amdgcn_exp2f(other - at);
-        m[nt] = top, sum[nt] = sum[nt] * f0 + y[64 + l] * f1;
+        m[nt] = top, sum[nt] = sum[nt] * f0 + y[64 + lane] * f1;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[nt][dt] = o[nt][dt] * f0 + reinterpret_cast<const f32x4 *>(y + 128)[64 * dt + l] * f1;
+        for (int dt = 0; dt < DT; ++dt) o[nt][dt] = o[nt][dt] * f0 + reinterpret_cast<const f32x4 *>(y + 128)[64 * dt + lane] * f1;
       }
     }
   }
@@ -1106,7 +1112,7 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
         for (int dt = 0; dt < DT; ++dt) {
           f32x4 odds;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) odds[i] = odd_value(vp[(16 * dt + 4 * g + i) * P], from);
+          for (int i = 0; i < 4; ++i) odds[i] = odd_value(vp[(16 * dt + 4 * group4 + i) * P], from);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const bool in = see[nt](j);
@@ -1125,23 +1131,23 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const float total = flags & 1u ? __uint_as_float(0x7fc00000u) : sum_lane16(sum[nt]);
-    const uint32_t r = mine + 16 * nt + n;
+    const uint32_t r = mine + 16 * nt + lane % 16;
     if (r >= sp.rows || u0) continue;
     if (sp.chunks > 1) {
       const uint32_t row = (r - row0) * kRecord<D>;
-      if (g == 0) store(row + D, f32x4{m[nt], total, 0.0f, 0.0f});
+      if (group4 == 0) store(row + D, f32x4{m[nt], total, 0.0f, 0.0f});
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) store(row + 16 * dt + 4 * g, o[nt][dt]);
+      for (int dt = 0; dt < DT; ++dt) store(row + 16 * dt + 4 * group4, o[nt][dt]);
       continue;
     }
     const uint64_t t = uint64_t(sp.first + r / group);
     const uint32_t h = head * group + r % group;
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const float row_sum = checked_sum(total, m[nt]), inv = row_sum == 0.0f ? 0.0f : 1.0f / row_sum;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
-      store_out(a.out, t * a.out.token + uint64_t(h) * a.out.head + 16 * dt + 4 * g, o[nt][dt][0] * inv,
+      store_out(a.out, t * a.out.token + uint64_t(h) * a.out.head + 16 * dt + 4 * group4, o[nt][dt][0] * inv,
                 o[nt][dt][1] * inv, o[nt][dt][2] * inv, o[nt][dt][3] * inv);
-    if (a.lse && g == 0) a.lse[t * a.heads + h] = total == 0.0f ? -INFINITY : m[nt] * kLn2 + __logf(total);
+    if (a.lse && group4 == 0) a.lse[t * a.heads + h] = row_sum == 0.0f ? -INFINITY : m[nt] * kLn2 + __logf(row_sum);
   }
 }
 
@@ -1191,6 +1197,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, PagedPlan p, co
   }
   const uint64_t t = uint64_t(sp.first + r / group);
   const uint32_t h = head * group + r % group;
+  if constexpr (D < 512) total = checked_sum(total, top);  // (wide heads: as in k_paged_wide)
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
   for (uint32_t i = 0; i < kSpan; ++i) {

@@ -269,7 +269,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(Prom
     const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
     top = fmaxf(m, fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])) * scale);
     if (__any(top > m + kRise)) {
-      const float fade = fade_of(m, top);
+      const float fade = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
       m = top;
       sum *= fade;
 #pragma unroll
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prompt_attention(Prom
 
   {
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
-    sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    sum = checked_sum(__uint_as_float(x[0]) + __uint_as_float(x[1]), m);
   }
   const bool mine = wrow + n < rows;
   const uint64_t t = uint64_t(blk.first + pos);
