@@ -229,6 +229,10 @@ class KvCache(C.Structure):
     ]
 
 
+class Kv4Cache(C.Structure):
+    _fields_ = KvCache._fields_
+
+
 class RouteDecisionC(C.Structure):
     _fields_ = [
         ("layer", C.c_uint8),
@@ -302,6 +306,21 @@ SIGNATURES = {
         I,
         [P, P, C.POINTER(Rows), C.POINTER(KvCache), U32, U32, U32, U32, Buffer, U32, Buffer, Buffer, C.POINTER(Rows),
          Buffer, F, U32],
+    ),
+    "s14_kv4_append": (
+        I,
+        [P, P, C.POINTER(Kv4Cache), U32, U32, U32, C.POINTER(Rows), C.POINTER(Rows), Buffer, U32, Buffer, Buffer, Buffer,
+         F, C.POINTER(Rope)],
+    ),
+    "s14_paged4_attention": (
+        I,
+        [P, P, C.POINTER(Rows), C.POINTER(Kv4Cache), U32, U32, U32, U32, Buffer, U32, Buffer, Buffer, C.POINTER(Rows),
+         Buffer, F, U32],
+    ),
+    "s14_add_rms_norm": (
+        I,
+        [P, P, U32, U32, C.POINTER(Rows), C.POINTER(Rows), C.POINTER(Rows), C.POINTER(Rows), Buffer, F, U32, Buffer,
+         Buffer],
     ),
     "s14_prompt_attention": (
         I,

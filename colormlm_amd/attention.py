@@ -4,12 +4,14 @@ the C ABI's attention entry points (include/s14_hip.h).
 A decode or verify step of a layer, around ``s14.fp8_linear`` and
 ``s14.moe_block_route``::
 
+    add_rms_norm(ctx, o, wn, residual=h, residual_out=h, q=x8, scales=xs)   # rows for fp8_linear
     qk_norm_rope(ctx, q, None, q16, None, q_weight=wq, rope=rope, positions=pos)
     kv_append(ctx, cache, k, v, table, cu, past, k_weight=wk, rope=rope, max_new=n)
     paged_attention(ctx, q16, cache, table, cu, lens, out, max_new=n, max_len=longest)
 
 and a whole prompt: ``qk_norm_rope`` of q and k, ``prompt_attention``, and
-``kv_append`` of the rotated keys for the steps that follow.
+``kv_append`` of the rotated keys for the steps that follow.  The cache is a
+``KvCache`` (8 bits) or a ``KvCache4`` (4 bits).
 
 Operands are torch tensors on the context's device, packed [tokens, heads,
 dim] with any strides that are multiples of 8 elements and a contiguous last
@@ -23,7 +25,7 @@ from __future__ import annotations
 import ctypes as C
 import importlib.util
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
@@ -54,7 +56,8 @@ def _load():
     spec = importlib.util.spec_from_file_location("_s14attn", path)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
-    names = ("s14_qk_norm_rope", "s14_kv_append", "s14_paged_attention", "s14_prompt_attention")
+    names = ("s14_qk_norm_rope", "s14_kv_append", "s14_paged_attention", "s14_prompt_attention", "s14_kv4_append",
+             "s14_paged4_attention", "s14_add_rms_norm")
     module.bind(tuple(C.cast(getattr(lib(), n), C.c_void_p).value for n in names), _refuse, check, _raw_stream())
     return module
 
@@ -108,28 +111,25 @@ class RopeScaling:
     amplitude: float = 1.0
 
 
-class KvCache:
-    """The paged 8-bit cache: uint8 E4M3 codes k [pages, heads, page_tokens,
-    dim] and v [pages, heads, dim, page_tokens], uint8 E8M0 scales [pages,
-    heads] of each."""
+class _PagedCache:
+    """What the caches of both formats keep: their tensors, and the address of
+    the C struct of them."""
 
-    def __init__(self, k_pages, k_scales, v_pages, v_scales):
-        for t, label in ((k_pages, "k codes"), (k_scales, "k scales"), (v_pages, "v codes"), (v_scales, "v scales")):
+    def __init__(self, struct, k_pages, k_scales, v_pages, v_scales, page_tokens, dim, shapes):
+        tensors = (k_pages, k_scales, v_pages, v_scales)
+        for t, label in zip(tensors, ("k codes", "k scales", "v codes", "v scales")):
             if t.dtype != torch.uint8 or not t.is_contiguous():
                 _refuse(N.S14_ERR_INVALID, f"{label} must be contiguous uint8")
             if t.device != k_pages.device:
                 _refuse(N.S14_ERR_INVALID, "the cache's tensors are on different devices")
-        if k_pages.dim() != 4:
-            _refuse(N.S14_ERR_SHAPE, "k codes must be [pages, heads, page_tokens, dim]")
-        pages, heads, page, dim = k_pages.shape
-        if tuple(v_pages.shape) != (pages, heads, dim, page):
-            _refuse(N.S14_ERR_SHAPE, f"v codes must be [{pages}, {heads}, {dim}, {page}]")
-        if tuple(k_scales.shape) != (pages, heads) or tuple(v_scales.shape) != (pages, heads):
-            _refuse(N.S14_ERR_SHAPE, f"scales must be [{pages}, {heads}]")
-        self._tensors = (k_pages, k_scales, v_pages, v_scales)
-        self.pages, self.heads, self.page_tokens, self.dim = pages, heads, page, dim
+        pages, heads = k_pages.shape[:2]
+        for t, label, shape in zip((v_pages, k_scales, v_scales), ("v codes", "k scales", "v scales"), shapes):
+            if tuple(t.shape) != (pages, heads, *shape):
+                _refuse(N.S14_ERR_SHAPE, f"{label} must be {[pages, heads, *shape]}")
+        self._tensors = tensors
+        self.pages, self.heads, self.page_tokens, self.dim = pages, heads, page_tokens, dim
         buf = [N.Buffer(t.data_ptr(), t.nbytes) for t in (k_pages, v_pages, k_scales, v_scales)]
-        self._c = N.KvCache(*buf, pages, heads, page, dim)
+        self._c = struct(*buf, pages, heads, page_tokens, dim)
         self._at, self._device = C.addressof(self._c), k_pages.get_device()
 
     # their addresses are held: not to be replaced, and a call refuses other memory behind them
@@ -137,6 +137,20 @@ class KvCache:
     k_scales = property(lambda self: self._tensors[1])
     v_pages = property(lambda self: self._tensors[2])
     v_scales = property(lambda self: self._tensors[3])
+
+
+class KvCache(_PagedCache):
+    """The paged 8-bit cache: uint8 E4M3 codes k [pages, heads, page_tokens,
+    dim] and v [pages, heads, dim, page_tokens], uint8 E8M0 scales [pages,
+    heads] of each."""
+
+    _append, _attend = staticmethod(_call.kv_append), staticmethod(_call.paged_attention)
+
+    def __init__(self, k_pages, k_scales, v_pages, v_scales):
+        if k_pages.dim() != 4:
+            _refuse(N.S14_ERR_SHAPE, "k codes must be [pages, heads, page_tokens, dim]")
+        page, dim = k_pages.shape[2:]
+        super().__init__(N.KvCache, k_pages, k_scales, v_pages, v_scales, page, dim, ((dim, page), (), ()))
 
     @classmethod
     def empty(cls, pages: int, heads: int, page_tokens: int, dim: int, device="cuda") -> "KvCache":
@@ -146,7 +160,38 @@ class KvCache:
                    new(pages, heads))
 
 
-def _cache(ctx: Context, cache: KvCache):
+class KvCache4(_PagedCache):
+    """The paged 4-bit cache: uint8 of two E2M1 codes k [pages, heads,
+    page_tokens, dim / 2] and v [pages, heads, dim / 32, page_tokens / 16, 16,
+    16], uint8 E8M0 scales of 32 dimensions of a key, [pages, heads, dim / 32,
+    page_tokens], and of 128 (64 at heads of 64) of a value, [pages, heads,
+    max(1, dim / 128), page_tokens].  Where in them a dimension and slot lies:
+    s14_kv4_cache in the C header."""
+
+    _append, _attend = staticmethod(_call.kv4_append), staticmethod(_call.paged4_attention)
+
+    def __init__(self, k_pages, k_scales, v_pages, v_scales):
+        if k_pages.dim() != 4:
+            _refuse(N.S14_ERR_SHAPE, "k codes must be [pages, heads, page_tokens, dim / 2]")
+        page, dim = k_pages.shape[2], 2 * k_pages.shape[3]
+        super().__init__(N.Kv4Cache, k_pages, k_scales, v_pages, v_scales, page, dim, self._shapes(page, dim))
+
+    @staticmethod
+    def _shapes(page: int, dim: int):
+        return (dim // 32, page // 16, 16, 16), (dim // 32, page), (max(1, dim // 128), page)
+
+    @classmethod
+    def empty(cls, pages: int, heads: int, page_tokens: int, dim: int, device="cuda") -> "KvCache4":
+        """An uninitialised cache: every slot is written before it is read."""
+        new = lambda *shape: torch.empty((pages, heads, *shape), dtype=torch.uint8, device=device)  # noqa: E731
+        v, ks, vs = cls._shapes(page_tokens, dim)
+        return cls(new(page_tokens, dim // 2), new(*ks), new(*v), new(*vs))
+
+
+Cache = Union[KvCache, KvCache4]
+
+
+def _cache(ctx: Context, cache):
     if cache._device != ctx.device:
         _here(ctx.device, cache.k_pages, "cache")
     return cache._at
@@ -177,18 +222,31 @@ def qk_norm_rope(ctx: Context, q, k, q_out, k_out, q_weight=None, k_weight=None,
                        positions, None if rope is None else rope._tensors)
 
 
-def kv_append(ctx: Context, cache: KvCache, k, v, page_table, cu, past, k_weight=None, eps: float = 1e-6,
+def add_rms_norm(ctx: Context, x, weight, residual=None, residual_out=None, y=None, q=None, scales=None, eps: float = 1e-6,
+                 stream=None) -> None:
+    """h = x + residual and its RMS norm h * rsqrt(mean(h^2) + eps) * weight of
+    each row of x [rows, k], in f32 and one launch.  Outputs, as far as given:
+    residual_out = h and y = the norm (f32 or bf16, x's shape), and its E4M3
+    codes q (uint8, x's shape) with their E8M0 scales (uint8 [rows, k / group],
+    group 32, 64 or 128; ``s14.fp8_linear`` takes 128), those of
+    ``s14.act_quant_e4m3`` of the f32 norm; y or the codes are asked for.  x and
+    residual: f32 or bf16; weight: f32 [k].  residual_out and y may be x or
+    residual themselves; outputs that share other memory are refused."""
+    _call.add_rms_norm(ctx._h.value, ctx.device, stream, x, weight, residual, residual_out, y, q, scales, eps)
+
+
+def kv_append(ctx: Context, cache: Cache, k, v, page_table, cu, past, k_weight=None, eps: float = 1e-6,
               rope: Optional[Rope] = None, max_new: Optional[int] = None, stream=None) -> None:
     """Rows cu[i] .. cu[i + 1] - 1 of k and v [tokens, heads, dim] (f32 or
     bf16) become positions past[i] .. of sequence i in the cache, K with the
     norm and rotation of ``qk_norm_rope`` on the way.  max_new: at least the
     most new tokens of a sequence, and at most the call's (which it is if left
     out); rows past it are not stored."""
-    _call.kv_append(ctx._h.value, ctx.device, stream, _cache(ctx, cache), cache.dim, k, v, page_table, cu, past, k_weight,
-                    eps, _rope(ctx, rope), max_new, cache._tensors, None if rope is None else rope._tensors)
+    cache._append(ctx._h.value, ctx.device, stream, _cache(ctx, cache), cache.dim, k, v, page_table, cu, past, k_weight, eps,
+                  _rope(ctx, rope), max_new, cache._tensors, None if rope is None else rope._tensors)
 
 
-def paged_attention(ctx: Context, q, cache: KvCache, page_table, cu, lens, out, lse=None, scale: Optional[float] = None,
+def paged_attention(ctx: Context, q, cache: Cache, page_table, cu, lens, out, lse=None, scale: Optional[float] = None,
                     window: int = 0, max_new: Optional[int] = None, max_len: Optional[int] = None, stream=None) -> None:
     """Attention of q's rows (bf16 [tokens, heads, dim]; cu[i] .. cu[i + 1] - 1
     are the last tokens of sequence i) over the sequences' lens[i] cached
@@ -198,8 +256,8 @@ def paged_attention(ctx: Context, q, cache: KvCache, page_table, cu, lens, out, 
     tokens, which it is if left out (the work is split for one sequence that has
     them all: give it for a batch); max_len: about the longest sequence (it
     sets how the work is split; the page table's reach if left out)."""
-    _call.paged_attention(ctx._h.value, ctx.device, stream, q, _cache(ctx, cache), cache.dim, page_table, cu, lens, out,
-                          lse, scale, window, max_new, max_len, cache.page_tokens, cache._tensors)
+    cache._attend(ctx._h.value, ctx.device, stream, q, _cache(ctx, cache), cache.dim, page_table, cu, lens, out, lse, scale,
+                  window, max_new, max_len, cache.page_tokens, cache._tensors)
 
 
 def prompt_attention(ctx: Context, q, k, v, cu, out, lse=None, scale: Optional[float] = None, window: int = 0,
@@ -212,8 +270,10 @@ def prompt_attention(ctx: Context, q, k, v, cu, out, lse=None, scale: Optional[f
 
 __all__ = [
     "KvCache",
+    "KvCache4",
     "Rope",
     "RopeScaling",
+    "add_rms_norm",
     "kv_append",
     "paged_attention",
     "prompt_attention",

@@ -37,7 +37,8 @@ OUT = PKG / "lib" / "libs14hip.so"
 PY_OUT = PKG / "lib" / "_s14attn.so"
 OBJ = PKG / "lib" / "obj"
 DEVICE_SOURCES = ["s14_device.hip", "s14_block.hip", "s14_prefill.hip", "s14_static.hip", "s14_linear.hip",
-                  "s14_attn_rows.hip", "s14_attn_paged.hip", "s14_attn_prompt.hip"]
+                  "s14_norm.hip", "s14_attn_rows.hip", "s14_attn_paged.hip", "s14_attn_append4.hip", "s14_attn_paged4.hip",
+                  "s14_attn_prompt.hip"]
 HOST_SOURCES = ["s14_api.cpp", "s14_attn_api.cpp", "s14_pool.cpp", "s14_loader.cpp"]
 SOURCES = DEVICE_SOURCES + HOST_SOURCES
 ARCH = os.environ.get("S14_OFFLOAD_ARCH", "gfx950")

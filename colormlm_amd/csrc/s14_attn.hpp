@@ -1,6 +1,7 @@
 // The attention operators between the FP8 projections and the expert layer:
-// per-head norms with the position rotation, the paged 8-bit key/value cache,
-// attention over it, and causal attention over packed prompts.  Shared
+// the residual norm before either, per-head norms with the position rotation,
+// the paged key/value caches of 8 and of 4 bits, attention over them, and causal
+// attention over packed prompts.  Shared
 // between the kernel files (s14_attn_*.hip) and s14_attn_api.cpp.
 #pragma once
 
@@ -46,9 +47,9 @@ struct NormRopeArgs {
   uint32_t *status;
 };
 
-struct CacheArgs {
-  uint8_t *k, *v;    // K codes [page][head][slot][dim], V codes [page][head][dim][slot]
-  uint8_t *ks, *vs;  // E8M0 [page][head]
+struct CacheArgs {     // of 8 bits, and of 4 (s14_hip.h has the layouts)
+  uint8_t *k, *v;      // K codes [page][head][slot][dim], V codes [page][head][dim][slot]
+  uint8_t *ks, *vs;    // E8M0 [page][head]
   uint32_t pages, heads, page, dim;  // page: tokens a page, a power of two
 };
 
@@ -89,16 +90,30 @@ struct PromptArgs {
   uint32_t window;
 };
 
+// Rows of k values; x.heads is 1 throughout.  A NULL p: absent.
+struct AddNormArgs {
+  uint32_t rows, k;
+  AttnRows x, residual;
+  AttnOut residual_out, y;
+  const float *weight;
+  float eps;
+  uint32_t group;  // of the codes' scales, 0: no codes
+  uint8_t *q, *scales;
+};
+
 struct RopeTableArgs {
   uint32_t positions, rot;
   double theta, factor, original, fast, slow, amplitude;
   float *out;
 };
 
+hipError_t launch_add_norm(hipStream_t s, const AddNormArgs &a);
 hipError_t launch_rope_table(hipStream_t s, const RopeTableArgs &a);
 hipError_t launch_norm_rope(hipStream_t s, const NormRopeArgs &a);
 hipError_t launch_kv_append(hipStream_t s, const AppendArgs &a);
+hipError_t launch_kv4_append(hipStream_t s, const AppendArgs &a);
 hipError_t launch_paged_attention(hipStream_t s, const PagedArgs &a, const PagedPlan &p, float *part);
+hipError_t launch_paged4_attention(hipStream_t s, const PagedArgs &a, const PagedPlan &p, float *part);
 hipError_t launch_prompt_attention(hipStream_t s, const PromptArgs &a);
 
 }  // namespace s14

@@ -51,6 +51,7 @@ bool head_dim(uint32_t dim) { return dim == 64 || dim == 128 || dim == 256 || di
 
 constexpr uint64_t kMaxStride = 1ull << 24;  // elements; a key tile's rows stay inside 32-bit offsets
 constexpr uint32_t kMaxTokens = 1u << 30, kMaxGrid = 65535;
+constexpr uint32_t kMaxNorm = 65536;  // values of a norm's row: 64 a thread of a workgroup
 constexpr uint64_t kMaxBlocks = 1u << 24;  // of 256 threads: a launch has below 2^32 in one dimension
 
 // A packed [tokens][heads][dim] operand: dtype, strides, and that its last
@@ -118,21 +119,40 @@ int check_weight(const s14_buffer &w, uint32_t dim, float eps, const char *label
   return require(w, 4ull * dim, 16, label);
 }
 
-int check_cache(const s14_kv_cache *c, s14::CacheArgs *out) {
+// Shape of either cache.
+template <class Cache>
+int check_pages(const Cache *c) {
   if (!c) return fail(S14_ERR_INVALID, "NULL cache");
   if (!head_dim(c->dim)) return fail(S14_ERR_SHAPE, "cache head size %u is not 64, 128, 256 or 512", c->dim);
   if (c->page_tokens != 16 && c->page_tokens != 32 && c->page_tokens != 64 && c->page_tokens != 128)
     return fail(S14_ERR_SHAPE, "cache pages of %u tokens: 16, 32, 64 or 128 are required", c->page_tokens);
   if (!c->pages || !c->heads || c->heads > kMaxGrid / 2 || c->pages > uint32_t(INT32_MAX))
     return fail(S14_ERR_SHAPE, "cache of %u pages and %u heads", c->pages, c->heads);
-  const uint64_t scales = uint64_t(c->pages) * c->heads, codes = scales * c->page_tokens * c->dim;
-  if (int rc = require(c->k, codes, 16, "k codes")) return rc;
-  if (int rc = require(c->v, codes, 16, "v codes")) return rc;
-  if (int rc = require(c->k_scale, scales, 1, "k scales")) return rc;
-  if (int rc = require(c->v_scale, scales, 1, "v scales")) return rc;
+  return S14_OK;
+}
+
+// Its buffers: bytes of codes and of scales of a (page, head), and the scales' alignment.
+template <class Cache>
+int check_codes(const Cache *c, uint64_t codes, uint64_t k_scales, uint64_t v_scales, uint32_t align, s14::CacheArgs *out) {
+  const uint64_t places = uint64_t(c->pages) * c->heads;
+  if (int rc = require(c->k, places * codes, 16, "k codes")) return rc;
+  if (int rc = require(c->v, places * codes, 16, "v codes")) return rc;
+  if (int rc = require(c->k_scale, places * k_scales, align, "k scales")) return rc;
+  if (int rc = require(c->v_scale, places * v_scales, align, "v scales")) return rc;
   *out = {static_cast<uint8_t *>(c->k.ptr), static_cast<uint8_t *>(c->v.ptr), static_cast<uint8_t *>(c->k_scale.ptr),
           static_cast<uint8_t *>(c->v_scale.ptr), c->pages, c->heads, c->page_tokens, c->dim};
   return S14_OK;
+}
+
+int check_cache(const s14_kv_cache *c, s14::CacheArgs *out) {
+  if (int rc = check_pages(c)) return rc;
+  return check_codes(c, uint64_t(c->page_tokens) * c->dim, 1, 1, 1, out);
+}
+
+int check_cache(const s14_kv4_cache *c, s14::CacheArgs *out) {
+  if (int rc = check_pages(c)) return rc;
+  const uint64_t slots = c->page_tokens;
+  return check_codes(c, slots * (c->dim / 2), slots * (c->dim / 32), slots * (c->dim < 128 ? 1 : c->dim / 128), 16, out);
 }
 
 int check_counts(uint32_t tokens, uint32_t seqs, uint32_t most) {
@@ -239,10 +259,82 @@ extern "C" int s14_qk_norm_rope(s14_ctx *ctx, void *stream, uint32_t tokens, uin
   return e == hipSuccess ? S14_OK : hip_fail(e, "qk_norm_rope launch");
 }
 
-extern "C" int s14_kv_append(s14_ctx *ctx, void *stream, const s14_kv_cache *cache, uint32_t tokens, uint32_t seqs,
-                             uint32_t max_new, const s14_rows *k, const s14_rows *v, s14_buffer page_table,
-                             uint32_t table_width, s14_buffer cu, s14_buffer past, s14_buffer k_weight, float eps,
-                             const s14_rope *rope) {
+// A row operand of add_rms_norm: one head of k values.
+static int check_flat(const s14_rows *r, uint32_t rows, uint32_t k, const char *label) {
+  if (int rc = check_rows(r, rows, k, false, label)) return rc;
+  return r->heads == 1 ? S14_OK : fail(S14_ERR_SHAPE, "%s has %u heads, one is required", label, r->heads);
+}
+
+extern "C" int s14_add_rms_norm(s14_ctx *ctx, void *stream, uint32_t rows, uint32_t k, const s14_rows *x,
+                                const s14_rows *residual, const s14_rows *residual_out, const s14_rows *y,
+                                s14_buffer weight, float eps, uint32_t group, s14_buffer q, s14_buffer scales) {
+  if (int rc = check_ctx(ctx)) return rc;
+  if (rows > kMaxTokens) return fail(S14_ERR_SHAPE, "%u rows, at most %u", rows, kMaxTokens);
+  if (!k || k % 8 || k > kMaxNorm) return fail(S14_ERR_SHAPE, "rows of %u values: multiples of 8, at most %u, are required", k, kMaxNorm);
+  if (group && group != 32 && group != 64 && group != 128) return fail(S14_ERR_SHAPE, "scale group %u is not 32, 64 or 128", group);
+  if (group && k % group) return fail(S14_ERR_SHAPE, "rows of %u values are not whole groups of %u", k, group);
+  if (!y && !group) return fail(S14_ERR_INVALID, "neither y nor codes are asked for");
+  if (int rc = check_flat(x, rows, k, "x")) return rc;
+  const s14_rows *outs[2] = {residual_out, y};
+  const char *const labels[2] = {"residual output", "y"};
+  if (residual)
+    if (int rc = check_flat(residual, rows, k, "residual")) return rc;
+  for (int i = 0; i < 2; ++i)
+    if (outs[i])
+      if (int rc = check_flat(outs[i], rows, k, labels[i])) return rc;
+  if (!weight.ptr) return fail(S14_ERR_INVALID, "norm weight buffer is NULL");
+  if (int rc = check_weight(weight, k, eps, "norm weight")) return rc;
+  if (!rows) return S14_OK;
+  const uint64_t values = uint64_t(rows) * k, n_scales = group ? values / group : 0;
+  if (group) {
+    if (int rc = require(q, values, 8, "codes")) return rc;
+    if (int rc = require(scales, n_scales, 1, "scales")) return rc;
+  }
+  // rows may be written in their input's place; nothing else is shared
+  const auto codes = [&](const s14_buffer &b, uint64_t bytes) {
+    return s14::RowBytes{reinterpret_cast<uintptr_t>(b.ptr), 0, 0, bytes, 1};
+  };
+  for (int i = 0; i < 2; ++i) {
+    if (!outs[i]) continue;
+    if (int rc = check_apart(outs[i], x, rows, k, true, labels[i])) return rc;
+    if (residual)
+      if (int rc = check_apart(outs[i], residual, rows, k, true, labels[i])) return rc;
+    if (s14::rows_share(bytes_of(outs[i], k), {reinterpret_cast<uintptr_t>(weight.ptr), 4ull * k, 0, 4ull * k, 1}, 1, false))
+      return fail(S14_ERR_INVALID, "%s shares memory with the norm weight", labels[i]);
+  }
+  if (residual_out && y && s14::rows_share(bytes_of(residual_out, k), bytes_of(y, k), rows, false))
+    return fail(S14_ERR_INVALID, "the residual output and y share memory");
+  if (group) {
+    const s14::RowBytes made[2] = {codes(q, values), codes(scales, n_scales)};
+    const auto apart = [&](const s14::RowBytes &m, uintptr_t at, uint64_t bytes) { return m.at + m.row <= at || at + bytes <= m.at; };
+    bool fine = apart(made[0], made[1].at, made[1].row);
+    for (const s14::RowBytes &m : made) {
+      fine = fine && apart(m, reinterpret_cast<uintptr_t>(weight.ptr), 4ull * k);
+      for (const s14_rows *r : {x, residual, residual_out, y})
+        if (r) fine = fine && apart(m, reinterpret_cast<uintptr_t>(r->buf.ptr), bytes_of(r, k).bytes(rows));
+    }
+    if (!fine) return fail(S14_ERR_INVALID, "codes or scales share memory with another operand");
+  }
+  s14::AddNormArgs a{};
+  a.rows = rows, a.k = k;
+  a.x = rows_of(x);
+  if (residual) a.residual = rows_of(residual);
+  if (residual_out) a.residual_out = out_of(residual_out);
+  if (y) a.y = out_of(y);
+  a.weight = static_cast<const float *>(weight.ptr), a.eps = eps, a.group = group;
+  a.q = static_cast<uint8_t *>(q.ptr), a.scales = static_cast<uint8_t *>(scales.ptr);
+  const OnDevice on(s14::ctx_device(ctx));
+  if (on.error() != hipSuccess) return hip_fail(on.error(), "hipSetDevice");
+  const hipError_t e = s14::launch_add_norm(reinterpret_cast<hipStream_t>(stream), a);
+  return e == hipSuccess ? S14_OK : hip_fail(e, "add_rms_norm launch");
+}
+
+// Both caches' appends and attentions: the same checks, and a kernel file each.
+template <class Cache>
+static int append_to(hipError_t (*launch)(hipStream_t, const s14::AppendArgs &), s14_ctx *ctx, void *stream,
+                     const Cache *cache, uint32_t tokens, uint32_t seqs, uint32_t max_new, const s14_rows *k,
+                     const s14_rows *v, s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer past,
+                     s14_buffer k_weight, float eps, const s14_rope *rope) {
   if (int rc = check_ctx(ctx)) return rc;
   s14::AppendArgs a{};
   if (int rc = check_cache(cache, &a.cache)) return rc;
@@ -263,14 +355,31 @@ extern "C" int s14_kv_append(s14_ctx *ctx, void *stream, const s14_kv_cache *cac
   a.status = s14::ctx_status(ctx);
   const OnDevice on(s14::ctx_device(ctx));
   if (on.error() != hipSuccess) return hip_fail(on.error(), "hipSetDevice");
-  const hipError_t e = s14::launch_kv_append(reinterpret_cast<hipStream_t>(stream), a);
-  return e == hipSuccess ? S14_OK : hip_fail(e, "kv_append launch");
+  const hipError_t e = launch(reinterpret_cast<hipStream_t>(stream), a);
+  return e == hipSuccess ? S14_OK : hip_fail(e, "append launch");
 }
 
-extern "C" int s14_paged_attention(s14_ctx *ctx, void *stream, const s14_rows *q, const s14_kv_cache *cache,
-                                   uint32_t tokens, uint32_t seqs, uint32_t max_new, uint32_t max_len,
-                                   s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer lens,
-                                   const s14_rows *out, s14_buffer lse, float scale, uint32_t window) {
+extern "C" int s14_kv_append(s14_ctx *ctx, void *stream, const s14_kv_cache *cache, uint32_t tokens, uint32_t seqs,
+                             uint32_t max_new, const s14_rows *k, const s14_rows *v, s14_buffer page_table,
+                             uint32_t table_width, s14_buffer cu, s14_buffer past, s14_buffer k_weight, float eps,
+                             const s14_rope *rope) {
+  return append_to(s14::launch_kv_append, ctx, stream, cache, tokens, seqs, max_new, k, v, page_table, table_width, cu,
+                   past, k_weight, eps, rope);
+}
+
+extern "C" int s14_kv4_append(s14_ctx *ctx, void *stream, const s14_kv4_cache *cache, uint32_t tokens, uint32_t seqs,
+                              uint32_t max_new, const s14_rows *k, const s14_rows *v, s14_buffer page_table,
+                              uint32_t table_width, s14_buffer cu, s14_buffer past, s14_buffer k_weight, float eps,
+                              const s14_rope *rope) {
+  return append_to(s14::launch_kv4_append, ctx, stream, cache, tokens, seqs, max_new, k, v, page_table, table_width, cu,
+                   past, k_weight, eps, rope);
+}
+
+template <class Cache>
+static int attend_over(hipError_t (*launch)(hipStream_t, const s14::PagedArgs &, const s14::PagedPlan &, float *),
+                       s14_ctx *ctx, void *stream, const s14_rows *q, const Cache *cache, uint32_t tokens, uint32_t seqs,
+                       uint32_t max_new, uint32_t max_len, s14_buffer page_table, uint32_t table_width, s14_buffer cu,
+                       s14_buffer lens, const s14_rows *out, s14_buffer lse, float scale, uint32_t window) {
   if (int rc = check_ctx(ctx)) return rc;
   s14::PagedArgs a{};
   if (int rc = check_cache(cache, &a.cache)) return rc;
@@ -304,8 +413,24 @@ extern "C" int s14_paged_attention(s14_ctx *ctx, void *stream, const s14_rows *q
   float *part = nullptr;
   if (p.chunks > 1)
     if (int rc = s14::ctx_attn_workspace(ctx, s14::kPagedPartFloats * sizeof(float), &part)) return rc;
-  const hipError_t e = s14::launch_paged_attention(reinterpret_cast<hipStream_t>(stream), a, p, part);
+  const hipError_t e = launch(reinterpret_cast<hipStream_t>(stream), a, p, part);
   return e == hipSuccess ? S14_OK : hip_fail(e, "paged_attention launch");
+}
+
+extern "C" int s14_paged_attention(s14_ctx *ctx, void *stream, const s14_rows *q, const s14_kv_cache *cache,
+                                   uint32_t tokens, uint32_t seqs, uint32_t max_new, uint32_t max_len,
+                                   s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer lens,
+                                   const s14_rows *out, s14_buffer lse, float scale, uint32_t window) {
+  return attend_over(s14::launch_paged_attention, ctx, stream, q, cache, tokens, seqs, max_new, max_len, page_table,
+                     table_width, cu, lens, out, lse, scale, window);
+}
+
+extern "C" int s14_paged4_attention(s14_ctx *ctx, void *stream, const s14_rows *q, const s14_kv4_cache *cache,
+                                    uint32_t tokens, uint32_t seqs, uint32_t max_new, uint32_t max_len,
+                                    s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer lens,
+                                    const s14_rows *out, s14_buffer lse, float scale, uint32_t window) {
+  return attend_over(s14::launch_paged4_attention, ctx, stream, q, cache, tokens, seqs, max_new, max_len, page_table,
+                     table_width, cu, lens, out, lse, scale, window);
 }
 
 extern "C" int s14_prompt_attention(s14_ctx *ctx, void *stream, uint32_t dim, const s14_rows *q, const s14_rows *k,

@@ -18,17 +18,23 @@
 
 typedef int (*norm_rope_fn)(s14_ctx *, void *, uint32_t, uint32_t, const s14_rows *, const s14_rows *, const s14_rows *,
                             const s14_rows *, s14_buffer, s14_buffer, float, const s14_rope *, s14_buffer);
-typedef int (*append_fn)(s14_ctx *, void *, const s14_kv_cache *, uint32_t, uint32_t, uint32_t, const s14_rows *,
-                         const s14_rows *, s14_buffer, uint32_t, s14_buffer, s14_buffer, s14_buffer, float,
-                         const s14_rope *);
-typedef int (*paged_fn)(s14_ctx *, void *, const s14_rows *, const s14_kv_cache *, uint32_t, uint32_t, uint32_t, uint32_t,
-                        s14_buffer, uint32_t, s14_buffer, s14_buffer, const s14_rows *, s14_buffer, float, uint32_t);
+typedef int (*add_norm_fn)(s14_ctx *, void *, uint32_t, uint32_t, const s14_rows *, const s14_rows *, const s14_rows *,
+                           const s14_rows *, s14_buffer, float, uint32_t, s14_buffer, s14_buffer);
+template <class Cache>
+using append_fn = int (*)(s14_ctx *, void *, const Cache *, uint32_t, uint32_t, uint32_t, const s14_rows *, const s14_rows *,
+                          s14_buffer, uint32_t, s14_buffer, s14_buffer, s14_buffer, float, const s14_rope *);
+template <class Cache>
+using paged_fn = int (*)(s14_ctx *, void *, const s14_rows *, const Cache *, uint32_t, uint32_t, uint32_t, uint32_t,
+                         s14_buffer, uint32_t, s14_buffer, s14_buffer, const s14_rows *, s14_buffer, float, uint32_t);
 typedef int (*prompt_fn)(s14_ctx *, void *, uint32_t, const s14_rows *, const s14_rows *, const s14_rows *, uint32_t,
                          uint32_t, s14_buffer, const s14_rows *, s14_buffer, float, uint32_t);
 
 static norm_rope_fn f_norm_rope;
-static append_fn f_append;
-static paged_fn f_paged;
+static add_norm_fn f_add_norm;
+template <class Cache>  // the cache of 8 bits, and of 4
+static append_fn<Cache> f_append;
+template <class Cache>
+static paged_fn<Cache> f_paged;
 static prompt_fn f_prompt;
 static PyObject *p_refuse, *p_check, *p_stream;      // attention.py's functions
 
@@ -142,8 +148,9 @@ static int held(PyObject *tensors, const s14_buffer *const *bufs, Py_ssize_t n, 
   }
   return 0;
 }
-static int cache_of(PyObject *at, PyObject *tensors, const s14_kv_cache **out) {
-  const s14_kv_cache *c = *out = (const s14_kv_cache *)pointer_of(at);
+template <class Cache>
+static int cache_of(PyObject *at, PyObject *tensors, const Cache **out) {
+  const Cache *c = *out = (const Cache *)pointer_of(at);
   if (!c) return refuse(S14_ERR_INVALID, "a cache is required");
   const s14_buffer *const bufs[4] = {&c->k, &c->k_scale, &c->v, &c->v_scale};
   return held(tensors, bufs, 4, "the cache");
@@ -202,12 +209,84 @@ static PyObject *qk_norm_rope(PyObject *, PyObject *const *v, Py_ssize_t argc) {
   return done(rc);
 }
 
+// The s14_rows of a [rows, k] tensor of the call's shape (shape[0] < 0: it sets that); None: absent.
+static int flat_rows(PyObject *t, const char *label, long device, s14_rows *r, long long shape[2], const s14_rows **out) {
+  *out = nullptr;
+  if (t == Py_None) return 0;
+  const at::Tensor *x = tensor_of(t, label, device);
+  if (!x) return -1;
+  const bool f32 = x->scalar_type() == at::kFloat;
+  if (!f32 && x->scalar_type() != at::kBFloat16) return refuse(S14_ERR_INVALID, "%s must be float32 or bfloat16", label);
+  const at::IntArrayRef size = x->sizes(), stride = x->strides();
+  if (size.size() != 2 || (stride[1] != 1 && size[1] > 1))
+    return refuse(S14_ERR_SHAPE, "%s must be [rows, k], its last dimension contiguous", label);
+  if (shape[0] < 0) shape[0] = size[0], shape[1] = size[1];
+  if (size[0] != shape[0] || size[1] != shape[1]) return refuse(S14_ERR_SHAPE, "%s must have x's shape", label);
+  if (size[0] > UINT32_MAX || size[1] > UINT32_MAX) return refuse(S14_ERR_SHAPE, "%s is too large", label);
+  const uint64_t row = size[0] < 2 ? 0 : uint64_t(stride[0]);  // a single row's may be anything
+  r->buf.ptr = x->data_ptr();
+  r->buf.bytes = size[0] ? ((size[0] - 1) * row + size[1]) * (f32 ? 4 : 2) : 0;
+  r->dtype = f32 ? S14_X_F32 : S14_X_BF16;
+  r->heads = 1, r->token_stride = row, r->head_stride = 0;
+  *out = r;
+  return 0;
+}
+
+// A contiguous uint8 [rows, columns] tensor (columns 0: it sets that).
+static int bytes_2d(PyObject *t, const char *label, long device, long long rows, long long *columns, s14_buffer *b) {
+  const at::Tensor *x = tensor_of(t, label, device);
+  if (!x) return -1;
+  if (x->scalar_type() != at::kByte || !x->is_contiguous()) return refuse(S14_ERR_INVALID, "%s must be a contiguous uint8 tensor", label);
+  const at::IntArrayRef size = x->sizes();
+  if (size.size() != 2 || size[0] != rows || (*columns && size[1] != *columns))
+    return refuse(S14_ERR_SHAPE, "%s must be [rows, %s]", label, *columns ? "k" : "k / group");
+  *columns = size[1];
+  b->ptr = x->data_ptr(), b->bytes = x->numel();
+  return 0;
+}
+
+// handle, device, stream, x, weight, residual, residual_out, y, q, scales, eps
+static PyObject *add_rms_norm(PyObject *, PyObject *const *v, Py_ssize_t argc) {
+  ARGUMENTS(11);
+  s14_ctx *ctx = (s14_ctx *)pointer_of(v[0]);
+  const long device = PyLong_AsLong(v[1]);
+  const double eps = PyFloat_AsDouble(v[10]);
+  void *stream;
+  s14_rows rows[4];
+  const s14_rows *r[4];
+  s14_buffer weight, q{}, scales{};
+  long long shape[2] = {-1, 0};
+  if (PyErr_Occurred()) return nullptr;
+  if (v[3] == Py_None) return refuse(S14_ERR_INVALID, "x is required"), nullptr;
+  if (flat_rows(v[3], "x", device, &rows[0], shape, &r[0]) || flat_rows(v[5], "residual", device, &rows[1], shape, &r[1]) ||
+      flat_rows(v[6], "residual output", device, &rows[2], shape, &r[2]) || flat_rows(v[7], "y", device, &rows[3], shape, &r[3]))
+    return nullptr;
+  if (flat_of(v[4], "norm weight", device, at::kFloat, shape[1], &weight)) return nullptr;
+  long long group = 0;
+  if ((v[8] == Py_None) != (v[9] == Py_None)) return refuse(S14_ERR_INVALID, "codes and scales go together"), nullptr;
+  if (v[8] != Py_None) {
+    long long k = shape[1], columns = 0;
+    if (!k) return refuse(S14_ERR_SHAPE, "rows of no values"), nullptr;
+    if (bytes_2d(v[8], "codes", device, shape[0], &k, &q) || bytes_2d(v[9], "scales", device, shape[0], &columns, &scales)) return nullptr;
+    if (!columns || k % columns || (group = k / columns) > 128)
+      return refuse(S14_ERR_SHAPE, "%lld scales of a row of %lld codes", columns, k), nullptr;
+  }
+  if (stream_of(v[2], device, &stream)) return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = f_add_norm(ctx, stream, (uint32_t)shape[0], (uint32_t)shape[1], r[0], r[1], r[2], r[3], weight, (float)eps,
+                  (uint32_t)group, q, scales);
+  Py_END_ALLOW_THREADS
+  return done(rc);
+}
+
 // handle, device, stream, cache, dim, k, v, page_table, cu, past, k_weight, eps, rope, max_new, the cache's and the rotation's tensors
+template <class Cache>
 static PyObject *kv_append(PyObject *, PyObject *const *v, Py_ssize_t argc) {
   ARGUMENTS(16);
   s14_ctx *ctx = (s14_ctx *)pointer_of(v[0]);
   const long device = PyLong_AsLong(v[1]);
-  const s14_kv_cache *cache;
+  const Cache *cache;
   const long long dim = PyLong_AsLongLong(v[4]);
   const double eps = PyFloat_AsDouble(v[11]);
   const s14_rope *rope;
@@ -226,7 +305,7 @@ static PyObject *kv_append(PyObject *, PyObject *const *v, Py_ssize_t argc) {
   if (stream_of(v[2], device, &stream)) return nullptr;
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = f_append(ctx, stream, cache, (uint32_t)shape[0], at.seqs, most, &k, &x, at.table, at.width, at.cu, at.len, kw,
+  rc = f_append<Cache>(ctx, stream, cache, (uint32_t)shape[0], at.seqs, most, &k, &x, at.table, at.width, at.cu, at.len, kw,
                 (float)eps, rope);
   Py_END_ALLOW_THREADS
   return done(rc);
@@ -240,11 +319,12 @@ static int scale_of(PyObject *v, long long dim, float *out) {
 }
 
 // handle, device, stream, q, cache, dim, page_table, cu, lens, out, lse, scale, window, max_new, max_len, tokens a page, the cache's tensors
+template <class Cache>
 static PyObject *paged_attention(PyObject *, PyObject *const *v, Py_ssize_t argc) {
   ARGUMENTS(17);
   s14_ctx *ctx = (s14_ctx *)pointer_of(v[0]);
   const long device = PyLong_AsLong(v[1]);
-  const s14_kv_cache *cache;
+  const Cache *cache;
   const long long dim = PyLong_AsLongLong(v[5]);
   const long long page = PyLong_AsLongLong(v[15]);
   void *stream;
@@ -268,7 +348,7 @@ static PyObject *paged_attention(PyObject *, PyObject *const *v, Py_ssize_t argc
   if (stream_of(v[2], device, &stream)) return nullptr;
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = f_paged(ctx, stream, &q, cache, (uint32_t)shape[0], at.seqs, most, length, at.table, at.width, at.cu, at.len, &out,
+  rc = f_paged<Cache>(ctx, stream, &q, cache, (uint32_t)shape[0], at.seqs, most, length, at.table, at.width, at.cu, at.len, &out,
                lse, scale, window);
   Py_END_ALLOW_THREADS
   return done(rc);
@@ -304,15 +384,18 @@ static PyObject *prompt_attention(PyObject *, PyObject *const *v, Py_ssize_t arg
   return done(rc);
 }
 
-// bind(addresses of the four entry points, refuse, check, current stream)
+// bind(addresses of the entry points, refuse, check, current stream)
 static PyObject *bind(PyObject *, PyObject *args) {
-  unsigned long long f[4];
+  unsigned long long f[7];
   PyObject *p[3];
-  if (!PyArg_ParseTuple(args, "(KKKK)OOO", &f[0], &f[1], &f[2], &f[3], &p[0], &p[1], &p[2])) return nullptr;
+  if (!PyArg_ParseTuple(args, "(KKKKKKK)OOO", &f[0], &f[1], &f[2], &f[3], &f[4], &f[5], &f[6], &p[0], &p[1], &p[2])) return nullptr;
   f_norm_rope = (norm_rope_fn)(uintptr_t)f[0];
-  f_append = (append_fn)(uintptr_t)f[1];
-  f_paged = (paged_fn)(uintptr_t)f[2];
+  f_append<s14_kv_cache> = (append_fn<s14_kv_cache>)(uintptr_t)f[1];
+  f_paged<s14_kv_cache> = (paged_fn<s14_kv_cache>)(uintptr_t)f[2];
   f_prompt = (prompt_fn)(uintptr_t)f[3];
+  f_append<s14_kv4_cache> = (append_fn<s14_kv4_cache>)(uintptr_t)f[4];
+  f_paged<s14_kv4_cache> = (paged_fn<s14_kv4_cache>)(uintptr_t)f[5];
+  f_add_norm = (add_norm_fn)(uintptr_t)f[6];
   PyObject **to[3] = {&p_refuse, &p_check, &p_stream};
   for (int i = 0; i < 3; ++i) {
     Py_INCREF(p[i]);
@@ -335,8 +418,11 @@ static PyObject *guarded(PyObject *self, PyObject *const *v, Py_ssize_t argc) {
 static PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, NULL},
     {"qk_norm_rope", (PyCFunction)(void (*)(void))guarded<qk_norm_rope>, METH_FASTCALL, NULL},
-    {"kv_append", (PyCFunction)(void (*)(void))guarded<kv_append>, METH_FASTCALL, NULL},
-    {"paged_attention", (PyCFunction)(void (*)(void))guarded<paged_attention>, METH_FASTCALL, NULL},
+    {"add_rms_norm", (PyCFunction)(void (*)(void))guarded<add_rms_norm>, METH_FASTCALL, NULL},
+    {"kv_append", (PyCFunction)(void (*)(void))guarded<kv_append<s14_kv_cache>>, METH_FASTCALL, NULL},
+    {"paged_attention", (PyCFunction)(void (*)(void))guarded<paged_attention<s14_kv_cache>>, METH_FASTCALL, NULL},
+    {"kv4_append", (PyCFunction)(void (*)(void))guarded<kv_append<s14_kv4_cache>>, METH_FASTCALL, NULL},
+    {"paged4_attention", (PyCFunction)(void (*)(void))guarded<paged_attention<s14_kv4_cache>>, METH_FASTCALL, NULL},
     {"prompt_attention", (PyCFunction)(void (*)(void))guarded<prompt_attention>, METH_FASTCALL, NULL},
     {NULL, NULL, 0, NULL},
 };

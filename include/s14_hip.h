@@ -497,6 +497,21 @@ int s14_qk_norm_rope(s14_ctx *ctx, void *stream, uint32_t tokens, uint32_t dim, 
                      s14_buffer q_weight, s14_buffer k_weight, float eps, const s14_rope *rope,
                      s14_buffer positions);
 
+/* The norm of the residual stream, before the projections and the experts:
+ *   h = x + residual, residual_out = h, y = h * rsqrt(mean(h^2) + eps) * weight,
+ *   q, scales = s14_act_quant_e4m3 of y (E4M3 codes [rows][k], E8M0 scales
+ *   [rows][k / group], group 32, 64 or 128; s14_fp8_linear takes group 128)
+ * of each row of k values (k a multiple of 8 and of the group, at most 65,536),
+ * f32 throughout, each output rounded once, the codes from y before its rounding.
+ * x, residual, residual_out and y: f32 or bf16 rows of one head (stride
+ * token_stride); residual NULL: h = x; residual_out NULL, y NULL and group 0
+ * leave that output out, y or the codes are asked for.  weight f32 [k].  An output
+ * may lie in x's or the residual's place, row on row; outputs that share memory
+ * with other rows, the weight or each other are refused. */
+int s14_add_rms_norm(s14_ctx *ctx, void *stream, uint32_t rows, uint32_t k, const s14_rows *x,
+                     const s14_rows *residual, const s14_rows *residual_out, const s14_rows *y,
+                     s14_buffer weight, float eps, uint32_t group, s14_buffer q, s14_buffer scales);
+
 /* The paged cache: E4M3 codes with one E8M0 scale for each page, key head and
  * side (value = code * 2^(scale - 127), as everywhere in this library).
  *   k codes [page][head][slot][dim], v codes [page][head][dim][slot],
@@ -546,6 +561,44 @@ int s14_paged_attention(s14_ctx *ctx, void *stream, const s14_rows *q, const s14
                         uint32_t tokens, uint32_t seqs, uint32_t max_new, uint32_t max_len,
                         s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer lens,
                         const s14_rows *out, s14_buffer lse, float scale, uint32_t window);
+
+/* The paged cache in 4 bits: E2M1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and, with
+ * bit 3, their negatives) with E8M0 scales of blocks of one token's dimensions,
+ * 32 of a key and 128 (64 at heads of 64) of a value; value = code * 2^(scale -
+ * 127), a block of scale 255 is NaN.  Pages and page tables as above.
+ *   k codes   [page][head][slot][dim / 2]: dimensions 2 i, 2 i + 1 in a byte's
+ *             low and high half
+ *   k scales  [page][head][dim / 32][page_tokens]: slot s at s - s % 16 +
+ *             4 (s % 4) + s % 16 / 4
+ *   v codes   [page][head][dim / 32][page_tokens / 16][16][16]: byte 8 h + j of
+ *             unit [u][b][d] holds dimension 32 u + 16 h + d of slots 16 b + 2 j
+ *             (low half) and 16 b + 2 j + 1
+ *   v scales  [page][head][dim / 128, at least 1][page_tokens]
+ * All four start on 16 bytes. */
+typedef struct {
+  s14_buffer k, v, k_scale, v_scale;
+  uint32_t pages, heads, page_tokens, dim;
+} s14_kv4_cache;
+
+/* s14_kv_append into it.  A block's scale is 2^e, e the least with 6 2^e >= its
+ * largest magnitude, held in -100 .. 100; codes are rounded to nearest, ties to
+ * even, and end at 6 (an infinity is stored as 6 * 2^100); a block with a NaN has
+ * scale 255 and codes 0.  A token's scales are its own: what was stored before
+ * stays as it is, to the bit. */
+int s14_kv4_append(s14_ctx *ctx, void *stream, const s14_kv4_cache *cache, uint32_t tokens,
+                   uint32_t seqs, uint32_t max_new, const s14_rows *k, const s14_rows *v,
+                   s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer past,
+                   s14_buffer k_weight, float eps, const s14_rope *rope);
+
+/* s14_paged_attention over it, in all it says but: a NaN block of a value that a
+ * row sees makes its 128 dimensions of the row NaN, one of a key the row; scales
+ * are 27 to 227 or 255, which is what the append stores (a value scale's power of
+ * two multiplies the weights before their rounding).  Blocks that no row sees may
+ * hold anything. */
+int s14_paged4_attention(s14_ctx *ctx, void *stream, const s14_rows *q, const s14_kv4_cache *cache,
+                         uint32_t tokens, uint32_t seqs, uint32_t max_new, uint32_t max_len,
+                         s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer lens,
+                         const s14_rows *out, s14_buffer lse, float scale, uint32_t window);
 
 /* Causal attention over packed prompts: sequence i is the rows cu[i] .. cu[i
  * + 1] - 1 of q, k and v (bf16), and row j of it sees its rows <= j (with
