@@ -4,6 +4,7 @@
 #include <hip/hip_runtime_api.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "s14_attn.hpp"
 #include "s14_attn_share.h"
@@ -261,8 +262,8 @@ extern "C" int s14_qk_norm_rope(s14_ctx *ctx, void *stream, uint32_t tokens, uin
 
 // A row operand of add_rms_norm: one head of k values.
 static int check_flat(const s14_rows *r, uint32_t rows, uint32_t k, const char *label) {
-  if (int rc = check_rows(r, rows, k, false, label)) return rc;
-  return r->heads == 1 ? S14_OK : fail(S14_ERR_SHAPE, "%s has %u heads, one is required", label, r->heads);
+  if (r && r->heads != 1) return fail(S14_ERR_SHAPE, "%s has %u heads, one is required", label, r->heads);
+  return check_rows(r, rows, k, false, label);
 }
 
 extern "C" int s14_add_rms_norm(s14_ctx *ctx, void *stream, uint32_t rows, uint32_t k, const s14_rows *x,
@@ -285,6 +286,9 @@ extern "C" int s14_add_rms_norm(s14_ctx *ctx, void *stream, uint32_t rows, uint3
   if (!weight.ptr) return fail(S14_ERR_INVALID, "norm weight buffer is NULL");
   if (int rc = check_weight(weight, k, eps, "norm weight")) return rc;
   if (!rows) return S14_OK;
+  // a thread for eight values at most
+  if (uint64_t(rows) * ((k / 8 + 63) / 64 * 64) >= kMaxBlocks * 256)
+    return fail(S14_ERR_SHAPE, "%u rows of %u values exceed one launch", rows, k);
   const uint64_t values = uint64_t(rows) * k, n_scales = group ? values / group : 0;
   if (group) {
     if (int rc = require(q, values, 8, "codes")) return rc;
@@ -347,6 +351,9 @@ static int append_to(hipError_t (*launch)(hipStream_t, const s14::AppendArgs &),
   if (int rc = check_rope(rope, cache->dim, &a.rope)) return rc;
   if (!tokens || !seqs || !max_new) return S14_OK;
   if (int rc = check_table(cu, past, page_table, seqs, table_width, "past")) return rc;
+  // 16 slots of D / 8 lanes a workgroup, and for each sequence two blocks that it may share
+  if (std::is_same_v<Cache, s14_kv4_cache> && (uint64_t(tokens) / 16 + 2ull * seqs + 1) * 2 * cache->dim >= kMaxBlocks * 256)
+    return fail(S14_ERR_SHAPE, "%u tokens of %u sequences exceed one launch", tokens, seqs);
   a.tokens = tokens, a.seqs = seqs, a.max_new = max_new, a.table_width = table_width;
   a.in[0] = rows_of(k), a.in[1] = rows_of(v);
   a.k_weight = static_cast<const float *>(k_weight.ptr), a.eps = eps;

@@ -39,10 +39,9 @@ __device__ __forceinline__ bf16x8 e2m1_bf16(uint32_t w, float scale = 1.0f) {
 __device__ __forceinline__ float rough_scale(uint32_t w, int i) {
   return __uint_as_float(i < 3 ? w << (23 - 8 * i) : w >> 1);
 }
-// And alone: 2^(code - 127), 0 for code 0, infinity for 255 (a block with a NaN,
-// whose codes are 0: times those it is NaN again).
+// And alone: 2^(code - 127), NaN for 255, by the conversion of an 8-bit one.
 __device__ __forceinline__ float clean_scale(uint32_t w, int i) {
-  return __uint_as_float(__float_as_uint(rough_scale(w, i)) & 0x7f800000u);
+  return __builtin_amdgcn_cvt_scalef32_f32_fp8(0x38, rough_scale(w, i), 0);
 }
 
 // A slot's place among a block's key scales: of each 16 slots the 4 x 4 transposed,
@@ -195,7 +194,7 @@ __global__ __launch_bounds__(256, D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2) void
         for (int c = 0; c < B; ++c)
           f[c][i] = clean_scale(i < 4 ? vsc[c].x : i < 8 ? vsc[c].y : i < 12 ? vsc[c].z : vsc[c].w, i % 4);
       }
-      if (partial) {  // a masked token's scale may be anything: no weight times infinity
+      if (partial) {  // a masked token's scale may be anything: no weight times NaN
         keep_branch();
 #pragma unroll
         for (int i = 0; i < 4 * T; ++i) {
@@ -495,7 +494,7 @@ __global__ __launch_bounds__(256, 2) void k_paged4_wide(PagedArgs a, PagedPlan p
         float w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = e[i] * f[c][i];
-        if (partial) {  // a masked token's scale may be anything: no weight times infinity
+        if (partial) {  // a masked token's scale may be anything: no weight times NaN
           keep_branch();
 #pragma unroll
           for (int i = 0; i < 4; ++i) w[i] = see[nt](tk + i) ? w[i] : 0.0f;
@@ -683,7 +682,7 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
       const uint32_t dim = v_dim + 16 * (w / 2);
       to[kPieces + dim * (TK / 8) + ((v_tok / 8 + w % 2) ^ turn_v<TK>(dim))] = __builtin_bit_cast(u32x4, e2m1_bf16(vv[w]));
     }
-    if (tid < B * TK) reinterpret_cast<float *>(s_vs)[tid] = __uint_as_float(uint32_t(vsc) << 23);
+    if (tid < B * TK) reinterpret_cast<float *>(s_vs)[tid] = clean_scale(vsc, 0);
   };
   const uint32_t k_row = 8 * (n / 4) + n % 4, k_turn = turn_k<D>(k_row), v_turn = turn_v<TK>(n);
 
@@ -754,7 +753,7 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
             float y[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] = e[j] * (j < 4 ? f0[j] : f1[j - 4]);
-            if (partial) {  // a masked token's scale may be anything: no weight times infinity
+            if (partial) {  // a masked token's scale may be anything: no weight times NaN
               keep_branch();
 #pragma unroll
               for (int j = 0; j < 8; ++j) y[j] = see[nt](tv + 32 * u + j) ? y[j] : 0.0f;
