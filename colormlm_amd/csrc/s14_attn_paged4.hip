@@ -48,6 +48,11 @@ __device__ __forceinline__ float clean_scale(uint32_t w, int i) {
 // so that the four tiles' scales of a lane are one word.
 __device__ __forceinline__ uint32_t scale_slot(uint32_t slot) { return (slot & ~15u) + 4 * (slot & 3u) + ((slot >> 2) & 3u); }
 
+// A weight times its token's value scale, 0 where the weight is 0 (the instruction's
+// own rule): a masked token's scale may be anything.
+extern "C" __device__ float s14_mul_zero(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
+__device__ __forceinline__ float weighted(float weight, float scale) { return s14_mul_zero(weight, scale); }
+
 // Scales above 0: a masked score times it stays -inf.
 __device__ __forceinline__ float score_scale(float scale) { return fmaxf(scale * kLog2e, 0x1p-126f); }
 
@@ -194,15 +199,10 @@ __global__ __launch_bounds__(256, D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2) void
         for (int c = 0; c < B; ++c)
           f[c][i] = clean_scale(i < 4 ? vsc[c].x : i < 8 ? vsc[c].y : i < 12 ? vsc[c].z : vsc[c].w, i % 4);
       }
-      if (partial) {  // a masked token's scale may be anything: no weight times NaN
+      if (partial) {
         keep_branch();
 #pragma unroll
-        for (int i = 0; i < 4 * T; ++i) {
-          const bool in = see[nt](tv + i);
-          x[i] = in ? x[i] : -INFINITY;
-#pragma unroll
-          for (int c = 0; c < B; ++c) f[c][i] = in ? f[c][i] : 0.0f;
-        }
+        for (int i = 0; i < 4 * T; ++i) x[i] = see[nt](tv + i) ? x[i] : -INFINITY;
       }
       float top = x[0];
 #pragma unroll
@@ -231,8 +231,8 @@ __global__ __launch_bounds__(256, D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2) void
 #pragma unroll
         for (int c = 0; c < B; ++c) {
           const float *v = &f[c][4 * t];
-          w[c][t / 2][2 * (t & 1)] = bf16_pair(e[0] * v[0], e[1] * v[1]);
-          w[c][t / 2][2 * (t & 1) + 1] = bf16_pair(e[2] * v[2], e[3] * v[3]);
+          w[c][t / 2][2 * (t & 1)] = bf16_pair(weighted(e[0], v[0]), weighted(e[1], v[1]));
+          w[c][t / 2][2 * (t & 1) + 1] = bf16_pair(weighted(e[2], v[2]), weighted(e[3], v[3]));
         }
       }
 #pragma unroll
@@ -493,12 +493,7 @@ __global__ __launch_bounds__(256, 2) void k_paged4_wide(PagedArgs a, PagedPlan p
       for (int c = 0; c < C; ++c) {
         float w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = e[i] * f[c][i];
-        if (partial) {  // a masked token's scale may be anything: no weight times NaN
-          keep_branch();
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = see[nt](tk + i) ? w[i] : 0.0f;
-        }
+        for (int i = 0; i < 4; ++i) w[i] = weighted(e[i], f[c][i]);
         // half a step of each weight: the matrix operand's type
         reinterpret_cast<uint2 *>(&s_p[c][nt][g / 2][16 * wave + n])[g & 1] =
             make_uint2(bf16_pair(w[0], w[1]), bf16_pair(w[2], w[3]));
@@ -584,7 +579,7 @@ __device__ __forceinline__ uint32_t turn_v(uint32_t dim) {
 // from LDS, where the workgroup has put them as bf16, the keys with their scales,
 // once for all its rows; the values' scales lie beside them.
 template <int D, int NT, int RW>
-__global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 ? 4 : 3) void k_paged4_rows(PagedArgs a, PagedPlan p, float *part) {
+__global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 4 : RW == 2 ? 4 : 3) void k_paged4_rows(PagedArgs a, PagedPlan p, float *part) {
   constexpr int TK = D <= 128 ? 64 : 32;  // tokens a step
   constexpr int TW = 4 / RW;              // wavefronts that share a row tile's tokens
   constexpr int U = TK / 32 / TW, T = 2 * U, DT = D / 16, C = D / 32;
@@ -752,12 +747,7 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 5 : RW == 2 
             const f32x4 f0 = s_vs[c * (TK / 4) + 8 * (u0 + u) + 2 * g], f1 = s_vs[c * (TK / 4) + 8 * (u0 + u) + 2 * g + 1];
             float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = e[j] * (j < 4 ? f0[j] : f1[j - 4]);
-            if (partial) {  // a masked token's scale may be anything: no weight times NaN
-              keep_branch();
-#pragma unroll
-              for (int j = 0; j < 8; ++j) y[j] = see[nt](tv + 32 * u + j) ? y[j] : 0.0f;
-            }
+            for (int j = 0; j < 8; ++j) y[j] = weighted(e[j], j < 4 ? f0[j] : f1[j - 4]);
             u32x4 w;
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = bf16_pair(y[2 * j], y[2 * j + 1]);  // half a step of each weight: the matrix operand's type
