@@ -410,7 +410,7 @@ static int attend_over(hipError_t (*launch)(hipStream_t, const s14::PagedArgs &,
   a.out = out_of(out), a.lse = static_cast<float *>(lse.ptr);
   a.scale = scale, a.window = window;
   const s14::PagedPlan p = s14::paged_plan(
-      {seqs, a.heads, cache->heads, cache->dim, max_new, max_len, window, table_width * cache->page_tokens});
+      {seqs, a.heads, cache->heads, cache->dim, max_new, max_len, window, table_width * cache->page_tokens, std::is_same_v<Cache, s14_kv4_cache>});
   if (p.blocks >= kMaxBlocks || uint64_t(max_new) * q->heads >= (1ull << 31))
     return fail(S14_ERR_SHAPE, "%u new tokens of %u sequences exceed one launch", max_new, seqs);
   if (int rc = check_apart(out, q, tokens, cache->dim, true, "out")) return rc;

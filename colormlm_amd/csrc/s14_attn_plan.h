@@ -11,6 +11,7 @@ namespace s14 {
 // hold, 2^31 - 2^16 at most; a promise (max_len) past it is one of that.
 struct PagedShape {
   uint32_t seqs, heads, kv_heads, dim, max_new, max_len, window, reach;
+  uint32_t four;  // the cache of 4 bits
 };
 
 // Work split of a paged launch.
@@ -22,8 +23,13 @@ struct PagedPlan {
   uint32_t chunks;     // of the longest sequence; above 1 the partial results go to the workspace
   uint32_t fused;      // the last workgroup of a row tile joins its chunks; else a second launch
   uint64_t blocks;     // workgroups
+  // Above 0: the chunk is set on the device, by what the sequences hold in all, so
+  // that `fill` workgroups a row tile and key head have it, `least` tokens at least
+  // each.  chunks is then the most that a sequence is cut into.
+  uint32_t fill, least;
 };
 constexpr uint64_t kPagedPartFloats = 16ull << 20;  // the workspace: 64 MiB
+constexpr uint32_t kMostBalanced = 256;             // sequences whose lengths a workgroup adds up
 constexpr uint32_t kPagedCounters = 16384;          // arrivals at a row tile, 0 between launches
 
 // The chunks of a row tile that reads `span` tokens: the plan's, and larger
@@ -69,6 +75,15 @@ constexpr int32_t paged_end(int32_t begin, int32_t hi, uint32_t chunk) {
 // (20 sequences of 300 tokens, 32 rows: 10 us, in two chunks 21; one of 500
 // tokens and 8 of them 11, 20), and small chunks start at shorter ones (4 of 48
 // rows of 300 tokens, heads of 256: 12 us in chunks of 64, 19 of 256).
+//
+// The cache of 4 bits.  Where a chunk's partial result is 64 KB (32 rows of heads
+// of 512, 128 of heads of 128) writing and reading it is what more chunks cost, and
+// how many the lengths need is only known on the device: there the chunk is what the
+// sequences hold in all over as many workgroups as the card holds at once (us, by
+// max_len / so: 8 of 64 new of 3,000 57 / 51; 2 of 256 of 4,000 71 / 61; 3 of 200 of
+// up to 6,000 94 / 88; 64 of 1 of 4,000, heads of 512, 79 / 65; 4 of 4 of up to 9,000
+// 33.7 / 34.8).  With smaller results the sum of the lengths costs more than it saves
+// (20 of 2 of up to 9,000, heads of 64: 18 / 21).
 inline PagedPlan paged_plan(const PagedShape &a) {
   PagedPlan p{};
   const uint64_t rows = uint64_t(a.max_new) * (a.heads / a.kv_heads);
@@ -95,7 +110,8 @@ inline PagedPlan paged_plan(const PagedShape &a) {
   p.rec_rows = uint32_t(rows < 16 * p.row_tiles ? rows : 16 * p.row_tiles);
   const uint64_t rec = uint64_t(p.rec_rows) * (dim + 4);
   uint64_t chunks = base < slots ? slots * (a.seqs > 1 ? 2 : 1) / base : (span + kMost - 1) / kMost;
-  const uint64_t fit = kPagedPartFloats / (rec * base);
+  const bool balance = a.four && a.seqs > 1 && a.seqs <= kMostBalanced && base < slots && rec * 4 >= kFuse;
+  const uint64_t fit = (kPagedPartFloats - (a.four ? 4 : 0)) / (rec * base);
   if (chunks > fit) chunks = fit;
   if (chunks > (span + least - 1) / least) chunks = (span + least - 1) / least;
   if (chunks < 1) chunks = 1;
@@ -104,6 +120,10 @@ inline PagedPlan paged_plan(const PagedShape &a) {
   p.chunk = uint32_t(((span + chunks - 1) / chunks + least - 1) / least * least);
   p.chunks = uint32_t((span + p.chunk - 1) / p.chunk);
   p.blocks = base * p.chunks;
+  if (balance && p.chunks > 1 && p.chunk > least) {
+    p.fill = uint32_t((slots + tiles * a.kv_heads - 1) / (tiles * a.kv_heads));
+    p.least = dim == 512 ? 320 : uint32_t(least);
+  }
   return p;
 }
 

@@ -6,7 +6,7 @@
 
 #include "s14_attn.hpp"
 #include "s14_attn_util.hpp"
-#include "s14_device.hpp"
+#include "s14_device_util.hpp"
 
 namespace s14 {
 namespace {
@@ -20,7 +20,35 @@ struct Span {
   uint32_t wrong;  // status: its length is outside the table, or it has rows that no workgroup takes
 };
 
-__device__ __forceinline__ Span paged_span(const PagedArgs &a, const PagedPlan &p, uint32_t seq, uint32_t row0) {
+// The sum of v over a wavefront.
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
+  v += uint32_t(dpp_i<0xb1>(0, int(v)));   // quad_perm [1,0,3,2]
+  v += uint32_t(dpp_i<0x4e>(0, int(v)));   // quad_perm [2,3,0,1]
+  v += uint32_t(dpp_i<0x141>(0, int(v)));  // row_half_mirror
+  v += uint32_t(dpp_i<0x140>(0, int(v)));  // row_mirror
+  return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) +
+         __builtin_amdgcn_readlane(v, 48);
+}
+
+// The chunk of a plan that balances (PagedPlan::fill): the cached tokens that the
+// launch reads in all, over the workgroups that shall have them.  The same in every
+// wavefront.
+__device__ __forceinline__ uint32_t balanced_chunk(const PagedArgs &a, const PagedPlan &p) {
+  uint32_t steps = 0;  // of 64 tokens: up to 2^25 of a sequence, of kMostBalanced / 64 sequences a lane
+  const int64_t room = int64_t(a.table_width) * a.cache.page;
+  for (uint32_t s = threadIdx.x & 63u; s < a.seqs; s += 64) {
+    const int64_t n = clamp_row(a.cu[s + 1], a.tokens) - clamp_row(a.cu[s], a.tokens), len = a.len[s];
+    const int64_t hi = n <= 0 || len < 0 ? 0 : len < room ? len : room;
+    const int64_t lo = a.window && hi - n - a.window + 1 > 0 ? hi - n - a.window + 1 : 0;
+    if (hi > lo) steps += uint32_t((hi - (lo & ~63ll) + 63) >> 6);
+  }
+  const uint64_t total = (uint64_t(wave_sum_u32(steps >> 16)) << 16) + wave_sum_u32(steps & 0xffffu);
+  const uint32_t most = 1u << 24;  // 2^30 tokens
+  const uint32_t each = total >> 31 ? most : (uint32_t(total) + p.fill - 1) / p.fill;
+  return 64 * max(p.least / 64, min(each, most));
+}
+
+__device__ __forceinline__ Span paged_span(const PagedArgs &a, const PagedPlan &p, uint32_t seq, uint32_t row0, uint32_t planned) {
   Span s;
   const uint32_t group = a.heads / a.cache.heads;
   s.first = uint32_t(clamp_row(a.cu[seq], a.tokens));
@@ -39,9 +67,29 @@ __device__ __forceinline__ Span paged_span(const PagedArgs &a, const PagedPlan &
   s.seen = int32_t(lo < 0 ? 0 : lo);
   s.lo = s.seen & ~63;
   const uint32_t span = s.hi > s.lo ? s.hi - s.lo : 0;
-  const PagedCut cut = paged_cut(span, p.chunk, p.chunks);
+  const PagedCut cut = paged_cut(span, planned, p.chunks);
   s.chunk = cut.chunk, s.chunks = cut.chunks;
   return s;
+}
+
+__device__ __forceinline__ Span paged_span(const PagedArgs &a, const PagedPlan &p, uint32_t seq, uint32_t row0) {
+  return paged_span(a, p, seq, row0, p.chunk);
+}
+
+// The same with a plan that may balance.  The joining launch takes the chunk from
+// the end of the workspace.
+__device__ __forceinline__ uint32_t *chunk_word(float *part) { return reinterpret_cast<uint32_t *>(part + kPagedPartFloats - 4); }
+__device__ __forceinline__ Span balanced_span(const PagedArgs &a, const PagedPlan &p, uint32_t seq, uint32_t row0, float *part) {
+  uint32_t planned = p.chunk;
+  if (p.fill) {
+    planned = balanced_chunk(a, p);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *chunk_word(part) = planned;
+  }
+  return paged_span(a, p, seq, row0, planned);
+}
+template <bool kBalanced>
+__device__ __forceinline__ Span joined_span(const PagedArgs &a, const PagedPlan &p, uint32_t seq, uint32_t row0, const float *part) {
+  return paged_span(a, p, seq, row0, kBalanced && p.fill ? *chunk_word(const_cast<float *>(part)) : p.chunk);
 }
 
 __device__ __forceinline__ void store_out(const AttnOut &o, uint64_t at, float a, float b, float c, float d) {
@@ -228,14 +276,14 @@ __device__ __forceinline__ void join_tile(const PagedArgs &a, const PagedPlan &p
 // Joins the chunks of one row a workgroup, in an order that its size alone
 // sets: the chunks' maxima in the lanes, then their rows in groups of
 // threads at once.
-template <int D>
+template <int D, bool kBalanced>
 __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, PagedPlan p, const float *part) {
   constexpr uint32_t kLanes = D / 4 < 64 ? D / 4 : 64, kSpan = D / (4 * kLanes);  // float4s of a row a thread
   constexpr uint32_t kGroups = 256 / kLanes;
   const uint32_t kvh = a.cache.heads, group = a.heads / kvh, tid = threadIdx.x;
   const uint32_t seq = blockIdx.y, head = blockIdx.z, r = blockIdx.x;
   const uint32_t per = 16 * p.row_tiles, tile = r / per;
-  const Span sp = paged_span(a, p, seq, tile * per);
+  const Span sp = joined_span<kBalanced>(a, p, seq, tile * per, part);
   if (r >= sp.rows || sp.chunks <= 1) return;
   const uint64_t rec = uint64_t(p.rec_rows) * kRecord<D>;
   const float *row = part + record_of(a, p, Item{tile, 0, seq, head}, kvh) * rec + r % per * kRecord<D>;
@@ -284,24 +332,24 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a, PagedPlan p, co
 // Up to 16 chunks of a row: a row a wavefront, which reads them at once (128
 // rows of 8 sequences, 8 key heads, 8 chunks, 69 MB: 78 us with the attention,
 // a row a workgroup 98).
-template <int D>
+template <int D, bool kBalanced>
 __global__ __launch_bounds__(256) void k_paged_join_rows(PagedArgs a, PagedPlan p, const float *part) {
   const uint32_t r = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / 64), per = 16 * p.row_tiles;
   const Item it{r / per, 0, blockIdx.y, blockIdx.z};
-  const Span sp = paged_span(a, p, it.seq, it.tile * per);
+  const Span sp = joined_span<kBalanced>(a, p, it.seq, it.tile * per, part);
   if (r >= sp.rows || sp.chunks <= 1) return;
   join_row<D, 0>(a, p, sp, it, it.tile * per, r % per, part);
 }
 
-template <int D, class Kernel>
+template <int D, bool kBalanced = false, class Kernel>
 hipError_t launch(hipStream_t s, const PagedArgs &a, const PagedPlan &p, float *part, Kernel kernel) {
   kernel<<<uint32_t(p.blocks), 256, 0, s>>>(a, p, part);
   if (p.chunks > 1 && !p.fused) {
     const uint32_t rows = uint32_t(a.max_new) * (a.heads / a.cache.heads);
     if (p.chunks <= 16)
-      k_paged_join_rows<D><<<dim3((rows + 3) / 4, a.seqs, a.cache.heads), 256, 0, s>>>(a, p, part);
+      k_paged_join_rows<D, kBalanced><<<dim3((rows + 3) / 4, a.seqs, a.cache.heads), 256, 0, s>>>(a, p, part);
     else
-      k_paged_join<D><<<dim3(rows, a.seqs, a.cache.heads), 256, 0, s>>>(a, p, part);
+      k_paged_join<D, kBalanced><<<dim3(rows, a.seqs, a.cache.heads), 256, 0, s>>>(a, p, part);
   }
   return hipGetLastError();
 }
