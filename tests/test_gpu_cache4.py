@@ -336,6 +336,45 @@ def test_append_slices_of_one_projection(ctx):
             assert torch.equal(getattr(p.cache, t), getattr(w.cache, t)), t
 
 
+@pytest.mark.parametrize("new", [[1, 1], [40, 9]])
+def test_append_operands_of_different_types(ctx, new):
+    say("append4 of f32 keys with bf16 values and the other way round")
+    for kt, vt in ((F32, BF16), (BF16, F32)):
+        p, w = (Paged4(5, [5 + n for n in new], 2, 128, 32) for _ in range(2))
+        x, y = rand(gen(1), sum(new), 2, 128, dtype=BF16).to(kt).cuda(), rand(gen(2), sum(new), 2, 128, dtype=BF16).to(vt).cuda()
+        A.kv_append(ctx, p.cache, x, y, p.dev_table, cumulative(new), ints([5, 5]), max_new=max(new))
+        A.kv_append(ctx, w.cache, x.float(), y.float(), w.dev_table, cumulative(new), ints([5, 5]), max_new=max(new))
+        for t in ("k_pages", "v_pages", "k_scales", "v_scales"):
+            assert torch.equal(getattr(p.cache, t), getattr(w.cache, t)), t
+
+
+@pytest.mark.parametrize("seqs,counts", [(256, 1), (257, 1), (70, 20), (2, 300), (5, 40)])
+def test_balanced_and_planned_splits(ctx, seqs, counts):
+    """Chunks set by the lengths (up to 256 sequences) and by max_len, with
+    sequences without tokens, without rows, and one far longer than the rest."""
+    say(f"paged4 {seqs} sequences of {counts} rows, ragged")
+    g = gen(seqs)
+    lengths = [int(x) for x in torch.randint(0, 200, (seqs,), generator=g)]
+    lengths[0], lengths[1], lengths[-1] = 6000, 0, 700
+    new = [counts] * seqs
+    new[seqs // 2] = 0 if seqs > 2 else counts
+    for heads, kv, dim in ((64, 1, 512), (8, 1, 128)):
+        p = Paged4(seqs, lengths, kv, dim, 64)
+        q = rand(gen(4), sum(new), heads, dim, dtype=BF16).cuda()
+        for window in (0, 1000):
+            out, lse = run_paged(ctx, p, q, new, heads, dim, window)
+            for i in (0, 1, seqs // 2, seqs - 1):
+                at, m = sum(new[:i]), new[i]
+                k, v = p.rows(i)
+                for n, end in ((min(m, 2), len(k) - m + min(m, 2)), (min(m, 1), len(k))):  # its first and last rows
+                    first = at if end < len(k) else at + m - n
+                    rows = slice(first, first + n)
+                    want = T.attention64(q[rows].cpu(), k[:max(end, 0)], v[:max(end, 0)], dim ** -0.5, window) if n else None
+                    if n:
+                        check_attention(out[rows], lse[rows], want, f"sequence {i}")
+    ctx.launch_status()
+
+
 def test_appends_in_pieces_are_one(ctx):
     say("append4: a token's codes do not depend on how the tokens came")
     x, y = rand(gen(8), 75, 2, 64).cuda(), rand(gen(9), 75, 2, 64).cuda()
