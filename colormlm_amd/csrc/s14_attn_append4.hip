@@ -6,8 +6,9 @@
 // and end at 6.  A token's scales are its own: nothing that was stored before is
 // touched, so the unit of work is a block of kSlots neighbouring slots of a page
 // (16, the slots of a unit of V codes, or 4 where few tokens are new), head and
-// side, of D / 8 lanes a slot.  Bound by the bytes moved, for a few tokens by the
-// launch.
+// side, of D / 8 lanes a slot.  Bound by the bytes moved (21 prompts of up to 4,000
+// tokens, 8 heads of 128: 78 MB in 22.2 us, 3.5 TB/s), for a few tokens by the chain
+// of loads, counts, then the page's id and the rows (96 single ones: 4.3 us).
 #include "s14_attn_rows.hpp"
 
 namespace s14 {
@@ -257,16 +258,19 @@ hipError_t append(hipStream_t s, const AppendArgs &a) {
   const bool turn = a.k_weight || a.rope.table;
   // more workgroups than the card holds at once: keys and values by one (21 prompts
   // of up to 4,000 tokens, 8 heads of 128: 22.4 us, apart 30.3); else apart (8 tokens
-  // of one head of 512: 4.6 us, by one 5.5)
+  // of one head of 512 in blocks of 16: 4.6 us, by one 5.5)
   if constexpr (kSlots == 16)
     if (uint64_t(blocks) * a.cache.heads * kThreads > 256 * 2048)
       return turn ? launch(k_kv_append4<kDim, kSlots, true, true>, 1) : launch(k_kv_append4<kDim, kSlots, true, false>, 1);
   return turn ? launch(k_kv_append4<kDim, kSlots, false, true>, 2) : launch(k_kv_append4<kDim, kSlots, false, false>, 2);
 }
 
+// Blocks of 4 slots for up to 16 tokens of a sequence, more and smaller workgroups (us
+// of 4 and 16 slots: 96 single tokens, 8 heads of 128, 4.4 / 6.0; 8 tokens of a head of
+// 512 4.3 / 5.1; 32 sequences of 8 4.5 / 5.3; 8 of 16 4.4 / 4.4).
 template <int kDim>
 hipError_t append_dim(hipStream_t s, const AppendArgs &a) {
-  return a.max_new <= 4 ? append<kDim, 4>(s, a) : append<kDim, 16>(s, a);
+  return a.max_new <= 16 ? append<kDim, 4>(s, a) : append<kDim, 16>(s, a);
 }
 
 }  // namespace

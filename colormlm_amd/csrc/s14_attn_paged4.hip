@@ -57,7 +57,11 @@ __device__ __forceinline__ float weighted(float weight, float scale) { return s1
 __device__ __forceinline__ float score_scale(float scale) { return fmaxf(scale * kLog2e, 0x1p-126f); }
 
 // Up to 16 NT rows: the four wavefronts take steps of 64 tokens in turn and join
-// through LDS.
+// through LDS.  Bound by the cache's bytes: 96 sequences of 2,048 tokens, 8 key heads
+// of 128, 40.5 us, 5.2 TB/s (a large read alone takes 5.7); 128 of up to 8,192 85 to
+// 90 us, 4.5 TB/s, by how their lengths fall on the compute units.  A fourth
+// wavefront a SIMD spills (128 us); with two row tiles eight wavefronts are no faster
+// (8 tokens of 40,000: 18.6 us, 19.8).
 template <int D, int NT>
 __global__ __launch_bounds__(256, D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2) void k_paged4(PagedArgs a, PagedPlan p, float *part) {
   constexpr int T = 4;                       // 16-token tiles a step
@@ -343,7 +347,11 @@ __global__ __launch_bounds__(256, D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2) void
 // first product, all dimensions of them, against Q from LDS; the wavefronts'
 // maxima meet there, each weights its own scores, once for each of the four value
 // scales of a token, and P goes through LDS for the second product, of which a
-// wavefront takes the 128 dimensions of one scale, all tokens.
+// wavefront takes the 128 dimensions of one scale, all tokens.  64 sequences of 4,000
+// tokens, 64 heads, 65 us, 519 TFLOP/s; issue bounds it, 480 instructions of the
+// vector unit a step beside 1,024 clocks of the matrix unit, and for few sequences
+// the partial results (33 MB of one of 4,000 tokens).  Codes two steps ahead are no
+// faster (256 sequences of 1,024: 59.6 us, 62.8).
 template <int NT>
 __global__ __launch_bounds__(256, 2) void k_paged4_wide(PagedArgs a, PagedPlan p, float *part) {
   constexpr int D = 512, C = 4, DT = 8;
@@ -577,7 +585,12 @@ __device__ __forceinline__ uint32_t turn_v(uint32_t dim) {
 // More rows: each wavefront has 16 NT of its own (of two row tiles, two
 // wavefronts share one, half the tokens each), and all read the same TK tokens
 // from LDS, where the workgroup has put them as bf16, the keys with their scales,
-// once for all its rows; the values' scales lie beside them.
+// once for all its rows; the values' scales lie beside them.  A step of 128 rows takes
+// 1.2 us a compute unit (880 TFLOP/s of a running one); what 8 sequences of 64 new of
+// 3,000 tokens take beyond that, 51 us in all, is the start, and 35 MB of partial
+// results written and read.  Tried without gain there: a step's products between the
+// next one's weights with two buffers (58 us), eight wavefronts that halve the partial
+// results (59), 64 rows a workgroup (54).
 template <int D, int NT, int RW>
 __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 4 : RW == 2 ? 4 : 3) void k_paged4_rows(PagedArgs a, PagedPlan p, float *part) {
   constexpr int TK = D <= 128 ? 64 : 32;  // tokens a step
