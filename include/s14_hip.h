@@ -432,9 +432,10 @@ int s14_fp8_linear(s14_ctx *ctx, void *stream, uint32_t m, uint32_t n, uint32_t 
                    int weight_scale_dtype, s14_buffer bias, s14_buffer y, int flags, int mode);
 
 /* ======================================================================
- * Attention between the FP8 projections and the expert layer: per-head norms
- * with the position rotation, a paged key/value cache in 8 bits, attention
- * over it, and causal attention over packed prompts.  No counterpart in the
+ * Attention between the FP8 projections and the expert layer: the residual
+ * norm before either, per-head norms with the position rotation, paged
+ * key/value caches in 8 and in 4 bits, attention over them, and causal
+ * attention over packed prompts.  No counterpart in the
  * reference, whose GPU code has no S14 attention; the projections (s14_fp8_linear)
  * give these calls their rows and take their outputs.
  *
@@ -504,7 +505,7 @@ int s14_qk_norm_rope(s14_ctx *ctx, void *stream, uint32_t tokens, uint32_t dim, 
  * of each row of k values (k a multiple of 8 and of the group, at most 65,536),
  * f32 throughout, each output rounded once, the codes from y before its rounding.
  * x, residual, residual_out and y: f32 or bf16 rows of one head (stride
- * token_stride); residual NULL: h = x; residual_out NULL, y NULL and group 0
+ * token_stride); codes start on 8 bytes.  residual NULL: h = x; residual_out NULL, y NULL and group 0
  * leave that output out, y or the codes are asked for.  weight f32 [k].  An output
  * may lie in x's or the residual's place, row on row; outputs that share memory
  * with other rows, the weight or each other are refused. */
