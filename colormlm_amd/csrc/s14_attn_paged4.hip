@@ -348,7 +348,7 @@ __global__ __launch_bounds__(256, D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2) void
 // maxima meet there, each weights its own scores, once for each of the four value
 // scales of a token, and P goes through LDS for the second product, of which a
 // wavefront takes the 128 dimensions of one scale, all tokens.  64 sequences of 4,000
-// tokens, 64 heads, 65 us, 519 TFLOP/s; issue bounds it, 480 instructions of the
+// tokens, 64 heads, 68 us, 495 TFLOP/s; issue bounds it, 480 instructions of the
 // vector unit a step beside 1,024 clocks of the matrix unit, and for few sequences
 // the partial results (33 MB of one of 4,000 tokens).  Codes two steps ahead are no
 // faster (256 sequences of 1,024: 59.6 us, 62.8).
@@ -448,17 +448,21 @@ __global__ __launch_bounds__(256, 2) void k_paged4_wide(PagedArgs a, PagedPlan p
     load_ids(min(b + 2 * kStep, last), idk2, idv2);
     const bool partial = b + kStep - 1 > pos_lo || (a.window && int64_t(b) <= int64_t(pos_hi) - a.window);
     f32x4 s[NT][2] = {};
+    // Q two words ahead of its use (read right before it, as the compiler leaves it: 68 -> 70 us)
+    bf16x8 qa[4][NT];
+    const auto read_q = [&](int w) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const float ks = __uint_as_float(uint32_t(ksc[c]) << 23);
-      const uint32_t word[4] = {kk[c].x, kk[c].y, kk[c].z, kk[c].w};
+      for (int nt = 0; nt < NT; ++nt) qa[w & 3][nt] = s_q[nt][w][l];
+    };
+    read_q(0), read_q(1);
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const bf16x8 k = e2m1_bf16(word[h], ks);
+    for (int w = 0; w < 4 * C; ++w) {
+      if (w + 2 < 4 * C) read_q(w + 2);
+      const uint32_t word = w % 4 == 0 ? kk[w / 4].x : w % 4 == 1 ? kk[w / 4].y : w % 4 == 2 ? kk[w / 4].z : kk[w / 4].w;
+      const bf16x8 k = e2m1_bf16(word, __uint_as_float(uint32_t(ksc[w / 4]) << 23));
+      __builtin_amdgcn_sched_barrier(0x1 | 0x2 | 0x4 | 0x8);  // LDS reads stay ahead
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          s[nt][h & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, s_q[nt][4 * c + h][l], s[nt][h & 1], 0, 0, 0);
-      }
+      for (int nt = 0; nt < NT; ++nt) s[nt][w & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qa[w & 3][nt], s[nt][w & 1], 0, 0, 0);
     }
     float f[C][4];
 #pragma unroll
