@@ -295,29 +295,28 @@ extern "C" int s14_add_rms_norm(s14_ctx *ctx, void *stream, uint32_t rows, uint3
     if (int rc = require(scales, n_scales, 1, "scales")) return rc;
   }
   // rows may be written in their input's place; nothing else is shared
-  const auto codes = [&](const s14_buffer &b, uint64_t bytes) {
-    return s14::RowBytes{reinterpret_cast<uintptr_t>(b.ptr), 0, 0, bytes, 1};
+  const auto touch = [&](const s14_rows *r, const void *p, uint64_t bytes) {
+    return r && s14::rows_touch(bytes_of(r, k), reinterpret_cast<uintptr_t>(p), bytes, rows);
   };
   for (int i = 0; i < 2; ++i) {
     if (!outs[i]) continue;
     if (int rc = check_apart(outs[i], x, rows, k, true, labels[i])) return rc;
     if (residual)
       if (int rc = check_apart(outs[i], residual, rows, k, true, labels[i])) return rc;
-    if (s14::rows_share(bytes_of(outs[i], k), {reinterpret_cast<uintptr_t>(weight.ptr), 4ull * k, 0, 4ull * k, 1}, 1, false))
-      return fail(S14_ERR_INVALID, "%s shares memory with the norm weight", labels[i]);
+    if (touch(outs[i], weight.ptr, 4ull * k)) return fail(S14_ERR_INVALID, "%s shares memory with the norm weight", labels[i]);
   }
   if (residual_out && y && s14::rows_share(bytes_of(residual_out, k), bytes_of(y, k), rows, false))
     return fail(S14_ERR_INVALID, "the residual output and y share memory");
   if (group) {
-    const s14::RowBytes made[2] = {codes(q, values), codes(scales, n_scales)};
-    const auto apart = [&](const s14::RowBytes &m, uintptr_t at, uint64_t bytes) { return m.at + m.row <= at || at + bytes <= m.at; };
-    bool fine = apart(made[0], made[1].at, made[1].row);
-    for (const s14::RowBytes &m : made) {
-      fine = fine && apart(m, reinterpret_cast<uintptr_t>(weight.ptr), 4ull * k);
+    const s14::RowBytes codes{reinterpret_cast<uintptr_t>(q.ptr), 0, 0, values, 1};
+    const s14::RowBytes byte_scales{reinterpret_cast<uintptr_t>(scales.ptr), 0, 0, n_scales, 1};
+    bool shared = s14::rows_touch(codes, byte_scales.at, n_scales, 1);
+    for (const s14::RowBytes &made : {codes, byte_scales}) {
+      shared |= s14::rows_touch(made, reinterpret_cast<uintptr_t>(weight.ptr), 4ull * k, 1);
       for (const s14_rows *r : {x, residual, residual_out, y})
-        if (r) fine = fine && apart(m, reinterpret_cast<uintptr_t>(r->buf.ptr), bytes_of(r, k).bytes(rows));
+        shared |= touch(r, reinterpret_cast<const void *>(made.at), made.row);
     }
-    if (!fine) return fail(S14_ERR_INVALID, "codes or scales share memory with another operand");
+    if (shared) return fail(S14_ERR_INVALID, "codes or scales share memory with another operand");
   }
   s14::AddNormArgs a{};
   a.rows = rows, a.k = k;

@@ -1,4 +1,4 @@
-// Do two packed [tokens][heads] operands share memory?  Plain C++ (no HIP
+// Do two packed [tokens][heads] operands, or one and a run of bytes, share memory?  Plain C++ (no HIP
 // types): the library and a host-only test include it.
 #pragma once
 
@@ -39,6 +39,14 @@ inline bool rows_share(const RowBytes &a, const RowBytes &b, uint32_t tokens, bo
     }
   }
   return false;
+}
+
+// Whether one of `tokens` >= 1 rows of a, which has one head, and the `bytes` from
+// address `from` have a byte in common.
+inline bool rows_touch(const RowBytes &a, uint64_t from, uint64_t bytes, uint32_t tokens) {
+  if (a.at + a.bytes(tokens) <= from || from + bytes <= a.at) return false;
+  const uint64_t t = from < a.at + a.row ? 0 : (from - a.at - a.row) / a.token + 1;  // the first that ends past it
+  return t < tokens && a.at + t * a.token < from + bytes;
 }
 
 }  // namespace s14

@@ -209,3 +209,19 @@ def test_python_norm_refusals(text, kw):
         A.add_rms_norm(CpuContext(), stream=0, **args)
     with pytest.raises(N.S14Error, match="context's device|required"):
         A.add_rms_norm(FakeContext(), stream=0, **args)
+
+
+@pytest.mark.parametrize("row", range(4))
+@pytest.mark.parametrize("which", ["ro", "y"])
+def test_norm_refuses_a_weight_in_any_row_of_an_output(native, which, row):
+    out = flat(at=FAR[7], stride=1024)
+    last = row * 4096 + 2048 - 16
+    refused(N.S14_ERR_INVALID, norm(native, **{which: out}, w=N.Buffer(FAR[7] + last, HUGE)), "norm weight")
+    refused(N.S14_ERR_INVALID, norm(native, **{which: out}, q=N.Buffer(FAR[7] + last, HUGE)), "codes or scales")
+
+
+@pytest.mark.parametrize("row", range(3))
+def test_norm_takes_a_weight_between_an_outputs_rows(native, row):
+    out = flat(at=FAR[7], stride=1024)
+    weight = N.Buffer(FAR[7] + row * 4096 + 2048, HUGE)
+    refused(N.S14_ERR_INVALID, norm(native, y=out, ro=out, w=weight), "the residual output and y share")
