@@ -460,6 +460,36 @@ def test_paged_without_cached_tokens_and_rows_that_see_nothing(ctx, heads, kv, d
 
 
 @pytest.mark.parametrize("heads,kv,dim,new", EVERY_TILE)
+def test_rows_behind_the_last_sequence_stay(ctx, heads, kv, dim, new):
+    """A padded batch: sequences without rows and packed rows of no sequence, on
+    another stream than the current one, over a page that two sequences share."""
+    say(f"paged4 padded heads={heads}/{kv} dim={dim} new={new}")
+    p = Paged4(dim + new, [40 + new, 70 + new, 33], kv, dim, 32)
+    p.table[1, 0] = p.table[0, 0]
+    p.upload()
+    counts, rows = [new, new, 0], 2 * new + 5
+    x, y = (rand(gen(i), rows, kv, dim).cuda() for i in (5, 6))
+    q = rand(gen(4), rows, heads, dim, dtype=BF16).cuda()
+    out, lse = torch.full((rows, heads, dim), 7.0, device="cuda"), torch.full((rows, heads), 7.0, device="cuda")
+    cu = ints([0, new, 2 * new, 2 * new])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    A.kv_append(ctx, p.cache, x, y, p.dev_table, cu, ints([40, 70, 33]), max_new=new, stream=stream.cuda_stream)
+    A.paged_attention(ctx, q, p.cache, p.dev_table, cu, p.lens, out, lse=lse, max_new=new, max_len=70 + new,
+                      stream=stream.cuda_stream)
+    stream.synchronize()
+    before = [t.clone() for t in (p.k, p.v, p.ks, p.vs)]
+    p.download()
+    new_pages = {int(p.table[i, j // 32]) for i, n in ((0, 40), (1, 70)) for j in range(n, n + new)}
+    kept = [i for i in range(p.cache.pages) if i not in new_pages]
+    for a, b in zip(before, (p.k, p.v, p.ks, p.vs)):
+        assert torch.equal(a[kept], b[kept])
+    assert bool((out[2 * new:] == 7.0).all()) and bool((lse[2 * new:] == 7.0).all())
+    check_attention(out[:2 * new], lse[:2 * new], paged_want(p, q[:2 * new], counts), "padded")
+    ctx.launch_status()
+
+
+@pytest.mark.parametrize("heads,kv,dim,new", EVERY_TILE)
 @pytest.mark.parametrize("page", [16, 128])
 @pytest.mark.parametrize("window", [0, 60])
 def test_paged_hidden_places_may_hold_anything(ctx, heads, kv, dim, new, page, window):
