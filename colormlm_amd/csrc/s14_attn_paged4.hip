@@ -48,10 +48,48 @@ __device__ __forceinline__ float clean_scale(uint32_t w, int i) {
 // so that the four tiles' scales of a lane are one word.
 __device__ __forceinline__ uint32_t scale_slot(uint32_t slot) { return (slot & ~15u) + 4 * (slot & 3u) + ((slot >> 2) & 3u); }
 
-// A weight times its token's value scale, 0 where the weight is 0 (the instruction's
-// own rule): a masked token's scale may be anything.
+// A value scale that is NaN.  A token that a row sees makes it NaN, however small its
+// weight is: else the order of the tokens and the cuts would decide whether the weight
+// was 0 when the scale came.  A masked token's scale may be anything.  Either its scale
+// is selected to 0 where a step has masked tokens (k_paged4 with one row tile, wide
+// heads), and the product is an ordinary one.  Or, where that takes registers that the
+// step has not (us, start / selects / this: 8 tokens of 40,000 21.0 / 22.5 / 21.2; 32
+// sequences of 8 of 4,000 54.2 / 61.8 / 54.8; but 16 of one token of up to 8,192, one
+// row tile, 24.7 / 24.8 / 25.9), the product is 0 where the weight is 0 (the
+// instruction's own rule), steps with a NaN among their scales are remembered, and
+// after the loop the rows look through those.
 extern "C" __device__ float s14_mul_zero(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
-__device__ __forceinline__ float weighted(float weight, float scale) { return s14_mul_zero(weight, scale); }
+template <bool kSelect>
+__device__ __forceinline__ float weighted(float weight, float scale) {
+  return kSelect ? weight * scale : s14_mul_zero(weight, scale);
+}
+
+// Bit c: of the tokens first .. last + 63 (steps of 64) one that the row sees has a NaN
+// scale of its 128 dimensions c.  By a whole wavefront, a token a lane.
+template <int B>
+__device__ uint32_t nan_parts(const PagedArgs &a, const Pages &pages, uint32_t head, int32_t first, int32_t last,
+                              const Visible &see) {
+  const uint32_t P = a.cache.page;
+  uint32_t hit = 0;
+  for (int32_t b = first; b <= last; b += 64) {
+    const int32_t tok = b + int32_t(threadIdx.x & 63u);
+    bool bad = false;  // (who loaded the step has said so)
+    const uint64_t at = uint64_t(pages.checked(pages.id(tok), bad)) * a.cache.heads + head;
+    for (int c = 0; c < B; ++c)
+      for (uint64_t m = __ballot(a.cache.vs[(at * B + c) * P + (uint32_t(tok) & (P - 1))] == 255); m; m &= m - 1)
+        if (see(b + __builtin_ctzll(m))) hit |= 1u << c;
+  }
+  return hit;
+}
+
+// The dimensions of `parts` of a row become NaN.
+template <int DT>
+__device__ __forceinline__ void spoil(f32x4 (&o)[DT], uint32_t parts) {
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[dt][i] = parts >> (dt / 8) & 1u ? __uint_as_float(0x7fc00000u) : o[dt][i];
+}
 
 // Scales above 0: a masked score times it stays -inf.
 __device__ __forceinline__ float score_scale(float scale) { return fmaxf(scale * kLog2e, 0x1p-126f); }
@@ -68,6 +106,7 @@ __global__ __launch_bounds__(256, D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2) void
   constexpr int H = D / 32;                  // words of K codes a lane holds of a token, products of a tile
   constexpr int B = D < 128 ? 1 : D / 128;   // key scales of those, and value scales of a token
   constexpr int U = D / 32, DT = D / 16;     // units of V a lane holds, 16-dimension tiles of O
+  constexpr bool kSelect = NT == 1;
   const uint32_t kvh = a.cache.heads, group = a.heads / kvh;
   const Item it = item_of(a, p, kvh);
   const uint32_t tile = it.tile, head = it.head, seq = it.seq, chunk = it.chunk;
@@ -147,6 +186,7 @@ __global__ __launch_bounds__(256, D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2) void
 #pragma unroll
     for (int u = 0; u < U; ++u) vv[u] = *reinterpret_cast<const uint4 *>(vp + u * P * 16);
   };
+  int32_t nan_first = INT_MAX, nan_last = -1;  // of the steps with a NaN value scale
   constexpr int32_t kStride = 4 * 16 * T;  // the wavefronts' steps interleave
   int32_t b = begin + 16 * T * int32_t(wave);
   const int32_t last = b + (end - 1 - b) / kStride * kStride;
@@ -193,6 +233,7 @@ __global__ __launch_bounds__(256, D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2) void
     load_k(next);
     const bool partial = b + 16 * T - 1 > pos_lo || (a.window && int64_t(b) <= int64_t(pos_hi) - a.window);
     bf16x8 pb[B][NT][T / 2];
+    uint32_t most = 0;  // the value scales' bits
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float x[4 * T], f[B][4 * T];
@@ -206,7 +247,14 @@ __global__ __launch_bounds__(256, D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2) void
       if (partial) {
         keep_branch();
 #pragma unroll
-        for (int i = 0; i < 4 * T; ++i) x[i] = see[nt](tv + i) ? x[i] : -INFINITY;
+        for (int i = 0; i < 4 * T; ++i) {
+          const bool in = see[nt](tv + i);
+          x[i] = in ? x[i] : -INFINITY;
+          if constexpr (kSelect) {
+#pragma unroll
+            for (int c = 0; c < B; ++c) f[c][i] = in ? f[c][i] : 0.0f;
+          }
+        }
       }
       float top = x[0];
 #pragma unroll
@@ -235,8 +283,12 @@ __global__ __launch_bounds__(256, D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2) void
 #pragma unroll
         for (int c = 0; c < B; ++c) {
           const float *v = &f[c][4 * t];
-          w[c][t / 2][2 * (t & 1)] = bf16_pair(weighted(e[0], v[0]), weighted(e[1], v[1]));
-          w[c][t / 2][2 * (t & 1) + 1] = bf16_pair(weighted(e[2], v[2]), weighted(e[3], v[3]));
+          if (!kSelect && nt == 0) {
+            most = max(most, max(__float_as_uint(v[0]), __float_as_uint(v[1])));
+            most = max(most, max(__float_as_uint(v[2]), __float_as_uint(v[3])));
+          }
+          w[c][t / 2][2 * (t & 1)] = bf16_pair(weighted<kSelect>(e[0], v[0]), weighted<kSelect>(e[1], v[1]));
+          w[c][t / 2][2 * (t & 1) + 1] = bf16_pair(weighted<kSelect>(e[2], v[2]), weighted<kSelect>(e[3], v[3]));
         }
       }
 #pragma unroll
@@ -257,8 +309,13 @@ __global__ __launch_bounds__(256, D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2) void
             o[nt][2 * u + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pb[u / 4][nt][h], o[nt][2 * u + d], 0, 0, 0);
         }
     }
+    if (!kSelect && __any(most > 0x7f800000u)) nan_first = min(nan_first, b), nan_last = b;
     load_v(next);
     idk = idk2, idv = idv2;
+  }
+  if (!kSelect && nan_last >= 0) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) spoil(o[nt], nan_parts<B>(a, pages, head, nan_first, nan_last, see[nt]));
   }
 
   // join the four wavefronts: 2 and 3 into 0 and 1, then 1 into 0
@@ -505,7 +562,12 @@ __global__ __launch_bounds__(256, 2) void k_paged4_wide(PagedArgs a, PagedPlan p
       for (int c = 0; c < C; ++c) {
         float w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = weighted(e[i], f[c][i]);
+        for (int i = 0; i < 4; ++i) w[i] = weighted<true>(e[i], f[c][i]);
+        if (partial) {
+          keep_branch();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = see[nt](tk + i) ? w[i] : 0.0f;
+        }
         // half a step of each weight: the matrix operand's type
         reinterpret_cast<uint2 *>(&s_p[c][nt][g / 2][16 * wave + n])[g & 1] =
             make_uint2(bf16_pair(w[0], w[1]), bf16_pair(w[2], w[3]));
@@ -638,7 +700,8 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 4 : RW == 2 
   __shared__ u32x4 s_rows[2 * kPieces];  // K, V
   __shared__ f32x4 s_vs[B * TK / 4];
   __shared__ uint32_t s_flags;
-  if (tid == 0) s_flags = 0;
+  __shared__ int32_t s_first, s_last;  // of the steps with a NaN value scale
+  if (tid == 0) s_flags = 0, s_first = INT_MAX, s_last = -1;
 
   f32x4 o[NT][DT] = {};
   float m[NT], sum[NT];
@@ -695,6 +758,7 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 4 : RW == 2 
       to[kPieces + dim * (TK / 8) + ((v_tok / 8 + w % 2) ^ turn_v<TK>(dim))] = __builtin_bit_cast(u32x4, e2m1_bf16(vv[w]));
     }
     if (tid < B * TK) reinterpret_cast<float *>(s_vs)[tid] = clean_scale(vsc, 0);
+    if (vsc == 255) atomicMin(&s_first, b), atomicMax(&s_last, b);
   };
   const uint32_t k_row = 8 * (n / 4) + n % 4, k_turn = turn_k<D>(k_row), v_turn = turn_v<TK>(n);
 
@@ -707,6 +771,7 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 4 : RW == 2 
   if (begin < end) {
     load(begin);
     if (begin + TK < end) load_ids(begin + TK);
+    __syncthreads();
     stage(begin, s_rows);
     if (begin + TK < end) load(begin + TK);
     if (begin + 2 * TK < end) load_ids(begin + 2 * TK);
@@ -764,7 +829,7 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 4 : RW == 2 
             const f32x4 f0 = s_vs[c * (TK / 4) + 8 * (u0 + u) + 2 * g], f1 = s_vs[c * (TK / 4) + 8 * (u0 + u) + 2 * g + 1];
             float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = weighted(e[j], j < 4 ? f0[j] : f1[j - 4]);
+            for (int j = 0; j < 8; ++j) y[j] = weighted<false>(e[j], j < 4 ? f0[j] : f1[j - 4]);
             u32x4 w;
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = bf16_pair(y[2 * j], y[2 * j + 1]);  // half a step of each weight: the matrix operand's type
@@ -799,6 +864,14 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 4 : RW == 2 
   if (bad) atomicOr(&s_flags, 1u);
   __syncthreads();
   const uint32_t flags = s_flags;
+  if (active && s_last >= 0) {
+    const int32_t first = __builtin_amdgcn_readfirstlane(s_first) & ~63, last = __builtin_amdgcn_readfirstlane(s_last);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const uint32_t r = mine + 16 * nt + lane % 16, rr = r < sp.rows ? r : sp.rows - 1;
+      spoil(o[nt], nan_parts<B>(a, pages, head, first, last, Visible(sp.pos0 + int32_t(rr / group), a.window)));
+    }
+  }
   if constexpr (TW == 2) {  // the token parts' sums: part 1 into 0, both taken from the larger maximum
     float *x = reinterpret_cast<float *>(s_rows) + (wave % RW) * (64 * NT * (4 * DT + 2));
     if (u0) {

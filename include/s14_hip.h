@@ -592,8 +592,8 @@ int s14_kv4_append(s14_ctx *ctx, void *stream, const s14_kv4_cache *cache, uint3
                    s14_buffer k_weight, float eps, const s14_rope *rope);
 
 /* s14_paged_attention over it, in all it says but: a NaN block of a value that a
- * row sees makes its 128 dimensions of the row NaN, unless its weight is 0 (a score
- * some 100 below the row's largest), one of a key the row; scales
+ * row sees makes its 128 dimensions of the row NaN, however small its weight is,
+ * one of a key the row; scales
  * are 27 to 227 or 255, which is what the append stores (a value scale's power of
  * two multiplies the weights before their rounding).  Blocks that no row sees may
  * hold anything. */

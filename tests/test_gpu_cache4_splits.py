@@ -1,0 +1,92 @@
+"""Attention over the paged 4-bit cache where the way its work is split could
+show: values that are NaN under weights too small for a number, chunks that the
+device sets by the sequences' lengths, and captured calls of those.  Against
+plain 64-bit implementations, with the tolerances of the cache's other tests."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import test_gpu_attention as T  # noqa: E402
+from test_gpu_attention import BF16, F32, U8, check_attention, gen, rand, run_paged, say  # noqa: E402
+from test_gpu_cache4 import Paged4, ctx  # noqa: E402, F401
+
+pytestmark = pytest.mark.gpu
+
+# ---------------------------------------------------------------------------
+# NaN values
+# ---------------------------------------------------------------------------
+
+# heads, key heads, head size, new tokens: every kernel, with one and two 16-row
+# tiles a wavefront or workgroup, and rows that share tokens
+TILES = [(4, 1, 64, 1), (4, 1, 64, 7), (8, 1, 64, 8), (8, 1, 64, 40), (4, 1, 128, 1), (4, 1, 128, 8), (8, 1, 128, 3),
+         (4, 1, 128, 12), (4, 1, 128, 30), (4, 1, 256, 2), (2, 1, 256, 11), (2, 1, 256, 32), (16, 1, 512, 1), (16, 1, 512, 2)]
+
+
+def loud_token(p, i, j, q):
+    """Key of position j of sequence i along q's signs, as far as E2M1 goes: its
+    scores pass every other key's by hundreds."""
+    page, slot = p.place(i, j)
+    codes = torch.where(q < 0, 15, 7).to(U8)
+    p.k[page, :, slot] = codes[0::2] | codes[1::2] << 4
+    p.set_scale(0, i, j, 127)
+
+
+@pytest.mark.parametrize("heads,kv,dim,new", TILES)
+@pytest.mark.parametrize("loud,nan", [(900, 40), (40, 900), (701, 700), (700, 701), (130, 70), (70, 130), (1990, 0), (2, 1930)])
+def test_nan_values_whatever_their_weight(ctx, heads, kv, dim, new, loud, nan):  # noqa: F811
+    """A row that sees a NaN block of a value has its dimensions NaN and no
+    others, though a key before, behind, in the same step or in another chunk
+    leaves it a weight of exp(-100) and less; a row that does not see it has none."""
+    say(f"paged4 NaN value at {nan}, loud key at {loud}, heads={heads}/{kv} dim={dim} new={new}")
+    g = gen(dim + new)
+    q = (rand(g, dim).sign() + 0.05 * rand(g, 2 * new, heads, dim)).to(BF16)
+    base = q.float().mean((0, 1))
+    p = Paged4(dim + new, [2000, 1000], kv, dim, 64, lo=123, hi=126)
+    loud_token(p, 0, loud, base)
+    last = (dim // 128 or 1) - 1
+    p.set_scale(1, 0, nan, 255, last)
+    p.upload()
+    scale = 64.0 / dim
+    window = 1900 if (loud, nan) == (1990, 0) else 0  # what lies before a window is not seen: no row has the NaN
+    k, v = p.rows(0)
+    s = (q[:new].double().flatten(0, 1) @ k[:, 0].T) * scale
+    assert bool((s[:, loud] - s[:, nan] > 100 + 2 * math.log(2) * 8).all())
+    want = [torch.cat(x) for x in zip(*(T.attention64(q[at:at + new], *p.rows(i), scale, window) for i, at in ((0, 0), (1, new))))]
+    seen = bool(want[0].isnan().any())
+    assert seen == (window == 0)
+    if seen:
+        assert bool(want[0][:new, :, -min(dim, 128):].isnan().all())
+    for max_len in (2000, 1, 1 << 20):
+        out, lse = run_paged(ctx, p, q.cuda(), [new, new], heads, dim, window, F32, max_len=max_len, scale=scale)
+        check_attention(out, lse, want, f"max_len {max_len}")
+    # one sequence: other kernels up to 32 rows
+    p.lens, p.dev_table = p.lens[:1], p.dev_table[:1].contiguous()
+    for max_len in (2000, 1):
+        out, lse = run_paged(ctx, p, q[:new].cuda(), [new], heads, dim, window, F32, max_len=max_len, scale=scale)
+        check_attention(out, lse, [x[:new] for x in want], f"alone, max_len {max_len}")
+    ctx.launch_status()
+
+
+@pytest.mark.parametrize("heads,kv,dim,new", TILES)
+@pytest.mark.parametrize("loud,nan", [(900, 40), (40, 900), (700, 701)])
+def test_nan_keys_whatever_the_other_scores(ctx, heads, kv, dim, new, loud, nan):  # noqa: F811
+    say(f"paged4 NaN key at {nan}, loud key at {loud}, heads={heads}/{kv} dim={dim} new={new}")
+    g = gen(dim + new)
+    q = (rand(g, dim).sign() + 0.05 * rand(g, 2 * new, heads, dim)).to(BF16)
+    p = Paged4(dim + new, [2000, 1000], kv, dim, 64, lo=123, hi=126)
+    loud_token(p, 0, loud, q.float().mean((0, 1)))
+    p.set_scale(0, 0, nan, 255, 0)
+    p.upload()
+    for max_len in (2000, 1):
+        out, lse = run_paged(ctx, p, q.cuda(), [new, new], heads, dim, 0, F32, max_len=max_len, scale=64.0 / dim)
+        assert bool(out[:new].isnan().all()) and bool(lse[:new].isnan().all())
+        assert bool(out[new:].isfinite().all()) and bool(lse[new:].isfinite().all())
+    p.lens, p.dev_table = p.lens[:1], p.dev_table[:1].contiguous()
+    out, lse = run_paged(ctx, p, q[:new].cuda(), [new], heads, dim, 0, F32, scale=64.0 / dim)
+    assert bool(out.isnan().all()) and bool(lse.isnan().all())
+    ctx.launch_status()
