@@ -23,9 +23,9 @@ struct PagedPlan {
   uint32_t chunks;     // of the longest sequence; above 1 the partial results go to the workspace
   uint32_t fused;      // the last workgroup of a row tile joins its chunks; else a second launch
   uint64_t blocks;     // workgroups
-  // Above 0: the chunk is set on the device, by what the sequences hold in all, so
-  // that `fill` workgroups a row tile and key head have it, `least` tokens at least
-  // each.  chunks is then the most that a sequence is cut into.
+  // Above 0: the chunk is set on the device, by what the sequences hold in all
+  // (balanced_steps), so that `fill` workgroups a row tile and key head have it.
+  // chunks is then the most that a sequence is cut into.
   uint32_t fill, least;
 };
 constexpr uint64_t kPagedPartFloats = 16ull << 20;  // the workspace: 64 MiB
@@ -47,6 +47,20 @@ constexpr PagedCut paged_cut(uint32_t span, uint32_t chunk, uint32_t chunks) {
 // and the chunk are.
 constexpr int32_t paged_end(int32_t begin, int32_t hi, uint32_t chunk) {
   return uint32_t(hi - begin) > chunk ? begin + int32_t(chunk) : hi;
+}
+
+// The steps of 64 tokens of a chunk where the sequences hold `total` of them: as many
+// as give `fill` workgroups one chunk each, and at least `least`.  Where there are fewer
+// steps than workgroups, least * sqrt(total / fill) to the nearest at least: chunks of c
+// steps take c of a step's time and total / c of a partial result's, and the least sum
+// of the two goes with the root of total.
+constexpr uint32_t balanced_steps(uint64_t total, uint32_t fill, uint32_t least) {
+  constexpr uint32_t kMost = 1u << 24;  // 2^30 tokens
+  if (total >> 31) return kMost;
+  const uint32_t each = (uint32_t(total) + fill - 1) / fill;
+  uint32_t c = 1;
+  while (c < least && (2 * c + 1) * (2 * c + 1) * uint64_t(fill) < 4ull * least * least * total) ++c;
+  return c > each ? c : each < kMost ? each : kMost;
 }
 
 // Rows of a workgroup: all of the longest new block's up to 64 (of 32 of
@@ -83,7 +97,12 @@ constexpr int32_t paged_end(int32_t begin, int32_t hi, uint32_t chunk) {
 // max_len / so: 8 of 64 new of 3,000 57 / 51; 2 of 256 of 4,000 71 / 61; 3 of 200 of
 // up to 6,000 94 / 88; 64 of 1 of 4,000, heads of 512, 79 / 65; 4 of 4 of up to 9,000
 // 33.7 / 34.8).  With smaller results the sum of the lengths costs more than it saves
-// (20 of 2 of up to 9,000, heads of 64: 18 / 21).
+// (20 of 2 of up to 9,000, heads of 64: 18 / 21).  At heads of 512 small chunks are
+// balanced too, with 256 tokens at least, whose codes are as many bytes as the partial
+// result (us, by max_len, chunks of 64 to 128 / at least 192 / 256 / 320: 8 of 1 of 2,048
+// 26.9 / 23.0 / 22.6 / 23.9; 7 of 1 of 4,096 39.8 / 27.8 / 24.9 / 25.9; 31 of 1 of 1,000
+// 42.0 / 27.0 / 24.2 / 25.1), and less where the card is not full (2 of 1 of 1,000:
+// chunks of 64 14.0, of 256 16.9).
 inline PagedPlan paged_plan(const PagedShape &a) {
   PagedPlan p{};
   const uint64_t rows = uint64_t(a.max_new) * (a.heads / a.kv_heads);
@@ -120,9 +139,9 @@ inline PagedPlan paged_plan(const PagedShape &a) {
   p.chunk = uint32_t(((span + chunks - 1) / chunks + least - 1) / least * least);
   p.chunks = uint32_t((span + p.chunk - 1) / p.chunk);
   p.blocks = base * p.chunks;
-  if (balance && p.chunks > 1 && p.chunk > least) {
+  if (balance && p.chunks > 1 && (dim == 512 || p.chunk > least)) {
     p.fill = uint32_t((slots + tiles * a.kv_heads - 1) / (tiles * a.kv_heads));
-    p.least = dim == 512 ? 320 : uint32_t(least);
+    p.least = dim == 512 ? 256 : uint32_t(least);
   }
   return p;
 }

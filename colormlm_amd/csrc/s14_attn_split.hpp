@@ -43,9 +43,7 @@ __device__ __forceinline__ uint32_t balanced_chunk(const PagedArgs &a, const Pag
     if (hi > lo) steps += uint32_t((hi - (lo & ~63ll) + 63) >> 6);
   }
   const uint64_t total = (uint64_t(wave_sum_u32(steps >> 16)) << 16) + wave_sum_u32(steps & 0xffffu);
-  const uint32_t most = 1u << 24;  // 2^30 tokens
-  const uint32_t each = total >> 31 ? most : (uint32_t(total) + p.fill - 1) / p.fill;
-  return 64 * max(p.least / 64, min(each, most));
+  return 64 * balanced_steps(total, p.fill, p.least / 64);
 }
 
 __device__ __forceinline__ Span paged_span(const PagedArgs &a, const PagedPlan &p, uint32_t seq, uint32_t row0, uint32_t planned) {

@@ -12,8 +12,11 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import test_gpu_attention as T  # noqa: E402
+from test_attention_balance import BALANCED  # noqa: E402
 from test_gpu_attention import BF16, F32, U8, check_attention, gen, rand, run_paged, say  # noqa: E402
 from test_gpu_cache4 import Paged4, ctx  # noqa: E402, F401
+
+from colormlm_amd import attention as A  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -89,4 +92,95 @@ def test_nan_keys_whatever_the_other_scores(ctx, heads, kv, dim, new, loud, nan)
     p.lens, p.dev_table = p.lens[:1], p.dev_table[:1].contiguous()
     out, lse = run_paged(ctx, p, q[:new].cuda(), [new], heads, dim, 0, F32, scale=64.0 / dim)
     assert bool(out.isnan().all()) and bool(lse.isnan().all())
+    ctx.launch_status()
+
+
+# ---------------------------------------------------------------------------
+# chunks by the lengths
+# ---------------------------------------------------------------------------
+
+
+def ragged(seed, seqs, new, most):
+    """Lengths with one past the promise, empty sequences, and short ones."""
+    g = gen(seed)
+    lengths = [int(x) for x in torch.randint(new, max(new + 1, most // 4), (seqs,), generator=g)]
+    lengths[0], lengths[-1] = most + 700, most
+    if seqs > 2:
+        lengths[1] = 0
+    return lengths
+
+
+def check_some(p, q, out, lse, counts, window, what):
+    """First and last rows of the first, the last and two other sequences, all heads' first and last."""
+    at, seqs = [0], len(counts)
+    for n in counts:
+        at.append(at[-1] + n)
+    for i in {0, 1, seqs // 2, seqs - 1}:
+        if not counts[i]:
+            continue
+        k, v = p.rows(i)
+        heads = q.shape[1]
+        for row in {0, counts[i] - 1}:
+            end = len(k) - counts[i] + row + 1
+            kv = k.shape[1]
+            group = heads // kv
+            pick = [0, heads - 1]
+            t = at[i] + row
+            parts = [T.attention64(q[t:t + 1, h:h + 1].cpu(), k[:max(end, 0), h // group:h // group + 1], v[:max(end, 0), h // group:h // group + 1],
+                                   q.shape[-1] ** -0.5, window) for h in pick]
+            want = [torch.cat(x, 1) for x in zip(*parts)]
+            check_attention(out[t:t + 1, pick], lse[t:t + 1, pick], want, f"{what}, sequence {i} row {row}")
+
+
+@pytest.mark.parametrize("seqs,heads,kv,dim,new,most", BALANCED)
+@pytest.mark.parametrize("window", [0, 900])
+def test_balanced_launches(ctx, seqs, heads, kv, dim, new, most, window):  # noqa: F811
+    """Chunks by what the sequences hold in all, one sequence longer than promised,
+    one without tokens and one without rows; and, one sequence more than the lengths
+    are added up of, by the promise."""
+    say(f"paged4 balanced: {seqs} sequences heads={heads}/{kv} dim={dim} new={new} window={window}")
+    for more in ((0, 1) if seqs == 256 else (0,)):
+        lengths = ragged(seqs, seqs + more, new, most)
+        counts = [new] * (seqs + more)
+        counts[seqs // 2] = 0
+        p = Paged4(seqs, lengths, kv, dim, 64)
+        q = rand(gen(4), sum(counts), heads, dim, dtype=BF16).cuda()
+        out, lse = run_paged(ctx, p, q, counts, heads, dim, window, F32, max_len=most)
+        again, _ = run_paged(ctx, p, q, counts, heads, dim, window, F32, max_len=most)
+        assert torch.equal(out, again)
+        check_some(p, q, out, lse, counts, window, "balanced")
+    ctx.launch_status()
+
+
+@pytest.mark.parametrize("seqs,heads,kv,dim,new,most", BALANCED)
+def test_balanced_launches_captured_and_replayed(ctx, seqs, heads, kv, dim, new, most):  # noqa: F811
+    """A captured launch, replayed with other lengths: the chunk, which the join takes
+    from the workspace, is another one each time.  Eager launches of the same context
+    lie between the replays; each replay equals an eager call bit for bit."""
+    say(f"paged4 balanced and captured: {seqs} sequences heads={heads}/{kv} dim={dim} new={new}")
+    counts = [new] * seqs
+    full = [most] * seqs
+    p = Paged4(seqs, full, kv, dim, 64)
+    q = rand(gen(4), sum(counts), heads, dim, dtype=BF16).cuda()
+    out, lse = torch.zeros(q.shape, device="cuda"), torch.zeros(q.shape[:2], device="cuda")
+    cu = T.cumulative(counts)
+    call = lambda o, l: A.paged_attention(ctx, q, p.cache, p.dev_table, cu, p.lens, o, lse=l, max_new=new, max_len=most)  # noqa: E731
+    call(out, lse)
+    torch.cuda.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        call(out, lse)
+    rows = p.rows
+    for step, lengths in enumerate((full, [new] * seqs, ragged(3, seqs, new, most - 700), [max(new, most // 8)] * seqs, full)):
+        p.lens.copy_(torch.tensor(lengths, dtype=torch.int32))
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager, eager_lse = torch.zeros_like(out), torch.zeros_like(lse)
+        call(eager, eager_lse)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager) and torch.equal(lse, eager_lse), step
+        p.rows = lambda i: rows(i, lengths[i])  # noqa: B023
+        check_some(p, q, out, lse, counts, 0, f"replay {step}")
     ctx.launch_status()
