@@ -97,7 +97,9 @@ constexpr uint32_t balanced_steps(uint64_t total, uint32_t fill, uint32_t least)
 // max_len / so: 8 of 64 new of 3,000 57 / 51; 2 of 256 of 4,000 71 / 61; 3 of 200 of
 // up to 6,000 94 / 88; 64 of 1 of 4,000, heads of 512, 79 / 65; 4 of 4 of up to 9,000
 // 33.7 / 34.8).  With smaller results the sum of the lengths costs more than it saves
-// (20 of 2 of up to 9,000, heads of 64: 18 / 21).  At heads of 512 small chunks are
+// (20 of 2 of up to 9,000, heads of 64: 18 / 21), and with 64 rows of heads of 256 it
+// decides nothing (16 of 16 of 4,096 35.4 / 35.5, 8 of 64 of 3,000 45.0 / 45.0, 32 of 16
+// of up to 4,000 46.8 / 46.2, 16 of 16 of 8,192 52.0 / 52.6).  At heads of 512 small chunks are
 // balanced too, with 256 tokens at least, whose codes are as many bytes as the partial
 // result (us, by max_len, chunks of 64 to 128 / at least 192 / 256 / 320: 8 of 1 of 2,048
 // 26.9 / 23.0 / 22.6 / 23.9; 7 of 1 of 4,096 39.8 / 27.8 / 24.9 / 25.9; 31 of 1 of 1,000
@@ -129,7 +131,7 @@ inline PagedPlan paged_plan(const PagedShape &a) {
   p.rec_rows = uint32_t(rows < 16 * p.row_tiles ? rows : 16 * p.row_tiles);
   const uint64_t rec = uint64_t(p.rec_rows) * (dim + 4);
   uint64_t chunks = base < slots ? slots * (a.seqs > 1 ? 2 : 1) / base : (span + kMost - 1) / kMost;
-  const bool balance = a.four && a.seqs > 1 && a.seqs <= kMostBalanced && base < slots && rec * 4 >= kFuse;
+  const bool balance = a.four && a.seqs > 1 && a.seqs <= kMostBalanced && base < slots && rec * 4 >= kFuse && dim != 256;
   const uint64_t fit = (kPagedPartFloats - (a.four ? 4 : 0)) / (rec * base);
   if (chunks > fit) chunks = fit;
   if (chunks > (span + least - 1) / least) chunks = (span + least - 1) / least;

@@ -59,6 +59,13 @@ def test_balanced_launches(lib, seqs, heads, kv, dim, new, most):  # noqa: F811
     assert not plan(lib, 257, heads, kv, dim, new, most).fill
 
 
+@pytest.mark.parametrize("heads,kv,dim,balances", [(64, 1, 512, True), (16, 8, 128, True), (8, 2, 256, False), (8, 8, 64, False)])
+def test_which_heads_balance(lib, heads, kv, dim, balances):  # noqa: F811
+    found = any(plan(lib, seqs, heads, kv, dim, new, most).fill for seqs in (2, 8, 30, 100, 256) for new in (1, 16, 64, 200)
+                for most in (500, 3000, 70000, REACH))
+    assert found == balances
+
+
 @pytest.mark.parametrize("heads", [32, 64, 128])
 def test_chunks_do_not_jump_with_the_lengths(lib, steps, heads):  # noqa: F811
     """Heads of 512, one token each: a step more of every sequence makes a chunk a
