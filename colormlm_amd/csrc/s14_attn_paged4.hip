@@ -111,7 +111,7 @@ __global__ __launch_bounds__(256, D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2) void
   const Item it = item_of(a, p, kvh);
   const uint32_t tile = it.tile, head = it.head, seq = it.seq, chunk = it.chunk;
   const uint32_t row0 = tile * 16 * NT;
-  const Span sp = balanced_span(a, p, seq, row0, part);
+  const Span sp = paged_span(a, p, seq, row0);
   if (row0 >= sp.rows || (chunk && chunk >= sp.chunks)) return;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page;
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(256, 2) void k_paged4_wide(PagedArgs a, PagedPlan p
   const Item it = item_of(a, p, kvh);
   const uint32_t tile = it.tile, head = it.head, seq = it.seq, chunk = it.chunk;
   const uint32_t row0 = tile * 16 * NT;
-  const Span sp = balanced_span(a, p, seq, row0, part);
+  const Span sp = balanced_span<paged_balances(D, NT)>(a, p, seq, row0, part);
   if (row0 >= sp.rows || (chunk && chunk >= sp.chunks)) return;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page, d0 = 128 * wave;
@@ -669,7 +669,7 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 4 : RW == 2 
   const Item it = item_of(a, p, kvh);
   const uint32_t tile = it.tile, head = it.head, seq = it.seq, chunk = it.chunk;
   const uint32_t row0 = tile * 16 * NT * RW;
-  const Span sp = balanced_span(a, p, seq, row0, part);
+  const Span sp = balanced_span<paged_balances(D, NT * RW)>(a, p, seq, row0, part);
   if (row0 >= sp.rows || (chunk && chunk >= sp.chunks)) return;
   const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), l = tid & 63u, n = l & 15u, g = l >> 4;
   const uint32_t P = a.cache.page;
@@ -925,16 +925,16 @@ __global__ __launch_bounds__(256, D * NT > 128 ? 2 : D * NT < 128 ? 4 : RW == 2 
 template <int D>
 hipError_t launch_dim(hipStream_t s, const PagedArgs &a, const PagedPlan &p, float *part) {
   if constexpr (D == 512) {
-    if (p.row_tiles == 2) return launch<D, true>(s, a, p, part, k_paged4_wide<2>);
-    return launch<D, true>(s, a, p, part, k_paged4_wide<1>);
+    if (p.row_tiles == 2) return launch<D, paged_balances(D, 2)>(s, a, p, part, k_paged4_wide<2>);
+    return launch<D>(s, a, p, part, k_paged4_wide<1>);
   } else {
     if constexpr (D <= 128) {
-      if (p.row_tiles == 8) return launch<D, true>(s, a, p, part, k_paged4_rows<D, 2, 4>);
-      if (p.row_tiles == 2 && p.staged) return launch<D, true>(s, a, p, part, k_paged4_rows<D, 1, 2>);
-      if (p.row_tiles == 2) return launch<D, true>(s, a, p, part, k_paged4<D, 2>);
+      if (p.row_tiles == 8) return launch<D, paged_balances(D, 8)>(s, a, p, part, k_paged4_rows<D, 2, 4>);
+      if (p.row_tiles == 2 && p.staged) return launch<D>(s, a, p, part, k_paged4_rows<D, 1, 2>);
+      if (p.row_tiles == 2) return launch<D>(s, a, p, part, k_paged4<D, 2>);
     }
-    if (p.row_tiles == 4) return launch<D, true>(s, a, p, part, k_paged4_rows<D, 1, 4>);
-    return launch<D, true>(s, a, p, part, k_paged4<D, 1>);
+    if (p.row_tiles == 4) return launch<D>(s, a, p, part, k_paged4_rows<D, 1, 4>);
+    return launch<D>(s, a, p, part, k_paged4<D, 1>);
   }
 }
 

@@ -49,6 +49,13 @@ constexpr int32_t paged_end(int32_t begin, int32_t hi, uint32_t chunk) {
   return uint32_t(hi - begin) > chunk ? begin + int32_t(chunk) : hi;
 }
 
+// Whether a workgroup of so many row tiles may have chunks that balance: the kernels
+// of the others are compiled without.
+constexpr uint32_t kBalancedBytes = 64 * 1024;  // of a chunk's partial result
+constexpr bool paged_balances(uint32_t dim, uint32_t row_tiles) {
+  return dim != 256 && 16 * row_tiles * (dim + 4) * 4 >= kBalancedBytes;
+}
+
 // The steps of 64 tokens of a chunk where the sequences hold `total` of them: as many
 // as give `fill` workgroups one chunk each, and at least `least`.  Where there are fewer
 // steps than workgroups, least * sqrt(total / fill) to the nearest at least: chunks of c
@@ -131,7 +138,8 @@ inline PagedPlan paged_plan(const PagedShape &a) {
   p.rec_rows = uint32_t(rows < 16 * p.row_tiles ? rows : 16 * p.row_tiles);
   const uint64_t rec = uint64_t(p.rec_rows) * (dim + 4);
   uint64_t chunks = base < slots ? slots * (a.seqs > 1 ? 2 : 1) / base : (span + kMost - 1) / kMost;
-  const bool balance = a.four && a.seqs > 1 && a.seqs <= kMostBalanced && base < slots && rec * 4 >= kFuse && dim != 256;
+  const bool balance = a.four && a.seqs > 1 && a.seqs <= kMostBalanced && base < slots && rec * 4 >= kBalancedBytes &&
+                       paged_balances(dim, p.row_tiles);
   const uint64_t fit = (kPagedPartFloats - (a.four ? 4 : 0)) / (rec * base);
   if (chunks > fit) chunks = fit;
   if (chunks > (span + least - 1) / least) chunks = (span + least - 1) / least;

@@ -74,12 +74,13 @@ __device__ __forceinline__ Span paged_span(const PagedArgs &a, const PagedPlan &
   return paged_span(a, p, seq, row0, p.chunk);
 }
 
-// The same with a plan that may balance.  The joining launch takes the chunk from
-// the end of the workspace.
+// The same of a kernel whose plans may balance (paged_balances).  The joining launch
+// takes the chunk from the end of the workspace.
 __device__ __forceinline__ uint32_t *chunk_word(float *part) { return reinterpret_cast<uint32_t *>(part + kPagedPartFloats - 4); }
+template <bool kBalanced>
 __device__ __forceinline__ Span balanced_span(const PagedArgs &a, const PagedPlan &p, uint32_t seq, uint32_t row0, float *part) {
   uint32_t planned = p.chunk;
-  if (p.fill) {
+  if (kBalanced && p.fill) {
     planned = balanced_chunk(a, p);
     if (blockIdx.x == 0 && threadIdx.x == 0) *chunk_word(part) = planned;
   }

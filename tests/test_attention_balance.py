@@ -28,8 +28,10 @@ def steps(tmp_path_factory):
          str(ROOT / "tests" / "native" / "attention_balance_check.cpp"), "-o", str(out)],
         check=True,
     )
-    f = C.CDLL(str(out)).attn_balanced
+    host = C.CDLL(str(out))
+    f = host.attn_balanced
     f.argtypes, f.restype = (C.c_uint64, C.c_uint32, C.c_uint32), C.c_uint32
+    f.may = host.attn_may_balance
     return f
 
 
@@ -64,6 +66,24 @@ def test_which_heads_balance(lib, heads, kv, dim, balances):  # noqa: F811
     found = any(plan(lib, seqs, heads, kv, dim, new, most).fill for seqs in (2, 8, 30, 100, 256) for new in (1, 16, 64, 200)
                 for most in (500, 3000, 70000, REACH))
     assert found == balances
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(64, 1, 512), (9, 1, 512), (16, 8, 128), (125, 1, 128), (31, 1, 128), (8, 2, 256), (8, 8, 64)])
+def test_plans_balance_only_for_kernels_that_do(lib, steps, heads, kv, dim):  # noqa: F811
+    """A plan with a chunk of the device's for a kernel that was compiled without would
+    be joined by another chunk than the one it ran by; a kernel that was compiled with
+    has plans that use it."""
+    used, may = set(), set()
+    for seqs in (2, 3, 8, 30, 100, 256):
+        for new in range(1, 300, 3 if dim < 512 else 1):
+            for most in (500, 3000, 70000, REACH):
+                p = plan(lib, seqs, heads, kv, dim, new, most)
+                if steps.may(dim, p.row_tiles):
+                    may.add(p.row_tiles)
+                if p.fill:
+                    used.add(p.row_tiles)
+                    assert steps.may(dim, p.row_tiles), (seqs, new, most)
+    assert used == may
 
 
 @pytest.mark.parametrize("heads", [32, 64, 128])
