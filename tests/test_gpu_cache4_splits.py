@@ -14,7 +14,7 @@ torch = pytest.importorskip("torch")
 import test_gpu_attention as T  # noqa: E402
 from test_attention_balance import BALANCED  # noqa: E402
 from test_gpu_attention import BF16, F32, U8, check_attention, gen, rand, run_paged, say  # noqa: E402
-from test_gpu_cache4 import Paged4, ctx  # noqa: E402, F401
+from test_gpu_cache4 import Layer, Paged4, ctx  # noqa: E402, F401
 
 from colormlm_amd import attention as A  # noqa: E402
 
@@ -183,4 +183,37 @@ def test_balanced_launches_captured_and_replayed(ctx, seqs, heads, kv, dim, new,
         assert torch.equal(out, eager) and torch.equal(lse, eager_lse), step
         p.rows = lambda i: rows(i, lengths[i])  # noqa: B023
         check_some(p, q, out, lse, counts, 0, f"replay {step}")
+    ctx.launch_status()
+
+
+def test_layer_replays_leave_the_same_cache(ctx):  # noqa: F811
+    """A captured layer step replayed from step to step against an eager one: every
+    byte of the cache, key scales too, as the tokens cross blocks of slots and pages."""
+    say("graph capture of a layer's step, all of the cache's bytes")
+    g = gen(23)
+    L, E = Layer(ctx, 2), Layer(ctx, 2)
+    x, cu = torch.empty(2, L.hidden, device="cuda"), T.cumulative([1, 1])
+    past, lens, pos = (T.ints([0, 0]) for _ in range(3))
+    tensors = lambda c: (c.k_pages, c.v_pages, c.k_scales, c.v_scales)  # noqa: E731
+    for a, b in zip(tensors(L.cache), tensors(E.cache)):
+        a.copy_(torch.randint(0, 120, a.shape, generator=g, dtype=U8))
+        b.copy_(a)
+    x.copy_(rand(g, 2, L.hidden))
+    L.step(x, cu, past, T.ints([1, 1]), pos, 1)  # warm
+    E.step(x, cu, past, T.ints([1, 1]), pos, 1)
+    torch.cuda.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        L.step(x, cu, past, lens, pos, 1)
+    for step, at in enumerate(([1, 1], [63, 2], [64, 150], [197, 65], [198, 66])):
+        x.copy_(rand(g, 2, L.hidden))
+        for t, v in ((past, at), (lens, [n + 1 for n in at]), (pos, at)):
+            t.copy_(torch.tensor(v, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        E.step(x, cu, past, lens, pos, 1)
+        torch.cuda.synchronize()
+        for a, b in zip((L.out, L.y2, L.h, *tensors(L.cache)), (E.out, E.y2, E.h, *tensors(E.cache))):
+            assert torch.equal(a, b), step
     ctx.launch_status()
