@@ -6,9 +6,12 @@
 // and end at 6.  A token's scales are its own: nothing that was stored before is
 // touched, so the unit of work is a block of kSlots neighbouring slots of a page
 // (16, the slots of a unit of V codes, or 4 where few tokens are new), head and
-// side, of D / 8 lanes a slot.  Bound by the bytes moved (21 prompts of up to 4,000
-// tokens, 8 heads of 128: 78 MB in 22.2 us, 3.5 TB/s), for a few tokens by the chain
-// of loads, counts, then the page's id and the rows (96 single ones: 4.3 us).
+// side, of D / 8 lanes a slot.  21 prompts of up to 4,000 tokens, 8 heads of 128: 78 MB
+// in 22.4 us, 3.5 TB/s, a third over what the bytes take: a workgroup of some 32 B a
+// thread starts with a chain of its own, the search for its sequence (64 counts and six
+// LDS permutes), the page's id, then the rows, and the card takes several rounds of
+// them.  With the keys' norm and rotation 30.4 (f32 rows 39.1).  For a few tokens that
+// chain is all (96 single ones: 4.3 us).
 #include "s14_attn_rows.hpp"
 
 namespace s14 {
@@ -193,7 +196,8 @@ __device__ __forceinline__ void store_values(const AppendArgs &a, const Block &b
 template <int kDim, int kSlots, bool kBoth, bool kTurn, bool kK16, bool kV16>
 __device__ __forceinline__ void append_block(const AppendArgs &a, const Touched &t, uint32_t head, uint32_t side) {
   const Block b = block_of<kSlots>(a, t, head);
-  // (the page's id is in flight with the rows)
+  // (the id is a scalar load that the compiler waits for here, and it has sunk the rows'
+  // loads behind: a trip to memory each)
   const auto good = [&] {
     if (b.id >= 0 && b.id < int64_t(a.cache.pages)) return true;
     if (threadIdx.x == 0) atomicOr(a.status, kStatusBadCachePage);
@@ -214,7 +218,7 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, const Touched 
   }
 }
 
-// kBoth: keys and values by one workgroup, which has twice the bytes in flight.
+// kBoth: keys and values by one workgroup, which looks for its sequence and page once.
 // kTurn: K takes a norm or a rotation on the way.
 template <int kDim, int kSlots, bool kBoth, bool kTurn>
 __global__ __launch_bounds__(kSlots * kDim / 8 < 64 ? 64 : kSlots * kDim / 8) void k_kv_append4(AppendArgs a, uint32_t direct) {

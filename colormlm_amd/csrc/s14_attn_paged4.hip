@@ -653,7 +653,7 @@ __device__ __forceinline__ uint32_t turn_v(uint32_t dim) {
 // from LDS, where the workgroup has put them as bf16, the keys with their scales,
 // once for all its rows; the values' scales lie beside them.  A step of 128 rows takes
 // 1.2 us a compute unit (880 TFLOP/s of a running one); what 8 sequences of 64 new of
-// 3,000 tokens take beyond that, 51 us in all, is the start, and 35 MB of partial
+// 3,000 tokens take beyond that, 52 us in all, is the start, and 35 MB of partial
 // results written and read.  Tried without gain there: a step's products between the
 // next one's weights with two buffers (58 us), eight wavefronts that halve the partial
 // results (59), 64 rows a workgroup (54).

@@ -81,7 +81,7 @@ constexpr uint32_t balanced_steps(uint64_t total, uint32_t fill, uint32_t least)
 // up to 51,525 40 / 30, 38 of up to 422, window 161, 18 / 12).
 //
 // Chunks.  Where the launch alone would leave compute units idle: as many
-// workgroups as the card holds at once (a second round for a few of them costs
+// workgroups as the card holds at once (counted as below; a second round for a few of them costs
 // as much as the first), of several sequences twice as many, since their
 // lengths differ and short ones leave chunks empty (us, once / twice: 16
 // sequences of up to 8,192 tokens 36 / 29 ragged, 55 / 55 equal; 4 of up to
@@ -128,7 +128,12 @@ inline PagedPlan paged_plan(const PagedShape &a) {
   uint64_t span = a.max_len < a.reach ? a.max_len : a.reach;
   if (!span) span = 1;  // a chunk is never of no tokens: the kernels divide by it
   if (a.window && uint64_t(a.window) + a.max_new + 63 < span) span = uint64_t(a.window) + a.max_new + 63;
-  // workgroups that the card holds at once, by a wavefront's registers and by LDS
+  // workgroups that the card holds at once, by the registers of a wavefront of the 8-bit
+  // cache's kernels and by LDS.  The 4-bit cache's have fewer registers, and one to a
+  // compute unit more would fit with most, but more chunks take longer there (us, by
+  // these / by all that fit: one sequence of 8 of 40,000 20.5 / 23.4, of 1 19.1 / 20.3; 16
+  // of 1 of up to 8,192 24.9 / 27.9, heads of 256 20.9 / 27.3; 96 of 1 of 2,048, 2 key
+  // heads, 20.9 / 24.6; the others of 63 shapes within 4 %)
   const uint32_t words = (dim == 512 ? 128 : dim) * p.row_tiles;
   const uint64_t per_cu = p.staged ? (dim == 256 ? 2 : (dim == 64 ? 4 : 3) - p.row_tiles / 8)
                                    : (words <= 64 ? 3 : words <= 128 || dim == 512 ? 2 : 1);

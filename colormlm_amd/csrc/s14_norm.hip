@@ -1,8 +1,10 @@
 // Residual addition, root-mean-square norm of the rows, and their E4M3 codes with
 // E8M0 scales, in one pass: a row stays in its threads' registers between the sum
-// of its squares and what is written.  Bound by the bytes moved (16,384 rows of 4,096,
-// f32 with a bf16 residual: 604 MB in 104 us, 5.8 TB/s); for a few rows by the launch
-// and two trips to memory, the row with its weight and the stores (one row: 3.4 us).
+// of its squares and what is written, but for rows of more than 32,768 values, of which
+// 43 to 70 registers a thread go to scratch memory and back.  Bound by the bytes
+// moved (16,384 rows of 4,096, f32 with a bf16 residual: 604 MB in 105 us, 5.8 TB/s);
+// for a few rows by the launch and two trips to memory, the row with its weight and
+// the stores (one row: 3.5 us).
 #include "s14_attn_rows.hpp"
 
 namespace s14 {
@@ -130,7 +132,9 @@ hipError_t add_norm(hipStream_t s, const AddNormArgs &a, uint32_t threads) {
 
 // As few values a thread as a workgroup's threads allow (us of 1 and of 16,384 rows of
 // 4,096 values: eight 3.6 and 152, sixteen 4.4 and 159, a wavefront a row 10.8 and 230;
-// 1 and 8,192 of 8,192: eight 4.2 and 167, sixteen 4.5 and 162).
+// 1 and 8,192 of 8,192: eight 4.2 and 167, sixteen 4.5 and 162).  2,048 rows, f32 with a
+// bf16 residual: of 16,384 values 61 us (5.0 TB/s), of 32,768 139 (4.4), with the spills
+// of 40,960 311 (2.4) and of 65,536 426 (2.8); one row of 65,536 27 us.
 hipError_t launch_add_norm(hipStream_t s, const AddNormArgs &a) {
   const uint32_t octets = a.k / 8;
   const auto threads = [&](uint32_t v) { return ((octets + v - 1) / v + 63) / 64 * 64; };

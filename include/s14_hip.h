@@ -596,7 +596,8 @@ int s14_kv4_append(s14_ctx *ctx, void *stream, const s14_kv4_cache *cache, uint3
  * one of a key the row; scales
  * are 27 to 227 or 255, which is what the append stores (a value scale's power of
  * two multiplies the weights before their rounding).  Blocks that no row sees may
- * hold anything. */
+ * hold anything.  The lengths set how the work is split too, so that a row's last
+ * bits depend on the call's other sequences. */
 int s14_paged4_attention(s14_ctx *ctx, void *stream, const s14_rows *q, const s14_kv4_cache *cache,
                          uint32_t tokens, uint32_t seqs, uint32_t max_new, uint32_t max_len,
                          s14_buffer page_table, uint32_t table_width, s14_buffer cu, s14_buffer lens,
