@@ -111,7 +111,7 @@ constexpr uint32_t balanced_steps(uint64_t total, uint32_t fill, uint32_t least)
 // result (us, by max_len, chunks of 64 to 128 / at least 192 / 256 / 320: 8 of 1 of 2,048
 // 26.9 / 23.0 / 22.6 / 23.9; 7 of 1 of 4,096 39.8 / 27.8 / 24.9 / 25.9; 31 of 1 of 1,000
 // 42.0 / 27.0 / 24.2 / 25.1), and less where the card is not full (2 of 1 of 1,000:
-// chunks of 64 14.0, of 256 16.9).
+// chunks of 64 14.0, the same balanced 14.7, of 256 16.9).
 inline PagedPlan paged_plan(const PagedShape &a) {
   PagedPlan p{};
   const uint64_t rows = uint64_t(a.max_new) * (a.heads / a.kv_heads);
@@ -154,9 +154,12 @@ inline PagedPlan paged_plan(const PagedShape &a) {
   p.chunk = uint32_t(((span + chunks - 1) / chunks + least - 1) / least * least);
   p.chunks = uint32_t((span + p.chunk - 1) / p.chunk);
   p.blocks = base * p.chunks;
-  if (balance && p.chunks > 1 && (dim == 512 || p.chunk > least)) {
+  const uint32_t floor = dim == 512 ? 256 : uint32_t(least);  // of a balanced chunk
+  // (at heads of 512 not where the longest lengths give chunks of a step each)
+  const bool longer = dim == 512 ? balanced_steps(p.blocks, uint32_t(slots), floor / 64) > 1 : p.chunk > least;
+  if (balance && p.chunks > 1 && longer) {
     p.fill = uint32_t((slots + tiles * a.kv_heads - 1) / (tiles * a.kv_heads));
-    p.least = dim == 512 ? 256 : uint32_t(least);
+    p.least = floor;
   }
   return p;
 }

@@ -94,8 +94,8 @@ def test_chunks_do_not_jump_with_the_lengths(lib, steps, heads):  # noqa: F811
         before = None
         for n in range(192, 20000, 64):
             p = plan(lib, seqs, heads, 1, 512, 1, n)
-            assert p.fill and p.chunks > 1, (seqs, n)
-            size = steps(seqs * n // 64, p.fill, p.least // 64)
+            assert p.chunks > 1 and (p.fill or p.chunk == 64), (seqs, n)
+            size = steps(seqs * n // 64, p.fill, p.least // 64) if p.fill else 1
             assert before is None or 0 <= size - before <= 1, (seqs, n, before, size)
             before = size
 
