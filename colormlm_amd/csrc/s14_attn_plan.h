@@ -24,8 +24,9 @@ struct PagedPlan {
   uint32_t fused;      // the last workgroup of a row tile joins its chunks; else a second launch
   uint64_t blocks;     // workgroups
   // Above 0: the chunk is set on the device, by what the sequences hold in all
-  // (balanced_steps), so that `fill` workgroups a row tile and key head have it.
-  // chunks is then the most that a sequence is cut into.
+  // (balanced_steps), so that `fill` workgroups a row tile and key head have it, in
+  // chunks of `least` tokens at least where the card is full.  chunks is then the most
+  // that a sequence is cut into.
   uint32_t fill, least;
 };
 constexpr uint64_t kPagedPartFloats = 16ull << 20;  // the workspace: 64 MiB
@@ -81,8 +82,8 @@ constexpr uint32_t balanced_steps(uint64_t total, uint32_t fill, uint32_t least)
 // up to 51,525 40 / 30, 38 of up to 422, window 161, 18 / 12).
 //
 // Chunks.  Where the launch alone would leave compute units idle: as many
-// workgroups as the card holds at once (counted as below; a second round for a few of them costs
-// as much as the first), of several sequences twice as many, since their
+// workgroups as the card holds at once (counted as below; a second round for a few
+// of them costs as much as the first), of several sequences twice as many, since their
 // lengths differ and short ones leave chunks empty (us, once / twice: 16
 // sequences of up to 8,192 tokens 36 / 29 ragged, 55 / 55 equal; 4 of up to
 // 9,000, 64 heads of 512, 49 / 37 and 56 / 72; 3 of 200 new of up to 6,000 96 /
@@ -105,10 +106,10 @@ constexpr uint32_t balanced_steps(uint64_t total, uint32_t fill, uint32_t least)
 // up to 6,000 94 / 88; 64 of 1 of 4,000, heads of 512, 79 / 65; 4 of 4 of up to 9,000
 // 33.7 / 34.8).  With smaller results the sum of the lengths costs more than it saves
 // (20 of 2 of up to 9,000, heads of 64: 18 / 21), and with 64 rows of heads of 256 it
-// decides nothing (16 of 16 of 4,096 35.4 / 35.5, 8 of 64 of 3,000 45.0 / 45.0, 32 of 16
-// of up to 4,000 46.8 / 46.2, 16 of 16 of 8,192 52.0 / 52.6).  At heads of 512 small chunks are
-// balanced too, with 256 tokens at least, whose codes are as many bytes as the partial
-// result (us, by max_len, chunks of 64 to 128 / at least 192 / 256 / 320: 8 of 1 of 2,048
+// decides nothing (16 of 16 of 4,096 35.4 / 35.5, 8 of 64 of 3,000 45.0 / 45.0, 32 of
+// 16 of up to 4,000 46.8 / 46.2, 16 of 16 of 8,192 52.0 / 52.6).  At heads of 512 small
+// chunks are balanced too, with 256 tokens at least, whose codes are as many bytes as
+// the partial result (us, by max_len, chunks of 64 to 128 / at least 192 / 256 / 320: 8 of 1 of 2,048
 // 26.9 / 23.0 / 22.6 / 23.9; 7 of 1 of 4,096 39.8 / 27.8 / 24.9 / 25.9; 31 of 1 of 1,000
 // 42.0 / 27.0 / 24.2 / 25.1), and less where the card is not full (2 of 1 of 1,000:
 // chunks of 64 14.0, the same balanced 14.7, of 256 16.9).
@@ -133,7 +134,7 @@ inline PagedPlan paged_plan(const PagedShape &a) {
   // compute unit more would fit with most, but more chunks take longer there (us, by
   // these / by all that fit: one sequence of 8 of 40,000 20.5 / 23.4, of 1 19.1 / 20.3; 16
   // of 1 of up to 8,192 24.9 / 27.9, heads of 256 20.9 / 27.3; 96 of 1 of 2,048, 2 key
-  // heads, 20.9 / 24.6; the others of 63 shapes within 4 %)
+  // heads, 20.9 / 24.6; the others of 63 shapes from 3 % shorter to 8 % longer)
   const uint32_t words = (dim == 512 ? 128 : dim) * p.row_tiles;
   const uint64_t per_cu = p.staged ? (dim == 256 ? 2 : (dim == 64 ? 4 : 3) - p.row_tiles / 8)
                                    : (words <= 64 ? 3 : words <= 128 || dim == 512 ? 2 : 1);
